@@ -486,6 +486,7 @@ typedef enum lwm_norm_kind {
     LWM_NORM_BATCH = 0, /* BatchNorm1d in eval mode (running statistics), eps 1e-5 */
     LWM_NORM_LAYER = 1, /* LayerNorm, eps 1e-5 */
     LWM_NORM_NONE = 2,
+    LWM_NORM_RMS = 3,   /* x / sqrt(mean(x^2) + eps): lwm_gated_norm_device only */
 } lwm_norm_kind;
 typedef enum lwm_encoder_kind {
     LWM_ENCODER_VECTOR_MLP = 0,
@@ -730,6 +731,198 @@ lwm_status lwm_lewm_plan_nv12_device(lwm_planner* planner, lwm_scorer* scorer, c
                                      const uint8_t* uv_plane, uint32_t batch, uint32_t history, uint32_t height,
                                      uint32_t width, int32_t color_space, const lwm_image_preprocess* cfg,
                                      const float* injected_noise, lwm_plan_device_result* out);
+
+/* ---------------------------------------------------------------- transformer blocks
+ * Device-buffer entry points for world models that a caller runs itself, in
+ * a callback scorer (lwm_scorer_callback_create) or around a planner: rotary
+ * positions with several axes, a paged cache of keys and values with the
+ * attention that reads it, and the norms around a block with its gate.  The
+ * reference has no counterpart: its predictor recomputes a window of a few
+ * frames each step (src/models/lewm/model.rs:94-147); a model with a longer
+ * history keeps a cache, whose pages all candidates of a vehicle share.
+ *
+ * All buffers are the caller's, all work is asynchronous on the context's
+ * stream, nothing is allocated and no state is kept between calls, so every
+ * call can be captured into a CUDA graph, and graphs or threads share
+ * nothing but the buffers that the caller gives them.  The calls leave the
+ * calling thread's current device as it was.  16-bit and 32-bit tensors
+ * start on 16-byte boundaries and have strides (in elements) that are
+ * multiples of 8, with the channels of a head contiguous. */
+typedef enum lwm_dtype {
+    LWM_DTYPE_F32 = 0,
+    LWM_DTYPE_BF16 = 1,
+    LWM_DTYPE_F16 = 2,
+} lwm_dtype;
+
+/* Rotary positions.  A head's first sum(dims) channels are split among
+ * `axes` axes in order (one for text-like sequences, two for the rows and
+ * columns of an image, three with time), `dims[a]` channels each; pair i of
+ * an axis with n channels is (i, i + n/2), or (2i, 2i + 1) when interleaved,
+ * and turns by position * base^(-2i/n) radians.  Channels behind the last
+ * axis pass through.  Filled by lwm_rotary_init; `turn` is a pair's
+ * frequency in 2^-64 turns per position, so that position * turn modulo 2^64
+ * is its angle with no loss at far positions. */
+#define LWM_ROTARY_MAX_AXES 4
+#define LWM_ROTARY_MAX_PAIRS 64
+typedef struct lwm_rotary {
+    uint32_t axes;
+    uint32_t dims[LWM_ROTARY_MAX_AXES];
+    int32_t interleaved;
+    uint64_t turn[LWM_ROTARY_MAX_PAIRS];
+} lwm_rotary;
+/* dims: multiples of 16 (of 8 when interleaved), 128 at most together;
+ * bases finite and > 0. */
+lwm_status lwm_rotary_init(uint32_t axes, const uint32_t* dims, const double* bases, int32_t interleaved,
+                           lwm_rotary* out);
+/* out = x turned by its token's positions (inverse: turned back, which is
+ * also the gradient of x for a gradient of out).  x, out [tokens, heads,
+ * head_dim] of `dtype` with the strides given (head_dim a multiple of 8 up
+ * to 256), out may be x; positions [tokens, axes] int32, any sign. */
+typedef struct lwm_rotary_args {
+    const void* x;
+    void* out;
+    uint64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+    const int32_t* positions;
+    uint32_t tokens, heads, head_dim;
+    int32_t dtype;
+    int32_t inverse;
+} lwm_rotary_args;
+lwm_status lwm_rotary_device(lwm_ctx* ctx, const lwm_rotary* rotary, const lwm_rotary_args* args);
+
+/* A layer's paged cache.  k, v [pages, kv_heads, page_tokens, head_dim];
+ * head_dim 32, 64 or 128; page_tokens 16, 32, 64 or 128.  LWM_CACHE_16BIT
+ * holds values of `dtype` (bf16 or f16); LWM_CACHE_E4M3 holds 8-bit codes
+ * (4-bit exponent, 3-bit mantissa) and one f32 scale for each page and head,
+ * k_scale and v_scale [pages, kv_heads]: a value is code * scale. */
+typedef enum lwm_cache_storage {
+    LWM_CACHE_16BIT = 0,
+    LWM_CACHE_E4M3 = 1,
+} lwm_cache_storage;
+typedef struct lwm_paged_cache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    uint32_t pages, kv_heads, page_tokens, head_dim;
+    int32_t dtype;   /* bf16 or f16: the queries, keys and values of the calls */
+    int32_t storage; /* lwm_cache_storage */
+} lwm_paged_cache;
+/* A batch of sequences of different lengths.  Device arrays, read when the
+ * kernels run: table [sequences, table_stride] (the page that holds tokens
+ * [j page_tokens, (j + 1) page_tokens) of a sequence), lengths [sequences]
+ * (cached tokens, those of this call included), starts [sequences + 1]
+ * (ascending from 0): sequence s owns packed rows [starts[s],
+ * starts[s + 1]), its newest tokens, at cache indices lengths[s] - n ..
+ * lengths[s] - 1.  `tokens` is the row count of the packed tensors (rows
+ * from starts[sequences] on are left as they are), `max_new` at least every
+ * n; `max_length` (0: the table's reach) says how long sequences get, for
+ * the shape of the launch only.  Sequences may share pages that this call
+ * does not append to; entries of pages that no visible token lies in are
+ * not read.
+ *
+ * A sequence whose starts or length are out of order, above max_new, below 0
+ * or beyond its table, and a visible token whose page is not in the pool,
+ * are skipped (a skipped row of an attention is zero or left as it was); the
+ * next lwm_ctx_synchronize returns LWM_INVALID_ARGUMENT naming one, once. */
+typedef struct lwm_cache_batch {
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* starts;
+    uint32_t sequences, table_stride, tokens, max_new, max_length;
+} lwm_cache_batch;
+/* Appends keys and values, turned on the way (rotary NULL: as they are).  k,
+ * v [tokens, kv_heads, head_dim] and, optionally, q [tokens, heads,
+ * head_dim] with q_out (which may be q) of the cache's dtype; only keys and
+ * queries are turned.  positions [tokens, axes] int32, or NULL: a token's
+ * cache index on every axis.
+ *
+ * LWM_CACHE_E4M3: the scale of a page and head becomes the least power of
+ * two s (2^-120 at least) with |x| <= 448 s for the tokens appended to the
+ * page by this call, or stays where it is larger and the page holds earlier
+ * tokens of the sequence; where it grows, the earlier tokens' codes are
+ * rounded again.  A power of two keeps the codes' own rounding the only one.
+ * Infinities and NaN do not count for the scale and are stored as NaN. */
+typedef struct lwm_cache_append_args {
+    const void* q;
+    void* q_out;
+    const void* k;
+    const void* v;
+    uint64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+    uint64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const int32_t* positions;
+    uint32_t heads; /* query heads (ignored without q) */
+} lwm_cache_append_args;
+lwm_status lwm_cache_append_device(lwm_ctx* ctx, const lwm_paged_cache* cache, const lwm_cache_batch* batch,
+                                   const lwm_rotary* rotary, const lwm_cache_append_args* args);
+/* Reads the batch's tokens back out of the pages, as the values they stand
+ * for: k_out, v_out [tokens, kv_heads, head_dim] of the cache's dtype. */
+typedef struct lwm_cache_gather_args {
+    void* k_out;
+    void* v_out;
+    uint64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} lwm_cache_gather_args;
+lwm_status lwm_cache_gather_device(lwm_ctx* ctx, const lwm_paged_cache* cache, const lwm_cache_batch* batch,
+                                   const lwm_cache_gather_args* args);
+/* Attention of the batch's tokens over their sequences' cached tokens: out =
+ * softmax(scale q . k) v over the visible keys, zero where there is none.
+ * q, out [tokens, heads, head_dim] of the cache's dtype (out may be q);
+ * query head h reads kv head h / (heads / kv_heads).  The token at cache
+ * index p of a sequence of length L sees index j when
+ *   j < L, or, causal, j < min(L, (p / f + 1) f)            and
+ *   window 0, or j >= (p / f + 1 - window) f, or j < sinks
+ * with f = frame_tokens (0: 1): tokens of a frame see each other, the window
+ * counts frames (tokens when f is 1), the first `sinks` tokens stay visible.
+ * Tokens before the first cached one (n > length) see nothing.  What a token
+ * does not see does not reach it, not even as infinities or NaN. */
+typedef struct lwm_cache_attention_args {
+    const void* q;
+    void* out;
+    uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    uint32_t heads;
+    float scale;
+    int32_t causal;
+    uint32_t window, sinks, frame_tokens;
+} lwm_cache_attention_args;
+lwm_status lwm_cache_attention_device(lwm_ctx* ctx, const lwm_paged_cache* cache, const lwm_cache_batch* batch,
+                                      const lwm_cache_attention_args* args);
+
+/* The end of one residual block and the norm that opens the next
+ * (ConditionalBlock, src/models/lewm/modules.rs:275-330, as one row pass):
+ *   x' = x + residual_scale * gate * post(y)        (y NULL: x' = x)
+ *   u  = pre(x') * (1 + scale) + shift
+ *   h  = out_weight ? LayerNorm(u; out_weight, out_bias, out_eps) : u
+ * post and pre are LWM_NORM_LAYER, LWM_NORM_RMS or LWM_NORM_NONE, with f32
+ * weights and biases [width] or NULL.  gate, shift, scale: [ceil(rows /
+ * rows_per_cond), width] of cond_dtype with row stride cond_stride (e.g. one
+ * modulation table's column ranges), or NULL; residual_scale f32 [width] or
+ * NULL.  x, x_out [rows, width] of residual_dtype, y, h of dtype, each with
+ * its row stride; x_out may be x or NULL, h may be y or NULL (x_out: y too,
+ * when the types agree).  width 1 to 8192; rows of any alignment.  Sums and
+ * statistics are f32, h comes from the unrounded x'. */
+typedef struct lwm_gated_norm_args {
+    const void* x;
+    const void* y;
+    void* x_out;
+    void* h;
+    uint64_t x_stride, y_stride, x_out_stride, h_stride;
+    uint32_t rows, width;
+    int32_t residual_dtype, dtype, cond_dtype;
+    const void* gate;
+    const void* shift;
+    const void* scale;
+    uint64_t cond_stride;
+    uint32_t rows_per_cond;
+    const float* residual_scale;
+    int32_t post_kind, pre_kind;
+    float post_eps, pre_eps, out_eps;
+    const float* post_weight;
+    const float* post_bias;
+    const float* pre_weight;
+    const float* pre_bias;
+    const float* out_weight;
+    const float* out_bias;
+} lwm_gated_norm_args;
+lwm_status lwm_gated_norm_device(lwm_ctx* ctx, const lwm_gated_norm_args* args);
 
 /* ---------------------------------------------------------------- allocation-free iteration */
 

@@ -22,6 +22,7 @@
 #include "../../include/lewm_b200.h"
 #include "lwm_kernels.hpp"
 #include "lwm_host.hpp"
+#include "lwm_blocks.hpp"
 #include "lwm_lewm.hpp"
 
 using lwm::MppiArgs;
@@ -151,6 +152,10 @@ struct lwm_ctx {
     // read after every stream synchronisation (allocated on first use)
     int* media_err = nullptr;
     int* media_err_dev = nullptr;
+    // error word of the paged-cache kernels (same kind of memory, made with
+    // the context so that a first call may be captured)
+    int* cache_err = nullptr;
+    int* cache_err_dev = nullptr;
     lwm_test_faults faults{};  // fault injection for tests (lwm_ctx_set_test_faults)
     // kernel timing (lwm_ctx_set_kernel_timing): events around the last
     // SkyJEPA rollout launch
@@ -163,6 +168,17 @@ struct lwm_ctx {
         kt_valid = true;
     }
 };
+
+namespace lwm {
+bool ctx_view(lwm_ctx* ctx, CtxView* out) {
+    if (!ctx) return false;
+    out->device = ctx->device;
+    out->stream = ctx->stream;
+    out->cache_err = ctx->cache_err_dev;
+    return true;
+}
+void ctx_add_launches(lwm_ctx* ctx, uint64_t n) { ctx->launches += n; }
+}  // namespace lwm
 
 enum class PlannerKind { Mppi, Cem, Icem };
 enum class ScorerKind { Nominal, Skyjepa, Callback, Lewm };
@@ -1058,6 +1074,17 @@ lwm_status lwm_ctx_create(int device, lwm_ctx** out) {
         delete ctx;
         return fail(LWM_CUDA_ERROR, std::string("cudaStreamCreate failed: ") + cudaGetErrorString(e));
     }
+    e = cudaHostAlloc(reinterpret_cast<void**>(&ctx->cache_err), 4 * sizeof(int), cudaHostAllocMapped);
+    if (e == cudaSuccess) {
+        for (int i = 0; i < 4; ++i) ctx->cache_err[i] = 0;
+        e = cudaHostGetDevicePointer(reinterpret_cast<void**>(&ctx->cache_err_dev), ctx->cache_err, 0);
+    }
+    if (e != cudaSuccess) {
+        if (ctx->cache_err) cudaFreeHost(ctx->cache_err);
+        cudaStreamDestroy(ctx->stream);
+        delete ctx;
+        return fail(LWM_CUDA_ERROR, std::string("cudaHostAlloc failed: ") + cudaGetErrorString(e));
+    }
     std::random_device rd;
     ctx->unseeded_seed = (static_cast<uint64_t>(rd()) << 32) ^ rd();
     *out = ctx;
@@ -1070,6 +1097,7 @@ lwm_status lwm_ctx_destroy(lwm_ctx* ctx) {
     cudaStreamSynchronize(ctx->stream);
     cudaStreamDestroy(ctx->stream);
     if (ctx->media_err) cudaFreeHost(ctx->media_err);
+    cudaFreeHost(ctx->cache_err);
     if (ctx->kt_begin) cudaEventDestroy(ctx->kt_begin);
     if (ctx->kt_end) cudaEventDestroy(ctx->kt_end);
     delete ctx;
@@ -1092,6 +1120,18 @@ lwm_status lwm_ctx_synchronize(lwm_ctx* ctx) {
         for (int i = 0; i < 4; ++i) ctx->media_err[i] = 0;
         return fail(LWM_CUDA_ERROR, "image preprocessing: a source-row copy never completed (" + where +
                                         "); that launch's output is incomplete");
+    }
+    if (const int code = static_cast<volatile int*>(ctx->cache_err)[0]) {
+        const std::string seq = "paged cache: sequence " + std::to_string(ctx->cache_err[1]);
+        const std::string at = std::to_string(ctx->cache_err[2]);
+        for (int i = 0; i < 4; ++i) ctx->cache_err[i] = 0;
+        switch (code) {
+            case lwm::kCacheErrStarts: return fail(LWM_INVALID_ARGUMENT, seq + ": starts are out of order or beyond the packed rows (" + at + ")");
+            case lwm::kCacheErrNew: return fail(LWM_INVALID_ARGUMENT, seq + ": more new tokens (" + at + ") than max_new or its length");
+            case lwm::kCacheErrLength: return fail(LWM_INVALID_ARGUMENT, seq + ": length " + at + " is negative or beyond its page table");
+            case lwm::kCacheErrPage: return fail(LWM_INVALID_ARGUMENT, seq + ": page " + at + " is not in the pool");
+            default: return fail(LWM_CUDA_ERROR, seq + ": a pipeline wait of the attention kernel gave up (site " + at + ")");
+        }
     }
     return LWM_OK;
 }

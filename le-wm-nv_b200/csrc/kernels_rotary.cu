@@ -1,0 +1,77 @@
+// kernels_rotary.cu — rotary positions with several axes, dense tensors
+// (lwm_rotary_device).  Bound: memory, each channel read and written once.
+//
+// A block takes a few tokens: it computes the cosine and sine of their pairs
+// once into shared memory (64-bit fixed-point angles, see turn_of), then its
+// threads turn the heads' 16-byte vectors.  With halves a thread owns both
+// vectors of 8 pairs, so no value is read twice.
+#include "lwm_blocks.cuh"
+
+namespace lwm {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, uint32_t block_tokens, FastDiv units_div,
+                                                          FastDiv heads_div, FastDiv pairs_div) {
+    extern __shared__ float2 trig[];  // [block_tokens][pairs]
+    const uint32_t t0 = blockIdx.x * block_tokens, nt = min(block_tokens, a.tokens - t0);
+    const HeadUnits hu(a.pairs, a.r.interleaved, a.head_dim);
+    for (uint32_t i = threadIdx.x; i < nt * a.pairs; i += kThreads) {
+        const uint32_t t = pairs_div.div(i), p = i - t * a.pairs;
+        float2 cs = turn_of(a.positions[static_cast<size_t>(t0 + t) * a.r.axes + axis_of(a.r, p)], a.r.turn[p]);
+        if (a.inverse) cs.y = -cs.y;
+        trig[i] = cs;
+    }
+    __syncthreads();
+    const T* x = static_cast<const T*>(a.x);
+    T* out = static_cast<T*>(a.out);
+    for (uint32_t i = threadIdx.x; i < nt * a.heads * hu.count; i += kThreads) {
+        const uint32_t row = units_div.div(i), u = i - row * hu.count;
+        const uint32_t t = heads_div.div(row), h = row - t * a.heads;
+        const T* xr = x + (t0 + t) * a.x_ts + h * a.x_hs;
+        T* orow = out + (t0 + t) * a.o_ts + h * a.o_hs;
+        if (u >= hu.turned) {
+            const uint32_t ch = 2 * a.pairs + 8 * (u - hu.turned);
+            store8(orow + ch, load8(xr + ch));
+            continue;
+        }
+        uint32_t ch, apart, pair;
+        unit_place(a.r, u, ch, apart, pair);
+        const float2* cs = trig + t * a.pairs + pair;
+        float v[8];
+        unpack(load8(xr + ch), v);
+        if (a.r.interleaved) {
+            turn_pairs(v, cs);
+        } else {
+            float w[8];
+            unpack(load8(xr + ch + apart), w);
+            turn_halves(v, w, cs);
+            store8(orow + ch + apart, pack<T>(w));
+        }
+        store8(orow + ch, pack<T>(v));
+    }
+}
+
+template <typename T> cudaError_t launch(const RotaryArgs& a, cudaStream_t s) {
+    const HeadUnits hu(a.pairs, a.r.interleaved, a.head_dim);
+    const uint32_t per_token = a.heads * hu.count;
+    // four units a thread, unless that leaves SMs without a block
+    uint32_t bt = max(1u, min(32u, 4 * kThreads / per_token));
+    while (bt > 1 && a.tokens / bt < 148 * 4) bt /= 2;
+    const uint32_t blocks = (a.tokens + bt - 1) / bt;
+    rotary_kernel<T><<<blocks, kThreads, bt * a.pairs * sizeof(float2), s>>>(
+        a, bt, FastDiv(hu.count), FastDiv(a.heads), FastDiv(a.pairs));
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_rotary(const RotaryArgs& a, int dtype, cudaStream_t s) {
+    if (dtype == LWM_DTYPE_F32) return launch<float>(a, s);
+    return dtype == LWM_DTYPE_BF16 ? launch<bf16>(a, s) : launch<__half>(a, s);
+}
+
+}  // namespace lwm

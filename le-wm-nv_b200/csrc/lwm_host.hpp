@@ -14,6 +14,15 @@ namespace lwm {
 // Stores `message` as this thread's lwm_last_error() text and returns `status`.
 lwm_status set_last_error(lwm_status status, const std::string& message);
 
+// What the entry points outside api.cpp need of a context.
+struct CtxView {
+    int device = 0;
+    void* stream = nullptr;   // cudaStream_t
+    int* cache_err = nullptr; // the paged-cache kernels' error word (device address, 4 ints)
+};
+bool ctx_view(lwm_ctx* ctx, CtxView* out);
+void ctx_add_launches(lwm_ctx* ctx, uint64_t n);
+
 // One tensor of a weight blob: its VarBuilder path, shape, place in the blob
 // and the file it lives in (SkyJEPA: 0 latent model, 1 prober).
 struct NamedTensor {

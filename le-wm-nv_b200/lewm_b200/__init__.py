@@ -290,6 +290,67 @@ class FleetStep(C.Structure):
                 ("reference_states", VP), ("reference_actions", VP)]
 
 
+class _PagedCache(C.Structure):
+    _fields_ = [("k", VP), ("v", VP), ("k_scale", VP), ("v_scale", VP), ("pages", U32), ("kv_heads", U32),
+                ("page_tokens", U32), ("head_dim", U32), ("dtype", I32), ("storage", I32)]
+
+
+class _CacheBatch(C.Structure):
+    _fields_ = [("table", VP), ("lengths", VP), ("starts", VP), ("sequences", U32), ("table_stride", U32),
+                ("tokens", U32), ("max_new", U32), ("max_length", U32)]
+
+
+class _RotaryArgs(C.Structure):
+    _fields_ = [("x", VP), ("out", VP), ("x_token_stride", U64), ("x_head_stride", U64), ("out_token_stride", U64),
+                ("out_head_stride", U64), ("positions", VP), ("tokens", U32), ("heads", U32), ("head_dim", U32),
+                ("dtype", I32), ("inverse", I32)]
+
+
+class _CacheAppendArgs(C.Structure):
+    _fields_ = [("q", VP), ("q_out", VP), ("k", VP), ("v", VP), ("q_token_stride", U64), ("q_head_stride", U64),
+                ("q_out_token_stride", U64), ("q_out_head_stride", U64), ("k_token_stride", U64),
+                ("k_head_stride", U64), ("v_token_stride", U64), ("v_head_stride", U64), ("positions", VP),
+                ("heads", U32)]
+
+
+class _CacheGatherArgs(C.Structure):
+    _fields_ = [("k_out", VP), ("v_out", VP), ("k_token_stride", U64), ("k_head_stride", U64),
+                ("v_token_stride", U64), ("v_head_stride", U64)]
+
+
+class _CacheAttentionArgs(C.Structure):
+    _fields_ = [("q", VP), ("out", VP), ("q_token_stride", U64), ("q_head_stride", U64), ("out_token_stride", U64),
+                ("out_head_stride", U64), ("heads", U32), ("scale", F), ("causal", I32), ("window", U32),
+                ("sinks", U32), ("frame_tokens", U32)]
+
+
+class _GatedNormArgs(C.Structure):
+    _fields_ = [("x", VP), ("y", VP), ("x_out", VP), ("h", VP), ("x_stride", U64), ("y_stride", U64),
+                ("x_out_stride", U64), ("h_stride", U64), ("rows", U32), ("width", U32), ("residual_dtype", I32),
+                ("dtype", I32), ("cond_dtype", I32), ("gate", VP), ("shift", VP), ("scale", VP), ("cond_stride", U64),
+                ("rows_per_cond", U32), ("residual_scale", VP), ("post_kind", I32), ("pre_kind", I32),
+                ("post_eps", F), ("pre_eps", F), ("out_eps", F), ("post_weight", VP), ("post_bias", VP),
+                ("pre_weight", VP), ("pre_bias", VP), ("out_weight", VP), ("out_bias", VP)]
+
+
+class Rotary(C.Structure):
+    """lwm_rotary: rotary positions with one to four axes (include/lewm_b200.h)."""
+    _fields_ = [("axes", U32), ("dims", U32 * 4), ("interleaved", I32), ("turn", U64 * 64)]
+
+    @staticmethod
+    def make(dims: Sequence[int], bases, interleaved: bool = False) -> "Rotary":
+        """`dims[a]` channels of every head turn by axis a, with base `bases[a]` (or one base for all)."""
+        n = len(dims)
+        b = list(bases) if hasattr(bases, "__len__") else [bases] * n
+        if len(b) != n:
+            raise LwmError(1, f"rotary has {n} axes and {len(b)} bases")
+        if n > 4:
+            raise LwmError(1, "rotary axes must be 1 to 4")
+        r = Rotary()
+        _check(lib.lwm_rotary_init(n, (U32 * 4)(*dims), (C.c_double * 4)(*b), int(interleaved), C.byref(r)))
+        return r
+
+
 SCORE_FN = C.CFUNCTYPE(C.c_int, VP, VP, U32, U32, U32, U32, VP, VP)
 EXCHANGE_FN = C.CFUNCTYPE(C.c_int, VP, VP, C.c_size_t, VP, VP)
 
@@ -400,6 +461,15 @@ _sig("lwm_preprocess_nv12_patches_device", C.c_int, VP, VP, VP, U32, U32, U32, I
 _sig("lwm_lewm_encode_nv12_device", C.c_int, VP, VP, VP, U32, U32, U32, I32, C.POINTER(ImagePreprocess), VP)
 _sig("lwm_lewm_plan_nv12_device", C.c_int, VP, VP, VP, VP, U32, U32, U32, U32, I32, C.POINTER(ImagePreprocess), VP,
      C.POINTER(_PlanDeviceResult))
+_sig("lwm_rotary_init", C.c_int, U32, C.POINTER(U32), C.POINTER(C.c_double), I32, C.POINTER(Rotary))
+_sig("lwm_rotary_device", C.c_int, VP, C.POINTER(Rotary), C.POINTER(_RotaryArgs))
+_sig("lwm_cache_append_device", C.c_int, VP, C.POINTER(_PagedCache), C.POINTER(_CacheBatch), C.POINTER(Rotary),
+     C.POINTER(_CacheAppendArgs))
+_sig("lwm_cache_gather_device", C.c_int, VP, C.POINTER(_PagedCache), C.POINTER(_CacheBatch),
+     C.POINTER(_CacheGatherArgs))
+_sig("lwm_cache_attention_device", C.c_int, VP, C.POINTER(_PagedCache), C.POINTER(_CacheBatch),
+     C.POINTER(_CacheAttentionArgs))
+_sig("lwm_gated_norm_device", C.c_int, VP, C.POINTER(_GatedNormArgs))
 _sig("lwm_lewm_encode_packed_device", C.c_int, VP, VP, U32, U32, U32, I32, C.POINTER(ImagePreprocess), VP)
 
 
@@ -1153,6 +1223,247 @@ def preprocess_nv12_device(ctx: Context, y_plane, uv_plane, batch: int, height: 
     cs = NV12_COLOR_SPACES[color_space] if isinstance(color_space, str) else int(color_space)
     _check(lib.lwm_preprocess_nv12_device(ctx.handle, VP(_ptr(y_plane)), VP(_ptr(uv_plane)), batch, height, width,
                                           cs, C.byref(cfg), history_len, history_slot, int(bf16), VP(_ptr(out))))
+
+
+# ------------------------------------------------------------ transformer blocks
+#
+# Operators of a world model that the caller runs itself (in a CallbackScorer,
+# or around a planner), on torch CUDA tensors and the context's stream.
+
+DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+
+
+def _dtype(t, name: str) -> int:
+    d = DTYPES.get(str(t.dtype))
+    if d is None:
+        raise LwmError(1, f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return d
+
+
+def _on(ctx: Context, name: str, t) -> int:
+    """The address of a tensor on the context's device."""
+    if not t.is_cuda or t.device.index != ctx.device:
+        raise LwmError(1, f"{name} must be on cuda:{ctx.device}, got {t.device}")
+    return t.data_ptr()
+
+
+def _heads(ctx: Context, name: str, t, shape, dtype) -> int:
+    """The address of a [tokens, heads, channels] tensor with contiguous channels."""
+    if tuple(t.shape) != shape:
+        raise LwmError(1, f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype != dtype:
+        raise LwmError(1, f"{name} must be {dtype}, got {t.dtype}")
+    if t.stride(2) != 1:
+        raise LwmError(1, f"{name} needs contiguous channels")
+    return _on(ctx, name, t)
+
+
+def _ints(name: str, t, shape) -> None:
+    if str(t.dtype) != "torch.int32" or tuple(t.shape) != shape or not t.is_contiguous():
+        raise LwmError(1, f"{name} must be a contiguous int32 tensor {list(shape)}, got {t.dtype} {list(t.shape)}")
+
+
+class PagedCache:
+    """lwm_paged_cache over torch tensors: k, v [pages, kv_heads, page_tokens,
+    head_dim] in bfloat16 or float16, or 8-bit codes (float8_e4m3fn or uint8)
+    with scales [pages, kv_heads] and the `dtype` of the values."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None, dtype=None):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise LwmError(1, "cache pools must be two [pages, kv_heads, page_tokens, head_dim] tensors of one type")
+        if not (k.is_contiguous() and v.is_contiguous()):
+            raise LwmError(1, "cache pools must be contiguous")
+        codes = k.element_size() == 1
+        if codes:
+            if str(k.dtype) not in ("torch.float8_e4m3fn", "torch.uint8"):
+                raise LwmError(1, f"8-bit cache pools hold float8_e4m3fn codes, got {k.dtype}")
+            if dtype is None or k_scale is None or v_scale is None:
+                raise LwmError(1, "an 8-bit cache needs k_scale, v_scale and the dtype of its values")
+            for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+                if str(t.dtype) != "torch.float32" or tuple(t.shape) != tuple(k.shape[:2]) or not t.is_contiguous():
+                    raise LwmError(1, f"{name} must be a contiguous float32 tensor {list(k.shape[:2])}")
+        self.dtype = dtype if codes else k.dtype
+        if str(self.dtype) not in ("torch.bfloat16", "torch.float16"):
+            raise LwmError(1, f"cache dtype must be bfloat16 or float16, got {self.dtype}")
+        self._keep = (k, v, k_scale, v_scale)
+        self.device = k.device
+        if any(t is not None and t.device != k.device for t in self._keep):
+            raise LwmError(1, "cache tensors are on different devices")
+        self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
+        self._c = _PagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if codes else None,
+                              v_scale.data_ptr() if codes else None, *k.shape, DTYPES[str(self.dtype)], int(codes))
+        self._ref = C.byref(self._c)
+
+
+class CacheBatch:
+    """lwm_cache_batch: the page table [sequences, pages], starts [sequences +
+    1] and lengths [sequences] (int32 device tensors, read when the kernels
+    run), the packed rows `tokens`, and bounds of a sequence's new tokens and
+    length."""
+
+    def __init__(self, table, starts, lengths, tokens: int, max_new: Optional[int] = None, max_length: int = 0):
+        if table.dim() != 2:
+            raise LwmError(1, "page table must be [sequences, pages]")
+        n = table.shape[0]
+        _ints("page table", table, tuple(table.shape))
+        _ints("starts", starts, (n + 1,))
+        _ints("lengths", lengths, (n,))
+        self._keep = (table, starts, lengths)
+        self.device = table.device
+        if starts.device != table.device or lengths.device != table.device:
+            raise LwmError(1, "batch tensors are on different devices")
+        self.tokens = tokens
+        self._c = _CacheBatch(table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), n, table.shape[1], tokens,
+                              tokens if max_new is None else max_new, max_length)
+        self._ref = C.byref(self._c)
+
+
+def _same_device(ctx: Context, cache: PagedCache, batch: CacheBatch) -> None:
+    for name, x in (("cache", cache), ("batch", batch)):
+        if x.device.type != "cuda" or x.device.index != ctx.device:
+            raise LwmError(1, f"{name} must be on cuda:{ctx.device}, got {x.device}")
+
+
+def rotary_device(ctx: Context, rotary: Rotary, x, out, positions, inverse: bool = False) -> None:
+    """out = x [tokens, heads, head_dim] turned by positions [tokens, axes] int32 (`inverse`: turned back)."""
+    if x.dim() != 3:
+        raise LwmError(1, f"x must be [tokens, heads, head_dim], got {list(x.shape)}")
+    tokens, heads, d = x.shape
+    shape = (tokens, heads, d)
+    _ints("positions", positions, (tokens, rotary.axes))
+    a = _RotaryArgs(_heads(ctx, "x", x, shape, x.dtype), _heads(ctx, "out", out, shape, x.dtype), x.stride(0),
+                    x.stride(1), out.stride(0), out.stride(1), _on(ctx, "positions", positions), tokens, heads, d,
+                    _dtype(x, "x"), int(inverse))
+    _check(lib.lwm_rotary_device(ctx.handle, C.byref(rotary), C.byref(a)))
+
+
+def cache_append_device(ctx: Context, cache: PagedCache, batch: CacheBatch, k, v, rotary: Optional[Rotary] = None,
+                        positions=None, q=None, q_out=None) -> None:
+    """Appends k, v [tokens, kv_heads, head_dim] to the batch's sequences, the
+    keys (and q [tokens, heads, head_dim] into q_out) turned by `positions`
+    [tokens, axes] (None: each token's cache index)."""
+    _same_device(ctx, cache, batch)
+    n, shape = batch.tokens, (batch.tokens, cache.kv_heads, cache.head_dim)
+    if positions is not None:
+        if rotary is None:
+            raise LwmError(1, "positions need a rotary")
+        _ints("positions", positions, (n, rotary.axes))
+    kp, vp = _heads(ctx, "k", k, shape, cache.dtype), _heads(ctx, "v", v, shape, cache.dtype)
+    if q is not None:
+        if q_out is None or q.dim() != 3:
+            raise LwmError(1, "q [tokens, heads, head_dim] needs q_out")
+        heads = q.shape[1]
+        shape = (n, heads, cache.head_dim)
+        qp, qo = _heads(ctx, "q", q, shape, cache.dtype), _heads(ctx, "q_out", q_out, shape, cache.dtype)
+        a = _CacheAppendArgs(qp, qo, kp, vp, q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1), k.stride(0),
+                             k.stride(1), v.stride(0), v.stride(1),
+                             None if positions is None else _on(ctx, "positions", positions), heads)
+    else:
+        a = _CacheAppendArgs(None, None, kp, vp, 0, 0, 0, 0, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                             None if positions is None else _on(ctx, "positions", positions), 0)
+    _check(lib.lwm_cache_append_device(ctx.handle, cache._ref, batch._ref,
+                                       None if rotary is None else C.byref(rotary), C.byref(a)))
+
+
+def cache_gather_device(ctx: Context, cache: PagedCache, batch: CacheBatch, k_out, v_out) -> None:
+    """The batch's cached tokens as values: k_out, v_out [tokens, kv_heads, head_dim] of the cache's dtype."""
+    _same_device(ctx, cache, batch)
+    shape = (batch.tokens, cache.kv_heads, cache.head_dim)
+    a = _CacheGatherArgs(_heads(ctx, "k_out", k_out, shape, cache.dtype),
+                         _heads(ctx, "v_out", v_out, shape, cache.dtype), k_out.stride(0), k_out.stride(1),
+                         v_out.stride(0), v_out.stride(1))
+    _check(lib.lwm_cache_gather_device(ctx.handle, cache._ref, batch._ref, C.byref(a)))
+
+
+def cache_attention_device(ctx: Context, cache: PagedCache, batch: CacheBatch, q, out, scale: Optional[float] = None,
+                           causal: bool = True, window: int = 0, sinks: int = 0, frame_tokens: int = 1) -> None:
+    """out = attention of q [tokens, heads, head_dim] over the sequences'
+    cached tokens (scale None: head_dim ** -0.5); `window` frames of
+    `frame_tokens` tokens and the first `sinks` tokens are visible, window 0:
+    everything before."""
+    _same_device(ctx, cache, batch)
+    if q.dim() != 3:
+        raise LwmError(1, f"q must be [tokens, heads, head_dim], got {list(q.shape)}")
+    shape = (batch.tokens, q.shape[1], cache.head_dim)
+    a = _CacheAttentionArgs(_heads(ctx, "q", q, shape, cache.dtype), _heads(ctx, "out", out, shape, cache.dtype),
+                            q.stride(0), q.stride(1), out.stride(0), out.stride(1), shape[1],
+                            cache.head_dim ** -0.5 if scale is None else scale, int(causal), window, sinks,
+                            frame_tokens)
+    _check(lib.lwm_cache_attention_device(ctx.handle, cache._ref, batch._ref, C.byref(a)))
+
+
+class GatedNorm:
+    """The weights and kinds of lwm_gated_norm_device: x' = x + residual_scale
+    * gate * post(y), h = pre(x') * (1 + scale) + shift, then a LayerNorm with
+    out_weight when given.  Weights are float32 [width] tensors or None."""
+
+    def __init__(self, post: str = "none", pre: str = "layer", post_weight=None, post_bias=None, post_eps: float = 1e-6,
+                 pre_weight=None, pre_bias=None, pre_eps: float = 1e-6, residual_scale=None, out_weight=None,
+                 out_bias=None, out_eps: float = 1e-5):
+        kinds = {"layer": 1, "none": 2, "rms": 3}
+        if post not in kinds or pre not in kinds:
+            raise LwmError(1, "gated norm kinds are layer, rms or none")
+        self._keep = dict(residual_scale=residual_scale, post_weight=post_weight, post_bias=post_bias,
+                          pre_weight=pre_weight, pre_bias=pre_bias, out_weight=out_weight, out_bias=out_bias)
+        self._c = _GatedNormArgs(post_kind=kinds[post], pre_kind=kinds[pre], post_eps=post_eps, pre_eps=pre_eps,
+                                 out_eps=out_eps)
+        self.width, self.device = None, None
+        for name, t in self._keep.items():
+            if t is None:
+                continue
+            if str(t.dtype) != "torch.float32" or t.dim() != 1 or not t.is_contiguous():
+                raise LwmError(1, f"{name} must be a contiguous float32 [width] tensor")
+            if self.width not in (None, t.shape[0]) or self.device not in (None, t.device):
+                raise LwmError(1, "gated norm weights differ in width or device")
+            self.width, self.device = t.shape[0], t.device
+            setattr(self._c, name, t.data_ptr())
+
+
+def gated_norm_device(ctx: Context, norm: GatedNorm, x, y=None, x_out=None, h=None, gate=None, shift=None, scale=None,
+                      rows_per_cond: int = 1) -> None:
+    """One pass over the rows of x [rows, width] and y (None: x' = x); gate,
+    shift, scale [ceil(rows / rows_per_cond), width] of one type and row
+    stride; writes x' to x_out and the normed rows to h (either may be None)."""
+    if x.dim() != 2:
+        raise LwmError(1, f"x must be [rows, width], got {list(x.shape)}")
+    rows, width = x.shape
+    if norm.width not in (None, width):
+        raise LwmError(1, f"gated norm weights have width {norm.width}, x has {width}")
+    if norm.device is not None and norm.device != x.device:
+        raise LwmError(1, f"gated norm weights are on {norm.device}, x on {x.device}")
+    a = _GatedNormArgs.from_buffer_copy(norm._c)
+    a.rows, a.width, a.rows_per_cond = rows, width, rows_per_cond
+    a.residual_dtype = _dtype(x, "x")
+    dtype = None
+    for name, t, stride in (("x", x, "x_stride"), ("x_out", x_out, "x_out_stride"), ("y", y, "y_stride"),
+                            ("h", h, "h_stride")):
+        if t is None:
+            continue
+        if t.shape != x.shape or t.stride(1) != 1 and width > 1:
+            raise LwmError(1, f"{name} must be [{rows}, {width}] with contiguous rows, got {list(t.shape)}")
+        if name == "x_out" and t.dtype != x.dtype:
+            raise LwmError(1, f"x_out must be {x.dtype}, got {t.dtype}")
+        if name in ("y", "h"):
+            if dtype not in (None, t.dtype):
+                raise LwmError(1, "y and h must have one type")
+            dtype = t.dtype
+            a.dtype = _dtype(t, name)
+        setattr(a, name, _on(ctx, name, t))
+        setattr(a, stride, t.stride(0))
+    cond = None
+    for name, t in (("gate", gate), ("shift", shift), ("scale", scale)):
+        if t is None:
+            continue
+        if rows_per_cond < 1 or t.dim() != 2 or t.shape[1] != width or t.shape[0] * rows_per_cond < rows or \
+                (t.stride(1) != 1 and width > 1):
+            raise LwmError(1, f"{name} must be [ceil(rows / rows_per_cond), {width}] with contiguous rows, "
+                              f"got {list(t.shape)}")
+        if cond not in (None, (t.dtype, t.stride(0))):
+            raise LwmError(1, "gate, shift and scale must have one type and row stride")
+        cond = (t.dtype, t.stride(0))
+        a.cond_dtype, a.cond_stride = _dtype(t, name), t.stride(0)
+        setattr(a, name, _on(ctx, name, t))
+    _check(lib.lwm_gated_norm_device(ctx.handle, C.byref(a)))
 
 
 # --------------------------------------------------------------- fleet loop
