@@ -1,0 +1,643 @@
+// kernels_cache_attn_tc.cu — attention over the paged cache for many query
+// rows a kv head (whole histories, frames, chunks): both products on the
+// tcgen05 tensor cores.
+//
+// A block takes 256 query rows (tokens x heads of the group) of one sequence
+// and kv head as two tiles of 128, and walks the visible keys in tiles of
+// 128.  S = Q K^T goes to TMEM, a softmax warpgroup a tile (one row a
+// thread, so no shuffles) reads it, writes P back over it in the operands'
+// type, and O += P V accumulates in TMEM with P as the A operand there.  The
+// two tiles alternate: while one is in its softmax the tensor cores work for
+// the other, and both use each K and V tile that is loaded.
+//
+// TMEM: S (and P) of tile 0 and 1 at columns 0 and 128, O at 256 and
+// 256 + D.  Shared memory: Q, two stages of K and of V, all rows of 64
+// channels (128 bytes, 128-byte swizzle); K is a K-major operand, V the
+// transposed (N-major) one with the same layout.
+//
+// Producers (a warpgroup) gather the pages' rows with cp.async; 8-bit codes
+// are loaded a tile ahead into registers and become halves (exact) on the
+// way to shared memory.  Their scales stay out of the products: a page's key
+// scale multiplies its 16-key groups' scores, its value scale, relative to
+// the block's largest, enters the exponent of the weight.
+//
+// O is rescaled only when a row's maximum rises by more than 2^kRaise.
+// Every wait is bounded: one that gives up marks the block, which unwinds.
+#include "lwm_blocks.cuh"
+#include "lwm_cache_attn.cuh"
+#include "lwm_tc.cuh"
+
+namespace lwm {
+
+namespace {
+
+constexpr int kTile = 128;           // rows of a tile, keys of a step
+constexpr int kThreads = 512;        // two softmax warpgroups, producers, MMA issuer
+constexpr int kProducers = 128;
+constexpr int kPanel = kTile * 128;  // bytes of 128 rows x 64 channels
+constexpr int kInfos = 4;
+constexpr uint32_t kOCol = 256;
+
+// What the softmax needs of a key tile, by 16-key groups.
+struct TileInfo {
+    float k_scale[8];  // codes: key scales
+    float v_log[8];    // log2 of the value scale relative to the block's
+    float v_inv[8];    // its reciprocal
+    uint32_t ok;       // groups whose page is in the pool
+    uint32_t pad[7];
+};
+
+struct Control {
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], info_full[kInfos], drain;
+    uint32_t tmem;
+    int dead;        // a wait gave up
+    int poisoned;    // infinities or NaN were taken out of a V tile
+    float v_ref;     // codes: the largest value scale of the visible pages
+    float reduce[4];
+    TileInfo info[kInfos];
+};
+
+template <int D, bool kCodes> struct Shape {
+    static constexpr int kPanels = D / 64;
+    static constexpr int kTileBytes = kPanels * kPanel;
+    static constexpr int kQ = 0, kK = 2 * kTileBytes, kV = kK + 2 * kTileBytes, kControl = kV + 2 * kTileBytes;
+    static constexpr int kBytes = kControl + static_cast<int>(sizeof(Control)) + 1024;  // + alignment
+};
+
+// Called by whole warps; the answer is the warp's, so that its lanes stay together.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Control* c, int site, int* err, uint32_t seq) {
+    bool done = false;
+    for (uint32_t i = 0; i < tc::kWaitLimit && !done; ++i) {
+        done = tc::mbar_try(bar, parity);
+        if ((i & 255u) == 255u && *static_cast<volatile int*>(&c->dead)) break;
+    }
+    if (__all_sync(0xffffffffu, done)) return true;
+    if (atomicExch(&c->dead, 1) == 0) cache_report(err, kCacheErrWait, seq, site);
+    return false;
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+// kind::f16 descriptor: f32 accumulation, both operands of type M; B
+// transposed (N-major) for V.
+template <typename M> __device__ __forceinline__ constexpr uint32_t idesc(uint32_t n, bool b_transposed) {
+    constexpr uint32_t t = std::is_same_v<M, bf16> ? 1u : 0u;
+    return (1u << 4) | (t << 7) | (t << 10) | ((b_transposed ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// The keys a block walks: tiles [0, sink_tiles) and from win_tile on.
+struct Walk {
+    uint32_t lo_min, lo_max, hi_min, hi_max, sinks_end, sink_tiles, win_tile, tiles;
+    __device__ __forceinline__ uint32_t key0(uint32_t i) const {
+        return (i < sink_tiles ? i : i - sink_tiles + win_tile) * kTile;
+    }
+    // whether every row sees all 128 keys from `key`
+    __device__ __forceinline__ bool whole(uint32_t key) const {
+        return (key >= lo_max || key + kTile <= sinks_end) && key + kTile <= hi_min;
+    }
+};
+__device__ __forceinline__ Walk walk_of(const CacheAttnArgs& a, const SeqView& v, uint32_t row0, uint32_t last) {
+    const VisibleRange r0 = visible(a, v, a.group_div.div(row0)), r1 = visible(a, v, a.group_div.div(last));
+    Walk w;
+    w.lo_min = r0.lo, w.lo_max = r1.lo, w.hi_min = r0.hi, w.hi_max = r1.hi;
+    w.sinks_end = min(a.sinks, min(w.lo_min, w.hi_max));
+    w.sink_tiles = (w.sinks_end + kTile - 1) / kTile;
+    w.win_tile = max(w.lo_min / kTile, w.sink_tiles);
+    w.tiles = w.sink_tiles + (w.hi_max > w.win_tile * kTile ? (w.hi_max - w.win_tile * kTile + kTile - 1) / kTile : 0);
+    return w;
+}
+
+// Zeroes the infinities and NaN of eight values; true if there were any.
+template <typename T> __device__ __forceinline__ bool take_out(uint4& x) {
+    uint32_t* w = &x.x;
+    constexpr uint32_t e = std::is_same_v<T, bf16> ? 0x7f80u : 0x7c00u;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((w[i] & e) == e) w[i] &= 0xffff0000u, any = true;
+        if (((w[i] >> 16) & e) == e) w[i] &= 0x0000ffffu, any = true;
+    }
+    return any;
+}
+
+template <typename T, int D, bool kCodes>
+__global__ void __launch_bounds__(kThreads, 1)
+    cache_attn_tc_kernel(const __grid_constant__ CacheAttnArgs a, uint32_t row_blocks) {
+    using M = std::conditional_t<kCodes, __half, T>;
+    using S = Shape<D, kCodes>;
+    constexpr int kSteps = D / 16;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
+    Control* ctl = reinterpret_cast<Control*>(smem + S::kControl);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the last rows of the sequences first: causal rows there see the most keys
+    const uint32_t pairs = a.c.sequences * a.c.kv_heads, turn = blockIdx.x / pairs, hs = blockIdx.x - turn * pairs;
+    const uint32_t h = hs % a.c.kv_heads, s = hs / a.c.kv_heads;
+    const SeqView v = sequence(a.c, s, false, threadIdx.x == 0 && h == 0 && turn == 0);
+    const uint32_t rows = v.n * a.group, row0 = (row_blocks - 1 - turn) * 2 * kTile;
+    if (row0 >= rows) return;
+    const uint32_t last = min(row0 + 2 * kTile, rows) - 1;
+    const bool two = last >= row0 + kTile;  // the second tile has rows
+    const Walk w = walk_of(a, v, row0, last);
+
+    if (threadIdx.x == 0) {
+        const int softmax = two ? 256 : 128;
+        tc::mbar_init(&ctl->q_full, softmax);
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&ctl->k_full[i], kProducers);
+            tc::mbar_init(&ctl->v_full[i], kProducers);
+            tc::mbar_init(&ctl->k_empty[i], 1);
+            tc::mbar_init(&ctl->v_empty[i], 1);
+            tc::mbar_init(&ctl->s_full[i], 1);
+            tc::mbar_init(&ctl->p_full[i], 128);
+            tc::mbar_init(&ctl->o_done[i], 1);
+        }
+        for (int i = 0; i < kInfos; ++i) tc::mbar_init(&ctl->info_full[i], 8);
+        tc::mbar_init(&ctl->drain, 1);
+        ctl->dead = 0;
+        ctl->poisoned = 0;
+        ctl->v_ref = 1.0f;
+        tc::mbar_fence_init();
+    }
+    if (warp == 12) tc::tmem_alloc(&ctl->tmem, 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = ctl->tmem;
+    int* const err = a.c.err;
+
+    if (warp < 8) {
+        // ---------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kCodes ? 168 : 192));
+        const int tile = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t R = row0 + tile * kTile + r;
+        if (tile == 0 || two) {
+            const bool live = R < rows;
+            const uint32_t tok = live ? a.group_div.div(R) : 0, head = h * a.group + (live ? R - tok * a.group : 0);
+            VisibleRange rr = {0, 0, 0};
+            float mul = a.scale_log2;
+            // Q: this thread's row into the swizzled tile
+            {
+                const T* q = static_cast<const T*>(a.q) + (v.start + tok) * a.q_ts + head * a.q_hs;
+                uint8_t* dst = smem + S::kQ + tile * S::kTileBytes;
+                if (live) rr = visible(a, v, tok);
+                float down = 1.0f;
+                if constexpr (kCodes && std::is_same_v<T, bf16>) {
+                    float amax = 0.0f;
+                    if (live)
+                        for (int c = 0; c < D / 8; ++c) {
+                            float f[8];
+                            unpack(load8(q + 8 * c), f);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
+                        }
+                    int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+                    if (amax == 0.0f || e == 128) e = 0;
+                    e = min(max(e, -126), 126);
+                    down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                    mul *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                }
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (live) {
+                        const Vec8<T> y = load8(q + 8 * c);
+                        if constexpr (kCodes && std::is_same_v<T, bf16>) {
+                            float f[8];
+                            unpack(y, f);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) f[e] *= down;
+                            x = pack<__half>(f).a;
+                        } else {
+                            x = y.a;
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(dst + (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+                }
+                tc::fence_async_smem();
+                tc::mbar_arrive(&ctl->q_full);
+            }
+            const Walk mine = walk_of(a, v, row0 + tile * kTile, min(row0 + (tile + 1) * kTile - 1, last));
+            const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+            const uint32_t t_s = t_lane + tile * kTile, t_o = t_lane + kOCol + tile * D;
+            float m = -INFINITY, l = 0.0f;
+            bool fine = true;
+            for (uint32_t i = 0; i < w.tiles; ++i) {
+                if (!wait(&ctl->s_full[tile], i & 1, ctl, 10 + tile, err, s)) { fine = false; break; }
+                const TileInfo& info = ctl->info[i % kInfos];
+                if (!wait(&ctl->info_full[i % kInfos], (i / kInfos) & 1, ctl, 12 + tile, err, s)) { fine = false; break; }
+                tc::fence_after();
+                float x[kTile];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, x + 32 * c);
+                tc::tmem_ld_wait();
+                const uint32_t key = w.key0(i), ok = info.ok;
+                float g_mul[8];
+#pragma unroll
+                for (int g = 0; g < 8; ++g) g_mul[g] = kCodes ? info.k_scale[g] * mul : mul;
+                float top = -INFINITY;
+                if (mine.whole(key) && ok == 0xffu) {
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        float t0 = x[16 * g], t1 = x[16 * g + 1];
+#pragma unroll
+                        for (int e = 2; e < 16; e += 2) {
+                            t0 = fmaxf(t0, x[16 * g + e]);
+                            t1 = fmaxf(t1, x[16 * g + e + 1]);
+                        }
+                        // a negative factor (scale < 0) turns the order round: see below
+                        top = fmaxf(top, fmaxf(t0, t1) * g_mul[g]);
+                    }
+                    if (a.scale_log2 < 0.0f) {
+                        top = -INFINITY;
+#pragma unroll
+                        for (int e = 0; e < kTile; ++e) top = fmaxf(top, x[e] * g_mul[e / 16]);
+                    }
+                } else {
+                    // rows that do not see a key: minus infinity
+#pragma unroll
+                    for (int e = 0; e < kTile; ++e) {
+                        const uint32_t j = key + e;
+                        const bool seen = ((ok >> (e / 16)) & 1) && j < rr.hi && (j >= rr.lo || j < rr.first);
+                        x[e] = seen ? x[e] * g_mul[e / 16] : -INFINITY;
+                        top = fmaxf(top, x[e]);
+                    }
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) g_mul[g] = 1.0f;
+                }
+                if (__any_sync(0xffffffffu, top > m + kRaise)) {
+                    const float to = fmaxf(m, top), down = m == -INFINITY ? 0.0f : exp2_fast(m - to);
+                    m = to;
+                    l *= down;
+                    if (i > 0) {
+                        if (!wait(&ctl->o_done[tile], (i - 1) & 1, ctl, 14 + tile, err, s)) { fine = false; break; }
+                        tc::fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            float o[16];
+                            tc::tmem_ld16(t_o + c, o);
+                            tc::tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] *= down;
+                            tc::tmem_st16(t_o + c, o);
+                        }
+                    }
+                }
+                const float sub = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    const float add = kCodes ? sub + info.v_log[g] : sub;
+                    float sum0 = 0.0f, sum1 = 0.0f;
+                    uint32_t p[8];
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float p0 = exp2_fast(fmaf(x[16 * g + e], g_mul[g], add));
+                        const float p1 = exp2_fast(fmaf(x[16 * g + e + 1], g_mul[g], add));
+                        sum0 += p0;
+                        sum1 += p1;
+                        p[e / 2] = pack2(p0, p1, M{});
+                    }
+                    l += kCodes ? (sum0 + sum1) * info.v_inv[g] : sum0 + sum1;
+                    tc::tmem_st8u(t_s + 8 * g, p);
+                }
+                tc::tmem_st_wait();
+                tc::fence_before();
+                tc::mbar_arrive(&ctl->p_full[tile]);
+            }
+            if (fine && w.tiles) fine = wait(&ctl->o_done[tile], (w.tiles - 1) & 1, ctl, 16 + tile, err, s);
+            tc::fence_after();
+            const float inv = l == 0.0f ? 0.0f : (kCodes ? ctl->v_ref : 1.0f) / l;
+            const bool poisoned = *static_cast<volatile int*>(&ctl->poisoned) != 0;
+            T* out = static_cast<T*>(a.out) + (v.start + tok) * a.o_ts + head * a.o_hs;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+                float o[16];
+                if (w.tiles) {
+                    tc::tmem_ld16(t_o + c, o);
+                    tc::tmem_ld_wait();
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = l == 0.0f ? 0.0f : o[e] * inv;
+                if (poisoned && live) {
+                    // a value that is not finite, in a tile where rows differ in what they see: its weight is
+                    // positive, so it decides its channel for the rows that see it
+                    for (uint32_t i = 0; i < w.tiles; ++i) {
+                        const uint32_t key = w.key0(i);
+                        if (w.whole(key)) continue;
+                        for (uint32_t j = key; j < min(key + kTile, rr.hi); ++j) {
+                            if (!(j >= rr.lo || j < rr.first)) continue;
+                            const int page = a.c.table[static_cast<size_t>(s) * a.c.table_stride + (j >> a.c.page_shift)];
+                            if (static_cast<uint32_t>(page) >= a.c.pages) continue;
+                            const size_t at = pool_at(a.c, page, h, j & (a.c.page_tokens - 1)) + c;
+#pragma unroll
+                            for (int b = 0; b < 16; b += 8) {
+                                float f[8];
+                                if constexpr (kCodes) {
+                                    from_e4m3(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.c.v) + at + b), f);
+                                    const float vs = a.c.v_scale[static_cast<size_t>(page) * a.c.kv_heads + h];
+                                    if (!isfinite(vs)) f[0] = f[1] = f[2] = f[3] = f[4] = f[5] = f[6] = f[7] = __int_as_float(0x7fc00000);
+                                } else {
+                                    unpack(load8(static_cast<const T*>(a.c.v) + at + b), f);
+                                }
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    if (!isfinite(f[e])) o[b + e] += f[e];
+                            }
+                        }
+                    }
+                }
+                if (live && fine) {
+                    float lo[8], hi[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) lo[e] = o[e], hi[e] = o[8 + e];
+                    store8(out + c, pack<T>(lo));
+                    store8(out + c + 8, pack<T>(hi));
+                }
+            }
+        }
+    } else if (warp < 12) {
+        // -------------------------------------------------------- producers
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCodes ? 120 : 72));
+        const int t = threadIdx.x - 256;
+        constexpr int kRowChunks = kCodes ? D / 16 : D / 8;  // 16-byte chunks of a cached row
+        constexpr int kEach = kTile * kRowChunks / kProducers, kRowStep = kProducers / kRowChunks;
+        const int ch = t % kRowChunks, r0 = t / kRowChunks;
+        constexpr size_t kElem = kCodes ? 1 : 2;
+        auto page_ids = [&](uint32_t i) {  // lane g: the page of group g of tile i, -1: nothing visible or no page
+            int p = -1;
+            if (i < w.tiles && lane < 8) {
+                const uint32_t j = w.key0(i) + 16 * lane;
+                if (j < w.hi_max && (j + 16 > w.lo_min || j < w.sinks_end)) p = page_of(a.c, s, j >> a.c.page_shift);
+            }
+            return p;
+        };
+        auto row_live = [&](uint32_t j) { return j < w.hi_max && (j >= w.lo_min || j < w.sinks_end); };
+        auto source = [&](const void* pool, int page, uint32_t j) {
+            return static_cast<const uint8_t*>(pool) +
+                   (pool_at(a.c, page < 0 ? 0 : page, h, j & (a.c.page_tokens - 1)) * kElem + ch * 16);
+        };
+        if constexpr (kCodes) {
+            // the largest value scale of the visible pages
+            float top = 0.0f;
+            for (uint32_t i = t; i < w.tiles * 8; i += kProducers) {
+                const uint32_t j = w.key0(i / 8) + 16 * (i % 8);
+                if (j < w.hi_max && (j + 16 > w.lo_min || j < w.sinks_end)) {
+                    const int p = a.c.table[static_cast<size_t>(s) * a.c.table_stride + (j >> a.c.page_shift)];
+                    if (static_cast<uint32_t>(p) < a.c.pages) {
+                        const float x = a.c.v_scale[static_cast<size_t>(p) * a.c.kv_heads + h];
+                        if (isfinite(x)) top = fmaxf(top, x);
+                    }
+                }
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (lane == 0) ctl->reduce[warp - 8] = top;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            top = fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]), fmaxf(ctl->reduce[2], ctl->reduce[3]));
+            if (top == 0.0f) top = 1.0f;
+            if (t == 0) ctl->v_ref = top;
+        }
+        const float v_ref_inv = kCodes ? 1.0f / fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]),
+                                                      fmaxf(ctl->reduce[2], ctl->reduce[3]))
+                                       : 1.0f;
+        bool fine = true;
+        int pages = page_ids(0);
+        uint4 kc[kCodes ? kEach : 1], vc[kCodes ? kEach : 1];
+        auto fetch = [&](uint4(&to)[kCodes ? kEach : 1], const void* pool, uint32_t i, int ids) {
+#pragma unroll
+            for (int c = 0; c < (kCodes ? kEach : 1); ++c) {
+                const uint32_t r = r0 + c * kRowStep, j = w.key0(i) + r;
+                const int page = __shfl_sync(0xffffffffu, ids, r >> 4);
+                to[c] = make_uint4(0, 0, 0, 0);
+                if (page >= 0 && row_live(j)) to[c] = *reinterpret_cast<const uint4*>(source(pool, page, j));
+            }
+        };
+        // 16 codes to two chunks of halves; NaN codes of a mixed tile are taken out
+        auto expand = [&](uint8_t* dst, uint32_t r, uint4 x, bool mixed, bool nan) {
+            const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
+            uint32_t o[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t y = wd[e];
+                if (mixed) {
+                    const uint32_t bad = __vcmpeq4(y | 0x80808080u, 0xffffffffu) | (nan ? 0xffffffffu : 0u);
+                    if (bad) ctl->poisoned = 1;
+                    y &= ~bad;
+                } else if (nan) {
+                    y = 0x7f7f7f7fu;
+                }
+                o[2 * e] = f16x2_from_e4m3x2(y);
+                o[2 * e + 1] = f16x2_from_e4m3x2(y >> 16);
+            }
+            const int c0 = 2 * ch;
+            uint8_t* row = dst + (c0 >> 3) * kPanel + r * 128;
+            *reinterpret_cast<uint4*>(row + (((c0 & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(row + ((((c0 + 1) & 7) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+        };
+        if constexpr (kCodes) {
+            if (w.tiles) {
+                fetch(kc, a.c.k, 0, pages);
+                fetch(vc, a.c.v, 0, pages);
+            }
+        }
+        for (uint32_t i = 0; i < w.tiles && fine; ++i) {
+            const uint32_t st = i & 1, use = (i >> 1) & 1, key = w.key0(i);
+            const bool mixed = !w.whole(key);
+            const int next_pages = page_ids(i + 1);
+            uint8_t* kd = smem + S::kK + st * S::kTileBytes;
+            uint8_t* vd = smem + S::kV + st * S::kTileBytes;
+            if (i >= 2 && !wait(&ctl->k_empty[st], use ^ 1, ctl, 20, err, s)) { fine = false; break; }
+            // what the softmax needs to know; the ring is four tiles deep, the stages two
+            float v_scale = 1.0f;
+            if (lane < 8) {
+                TileInfo& info = ctl->info[i % kInfos];
+                if (warp == 8) {
+                    if constexpr (kCodes) {
+                        float ks = 1.0f;
+                        if (pages >= 0) {
+                            const size_t at = static_cast<size_t>(pages) * a.c.kv_heads + h;
+                            ks = a.c.k_scale[at];
+                            v_scale = a.c.v_scale[at];
+                        }
+                        float ratio = isfinite(v_scale) && pages >= 0 ? v_scale * v_ref_inv : 1.0f;
+                        ratio = fmaxf(ratio, 0x1p-60f);  // halves of such weights are zero
+                        info.k_scale[lane] = ks;
+                        info.v_log[lane] = log2f(ratio);
+                        info.v_inv[lane] = 1.0f / ratio;
+                    }
+                    const uint32_t ok = __ballot_sync(0xffu, pages >= 0);
+                    if (lane == 0) info.ok = ok;
+                    tc::mbar_arrive(&ctl->info_full[i % kInfos]);
+                } else if constexpr (kCodes) {
+                    if (pages >= 0) v_scale = a.c.v_scale[static_cast<size_t>(pages) * a.c.kv_heads + h];
+                }
+            }
+            if constexpr (kCodes) {
+#pragma unroll
+                for (int c = 0; c < kEach; ++c) expand(kd, r0 + c * kRowStep, kc[c], false, false);
+                tc::fence_async_smem();
+                tc::mbar_arrive(&ctl->k_full[st]);
+                if (i + 1 < w.tiles) fetch(kc, a.c.k, i + 1, next_pages);
+                if (i >= 2 && !wait(&ctl->v_empty[st], use ^ 1, ctl, 21, err, s)) { fine = false; break; }
+#pragma unroll
+                for (int c = 0; c < kEach; ++c) {
+                    const uint32_t r = r0 + c * kRowStep;
+                    const float vs = __shfl_sync(0xffffffffu, v_scale, r >> 4);
+                    expand(vd, r, vc[c], mixed, !isfinite(vs));
+                }
+                tc::fence_async_smem();
+                tc::mbar_arrive(&ctl->v_full[st]);
+                if (i + 1 < w.tiles) fetch(vc, a.c.v, i + 1, next_pages);
+            } else {
+                const uint32_t ka = tc::smem_u32(kd) + (ch >> 3) * kPanel, va = tc::smem_u32(vd) + (ch >> 3) * kPanel;
+#pragma unroll 4
+                for (int c = 0; c < kEach; ++c) {
+                    const uint32_t r = r0 + c * kRowStep, j = key + r;
+                    const int page = __shfl_sync(0xffffffffu, pages, r >> 4);
+                    cp_async16(ka + r * 128 + (((ch & 7) ^ (r & 7)) << 4), source(a.c.k, page, j), page >= 0 && row_live(j));
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (i >= 2 && !wait(&ctl->v_empty[st], use ^ 1, ctl, 21, err, s)) { fine = false; break; }
+#pragma unroll 4
+                for (int c = 0; c < kEach; ++c) {
+                    const uint32_t r = r0 + c * kRowStep, j = key + r;
+                    const int page = __shfl_sync(0xffffffffu, pages, r >> 4);
+                    cp_async16(va + r * 128 + (((ch & 7) ^ (r & 7)) << 4), source(a.c.v, page, j), page >= 0 && row_live(j));
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                tc::fence_async_smem();
+                tc::mbar_arrive(&ctl->k_full[st]);
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                if (mixed) {
+#pragma unroll 4
+                    for (int c = 0; c < kEach; ++c) {
+                        const uint32_t r = r0 + c * kRowStep;
+                        uint4* at = reinterpret_cast<uint4*>(vd + (ch >> 3) * kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                        uint4 x = *at;
+                        if (take_out<T>(x)) {
+                            *at = x;
+                            ctl->poisoned = 1;
+                        }
+                    }
+                }
+                tc::fence_async_smem();
+                tc::mbar_arrive(&ctl->v_full[st]);
+            }
+            pages = next_pages;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(56));
+        if (warp == 12) {
+            // ------------------------------------------------------ MMA issuer
+            constexpr uint32_t kS = idesc<M>(kTile, false), kO = idesc<M>(D, true);
+            // descriptors of the first step; later ones start a few 16-byte units further
+            const uint64_t qd = tc::smem_desc(tc::smem_u32(smem + S::kQ), 16, 1024, tc::kSwizzle128);
+            const uint64_t kd = tc::smem_desc(tc::smem_u32(smem + S::kK), 16, 1024, tc::kSwizzle128);
+            const uint64_t vd = tc::smem_desc(tc::smem_u32(smem + S::kV), kPanel, 1024, tc::kSwizzle128);
+            // (the loops stay rolled: unrolled, their descriptors would not fit this role's registers)
+            auto issue_s = [&](int tile, uint32_t st) {
+                uint64_t qk = qd + tile * (S::kTileBytes >> 4), kk = kd + st * (S::kTileBytes >> 4);
+#pragma unroll 1
+                for (int k = 0; k < kSteps; ++k) {
+                    tc::mma_bf16_w(tmem + tile * kTile, qk, kk, kS, k > 0);
+                    const uint32_t on = (k & 3) == 3 ? (kPanel >> 4) - 6 : 2;  // the next 16 channels
+                    qk += on;
+                    kk += on;
+                }
+                tc::commit_w(&ctl->s_full[tile]);
+            };
+            auto issue_o = [&](int tile, uint32_t st, bool more) {
+                uint64_t vk = vd + st * (S::kTileBytes >> 4);
+                uint32_t p = tmem + tile * kTile;
+#pragma unroll 1
+                for (int k = 0; k < kTile / 16; ++k) {
+                    tc::mma_bf16_ta_w(tmem + kOCol + tile * D, p, vk, kO, more || k > 0);
+                    vk += 2048 >> 4;  // the next 16 keys
+                    p += 8;
+                }
+                tc::commit_w(&ctl->o_done[tile]);
+            };
+            bool fine = w.tiles == 0 || (wait(&ctl->q_full, 0, ctl, 30, err, s) && wait(&ctl->k_full[0], 0, ctl, 31, err, s));
+            if (fine && w.tiles) {
+                tc::fence_after();
+                issue_s(0, 0);
+                if (two) issue_s(1, 0);
+                tc::commit_w(&ctl->k_empty[0]);
+            }
+            for (uint32_t i = 0; i < w.tiles && fine; ++i) {
+                const uint32_t st = i & 1, use = (i >> 1) & 1, st1 = (i + 1) & 1, use1 = ((i + 1) >> 1) & 1;
+                const bool next = i + 1 < w.tiles;
+                fine = wait(&ctl->v_full[st], use, ctl, 32, err, s) && wait(&ctl->p_full[0], i & 1, ctl, 33, err, s);
+                if (!fine) break;
+                tc::fence_after();
+                issue_o(0, st, i > 0);
+                if (next) {
+                    fine = wait(&ctl->k_full[st1], use1, ctl, 34, err, s);
+                    if (!fine) break;
+                    tc::fence_after();
+                    issue_s(0, st1);
+                }
+                if (two) {
+                    fine = wait(&ctl->p_full[1], i & 1, ctl, 35, err, s);
+                    if (!fine) break;
+                    tc::fence_after();
+                    issue_o(1, st, i > 0);
+                }
+                tc::commit_w(&ctl->v_empty[st]);
+                if (next) {
+                    if (two) issue_s(1, st1);
+                    tc::commit_w(&ctl->k_empty[st1]);
+                }
+            }
+            // every MMA has read its operands before the block ends
+            tc::commit_w(&ctl->drain);
+            tc::mbar_wait_landing(&ctl->drain, 0);
+            tc::fence_before();
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    if (warp == 12) tc::tmem_free(tmem, 512);
+}
+
+template <typename T, int D, bool kCodes> cudaError_t launch(const CacheAttnArgs& a, cudaStream_t s) {
+    using S = Shape<D, kCodes>;
+    static_assert(S::kBytes <= 227 * 1024, "shared memory");
+    const uint32_t row_blocks = (a.c.max_new * a.group + 2 * kTile - 1) / (2 * kTile);
+    auto* kernel = cache_attn_tc_kernel<T, D, kCodes>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (e != cudaSuccess) return e;
+    kernel<<<row_blocks * a.c.sequences * a.c.kv_heads, kThreads, S::kBytes, s>>>(a, row_blocks);
+    return cudaGetLastError();
+}
+
+template <typename T, bool kCodes> cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t s) {
+    return a.c.head_dim == 64 ? launch<T, 64, kCodes>(a, s) : launch<T, 128, kCodes>(a, s);
+}
+
+}  // namespace
+
+cudaError_t launch_cache_attention_tc(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s) {
+    if (storage == LWM_CACHE_E4M3)
+        return dtype == LWM_DTYPE_BF16 ? by_dim<bf16, true>(a, s) : by_dim<__half, true>(a, s);
+    return dtype == LWM_DTYPE_BF16 ? by_dim<bf16, false>(a, s) : by_dim<__half, false>(a, s);
+}
+
+}  // namespace lwm

@@ -91,7 +91,9 @@ struct CacheAttnArgs {
     uint32_t window, sinks, frame;
     FastDiv group_div, frame_div;
 };
+// Few query rows a kv head (any head width), and many (head_dim 64 or 128).
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
+cudaError_t launch_cache_attention_tc(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
 
 struct GatedNormArgs {
     lwm_gated_norm_args a;
