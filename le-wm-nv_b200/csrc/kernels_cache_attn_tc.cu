@@ -3,26 +3,38 @@
 // tcgen05 tensor cores.
 //
 // A block takes 256 query rows (tokens x heads of the group) of one sequence
-// and kv head as two tiles of 128, and walks the visible keys in tiles of
-// 128.  S = Q K^T goes to TMEM, a softmax warpgroup a tile (one row a
-// thread, so no shuffles) reads it, writes P back over it in the operands'
-// type, and O += P V accumulates in TMEM with P as the A operand there.  The
-// two tiles alternate: while one is in its softmax the tensor cores work for
-// the other, and both use each K and V tile that is loaded.
+// and kv head as two tiles of 128, and walks the visible keys 128 at a time.
+// S = Q K^T goes to TMEM, a softmax warpgroup a tile (one row a thread, so no
+// shuffles) reads it, writes P back over it in the operands' type, and O +=
+// P V accumulates in TMEM with P as the A operand there.  The two tiles
+// alternate: while one is in its softmax the tensor cores work for the other,
+// and both use each K and V tile that is loaded.  The weights go to the
+// product with V in two halves of 64 keys, which shortens the chain of
+// scores, softmax and product that bounds a tile.  Measured and left: an
+// issuing warp for each tile (their products interleave and delay each other:
+// 427 us on whole histories against 373), and 64 keys a step with two buffers
+// of S (375: an N = 64 product reads A as an N = 128 one does and takes three
+// quarters of its time).
 //
-// TMEM: S (and P) of tile 0 and 1 at columns 0 and 128, O at 256 and
-// 256 + D.  Shared memory: Q, two stages of K and of V, all rows of 64
-// channels (128 bytes, 128-byte swizzle); K is a K-major operand, V the
-// transposed (N-major) one with the same layout.
+// TMEM: S (and P) of tile t at column 128 t, O at 256 and 256 + D.  Shared
+// memory: Q, two stages of K and of V, all rows of 64 channels (128 bytes,
+// 128-byte swizzle); K is a K-major operand, V the transposed (N-major) one
+// with the same layout.
 //
-// Producers (a warpgroup) gather the pages' rows with cp.async; 8-bit codes
-// are loaded a tile ahead into registers and become halves (exact) on the
-// way to shared memory.  Their scales stay out of the products: a page's key
+// Producers (a warpgroup): a tile that every row sees comes by TMA, a box of
+// 64 channels for each page; the few tiles at the edges of the masks are
+// gathered row by row with cp.async, rows that no query sees as zeros.
+// 8-bit codes are loaded a tile ahead into registers and become halves
+// (exact) on the way to shared memory.  Their scales stay out of the products: a page's key
 // scale multiplies its 16-key groups' scores, its value scale, relative to
 // the block's largest, enters the exponent of the weight.
 //
-// O is rescaled only when a row's maximum rises by more than 2^kRaise.
+// O is rescaled only when a score passes a row's maximum by more than kRaise
+// (a factor of 2^8).
 // Every wait is bounded: one that gives up marks the block, which unwinds.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "lwm_blocks.cuh"
 #include "lwm_cache_attn.cuh"
 #include "lwm_tc.cuh"
@@ -32,7 +44,8 @@ namespace lwm {
 namespace {
 
 constexpr int kTile = 128;           // rows of a tile, keys of a step
-constexpr int kThreads = 512;        // two softmax warpgroups, producers, MMA issuer
+constexpr int kHalf = 64;            // keys whose weights go to the product at once
+constexpr int kThreads = 512;        // two softmax warpgroups, producers, MMA issuers
 constexpr int kProducers = 128;
 constexpr int kPanel = kTile * 128;  // bytes of 128 rows x 64 channels
 constexpr int kInfos = 4;
@@ -48,7 +61,7 @@ struct TileInfo {
 };
 
 struct Control {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], info_full[kInfos], drain;
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_half[2], o_done[2], info_full[kInfos], drain;
     uint32_t tmem;
     int dead;        // a wait gave up
     int poisoned;    // infinities or NaN were taken out of a V tile
@@ -66,7 +79,7 @@ template <int D, bool kCodes> struct Shape {
 
 // Called by whole warps; the answer is the warp's, so that its lanes stay together.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Control* c, int site, int* err, uint32_t seq) {
-    bool done = false;
+    bool done = tc::mbar_try(bar, parity);
     for (uint32_t i = 0; i < tc::kWaitLimit && !done; ++i) {
         done = tc::mbar_try(bar, parity);
         if ((i & 255u) == 255u && *static_cast<volatile int*>(&c->dead)) break;
@@ -90,6 +103,78 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+// A product's K = 16 steps as one run of instructions by a whole warp (one
+// elected lane): D (+)= A B^T.  The descriptors' low words advance by
+// constants, so that between two instructions there is next to nothing; a
+// call a step cost the issuing warp about 55 cycles each, as long as the
+// tensor core takes for it.
+#define LWM_SS(on)                                                                                      \
+    "add.u32 al, %1, " on ";\n\tadd.u32 bl, %2, " on ";\n\tmov.b64 x, {al, %3};\n\tmov.b64 y, {bl, %3};\n\t" \
+    "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, "
+// S: 4 or 8 steps; 16 channels are 2 units of 16 bytes, a panel 1024.
+template <int kSteps>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t high, uint32_t idesc) {
+    if constexpr (kSteps == 8)
+        asm volatile(
+            "{\n\t.reg .pred e;\n\t.reg .b32 al, bl;\n\t.reg .b64 x, y;\n\telect.sync _|e, 0xffffffff;\n\t"
+            LWM_SS("0") "0;\n\t" LWM_SS("2") "1;\n\t" LWM_SS("4") "1;\n\t" LWM_SS("6") "1;\n\t"
+            LWM_SS("1024") "1;\n\t" LWM_SS("1026") "1;\n\t" LWM_SS("1028") "1;\n\t" LWM_SS("1030") "1;\n\t}\n" ::"r"(d),
+            "r"(a_low), "r"(b_low), "r"(high), "r"(idesc)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred e;\n\t.reg .b32 al, bl;\n\t.reg .b64 x, y;\n\telect.sync _|e, 0xffffffff;\n\t"
+            LWM_SS("0") "0;\n\t" LWM_SS("2") "1;\n\t" LWM_SS("4") "1;\n\t" LWM_SS("6") "1;\n\t}\n" ::"r"(d),
+            "r"(a_low), "r"(b_low), "r"(high), "r"(idesc)
+            : "memory");
+}
+#undef LWM_SS
+// O: the four steps of 64 keys; 16 keys are 8 columns of P and 128 units of V.
+__device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a, uint32_t b_low, uint32_t high, uint32_t idesc, bool more) {
+#define LWM_TS(p, on) \
+    "add.u32 al, %1, " p ";\n\tadd.u32 bl, %2, " on ";\n\tmov.b64 y, {bl, %3};\n\t" \
+    "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [al], y, %4, "
+    asm volatile(
+        "{\n\t.reg .pred e, m;\n\t.reg .b32 al, bl;\n\t.reg .b64 y;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 m, %5, 0;\n\t"
+        LWM_TS("0", "0") "m;\n\t" LWM_TS("8", "128") "1;\n\t" LWM_TS("16", "256") "1;\n\t" LWM_TS("24", "384") "1;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b_low), "r"(high), "r"(idesc), "r"(static_cast<uint32_t>(more))
+        : "memory");
+#undef LWM_TS
+}
+// Packed pairs and the three-operand maximum.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(r)
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+          "l"(reinterpret_cast<const uint64_t&>(c)));
+    return reinterpret_cast<const float2&>(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return reinterpret_cast<const float2&>(r);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// Bits e of the keys k32 + e below `end`.
+__device__ __forceinline__ uint32_t below(uint32_t end, uint32_t k32) {
+    return end <= k32 ? 0u : end - k32 >= 32 ? 0xffffffffu : (1u << (end - k32)) - 1u;
+}
+
+// 64 channels of the rows of a box to shared memory (no multicast).
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int channel, int row, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            dst),
+        "l"(map), "r"(tc::smem_u32(bar)), "r"(channel), "r"(row), "r"(page)
+        : "memory");
 }
 
 // kind::f16 descriptor: f32 accumulation, both operands of type M; B
@@ -134,9 +219,48 @@ template <typename T> __device__ __forceinline__ bool take_out(uint4& x) {
     return any;
 }
 
+// The weights exp2(score - maximum) of a row's 64 keys, packed for the
+// product, their sum (the value scales taken out again) and the largest
+// exponent.  kMasked: only the keys that the row sees.
+template <typename M, bool kCodes, bool kMasked>
+__device__ __forceinline__ float weights(const float (&x)[64], uint32_t (&p)[32], float2& sum, const TileInfo& info,
+                                         int half, float mul, float sub, const VisibleRange& rr, uint32_t key, uint32_t ok) {
+    float top0 = -INFINITY, top1 = -INFINITY;
+    sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int group = 4 * half + g;
+        const float gm = kCodes ? info.k_scale[group] * mul : mul;
+        const float add = kCodes ? sub + info.v_log[group] : sub;
+        uint32_t seen = 0;
+        if constexpr (kMasked) {
+            const uint32_t k16 = key + 16 * group;
+            seen = (ok >> group) & 1 ? below(rr.hi, k16) & (~below(rr.lo, k16) | below(rr.first, k16)) : 0u;
+        }
+        float2 part = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            float2 y = fma2(make_float2(x[16 * g + e], x[16 * g + e + 1]), make_float2(gm, gm), make_float2(add, add));
+            if constexpr (kMasked) {
+                if (!((seen >> e) & 1)) y.x = -INFINITY;
+                if (!((seen >> (e + 1)) & 1)) y.y = -INFINITY;
+            }
+            if (e & 2) top1 = max3(top1, y.x, y.y);
+            else top0 = max3(top0, y.x, y.y);
+            y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+            part = add2(part, y);
+            p[8 * g + e / 2] = pack2(y.x, y.y, M{});
+        }
+        if constexpr (kCodes) sum = fma2(part, make_float2(info.v_inv[group], info.v_inv[group]), sum);
+        else sum = add2(sum, part);
+    }
+    return fmaxf(top0, top1);
+}
+
 template <typename T, int D, bool kCodes>
 __global__ void __launch_bounds__(kThreads, 1)
-    cache_attn_tc_kernel(const __grid_constant__ CacheAttnArgs a, uint32_t row_blocks) {
+    cache_attn_tc_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ CUtensorMap k_map,
+                         const __grid_constant__ CUtensorMap v_map, uint32_t row_blocks) {
     using M = std::conditional_t<kCodes, __half, T>;
     using S = Shape<D, kCodes>;
     constexpr int kSteps = D / 16;
@@ -163,7 +287,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::mbar_init(&ctl->k_empty[i], 1);
             tc::mbar_init(&ctl->v_empty[i], 1);
             tc::mbar_init(&ctl->s_full[i], 1);
-            tc::mbar_init(&ctl->p_full[i], 128);
+            for (int b = 0; b < 2; ++b) tc::mbar_init(&ctl->p_full[i][b], 4);
+            tc::mbar_init(&ctl->o_half[i], 1);
             tc::mbar_init(&ctl->o_done[i], 1);
         }
         for (int i = 0; i < kInfos; ++i) tc::mbar_init(&ctl->info_full[i], 8);
@@ -187,46 +312,53 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t R = row0 + tile * kTile + r;
         if (tile == 0 || two) {
             const bool live = R < rows;
-            const uint32_t tok = live ? a.group_div.div(R) : 0, head = h * a.group + (live ? R - tok * a.group : 0);
+            const uint32_t tok = live ? a.group_div.div(R) : 0;
             VisibleRange rr = {0, 0, 0};
             float mul = a.scale_log2;
-            // Q: this thread's row into the swizzled tile
+            if (live) rr = visible(a, v, tok);
+            // Q: the warp's 32 rows into the swizzled tile, whole rows at a time
             {
-                const T* q = static_cast<const T*>(a.q) + (v.start + tok) * a.q_ts + head * a.q_hs;
-                uint8_t* dst = smem + S::kQ + tile * S::kTileBytes;
-                if (live) rr = visible(a, v, tok);
-                float down = 1.0f;
-                if constexpr (kCodes && std::is_same_v<T, bf16>) {
-                    float amax = 0.0f;
-                    if (live)
-                        for (int c = 0; c < D / 8; ++c) {
-                            float f[8];
-                            unpack(load8(q + 8 * c), f);
+                constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;  // lanes a row, rows a load
+                const int c = lane % kLanes;
+                uint8_t* dst = smem + S::kQ + tile * S::kTileBytes + (c >> 3) * kPanel;
+                Vec8<T> x[kLanes];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
-                        }
-                    int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-                    if (amax == 0.0f || e == 128) e = 0;
-                    e = min(max(e, -126), 126);
-                    down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                    mul *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                for (int k = 0; k < kLanes; ++k) {
+                    const uint32_t Rk = row0 + tile * kTile + (warp & 3) * 32 + k * kAtOnce + lane / kLanes;
+                    const uint32_t tk = Rk < rows ? a.group_div.div(Rk) : 0;
+                    x[k].a = make_uint4(0, 0, 0, 0);
+                    if (Rk < rows)
+                        x[k] = load8(static_cast<const T*>(a.q) + (v.start + tk) * a.q_ts +
+                                     (h * a.group + (Rk - tk * a.group)) * a.q_hs + 8 * c);
                 }
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (live) {
-                        const Vec8<T> y = load8(q + 8 * c);
-                        if constexpr (kCodes && std::is_same_v<T, bf16>) {
-                            float f[8];
-                            unpack(y, f);
+                for (int k = 0; k < kLanes; ++k) {
+                    const int rk = (warp & 3) * 32 + k * kAtOnce + lane / kLanes;
+                    uint4 y = x[k].a;
+                    if constexpr (kCodes && std::is_same_v<T, bf16>) {
+                        // to fp16 by a power of two a row, which the scores' factor takes back
+                        float f[8], amax = 0.0f;
+                        unpack(x[k], f);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) f[e] *= down;
-                            x = pack<__half>(f).a;
-                        } else {
-                            x = y.a;
+                        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
+#pragma unroll
+                        for (int o = kLanes / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                        int e2 = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+                        if (amax == 0.0f || e2 == 128) e2 = 0;
+                        e2 = min(max(e2, -126), 126);
+                        const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] *= down;
+                        y = pack<__half>(f).a;
+                        // the factor of row k * kAtOnce + j to the lane that owns the row
+                        const float up = __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+#pragma unroll
+                        for (int j = 0; j < kAtOnce; ++j) {
+                            const float u = __shfl_sync(0xffffffffu, up, j * kLanes);
+                            if (lane == k * kAtOnce + j) mul *= u;
                         }
                     }
-                    *reinterpret_cast<uint4*>(dst + (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+                    *reinterpret_cast<uint4*>(dst + rk * 128 + (((c & 7) ^ (rk & 7)) << 4)) = y;
                 }
                 tc::fence_async_smem();
                 tc::mbar_arrive(&ctl->q_full);
@@ -236,93 +368,72 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t t_s = t_lane + tile * kTile, t_o = t_lane + kOCol + tile * D;
             float m = -INFINITY, l = 0.0f;
             bool fine = true;
-            for (uint32_t i = 0; i < w.tiles; ++i) {
-                if (!wait(&ctl->s_full[tile], i & 1, ctl, 10 + tile, err, s)) { fine = false; break; }
+            for (uint32_t i = 0; i < w.tiles && fine; ++i) {
+                // (the producers' notes are there long before the scores)
                 const TileInfo& info = ctl->info[i % kInfos];
-                if (!wait(&ctl->info_full[i % kInfos], (i / kInfos) & 1, ctl, 12 + tile, err, s)) { fine = false; break; }
-                tc::fence_after();
-                float x[kTile];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, x + 32 * c);
-                tc::tmem_ld_wait();
+                fine = wait(&ctl->info_full[i % kInfos], (i / kInfos) & 1, ctl, 12 + tile, err, s);
+                if (!fine) break;
                 const uint32_t key = w.key0(i), ok = info.ok;
-                float g_mul[8];
-#pragma unroll
-                for (int g = 0; g < 8; ++g) g_mul[g] = kCodes ? info.k_scale[g] * mul : mul;
-                float top = -INFINITY;
-                if (mine.whole(key) && ok == 0xffu) {
-#pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        float t0 = x[16 * g], t1 = x[16 * g + 1];
-#pragma unroll
-                        for (int e = 2; e < 16; e += 2) {
-                            t0 = fmaxf(t0, x[16 * g + e]);
-                            t1 = fmaxf(t1, x[16 * g + e + 1]);
-                        }
-                        // a negative factor (scale < 0) turns the order round: see below
-                        top = fmaxf(top, fmaxf(t0, t1) * g_mul[g]);
-                    }
-                    if (a.scale_log2 < 0.0f) {
-                        top = -INFINITY;
-#pragma unroll
-                        for (int e = 0; e < kTile; ++e) top = fmaxf(top, x[e] * g_mul[e / 16]);
-                    }
-                } else {
-                    // rows that do not see a key: minus infinity
-#pragma unroll
-                    for (int e = 0; e < kTile; ++e) {
-                        const uint32_t j = key + e;
-                        const bool seen = ((ok >> (e / 16)) & 1) && j < rr.hi && (j >= rr.lo || j < rr.first);
-                        x[e] = seen ? x[e] * g_mul[e / 16] : -INFINITY;
-                        top = fmaxf(top, x[e]);
-                    }
-#pragma unroll
-                    for (int g = 0; g < 8; ++g) g_mul[g] = 1.0f;
-                }
-                if (__any_sync(0xffffffffu, top > m + kRaise)) {
-                    const float to = fmaxf(m, top), down = m == -INFINITY ? 0.0f : exp2_fast(m - to);
-                    m = to;
-                    l *= down;
-                    if (i > 0) {
-                        if (!wait(&ctl->o_done[tile], (i - 1) & 1, ctl, 14 + tile, err, s)) { fine = false; break; }
-                        tc::fence_after();
+                const bool whole = mine.whole(key) && ok == 0xffu;
+                fine = wait(&ctl->s_full[tile], i & 1, ctl, 10 + tile, err, s);
+                tc::fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 16) {
-                            float o[16];
-                            tc::tmem_ld16(t_o + c, o);
-                            tc::tmem_ld_wait();
+                for (int half = 0; half < 2 && fine; ++half) {
+                    // The weights are taken against the row's old maximum while the new one is found; only when a
+                    // score passes it by kRaise (or it is the first) are they taken again.
+                    float x[kHalf];
+                    tmem_ld32(t_s + kHalf * half, x);
+                    tmem_ld32(t_s + kHalf * half + 32, x + 32);
+                    tc::tmem_ld_wait();
+                    uint32_t p[32];
+                    float2 sum;
+                    bool again = false;
+                    while (true) {
+                        const bool first = m == -INFINITY;
+                        const float sub = first ? 0.0f : -m;
+                        const float top = whole ? weights<M, kCodes, false>(x, p, sum, info, half, mul, sub, rr, key, ok)
+                                                : weights<M, kCodes, true>(x, p, sum, info, half, mul, sub, rr, key, ok);
+                        if (again || !__any_sync(0xffffffffu, top > (first ? -INFINITY : kRaise))) break;
+                        again = true;
+                        const float up = first ? top : fmaxf(top, 0.0f), down = first ? 0.0f : exp2_fast(-up);
+                        m = first ? top : m + up;
+                        l *= down;
+                        if (i > 0 || half) {  // O holds every product up to here once the last one is done
+                            fine = half ? wait(&ctl->o_half[tile], i & 1, ctl, 14 + tile, err, s)
+                                        : wait(&ctl->o_done[tile], (i - 1) & 1, ctl, 14 + tile, err, s);
+                            if (!fine) break;
+                            tc::fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                float o[16];
+                                tc::tmem_ld16(t_o + c, o);
+                                tc::tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] *= down;
-                            tc::tmem_st16(t_o + c, o);
+                                for (int e = 0; e < 16; ++e) o[e] *= down;
+                                tc::tmem_st16(t_o + c, o);
+                            }
                         }
+                        tmem_ld32(t_s + kHalf * half, x);  // still there: P covers what has been read
+                        tmem_ld32(t_s + kHalf * half + 32, x + 32);
+                        tc::tmem_ld_wait();
                     }
-                }
-                const float sub = m == -INFINITY ? 0.0f : -m;
+                    if (!fine) break;
+                    l += sum.x + sum.y;
 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    const float add = kCodes ? sub + info.v_log[g] : sub;
-                    float sum0 = 0.0f, sum1 = 0.0f;
-                    uint32_t p[8];
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float p0 = exp2_fast(fmaf(x[16 * g + e], g_mul[g], add));
-                        const float p1 = exp2_fast(fmaf(x[16 * g + e + 1], g_mul[g], add));
-                        sum0 += p0;
-                        sum1 += p1;
-                        p[e / 2] = pack2(p0, p1, M{});
-                    }
-                    l += kCodes ? (sum0 + sum1) * info.v_inv[g] : sum0 + sum1;
-                    tc::tmem_st8u(t_s + 8 * g, p);
+                    for (int c = 0; c < 32; c += 8)
+                        tc::tmem_st8u(t_s + 32 * half + c, reinterpret_cast<const uint32_t(&)[8]>(p[c]));
+                    tc::tmem_st_wait();
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&ctl->p_full[tile][half]);
                 }
-                tc::tmem_st_wait();
-                tc::fence_before();
-                tc::mbar_arrive(&ctl->p_full[tile]);
             }
             if (fine && w.tiles) fine = wait(&ctl->o_done[tile], (w.tiles - 1) & 1, ctl, 16 + tile, err, s);
             tc::fence_after();
             const float inv = l == 0.0f ? 0.0f : (kCodes ? ctl->v_ref : 1.0f) / l;
             const bool poisoned = *static_cast<volatile int*>(&ctl->poisoned) != 0;
-            T* out = static_cast<T*>(a.out) + (v.start + tok) * a.o_ts + head * a.o_hs;
+            // rows go through the tile's Q, which no product reads any more, and out in whole 16-byte runs
+            uint8_t* stage = smem + S::kQ + tile * S::kTileBytes;
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
                 float o[16];
@@ -360,12 +471,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                if (live && fine) {
-                    float lo[8], hi[8];
+                float f[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) lo[e] = o[e], hi[e] = o[8 + e];
-                    store8(out + c, pack<T>(lo));
-                    store8(out + c + 8, pack<T>(hi));
+                for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] = o[8 * b + e];
+                    const int ch = c / 8 + b;
+                    *reinterpret_cast<uint4*>(stage + (ch >> 3) * kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = pack<T>(f).a;
+                }
+            }
+            __syncwarp();
+            if (fine) {
+                constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+                const int c = lane % kLanes;
+#pragma unroll
+                for (int k = 0; k < kLanes; ++k) {
+                    const int rk = (warp & 3) * 32 + k * kAtOnce + lane / kLanes;
+                    const uint32_t Rk = row0 + tile * kTile + rk;
+                    if (Rk >= rows) continue;
+                    const uint32_t tk = a.group_div.div(Rk);
+                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (v.start + tk) * a.o_ts +
+                                              (h * a.group + (Rk - tk * a.group)) * a.o_hs + 8 * c) =
+                        *reinterpret_cast<const uint4*>(stage + (c >> 3) * kPanel + rk * 128 + (((c & 7) ^ (rk & 7)) << 4));
                 }
             }
         }
@@ -502,6 +629,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::fence_async_smem();
                 tc::mbar_arrive(&ctl->v_full[st]);
                 if (i + 1 < w.tiles) fetch(vc, a.c.v, i + 1, next_pages);
+            } else if (!mixed && __all_sync(0xffffffffu, lane >= 8 || pages >= 0)) {
+                // (the lookups of all warps agree, so all of them come here)
+                const uint32_t box = min(a.c.page_tokens, static_cast<uint32_t>(kTile));  // rows a box
+                const uint32_t g = lane * box / 16;  // this lane's box starts at this group
+                const int page = __shfl_sync(0xffffffffu, pages, g & 7);
+                if (warp == 8 && lane == 0) tc::mbar_expect_tx(&ctl->k_full[st], S::kTileBytes);
+                __syncwarp();
+                const int row = h * a.c.page_tokens + (key & (a.c.page_tokens - 1));
+                if (warp == 8 && g < 8)
+#pragma unroll
+                    for (int p = 0; p < S::kPanels; ++p)
+                        tma_rows(tc::smem_u32(kd) + p * kPanel + lane * box * 128, &k_map, 64 * p, row, page, &ctl->k_full[st]);
+                if (t != 0) tc::mbar_arrive(&ctl->k_full[st]);
+                if (i >= 2 && !wait(&ctl->v_empty[st], use ^ 1, ctl, 21, err, s)) { fine = false; break; }
+                if (warp == 8 && lane == 0) tc::mbar_expect_tx(&ctl->v_full[st], S::kTileBytes);
+                __syncwarp();
+                if (warp == 8 && g < 8)
+#pragma unroll
+                    for (int p = 0; p < S::kPanels; ++p)
+                        tma_rows(tc::smem_u32(vd) + p * kPanel + lane * box * 128, &v_map, 64 * p, row, page, &ctl->v_full[st]);
+                if (t != 0) tc::mbar_arrive(&ctl->v_full[st]);
             } else {
                 const uint32_t ka = tc::smem_u32(kd) + (ch >> 3) * kPanel, va = tc::smem_u32(vd) + (ch >> 3) * kPanel;
 #pragma unroll 4
@@ -541,68 +689,61 @@ __global__ void __launch_bounds__(kThreads, 1)
             pages = next_pages;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+        // a block that gave up: its TMA boxes in flight land long before this
+        if (!fine)
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(56));
         if (warp == 12) {
             // ------------------------------------------------------ MMA issuer
             constexpr uint32_t kS = idesc<M>(kTile, false), kO = idesc<M>(D, true);
-            // descriptors of the first step; later ones start a few 16-byte units further
-            const uint64_t qd = tc::smem_desc(tc::smem_u32(smem + S::kQ), 16, 1024, tc::kSwizzle128);
-            const uint64_t kd = tc::smem_desc(tc::smem_u32(smem + S::kK), 16, 1024, tc::kSwizzle128);
-            const uint64_t vd = tc::smem_desc(tc::smem_u32(smem + S::kV), kPanel, 1024, tc::kSwizzle128);
-            // (the loops stay rolled: unrolled, their descriptors would not fit this role's registers)
-            auto issue_s = [&](int tile, uint32_t st) {
-                uint64_t qk = qd + tile * (S::kTileBytes >> 4), kk = kd + st * (S::kTileBytes >> 4);
-#pragma unroll 1
-                for (int k = 0; k < kSteps; ++k) {
-                    tc::mma_bf16_w(tmem + tile * kTile, qk, kk, kS, k > 0);
-                    const uint32_t on = (k & 3) == 3 ? (kPanel >> 4) - 6 : 2;  // the next 16 channels
-                    qk += on;
-                    kk += on;
-                }
+            // the descriptors' high words are constants; their low words hold the address in 16-byte units, which
+            // the steps' offsets only add to
+            constexpr uint32_t kHigh = (1024u >> 4) | (1u << 14) | (tc::kSwizzle128 << 29);
+            const uint32_t q_low = (tc::smem_u32(smem + S::kQ) >> 4) | ((16u >> 4) << 16);
+            const uint32_t k_low = (tc::smem_u32(smem + S::kK) >> 4) | ((16u >> 4) << 16);
+            const uint32_t v_low = (tc::smem_u32(smem + S::kV) >> 4) | ((static_cast<uint32_t>(kPanel) >> 4) << 16);
+            auto scores = [&](int tile, uint32_t i) {
+                mma_scores<kSteps>(tmem + tile * kTile, q_low + tile * (S::kTileBytes >> 4),
+                                   k_low + (i & 1) * (S::kTileBytes >> 4), kHigh, kS);
                 tc::commit_w(&ctl->s_full[tile]);
             };
-            auto issue_o = [&](int tile, uint32_t st, bool more) {
-                uint64_t vk = vd + st * (S::kTileBytes >> 4);
-                uint32_t p = tmem + tile * kTile;
-#pragma unroll 1
-                for (int k = 0; k < kTile / 16; ++k) {
-                    tc::mma_bf16_ta_w(tmem + kOCol + tile * D, p, vk, kO, more || k > 0);
-                    vk += 2048 >> 4;  // the next 16 keys
-                    p += 8;
+            // the product of a tile's weights with V, half by half as they come
+            auto weighted = [&](int tile, uint32_t i) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (!wait(&ctl->p_full[tile][half], i & 1, ctl, 33 + tile, err, s)) return false;
+                    tc::fence_after();
+                    mma_weighted(tmem + kOCol + tile * D, tmem + tile * kTile + 32 * half,
+                                 v_low + (i & 1) * (S::kTileBytes >> 4) + half * (kHalf * 128 >> 4), kHigh, kO, i > 0 || half);
+                    tc::commit_w(half ? &ctl->o_done[tile] : &ctl->o_half[tile]);
                 }
-                tc::commit_w(&ctl->o_done[tile]);
+                return true;
             };
             bool fine = w.tiles == 0 || (wait(&ctl->q_full, 0, ctl, 30, err, s) && wait(&ctl->k_full[0], 0, ctl, 31, err, s));
             if (fine && w.tiles) {
                 tc::fence_after();
-                issue_s(0, 0);
-                if (two) issue_s(1, 0);
+                scores(0, 0);
+                if (two) scores(1, 0);
                 tc::commit_w(&ctl->k_empty[0]);
             }
             for (uint32_t i = 0; i < w.tiles && fine; ++i) {
-                const uint32_t st = i & 1, use = (i >> 1) & 1, st1 = (i + 1) & 1, use1 = ((i + 1) >> 1) & 1;
-                const bool next = i + 1 < w.tiles;
-                fine = wait(&ctl->v_full[st], use, ctl, 32, err, s) && wait(&ctl->p_full[0], i & 1, ctl, 33, err, s);
+                // K and V are there early as a rule: nothing but the weights is waited for between two products.
+                // The next scores overwrite this step's weights; a thread's products run in the order of issue.
+                const uint32_t st = i & 1, next = i + 1;
+                fine = wait(&ctl->v_full[st], (i >> 1) & 1, ctl, 32, err, s);
+                if (fine && next < w.tiles) fine = wait(&ctl->k_full[next & 1], (next >> 1) & 1, ctl, 31, err, s);
+                fine = fine && weighted(0, i);
                 if (!fine) break;
-                tc::fence_after();
-                issue_o(0, st, i > 0);
-                if (next) {
-                    fine = wait(&ctl->k_full[st1], use1, ctl, 34, err, s);
-                    if (!fine) break;
-                    tc::fence_after();
-                    issue_s(0, st1);
-                }
+                if (next < w.tiles) scores(0, next);
                 if (two) {
-                    fine = wait(&ctl->p_full[1], i & 1, ctl, 35, err, s);
+                    fine = weighted(1, i);
                     if (!fine) break;
-                    tc::fence_after();
-                    issue_o(1, st, i > 0);
                 }
                 tc::commit_w(&ctl->v_empty[st]);
-                if (next) {
-                    if (two) issue_s(1, st1);
-                    tc::commit_w(&ctl->k_empty[st1]);
+                if (next < w.tiles) {
+                    if (two) scores(1, next);
+                    tc::commit_w(&ctl->k_empty[next & 1]);
                 }
             }
             // every MMA has read its operands before the block ends
@@ -617,14 +758,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 12) tc::tmem_free(tmem, 512);
 }
 
+// The pool as [pages][kv_heads x page_tokens][head_dim], boxes of one page's
+// rows and 64 channels, 128-byte swizzle.
+cudaError_t page_map(const CacheArgs& c, void* pool, bool is_bf16, CUtensorMap* map) {
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found{};
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    if (!encode) return cudaErrorNotSupported;
+    const uint64_t row = c.head_dim * 2ull, rows = static_cast<uint64_t>(c.kv_heads) * c.page_tokens;
+    const cuuint64_t dims[3] = {c.head_dim, rows, c.pages};
+    const cuuint64_t strides[2] = {row, row * rows};
+    const cuuint32_t box[3] = {64, c.page_tokens, 1}, ones[3] = {1, 1, 1};
+    const CUresult r = encode(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, pool,
+                              dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 template <typename T, int D, bool kCodes> cudaError_t launch(const CacheAttnArgs& a, cudaStream_t s) {
     using S = Shape<D, kCodes>;
     static_assert(S::kBytes <= 227 * 1024, "shared memory");
     const uint32_t row_blocks = (a.c.max_new * a.group + 2 * kTile - 1) / (2 * kTile);
     auto* kernel = cache_attn_tc_kernel<T, D, kCodes>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    CUtensorMap k_map{}, v_map{};
+    if constexpr (!kCodes) {
+        if (e == cudaSuccess) e = page_map(a.c, a.c.k, std::is_same_v<T, bf16>, &k_map);
+        if (e == cudaSuccess) e = page_map(a.c, a.c.v, std::is_same_v<T, bf16>, &v_map);
+    }
     if (e != cudaSuccess) return e;
-    kernel<<<row_blocks * a.c.sequences * a.c.kv_heads, kThreads, S::kBytes, s>>>(a, row_blocks);
+    kernel<<<row_blocks * a.c.sequences * a.c.kv_heads, kThreads, S::kBytes, s>>>(a, k_map, v_map, row_blocks);
     return cudaGetLastError();
 }
 
