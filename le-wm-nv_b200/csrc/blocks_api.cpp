@@ -104,9 +104,9 @@ lwm_status check_cache(const lwm_paged_cache* c, const lwm_cache_batch* b, lwm::
     return LWM_OK;
 }
 
-// Blocks of a launch with one block per (sequence, page of new tokens).
-lwm_status check_page_blocks(const lwm::CacheArgs& a) {
-    const uint64_t per = (static_cast<uint64_t>(a.max_new) + a.page_tokens - 2) / a.page_tokens + 1;
+// Blocks of a launch with one block per (sequence, run of 16 new tokens).
+lwm_status check_run_blocks(const lwm::CacheArgs& a) {
+    const uint64_t per = (static_cast<uint64_t>(a.max_new) + 14) / 16 + 1;
     if (per * a.sequences > 0x7fffffffull) return fail(LWM_UNSUPPORTED, "batch is too large for one call");
     return LWM_OK;
 }
@@ -183,7 +183,7 @@ lwm_status lwm_cache_append_device(lwm_ctx* ctx, const lwm_paged_cache* cache, c
     if (!x) return bad("null argument");
     lwm::AppendArgs a{};
     LWM_TRY(check_cache(cache, batch, &a.c));
-    LWM_TRY(check_page_blocks(a.c));
+    LWM_TRY(check_run_blocks(a.c));
     if (rotary) {
         LWM_TRY(check_rotary(rotary, cache->head_dim, &a.pairs));
         a.r = *rotary;
@@ -228,7 +228,7 @@ lwm_status lwm_cache_gather_device(lwm_ctx* ctx, const lwm_paged_cache* cache, c
     if (!x) return bad("null argument");
     lwm::GatherArgs a{};
     LWM_TRY(check_cache(cache, batch, &a.c));
-    LWM_TRY(check_page_blocks(a.c));
+    LWM_TRY(check_run_blocks(a.c));
     const bool work = a.c.sequences && a.c.max_new;
     if (work) {
         LWM_TRY(check_heads("k_out", x->k_out, x->k_token_stride, x->k_head_stride));

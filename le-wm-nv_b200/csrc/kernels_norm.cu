@@ -12,21 +12,10 @@ namespace lwm {
 
 namespace {
 
-// Eight values at `p` (any of the three types, uniform over the launch).
-__device__ __forceinline__ void load_any(const void* p, size_t at, int dtype, float (&f)[8]) {
-    if (dtype == LWM_DTYPE_F32) unpack(load8(static_cast<const float*>(p) + at), f);
-    else if (dtype == LWM_DTYPE_BF16) unpack(load8(static_cast<const bf16*>(p) + at), f);
-    else unpack(load8(static_cast<const __half*>(p) + at), f);
-}
 __device__ __forceinline__ float load_one(const void* p, size_t at, int dtype) {
     if (dtype == LWM_DTYPE_F32) return static_cast<const float*>(p)[at];
     if (dtype == LWM_DTYPE_BF16) return __bfloat162float(static_cast<const bf16*>(p)[at]);
     return __half2float(static_cast<const __half*>(p)[at]);
-}
-__device__ __forceinline__ void store_any(void* p, size_t at, int dtype, const float (&f)[8]) {
-    if (dtype == LWM_DTYPE_F32) store8(static_cast<float*>(p) + at, pack<float>(f));
-    else if (dtype == LWM_DTYPE_BF16) store8(static_cast<bf16*>(p) + at, pack<bf16>(f));
-    else store8(static_cast<__half*>(p) + at, pack<__half>(f));
 }
 __device__ __forceinline__ void store_one(void* p, size_t at, int dtype, float f) {
     if (dtype == LWM_DTYPE_F32) static_cast<float*>(p)[at] = f;
@@ -95,8 +84,10 @@ __device__ __forceinline__ void norm_row(float (&v)[NV][8], int kind, const floa
     }
 }
 
-// Rows whose width is a multiple of 8 and whose buffers are 16-byte aligned.
-template <int kRow, int NV>
+// Rows whose width is a multiple of 8 and whose buffers are 16-byte aligned;
+// R, T, C: types of the residual stream, of y and h, and of the conditioning.
+// Everything a row needs is asked for before any of it is used.
+template <typename R, typename T, typename C, int kRow, int NV>
 __global__ void __launch_bounds__(256) gated_norm_kernel(GatedNormArgs g) {
     __shared__ float red[8];
     const lwm_gated_norm_args& a = g.a;
@@ -104,18 +95,37 @@ __global__ void __launch_bounds__(256) gated_norm_kernel(GatedNormArgs g) {
     const uint32_t r = blockIdx.x * (blockDim.x / kRow) + threadIdx.x / kRow;
     if (r >= a.rows) return;  // whole warps, or (kRow 256) never
     const size_t cond = static_cast<size_t>(g.cond_div.div(r)) * a.cond_stride;
-    float x[NV][8], y[NV][8];
+    const R* xr = static_cast<const R*>(a.x) + r * a.x_stride;
+    const T* yr = static_cast<const T*>(a.y) + r * a.y_stride;
+    const C* gate = static_cast<const C*>(a.gate) + cond;
+    Vec8<R> xv[NV];
+    Vec8<T> yv[NV];
+    Vec8<C> gv[NV];
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
         const uint32_t c = (lane + q * kRow) * 8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[q][e] = y[q][e] = 0.0f;
-        if (c < a.width) {
-            load_any(a.x, r * a.x_stride + c, a.residual_dtype, x[q]);
-            if (a.y) load_any(a.y, r * a.y_stride + c, a.dtype, y[q]);
+        if (c >= a.width) continue;
+        xv[q] = load8(xr + c);
+        if (a.y) {
+            yv[q] = load8(yr + c);
+            if (a.gate) gv[q] = load8(gate + c);
         }
     }
+    float x[NV][8];
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[q][e] = 0.0f;
+        if ((lane + q * kRow) * 8 < a.width) unpack(xv[q], x[q]);
+    }
     if (a.y) {
+        float y[NV][8];
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[q][e] = 0.0f;
+            if ((lane + q * kRow) * 8 < a.width) unpack(yv[q], y[q]);
+        }
         norm_row<kRow, NV>(y, a.post_kind, a.post_weight, a.post_bias, a.post_eps, a.width, lane, red);
 #pragma unroll
         for (int q = 0; q < NV; ++q) {
@@ -128,7 +138,7 @@ __global__ void __launch_bounds__(256) gated_norm_kernel(GatedNormArgs g) {
                 for (int e = 0; e < 8; ++e) y[q][e] *= t[e];
             }
             if (a.gate) {
-                load_any(a.gate, cond + c, a.cond_dtype, t);
+                unpack(gv[q], t);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[q][e] *= t[e];
             }
@@ -137,13 +147,22 @@ __global__ void __launch_bounds__(256) gated_norm_kernel(GatedNormArgs g) {
         }
     }
     if (a.x_out) {
+        R* out = static_cast<R*>(a.x_out) + r * a.x_out_stride;
 #pragma unroll
         for (int q = 0; q < NV; ++q) {
             const uint32_t c = (lane + q * kRow) * 8;
-            if (c < a.width) store_any(a.x_out, r * a.x_out_stride + c, a.residual_dtype, x[q]);
+            if (c < a.width) store8(out + c, pack<R>(x[q]));
         }
     }
     if (!a.h) return;
+    Vec8<C> sv[NV], bv[NV];
+    const C *scale = static_cast<const C*>(a.scale) + cond, *shift = static_cast<const C*>(a.shift) + cond;
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+        const uint32_t c = (lane + q * kRow) * 8;
+        if (c < a.width && a.scale) sv[q] = load8(scale + c);
+        if (c < a.width && a.shift) bv[q] = load8(shift + c);
+    }
     norm_row<kRow, NV>(x, a.pre_kind, a.pre_weight, a.pre_bias, a.pre_eps, a.width, lane, red);
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
@@ -151,22 +170,23 @@ __global__ void __launch_bounds__(256) gated_norm_kernel(GatedNormArgs g) {
         if (c >= a.width) continue;
         float t[8];
         if (a.scale) {
-            load_any(a.scale, cond + c, a.cond_dtype, t);
+            unpack(sv[q], t);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[q][e] *= 1.0f + t[e];
         }
         if (a.shift) {
-            load_any(a.shift, cond + c, a.cond_dtype, t);
+            unpack(bv[q], t);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[q][e] += t[e];
         }
     }
     if (g.out_norm)
         norm_row<kRow, NV>(x, LWM_NORM_LAYER, a.out_weight, a.out_bias, a.out_eps, a.width, lane, red);
+    T* h = static_cast<T*>(a.h) + r * a.h_stride;
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
         const uint32_t c = (lane + q * kRow) * 8;
-        if (c < a.width) store_any(a.h, r * a.h_stride + c, a.dtype, x[q]);
+        if (c < a.width) store8(h + c, pack<T>(x[q]));
     }
 }
 
@@ -229,10 +249,19 @@ bool aligned(const void* p, uint64_t stride, size_t elem) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * elem % 16 == 0);
 }
 
-template <int kRow, int NV> cudaError_t launch_rows(const GatedNormArgs& g, cudaStream_t s) {
+template <typename R, typename T, typename C, int kRow, int NV> cudaError_t launch_rows(const GatedNormArgs& g, cudaStream_t s) {
     const uint32_t per = kRow == 32 ? 4 : 1;  // rows a block
-    gated_norm_kernel<kRow, NV><<<(g.a.rows + per - 1) / per, per * kRow, 0, s>>>(g);
+    gated_norm_kernel<R, T, C, kRow, NV><<<(g.a.rows + per - 1) / per, per * kRow, 0, s>>>(g);
     return cudaGetLastError();
+}
+template <typename R, typename T, typename C> cudaError_t launch_vectors(const GatedNormArgs& g, cudaStream_t s) {
+    const uint32_t v = g.a.width / 8;
+    if (v <= 32) return launch_rows<R, T, C, 32, 1>(g, s);
+    if (v <= 64) return launch_rows<R, T, C, 32, 2>(g, s);
+    if (v <= 128) return launch_rows<R, T, C, 32, 4>(g, s);
+    if (v <= 256) return launch_rows<R, T, C, 256, 1>(g, s);
+    if (v <= 512) return launch_rows<R, T, C, 256, 2>(g, s);
+    return launch_rows<R, T, C, 256, 4>(g, s);
 }
 
 }  // namespace
@@ -241,23 +270,33 @@ cudaError_t launch_gated_norm(const GatedNormArgs& g, cudaStream_t s) {
     const lwm_gated_norm_args& a = g.a;
     const size_t re = a.residual_dtype == LWM_DTYPE_F32 ? 4 : 2, te = a.dtype == LWM_DTYPE_F32 ? 4 : 2,
                  ce = a.cond_dtype == LWM_DTYPE_F32 ? 4 : 2;
+    const bool cond = a.gate || a.shift || a.scale;
     const bool vectors = a.width % 8 == 0 && aligned(a.x, a.x_stride, re) && aligned(a.x_out, a.x_out_stride, re) &&
                          aligned(a.y, a.y_stride, te) && aligned(a.h, a.h_stride, te) &&
                          aligned(a.gate, a.cond_stride, ce) && aligned(a.shift, a.cond_stride, ce) &&
                          aligned(a.scale, a.cond_stride, ce) && aligned(a.residual_scale, 0, 4) &&
                          aligned(a.post_weight, 0, 4) && aligned(a.post_bias, 0, 4) && aligned(a.pre_weight, 0, 4) &&
                          aligned(a.pre_bias, 0, 4) && aligned(a.out_weight, 0, 4) && aligned(a.out_bias, 0, 4);
-    if (!vectors) {
-        gated_norm_any_kernel<<<a.rows, 256, a.width * sizeof(float), s>>>(g);
-        return cudaGetLastError();
+    // the types that go together: a 32-bit residual stream or one in the block's type, conditioning likewise
+    if (vectors) {
+        const bool rf = a.residual_dtype == LWM_DTYPE_F32, cf = !cond || a.cond_dtype == LWM_DTYPE_F32;
+        const bool rt = a.residual_dtype == a.dtype, ct = cond && a.cond_dtype == a.dtype;
+        if (a.dtype == LWM_DTYPE_F32 && rf && cf) return launch_vectors<float, float, float>(g, s);
+        if (a.dtype == LWM_DTYPE_BF16) {
+            if (rf && cf) return launch_vectors<float, bf16, float>(g, s);
+            if (rf && ct) return launch_vectors<float, bf16, bf16>(g, s);
+            if (rt && cf) return launch_vectors<bf16, bf16, float>(g, s);
+            if (rt && ct) return launch_vectors<bf16, bf16, bf16>(g, s);
+        }
+        if (a.dtype == LWM_DTYPE_F16) {
+            if (rf && cf) return launch_vectors<float, __half, float>(g, s);
+            if (rf && ct) return launch_vectors<float, __half, __half>(g, s);
+            if (rt && cf) return launch_vectors<__half, __half, float>(g, s);
+            if (rt && ct) return launch_vectors<__half, __half, __half>(g, s);
+        }
     }
-    const uint32_t v = a.width / 8;
-    if (v <= 32) return launch_rows<32, 1>(g, s);
-    if (v <= 64) return launch_rows<32, 2>(g, s);
-    if (v <= 128) return launch_rows<32, 4>(g, s);
-    if (v <= 256) return launch_rows<256, 1>(g, s);
-    if (v <= 512) return launch_rows<256, 2>(g, s);
-    return launch_rows<256, 4>(g, s);
+    gated_norm_any_kernel<<<a.rows, 256, a.width * sizeof(float), s>>>(g);
+    return cudaGetLastError();
 }
 
 }  // namespace lwm

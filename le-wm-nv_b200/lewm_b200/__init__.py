@@ -1231,35 +1231,42 @@ def preprocess_nv12_device(ctx: Context, y_plane, uv_plane, batch: int, height: 
 # or around a planner), on torch CUDA tensors and the context's stream.
 
 DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+_dtype_codes: dict = {}  # the same by torch dtype, as they are met
 
 
 def _dtype(t, name: str) -> int:
-    d = DTYPES.get(str(t.dtype))
+    d = _dtype_codes.get(t.dtype)
     if d is None:
-        raise LwmError(1, f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+        d = DTYPES.get(str(t.dtype))
+        if d is None:
+            raise LwmError(1, f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+        _dtype_codes[t.dtype] = d
     return d
 
 
 def _on(ctx: Context, name: str, t) -> int:
     """The address of a tensor on the context's device."""
-    if not t.is_cuda or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:
         raise LwmError(1, f"{name} must be on cuda:{ctx.device}, got {t.device}")
     return t.data_ptr()
 
 
-def _heads(ctx: Context, name: str, t, shape, dtype) -> int:
-    """The address of a [tokens, heads, channels] tensor with contiguous channels."""
-    if tuple(t.shape) != shape:
+def _heads(ctx: Context, name: str, t, shape, dtype):
+    """(address, token stride, head stride) of a [tokens, heads, channels] tensor with contiguous channels."""
+    if t.shape != shape:
         raise LwmError(1, f"{name} must be {list(shape)}, got {list(t.shape)}")
     if t.dtype != dtype:
         raise LwmError(1, f"{name} must be {dtype}, got {t.dtype}")
-    if t.stride(2) != 1:
+    ts, hs, cs = t.stride()
+    if cs != 1:
         raise LwmError(1, f"{name} needs contiguous channels")
-    return _on(ctx, name, t)
+    if t.get_device() != ctx.device:
+        raise LwmError(1, f"{name} must be on cuda:{ctx.device}, got {t.device}")
+    return t.data_ptr(), ts, hs
 
 
 def _ints(name: str, t, shape) -> None:
-    if str(t.dtype) != "torch.int32" or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.shape != shape or not t.is_contiguous() or str(t.dtype) != "torch.int32":
         raise LwmError(1, f"{name} must be a contiguous int32 tensor {list(shape)}, got {t.dtype} {list(t.shape)}")
 
 
@@ -1286,7 +1293,7 @@ class PagedCache:
         if str(self.dtype) not in ("torch.bfloat16", "torch.float16"):
             raise LwmError(1, f"cache dtype must be bfloat16 or float16, got {self.dtype}")
         self._keep = (k, v, k_scale, v_scale)
-        self.device = k.device
+        self.device, self.device_index = k.device, k.get_device()
         if any(t is not None and t.device != k.device for t in self._keep):
             raise LwmError(1, "cache tensors are on different devices")
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
@@ -1309,7 +1316,7 @@ class CacheBatch:
         _ints("starts", starts, (n + 1,))
         _ints("lengths", lengths, (n,))
         self._keep = (table, starts, lengths)
-        self.device = table.device
+        self.device, self.device_index = table.device, table.get_device()
         if starts.device != table.device or lengths.device != table.device:
             raise LwmError(1, "batch tensors are on different devices")
         self.tokens = tokens
@@ -1319,21 +1326,20 @@ class CacheBatch:
 
 
 def _same_device(ctx: Context, cache: PagedCache, batch: CacheBatch) -> None:
-    for name, x in (("cache", cache), ("batch", batch)):
-        if x.device.type != "cuda" or x.device.index != ctx.device:
-            raise LwmError(1, f"{name} must be on cuda:{ctx.device}, got {x.device}")
+    if cache.device_index != ctx.device or batch.device_index != ctx.device:
+        raise LwmError(1, f"cache and batch must be on cuda:{ctx.device}, got {cache.device} and {batch.device}")
 
 
 def rotary_device(ctx: Context, rotary: Rotary, x, out, positions, inverse: bool = False) -> None:
     """out = x [tokens, heads, head_dim] turned by positions [tokens, axes] int32 (`inverse`: turned back)."""
     if x.dim() != 3:
         raise LwmError(1, f"x must be [tokens, heads, head_dim], got {list(x.shape)}")
-    tokens, heads, d = x.shape
-    shape = (tokens, heads, d)
+    tokens, heads, d = shape = x.shape
     _ints("positions", positions, (tokens, rotary.axes))
-    a = _RotaryArgs(_heads(ctx, "x", x, shape, x.dtype), _heads(ctx, "out", out, shape, x.dtype), x.stride(0),
-                    x.stride(1), out.stride(0), out.stride(1), _on(ctx, "positions", positions), tokens, heads, d,
-                    _dtype(x, "x"), int(inverse))
+    xp, xt, xh = _heads(ctx, "x", x, shape, x.dtype)
+    op, ot, oh = _heads(ctx, "out", out, shape, x.dtype)
+    a = _RotaryArgs(xp, op, xt, xh, ot, oh, _on(ctx, "positions", positions), tokens, heads, d, _dtype(x, "x"),
+                    int(inverse))
     _check(lib.lwm_rotary_device(ctx.handle, C.byref(rotary), C.byref(a)))
 
 
@@ -1343,24 +1349,25 @@ def cache_append_device(ctx: Context, cache: PagedCache, batch: CacheBatch, k, v
     keys (and q [tokens, heads, head_dim] into q_out) turned by `positions`
     [tokens, axes] (None: each token's cache index)."""
     _same_device(ctx, cache, batch)
-    n, shape = batch.tokens, (batch.tokens, cache.kv_heads, cache.head_dim)
+    n, dtype, shape = batch.tokens, cache.dtype, (batch.tokens, cache.kv_heads, cache.head_dim)
+    pos = None
     if positions is not None:
         if rotary is None:
             raise LwmError(1, "positions need a rotary")
         _ints("positions", positions, (n, rotary.axes))
-    kp, vp = _heads(ctx, "k", k, shape, cache.dtype), _heads(ctx, "v", v, shape, cache.dtype)
+        pos = _on(ctx, "positions", positions)
+    kp, kt, kh = _heads(ctx, "k", k, shape, dtype)
+    vp, vt, vh = _heads(ctx, "v", v, shape, dtype)
     if q is not None:
         if q_out is None or q.dim() != 3:
             raise LwmError(1, "q [tokens, heads, head_dim] needs q_out")
         heads = q.shape[1]
         shape = (n, heads, cache.head_dim)
-        qp, qo = _heads(ctx, "q", q, shape, cache.dtype), _heads(ctx, "q_out", q_out, shape, cache.dtype)
-        a = _CacheAppendArgs(qp, qo, kp, vp, q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1), k.stride(0),
-                             k.stride(1), v.stride(0), v.stride(1),
-                             None if positions is None else _on(ctx, "positions", positions), heads)
+        qp, qt, qh = _heads(ctx, "q", q, shape, dtype)
+        op, ot, oh = _heads(ctx, "q_out", q_out, shape, dtype)
+        a = _CacheAppendArgs(qp, op, kp, vp, qt, qh, ot, oh, kt, kh, vt, vh, pos, heads)
     else:
-        a = _CacheAppendArgs(None, None, kp, vp, 0, 0, 0, 0, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                             None if positions is None else _on(ctx, "positions", positions), 0)
+        a = _CacheAppendArgs(None, None, kp, vp, 0, 0, 0, 0, kt, kh, vt, vh, pos, 0)
     _check(lib.lwm_cache_append_device(ctx.handle, cache._ref, batch._ref,
                                        None if rotary is None else C.byref(rotary), C.byref(a)))
 
@@ -1369,9 +1376,9 @@ def cache_gather_device(ctx: Context, cache: PagedCache, batch: CacheBatch, k_ou
     """The batch's cached tokens as values: k_out, v_out [tokens, kv_heads, head_dim] of the cache's dtype."""
     _same_device(ctx, cache, batch)
     shape = (batch.tokens, cache.kv_heads, cache.head_dim)
-    a = _CacheGatherArgs(_heads(ctx, "k_out", k_out, shape, cache.dtype),
-                         _heads(ctx, "v_out", v_out, shape, cache.dtype), k_out.stride(0), k_out.stride(1),
-                         v_out.stride(0), v_out.stride(1))
+    kp, kt, kh = _heads(ctx, "k_out", k_out, shape, cache.dtype)
+    vp, vt, vh = _heads(ctx, "v_out", v_out, shape, cache.dtype)
+    a = _CacheGatherArgs(kp, vp, kt, kh, vt, vh)
     _check(lib.lwm_cache_gather_device(ctx.handle, cache._ref, batch._ref, C.byref(a)))
 
 
@@ -1384,11 +1391,12 @@ def cache_attention_device(ctx: Context, cache: PagedCache, batch: CacheBatch, q
     _same_device(ctx, cache, batch)
     if q.dim() != 3:
         raise LwmError(1, f"q must be [tokens, heads, head_dim], got {list(q.shape)}")
-    shape = (batch.tokens, q.shape[1], cache.head_dim)
-    a = _CacheAttentionArgs(_heads(ctx, "q", q, shape, cache.dtype), _heads(ctx, "out", out, shape, cache.dtype),
-                            q.stride(0), q.stride(1), out.stride(0), out.stride(1), shape[1],
-                            cache.head_dim ** -0.5 if scale is None else scale, int(causal), window, sinks,
-                            frame_tokens)
+    heads = q.shape[1]
+    shape = (batch.tokens, heads, cache.head_dim)
+    qp, qt, qh = _heads(ctx, "q", q, shape, cache.dtype)
+    op, ot, oh = _heads(ctx, "out", out, shape, cache.dtype)
+    a = _CacheAttentionArgs(qp, op, qt, qh, ot, oh, heads, cache.head_dim ** -0.5 if scale is None else scale,
+                            int(causal), window, sinks, frame_tokens)
     _check(lib.lwm_cache_attention_device(ctx.handle, cache._ref, batch._ref, C.byref(a)))
 
 
@@ -1405,10 +1413,10 @@ class GatedNorm:
             raise LwmError(1, "gated norm kinds are layer, rms or none")
         self._keep = dict(residual_scale=residual_scale, post_weight=post_weight, post_bias=post_bias,
                           pre_weight=pre_weight, pre_bias=pre_bias, out_weight=out_weight, out_bias=out_bias)
-        self._c = _GatedNormArgs(post_kind=kinds[post], pre_kind=kinds[pre], post_eps=post_eps, pre_eps=pre_eps,
-                                 out_eps=out_eps)
         self.width, self.device = None, None
+        at = {}
         for name, t in self._keep.items():
+            at[name] = None
             if t is None:
                 continue
             if str(t.dtype) != "torch.float32" or t.dim() != 1 or not t.is_contiguous():
@@ -1416,7 +1424,21 @@ class GatedNorm:
             if self.width not in (None, t.shape[0]) or self.device not in (None, t.device):
                 raise LwmError(1, "gated norm weights differ in width or device")
             self.width, self.device = t.shape[0], t.device
-            setattr(self._c, name, t.data_ptr())
+            at[name] = t.data_ptr()
+        self.device_index = None if self.device is None else -1 if self.device.type == "cpu" else self.device.index
+        # the fields of lwm_gated_norm_args from residual_scale on
+        self._tail = (at["residual_scale"], kinds[post], kinds[pre], post_eps, pre_eps, out_eps, at["post_weight"],
+                      at["post_bias"], at["pre_weight"], at["pre_bias"], at["out_weight"], at["out_bias"])
+
+
+def _rows(ctx: Context, name: str, t, x, width: int):
+    """(address, row stride) of a tensor shaped like x with contiguous rows."""
+    stride, unit = t.stride()
+    if t.shape != x.shape or (unit != 1 and width > 1):
+        raise LwmError(1, f"{name} must be {list(x.shape)} with contiguous rows, got {list(t.shape)}")
+    if t.get_device() != ctx.device:
+        raise LwmError(1, f"{name} must be on cuda:{ctx.device}, got {t.device}")
+    return t.data_ptr(), stride
 
 
 def gated_norm_device(ctx: Context, norm: GatedNorm, x, y=None, x_out=None, h=None, gate=None, shift=None, scale=None,
@@ -1427,42 +1449,38 @@ def gated_norm_device(ctx: Context, norm: GatedNorm, x, y=None, x_out=None, h=No
     if x.dim() != 2:
         raise LwmError(1, f"x must be [rows, width], got {list(x.shape)}")
     rows, width = x.shape
-    if norm.width not in (None, width):
-        raise LwmError(1, f"gated norm weights have width {norm.width}, x has {width}")
-    if norm.device is not None and norm.device != x.device:
-        raise LwmError(1, f"gated norm weights are on {norm.device}, x on {x.device}")
-    a = _GatedNormArgs.from_buffer_copy(norm._c)
-    a.rows, a.width, a.rows_per_cond = rows, width, rows_per_cond
-    a.residual_dtype = _dtype(x, "x")
-    dtype = None
-    for name, t, stride in (("x", x, "x_stride"), ("x_out", x_out, "x_out_stride"), ("y", y, "y_stride"),
-                            ("h", h, "h_stride")):
+    if norm.width is not None and (norm.width != width or norm.device_index != ctx.device):
+        raise LwmError(1, f"gated norm weights are [{norm.width}] on {norm.device}, x is {list(x.shape)} on {x.device}")
+    xp, xs = _rows(ctx, "x", x, x, width)
+    yp = op = hp = None
+    ys = os_ = hs = 0
+    if x_out is not None:
+        op, os_ = _rows(ctx, "x_out", x_out, x, width)
+        if x_out.dtype != x.dtype:
+            raise LwmError(1, f"x_out must be {x.dtype}, got {x_out.dtype}")
+    if y is not None:
+        yp, ys = _rows(ctx, "y", y, x, width)
+    if h is not None:
+        hp, hs = _rows(ctx, "h", h, x, width)
+        if y is not None and y.dtype != h.dtype:
+            raise LwmError(1, "y and h must have one type")
+    t = y if y is not None else h
+    dtype = _dtype(t, "y") if t is not None else 0
+    cond_dtype, cond_stride, at = None, 0, [None, None, None]
+    for i, t in enumerate((gate, shift, scale)):
         if t is None:
             continue
-        if t.shape != x.shape or t.stride(1) != 1 and width > 1:
-            raise LwmError(1, f"{name} must be [{rows}, {width}] with contiguous rows, got {list(t.shape)}")
-        if name == "x_out" and t.dtype != x.dtype:
-            raise LwmError(1, f"x_out must be {x.dtype}, got {t.dtype}")
-        if name in ("y", "h"):
-            if dtype not in (None, t.dtype):
-                raise LwmError(1, "y and h must have one type")
-            dtype = t.dtype
-            a.dtype = _dtype(t, name)
-        setattr(a, name, _on(ctx, name, t))
-        setattr(a, stride, t.stride(0))
-    cond = None
-    for name, t in (("gate", gate), ("shift", shift), ("scale", scale)):
-        if t is None:
-            continue
-        if rows_per_cond < 1 or t.dim() != 2 or t.shape[1] != width or t.shape[0] * rows_per_cond < rows or \
-                (t.stride(1) != 1 and width > 1):
-            raise LwmError(1, f"{name} must be [ceil(rows / rows_per_cond), {width}] with contiguous rows, "
-                              f"got {list(t.shape)}")
-        if cond not in (None, (t.dtype, t.stride(0))):
+        stride, unit = t.stride()
+        if rows_per_cond < 1 or t.shape[1] != width or t.shape[0] * rows_per_cond < rows or (unit != 1 and width > 1):
+            raise LwmError(1, f"{('gate', 'shift', 'scale')[i]} must be [ceil(rows / rows_per_cond), {width}] with "
+                              f"contiguous rows, got {list(t.shape)}")
+        if cond_dtype is not None and (t.dtype != cond_dtype or stride != cond_stride):
             raise LwmError(1, "gate, shift and scale must have one type and row stride")
-        cond = (t.dtype, t.stride(0))
-        a.cond_dtype, a.cond_stride = _dtype(t, name), t.stride(0)
-        setattr(a, name, _on(ctx, name, t))
+        cond_dtype, cond_stride = t.dtype, stride
+        at[i] = _on(ctx, ("gate", "shift", "scale")[i], t)
+        code = _dtype(t, "gate, shift and scale")
+    a = _GatedNormArgs(xp, yp, op, hp, xs, ys, os_, hs, rows, width, _dtype(x, "x"), dtype,
+                       0 if cond_dtype is None else code, at[0], at[1], at[2], cond_stride, rows_per_cond, *norm._tail)
     _check(lib.lwm_gated_norm_device(ctx.handle, C.byref(a)))
 
 
