@@ -1,13 +1,15 @@
 // kernels_cache_attn.cu — attention over the paged cache for few query rows
 // a kv head (lwm_cache_attention_device).
 //
-// A job is (sequence, kv head, 16 query rows = tokens x heads of the group).
-// A warp walks 16-key units: scores = Q K^T on mma.sync m16n8k16, a running
-// maximum and sum in 32 bits, O += P V.  The units of a job are dealt to the
-// four warps of a block and, for long contexts, to the blocks of a cluster;
-// their (maximum, sum, O) are joined in shared memory and over distributed
-// shared memory, so a call needs no workspace and no second kernel and its
-// sums have one order.
+// A job is (sequence, kv head, 8 or 16 query rows = tokens x heads of the
+// group).  A warp walks 16-key units: scores S^T = K Q^T on mma.sync m16n8k16
+// (the keys are the wide side: a single token's few rows fill half of a
+// 16-row tile at best), a running maximum and sum in 32 bits, O^T += V^T P^T,
+// P turned over by movmatrix.  The units of a job are dealt to the four warps
+// of a block and, for long contexts, to the blocks of a cluster; their
+// (maximum, sum, O) are joined in shared memory and over distributed shared
+// memory, so a call needs no workspace and no second kernel and its sums have
+// one order.  Where contexts are short and jobs many, a warp has a job alone.
 //
 // Bound: memory (each K and V byte is used by at most 16 rows, 32 flops a
 // byte).  Every warp keeps its own ring of units in flight with cp.async, so
@@ -53,6 +55,12 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(addr)
                  : "memory");
+}
+// An 8 x 8 tile of 16-bit values turned over.
+__device__ __forceinline__ uint32_t turn_over(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 template <typename M>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -100,52 +108,71 @@ __device__ __forceinline__ float value_at(const uint8_t* unit, uint32_t key, uin
     }
 }
 
-template <int D, bool kCodes> struct Shape {
+// kRows: query rows of a job, 8 or 16.
+template <int D, bool kCodes, int kRows, bool kShared> struct Shape {
     static constexpr int kUnitBytes = kUnit * D * (kCodes ? 1 : 2);  // of K, and of V
-    static constexpr int kStages = kCodes ? (D == 128 ? 6 : 8) : (D == 128 ? 4 : 6);
+    static constexpr int kStages = kShared ? 3 : 2;
     static constexpr int kWarpBytes = kStages * 2 * kUnitBytes;
-    static constexpr int kPartFloats = 16 * D;                       // a warp's O
-    static constexpr int kPartBytes = (kPartFloats + 32) * 4;        // and its maxima and sums
-    static constexpr int kBytes = kWarps * (kWarpBytes > kPartBytes ? kWarpBytes : kPartBytes);
+    static constexpr int kPitch = D + 4;                             // floats of a row of O in shared memory
+    static constexpr int kPartFloats = kRows * kPitch;               // a warp's O
+    static constexpr int kPartBytes = kShared ? (kPartFloats + 2 * kRows) * 4 : kRows * D * 2;  // maxima and sums too
+    static constexpr int kRings = kWarps * (kWarpBytes > kPartBytes ? kWarpBytes : kPartBytes);
+    static constexpr int kBytes = kRings + kWarps * kStages * 16;    // and the units' pages and scales
+    // blocks a SM, by shared memory and registers
+    static constexpr int kBySmem = 220 * 1024 / (kBytes + 1024), kByRegs = kRows == 8 ? (D == 128 ? 4 : 5) : (D == 128 ? 3 : 4);
+    static constexpr int kBlocks = kBySmem < kByRegs ? kBySmem : kByRegs;
+};
+
+// A unit in flight: its page (-1: none) and, of codes, the page's scales.
+struct UnitNote {
+    int page;
+    float k_scale, v_scale, pad;
 };
 
 // Visible keys of one row: [0, first) and [lo, hi).
 struct RowRange { uint32_t lo, hi, first; };
 
-template <typename T, int D, bool kCodes, bool kShared>
-__global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a, uint32_t tiles, uint32_t split) {
+template <typename T, int D, bool kCodes, int kRows, bool kShared>
+__global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kBlocks)
+    cache_attn_kernel(const __grid_constant__ CacheAttnArgs a, uint32_t tiles, uint32_t split) {
     using M = std::conditional_t<kCodes, __half, T>;  // the operands' type
-    using S = Shape<D, kCodes>;
-    constexpr int kSteps = D / 16, kTiles = D / 8;
+    using S = Shape<D, kCodes, kRows, kShared>;
+    constexpr int kSteps = D / 16, kQ = kRows / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     // job: four warps (and `split` blocks) share one, or a warp has its own
     const uint32_t rank = kShared ? blockIdx.x % split : 0;
     const uint32_t job = kShared ? blockIdx.x / split : blockIdx.x * kWarps + warp;
-    const uint32_t tile = job % tiles, hs = job / tiles, h = hs % a.c.kv_heads, s = hs / a.c.kv_heads;
+    const uint32_t hs = a.tile_div.div(job), tile = job - hs * tiles, s = a.kv_div.div(hs), h = hs - s * a.c.kv_heads;
+    // a short table's row comes along with the lengths
+    int entry = -1;
+    const bool small_table = !kShared && a.c.table_stride <= 32;
     SeqView v;
-    if (s < a.c.sequences) v = sequence(a.c, s, false, h == 0 && tile == 0 && rank == 0 && lane == 0);
-    const uint32_t rows = v.n * a.group, row0 = tile * 16;
+    if (s < a.c.sequences) {
+        if (small_table && lane < a.c.table_stride)
+            entry = a.c.table[static_cast<size_t>(s) * a.c.table_stride + lane];
+        v = sequence(a.c, s, false, h == 0 && tile == 0 && rank == 0 && lane == 0);
+    }
+    const uint32_t rows = v.n * a.group, row0 = tile * kRows;
     const bool live = row0 < rows;
     if (!live && (!kShared || split == 1)) return;  // uniform over what waits together
 
-    // this thread's rows g and g + 8, and the tile's union
-    RowRange rr[2];
-    const void* q_row[2] = {nullptr, nullptr};
+    // the keys that this thread's queries 8 n + 2 t + e see, and the tile's union
+    RowRange rr[kQ][2];
     uint32_t lo_min = 0, lo_max = 0, hi_min = 0, hi_max = 0;
     if (live) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t R = row0 + g + 8 * i;
-            rr[i] = {0, 0, 0};
-            if (R < rows) {
-                const uint32_t tok = a.group_div.div(R), head = h * a.group + (R - tok * a.group);
-                const VisibleRange vr = visible(a, v, tok);
-                rr[i] = {vr.lo, vr.hi, vr.first};
-                q_row[i] = static_cast<const T*>(a.q) + (v.start + tok) * a.q_ts + head * a.q_hs;
+        for (int n = 0; n < kQ; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t R = row0 + 8 * n + 2 * t + e;
+                rr[n][e] = {0, 0, 0};
+                if (R < rows) {
+                    const VisibleRange vr = visible(a, v, a.group_div.div(R));
+                    rr[n][e] = {vr.lo, vr.hi, vr.first};
+                }
             }
-        }
-        const uint32_t tok0 = a.group_div.div(row0), tok1 = a.group_div.div(min(row0 + 15, rows - 1));
+        const uint32_t tok0 = a.group_div.div(row0), tok1 = a.group_div.div(min(row0 + kRows - 1, rows - 1));
         const VisibleRange r0 = visible(a, v, tok0), r1 = visible(a, v, tok1);
         lo_min = r0.lo, hi_min = r0.hi;
         lo_max = r1.lo, hi_max = r1.hi;
@@ -158,335 +185,360 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a, u
     // this warp's units: walk, walk + step, ... below end
     const uint32_t per = kShared ? (units + split - 1) / split : units;
     const uint32_t end = kShared ? min(units, (rank + 1) * per) : units;
-    uint32_t walk = kShared ? rank * per + warp : 0;
+    const uint32_t walk = kShared ? rank * per + warp : 0;
     const uint32_t step = kShared ? kWarps : 1;
 
     uint8_t* ring = smem + warp * S::kWarpBytes;
     const uint32_t ring_a = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
     const uint32_t count = walk < end ? (end - walk + step - 1) / step : 0;
-    // page and first key of the warp's unit i, looked up 32 units at a time
-    int pages_ahead = -1;
     auto key_of = [&](uint32_t i) {
         const uint32_t u = walk + i * step;
         return (u < sink_units ? u : u - sink_units + win_unit) * kUnit;
     };
-    auto look_ahead = [&](uint32_t i) {
-        pages_ahead = i + lane < count ? page_of(a.c, s, key_of(i + lane) >> a.c.page_shift) : -1;
+    // page of the warp's unit i: from the table's row, or looked up 32 units at a time
+    int pages_ahead = -1;
+    auto page_at = [&](uint32_t i) {
+        if (small_table) {
+            const int p = __shfl_sync(0xffffffffu, entry, key_of(i) >> a.c.page_shift);
+            if (static_cast<uint32_t>(p) < a.c.pages) return p;
+            if (lane == 0) cache_report(a.c.err, kCacheErrPage, s, p);
+            return -1;
+        }
+        if ((i & 31) == 0) pages_ahead = i + lane < count ? page_of(a.c, s, key_of(i + lane) >> a.c.page_shift) : -1;
+        return __shfl_sync(0xffffffffu, pages_ahead, i & 31);
     };
-    int unit_pages[S::kStages];  // of the units in flight, by ring slot (8 bits: their scales)
-    auto load = [&](uint32_t i, int slot) {
-        if ((i & 31) == 0) look_ahead(i);
-        const int page = __shfl_sync(0xffffffffu, pages_ahead, i & 31);
+    UnitNote* notes = reinterpret_cast<UnitNote*>(smem + S::kRings) + warp * S::kStages;
+    auto load = [&](uint32_t i, uint32_t slot) {
+        const int page = page_at(i);
         const uint32_t key = key_of(i);
-        const uint32_t at = key & (a.c.page_tokens - 1);
         constexpr int kRowChunks = S::kUnitBytes / kUnit / 16;
-        const size_t base = pool_at(a.c, page < 0 ? 0 : page, h, at) * (kCodes ? 1 : 2);
+        const size_t base = pool_at(a.c, page < 0 ? 0 : page, h, key & (a.c.page_tokens - 1)) * (kCodes ? 1 : 2);
         const uint32_t dst = ring_a + slot * 2 * S::kUnitBytes;
+        if (lane == 0) notes[slot].page = page;
+        if (kCodes && lane < 2 && page >= 0) {
+            const float* scale = (lane ? a.c.v_scale : a.c.k_scale) + static_cast<size_t>(page) * a.c.kv_heads + h;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(
+                             static_cast<uint32_t>(__cvta_generic_to_shared(lane ? &notes[slot].v_scale : &notes[slot].k_scale))),
+                         "l"(scale)
+                         : "memory");
+        }
+        const uint8_t* kp = static_cast<const uint8_t*>(a.c.k) + base + lane * 16;
+        const uint8_t* vp = static_cast<const uint8_t*>(a.c.v) + base + lane * 16;
+        // rows that no query sees come as zeros
+        const bool all = page >= 0 && key + kUnit <= hi_max && (key >= lo_min || key + kUnit <= sinks_end);
 #pragma unroll
         for (int c = 0; c < kUnit * kRowChunks / 32; ++c) {
             const uint32_t x = c * 32 + lane, r = x / kRowChunks, ch = x % kRowChunks;
             const uint32_t j = key + r;
-            const bool ok = page >= 0 && j < hi_max && (j >= lo_min || j < sinks_end);
-            cp_async16(dst + chunk_at<D, kCodes>(r, ch), static_cast<const uint8_t*>(a.c.k) + base + x * 16, ok);
-            cp_async16(dst + S::kUnitBytes + chunk_at<D, kCodes>(r, ch),
-                       static_cast<const uint8_t*>(a.c.v) + base + x * 16, ok);
+            const bool ok = all || (page >= 0 && j < hi_max && (j >= lo_min || j < sinks_end));
+            cp_async16(dst + chunk_at<D, kCodes>(r, ch), kp + c * 512, ok);
+            cp_async16(dst + S::kUnitBytes + chunk_at<D, kCodes>(r, ch), vp + c * 512, ok);
         }
-        return page;
     };
-#pragma unroll
-    for (int i = 0; i < S::kStages; ++i) unit_pages[i] = -1;
-#pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) {
-        if (i < count) unit_pages[i] = load(i, i);
+#pragma unroll 1
+    for (uint32_t i = 0; i < S::kStages - 1; ++i) {
+        if (i < count) load(i, i);
         cp_commit();
     }
 
-    // queries, in the order of the contraction
-    uint32_t q[kSteps][4];
-    float row_mul[2] = {a.scale_log2, a.scale_log2};
-    if (live) {
+    // queries 8 n + g, in the order of the contraction
+    uint32_t q[kQ][kSteps][2];
+    float row_mul[kQ][2];  // of queries 8 n + 2 t + e
+#pragma unroll
+    for (int n = 0; n < kQ; ++n) {
+        const uint32_t R = row0 + 8 * n + g;
+        const T* qr = nullptr;
+        if (live && R < rows) {
+            const uint32_t tok = a.group_div.div(R);
+            qr = static_cast<const T*>(a.q) + (v.start + tok) * a.q_ts + (h * a.group + (R - tok * a.group)) * a.q_hs;
+        }
+        row_mul[n][0] = row_mul[n][1] = a.scale_log2;
         if constexpr (!kCodes) {
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    q[k][i] = q_row[i & 1] ? *reinterpret_cast<const uint32_t*>(static_cast<const T*>(q_row[i & 1]) +
-                                                                               16 * k + 8 * (i >> 1) + 2 * t)
-                                           : 0u;
+                for (int i = 0; i < 2; ++i)
+                    q[n][k][i] = qr ? *reinterpret_cast<const uint32_t*>(qr + 16 * k + 8 * i + 2 * t) : 0u;
         } else {
             constexpr int kRun = D >= 64 ? 16 : 8;  // channels a thread reads of each 4 * kRun
-            float f[2][kSteps][4];
+            float f[kSteps][4], amax = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float amax = 0.0f;
+            for (int k = 0; k < kSteps; ++k) {
+                const int ch = (k / (kRun / 4)) * 4 * kRun + t * kRun + (k % (kRun / 4)) * 4;
+                uint2 w = make_uint2(0, 0);
+                if (qr) w = *reinterpret_cast<const uint2*>(qr + ch);
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    const int ch = (k / (kRun / 4)) * 4 * kRun + t * kRun + (k % (kRun / 4)) * 4;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        f[i][k][e] = q_row[i] ? static_cast<float>(static_cast<const T*>(q_row[i])[ch + e]) : 0.0f;
-                        amax = fmaxf(amax, fabsf(f[i][k][e]));
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const uint16_t x = static_cast<uint16_t>((e < 2 ? w.x : w.y) >> (16 * (e & 1)));
+                    f[k][e] = static_cast<float>(*reinterpret_cast<const T*>(&x));
+                    amax = fmaxf(amax, fabsf(f[k][e]));
                 }
-                if constexpr (std::is_same_v<T, bf16>) {
-                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                    int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-                    if (amax == 0.0f || e == 128) e = 0;
-                    e = min(max(e, -126), 126);
-                    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                    row_mul[i] *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            }
+            if constexpr (std::is_same_v<T, bf16>) {
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+                if (amax == 0.0f || e == 128) e = 0;
+                e = min(max(e, -126), 126);
+                const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k)
+                for (int i = 0; i < 2; ++i) row_mul[n][i] *= __shfl_sync(0xffffffffu, up, (2 * t + i) * 4);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) f[i][k][x] *= down;
-                }
+                for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) f[k][x] *= down;
             }
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    q[k][i] = pack2(f[i & 1][k][2 * (i >> 1)], f[i & 1][k][2 * (i >> 1) + 1], __half{});
+                for (int i = 0; i < 2; ++i) q[n][k][i] = pack2(f[k][2 * i], f[k][2 * i + 1], __half{});
         }
     }
 
-    float o[kTiles][4];
+    // O^T: tile n of queries, tile d of channels; element i is query 2 t + (i & 1), channel of row g + 8 (i >> 1)
+    float o[kQ][kSteps][4];
+    float m[kQ][2], l[kQ][2];
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n)
+    for (int n = 0; n < kQ; ++n) {
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][d][e] = 0.0f;
+    }
     float v_ref = 0.0f;  // 8 bits: O is in units of this value scale
+    auto channel = [&](int d, int half) {  // of row g + 8 half of channel tile d
+        return kCodes ? 32 * (d >> 1) + 4 * g + 2 * (d & 1) + half : 16 * d + 8 * half + g;
+    };
 
-    for (uint32_t base = 0; base < count; base += S::kStages) {
+    // (not unrolled over the ring: copies of the body missed the instruction cache)
+    uint32_t slot = 0;
+#pragma unroll 1
+    for (uint32_t i = 0; i < count; ++i) {
+        cp_wait<S::kStages - 2>();
+        __syncwarp();
+        const int page = notes[slot].page;
+        const uint32_t key = key_of(i);
+        const uint32_t k_at = ring_a + slot * 2 * S::kUnitBytes, v_at = k_at + S::kUnitBytes;
+        float k_scale = 1.0f, v_scale = 1.0f;
+        if constexpr (kCodes) {
+            k_scale = notes[slot].k_scale;
+            v_scale = page < 0 ? 1.0f : notes[slot].v_scale;
+            if (!isfinite(v_scale)) v_scale = __int_as_float(0x7fc00000);
+        }
+        // scores: element e is key g + 8 (e >> 1), query 2 t + (e & 1); two chains of products
+        float sc[kQ][4], odd[kQ][4];
 #pragma unroll
-        for (int slot = 0; slot < S::kStages; ++slot) {
-            const uint32_t i = base + slot;
-            if (i >= count) break;
-            cp_wait<S::kStages - 2>();
-            __syncwarp();
-            const int page = unit_pages[slot];
-            const uint32_t key = key_of(i);
-            const uint32_t k_at = ring_a + slot * 2 * S::kUnitBytes, v_at = k_at + S::kUnitBytes;
-            float k_scale = 1.0f, v_scale = 1.0f;
-            if constexpr (kCodes) {
-                if (page >= 0) {
-                    const size_t at = static_cast<size_t>(page) * a.c.kv_heads + h;
-                    k_scale = a.c.k_scale[at];
-                    v_scale = a.c.v_scale[at];
-                    if (!isfinite(v_scale)) v_scale = __int_as_float(0x7fc00000);
-                }
+        for (int n = 0; n < kQ; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][e] = odd[n][e] = 0.0f;
+        if constexpr (!kCodes) {
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                uint32_t b[4];  // keys 0-7 and 8-15 of channels 0-7, then of channels 8-15
+                ldsm4(b, k_at + chunk_at<D, false>(lane & 15, 2 * k + (lane >> 4)));
+#pragma unroll
+                for (int n = 0; n < kQ; ++n) mma<M>(k & 1 ? odd[n] : sc[n], b, q[n][k][0], q[n][k][1]);
             }
-            float sc[2][4];
+        } else {
+            uint32_t w[2][kSteps];
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
-            if constexpr (!kCodes) {
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    uint32_t b[4];  // keys 0-7 and 8-15, each channels 0-7 and 8-15 of the step
-                    ldsm4(b, k_at + chunk_at<D, false>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
-                    mma<M>(sc[0], q[k], b[0], b[1]);
-                    mma<M>(sc[1], q[k], b[2], b[3]);
-                }
-            } else {
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    uint32_t w[kSteps];
-                    if constexpr (D == 32) {
-                        const uint32_t at = k_at + chunk_at<D, true>(g + 8 * n, t >> 1) + (t & 1) * 8;
-                        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < D / 64; ++c) {
-                            const uint32_t at = k_at + chunk_at<D, true>(g + 8 * n, 4 * c + t);
-                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                                         : "=r"(w[4 * c]), "=r"(w[4 * c + 1]), "=r"(w[4 * c + 2]), "=r"(w[4 * c + 3])
-                                         : "r"(at)
-                                         : "memory");
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k)
-                        mma<M>(sc[n], q[k], f16x2_from_e4m3x2(w[k]), f16x2_from_e4m3x2(w[k] >> 16));
-                }
-            }
-            // scores in units of log2, masked where this row does not see the key
-            const bool whole = page >= 0 && (key >= lo_max || key + kUnit <= sinks_end) &&
-                               key + kUnit <= hi_min;
-            bool seen[2][4];
-            bool above = false;
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i2 = e >> 1;
-                    const uint32_t j = key + 8 * n + 2 * t + (e & 1);
-                    seen[n][e] = whole || (page >= 0 && j < rr[i2].hi && (j >= rr[i2].lo || j < rr[i2].first));
-                    sc[n][e] = seen[n][e] ? sc[n][e] * (k_scale * row_mul[i2]) : -INFINITY;
-                    above |= sc[n][e] > m[i2] + kRaise;
-                }
-            // the maximum moves only when a score passes it by kRaise: until
-            // then exp2(score - m) stays below 2^kRaise
-            if (__any_sync(0xffffffffu, above)) {
-#pragma unroll
-                for (int i2 = 0; i2 < 2; ++i2) {
-                    float x = fmaxf(fmaxf(sc[0][2 * i2], sc[0][2 * i2 + 1]), fmaxf(sc[1][2 * i2], sc[1][2 * i2 + 1]));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                    x = fmaxf(x, m[i2]);
-                    const float down = m[i2] == -INFINITY ? 0.0f : exp2_fast(m[i2] - x);
-                    m[i2] = x;
-                    l[i2] *= down;
-#pragma unroll
-                    for (int n = 0; n < kTiles; ++n) {
-                        o[n][2 * i2] *= down;
-                        o[n][2 * i2 + 1] *= down;
-                    }
-                }
-            }
-            float v_mul = 1.0f;
-            if constexpr (kCodes) {
-                if (v_scale > v_ref) {
-                    const float down = v_ref / v_scale;
-#pragma unroll
-                    for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[n][e] *= down;
-                    v_ref = v_scale;
-                }
-                v_mul = v_scale == 0.0f ? 0.0f : v_scale / v_ref;
-            }
-            float p[2][4];
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float top = m[e >> 1] == -INFINITY ? 0.0f : m[e >> 1];
-                    p[n][e] = exp2_fast(sc[n][e] - top);
-                    l[e >> 1] += p[n][e];
-                    p[n][e] *= v_mul;
-                }
-            // P in the operands' type: 2^-9 (bf16) or 2^-12 (fp16) of itself,
-            // no more than rounding the output costs
-            const uint32_t pa[4] = {pack2(p[0][0], p[0][1], M{}), pack2(p[0][2], p[0][3], M{}),
-                                    pack2(p[1][0], p[1][1], M{}), pack2(p[1][2], p[1][3], M{})};
-            // a key that some rows of the tile see and others do not: zero
-            // times an infinity or NaN would reach the others
-            bool poison = false;
-            if (!whole) {
-                constexpr int kVecs = S::kUnitBytes / 16 / 32;
-#pragma unroll
-                for (int c = 0; c < kVecs; ++c) {
-                    uint32_t w[4];
-                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                 : "r"(v_at + (c * 32 + lane) * 16)
-                                 : "memory");
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) poison |= any_not_finite<T, kCodes>(w[e]);
-                }
-                poison |= kCodes && v_scale != v_scale;
-                poison = __any_sync(0xffffffffu, poison);
-            }
-            if (!poison) {
-                if constexpr (!kCodes) {
-#pragma unroll
-                    for (int n = 0; n < kTiles; n += 2) {
-                        uint32_t b[4];  // channels 8n.. and 8n + 8.., each keys 0-7 and 8-15
-                        ldsm4t(b, v_at + chunk_at<D, false>((lane & 7) + (((lane >> 3) & 1) << 3), n + (lane >> 4)));
-                        mma<M>(o[n], pa, b[0], b[1]);
-                        mma<M>(o[n + 1], pa, b[2], b[3]);
-                    }
+            for (int r = 0; r < 2; ++r) {
+                if constexpr (D == 32) {
+                    const uint32_t at = k_at + chunk_at<D, true>(g + 8 * r, t >> 1) + (t & 1) * 8;
+                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[r][0]), "=r"(w[r][1]) : "r"(at) : "memory");
                 } else {
 #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t w[4];  // channels 32 c + 4 g .. + 3 of keys 2t, 2t + 1, 2t + 8, 2t + 9
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t r = 2 * t + (e & 1) + 8 * (e >> 1);
-                            const uint32_t at = v_at + chunk_at<D, true>(r, 2 * c + (g >> 2)) + (g & 3) * 4;
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[e]) : "r"(at) : "memory");
-                        }
-#pragma unroll
-                        for (int j = 0; j < 4; j += 2) {
-                            const uint32_t sel = j == 0 ? 0x5140 : 0x7362;
-                            const uint32_t lo2 = __byte_perm(w[0], w[1], sel), hi2 = __byte_perm(w[2], w[3], sel);
-                            mma<M>(o[4 * c + j], pa, f16x2_from_e4m3x2(lo2), f16x2_from_e4m3x2(hi2));
-                            mma<M>(o[4 * c + j + 1], pa, f16x2_from_e4m3x2(lo2 >> 16), f16x2_from_e4m3x2(hi2 >> 16));
-                        }
-                    }
-                }
-            } else {
-                // one key after another, for the rows that see it
-#pragma unroll 1
-                for (int key_i = 0; key_i < kUnit; ++key_i) {
-#pragma unroll
-                    for (int i2 = 0; i2 < 2; ++i2) {
-                        const int from = g * 4 + (key_i & 7) / 2;
-                        float pk = 0.0f;
-                        bool sk = false;
-#pragma unroll
-                        for (int n = 0; n < 2; ++n)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const float x = __shfl_sync(0xffffffffu, p[n][2 * i2 + e], from);
-                                const bool y = __shfl_sync(0xffffffffu, seen[n][2 * i2 + e], from);
-                                if (n == key_i >> 3 && e == (key_i & 1)) {
-                                    pk = x;
-                                    sk = y;
-                                }
-                            }
-                        if (!sk) continue;
-#pragma unroll
-                        for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int ch = kCodes ? 32 * (n >> 2) + 8 * t + 4 * e + (n & 3) : 8 * n + 2 * t + e;
-                                o[n][2 * i2 + e] += pk * value_at<T, D, kCodes>(ring + slot * 2 * S::kUnitBytes +
-                                                                                     S::kUnitBytes, key_i, ch);
-                            }
+                    for (int c = 0; c < D / 64; ++c) {
+                        const uint32_t at = k_at + chunk_at<D, true>(g + 8 * r, 4 * c + t);
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                     : "=r"(w[r][4 * c]), "=r"(w[r][4 * c + 1]), "=r"(w[r][4 * c + 2]), "=r"(w[r][4 * c + 3])
+                                     : "r"(at)
+                                     : "memory");
                     }
                 }
             }
-            __syncwarp();
-            // refill: this slot's unit is done, the one kStages - 1 ahead goes to the slot before
-            const uint32_t next = i + S::kStages - 1;
-            const int to = (slot + S::kStages - 1) % S::kStages;
-            if (next < count) unit_pages[to] = load(next, to);
-            cp_commit();
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const uint32_t b[4] = {f16x2_from_e4m3x2(w[0][k]), f16x2_from_e4m3x2(w[1][k]),
+                                       f16x2_from_e4m3x2(w[0][k] >> 16), f16x2_from_e4m3x2(w[1][k] >> 16)};
+#pragma unroll
+                for (int n = 0; n < kQ; ++n) mma<M>(k & 1 ? odd[n] : sc[n], b, q[n][k][0], q[n][k][1]);
+            }
         }
+        // in units of log2, masked where a query does not see the key
+        const bool whole = page >= 0 && (key >= lo_max || key + kUnit <= sinks_end) && key + kUnit <= hi_min;
+        auto sees = [&](int n, int e) {
+            const uint32_t j = key + g + 8 * (e >> 1);
+            return page >= 0 && j < rr[n][e & 1].hi && (j >= rr[n][e & 1].lo || j < rr[n][e & 1].first);
+        };
+        bool above = false;
+#pragma unroll
+        for (int n = 0; n < kQ; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sc[n][e] = (sc[n][e] + odd[n][e]) * (k_scale * row_mul[n][e & 1]);
+                if (!whole && !sees(n, e)) sc[n][e] = -INFINITY;
+                above |= sc[n][e] > m[n][e & 1] + kRaise;
+            }
+        // the maximum moves only when a score passes it by kRaise: until
+        // then exp2(score - m) stays below 2^kRaise
+        if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+            for (int n = 0; n < kQ; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = fmaxf(sc[n][e], sc[n][e + 2]);
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    x = fmaxf(x, m[n][e]);
+                    const float down = m[n][e] == -INFINITY ? 0.0f : exp2_fast(m[n][e] - x);
+                    m[n][e] = x;
+                    l[n][e] *= down;
+#pragma unroll
+                    for (int d = 0; d < kSteps; ++d) {
+                        o[n][d][e] *= down;
+                        o[n][d][e + 2] *= down;
+                    }
+                }
+        }
+        float v_mul = 1.0f;
+        if constexpr (kCodes) {
+            if (v_scale > v_ref) {
+                const float down = v_ref / v_scale;
+#pragma unroll
+                for (int n = 0; n < kQ; ++n)
+#pragma unroll
+                    for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[n][d][e] *= down;
+                v_ref = v_scale;
+            }
+            v_mul = v_scale == v_ref ? 1.0f : v_scale == 0.0f ? 0.0f : v_scale / v_ref;
+        }
+        // P in the operands' type: 2^-9 (bf16) or 2^-12 (fp16) of itself,
+        // no more than rounding the output costs
+        float p[kQ][4];
+        uint32_t pb[kQ][2];
+#pragma unroll
+        for (int n = 0; n < kQ; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float top = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
+                p[n][e] = exp2_fast(sc[n][e] - top);
+                l[n][e & 1] += p[n][e];
+                if constexpr (kCodes) p[n][e] *= v_mul;
+            }
+            pb[n][0] = turn_over(pack2(p[n][0], p[n][1], M{}));
+            pb[n][1] = turn_over(pack2(p[n][2], p[n][3], M{}));
+        }
+        // a key that some rows of the tile see and others do not: zero
+        // times an infinity or NaN would reach the others
+        bool poison = false;
+        if (!whole) {
+            constexpr int kVecs = S::kUnitBytes / 16 / 32;
+#pragma unroll
+            for (int c = 0; c < kVecs; ++c) {
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                             : "r"(v_at + (c * 32 + lane) * 16)
+                             : "memory");
+#pragma unroll
+                for (int e = 0; e < 4; ++e) poison |= any_not_finite<T, kCodes>(w[e]);
+            }
+            poison |= kCodes && v_scale != v_scale;
+            poison = __any_sync(0xffffffffu, poison);
+        }
+        if (!poison) {
+            if constexpr (!kCodes) {
+#pragma unroll
+                for (int d = 0; d < kSteps; ++d) {
+                    uint32_t b[4];  // channels 0-7 and 8-15 of keys 0-7, then of keys 8-15
+                    ldsm4t(b, v_at + chunk_at<D, false>((lane & 7) + ((lane >> 4) << 3), 2 * d + ((lane >> 3) & 1)));
+#pragma unroll
+                    for (int n = 0; n < kQ; ++n) mma<M>(o[n][d], b, pb[n][0], pb[n][1]);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t w[4];  // channels 32 c + 4 g .. + 3 of keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t r = 2 * t + (e & 1) + 8 * (e >> 1);
+                        const uint32_t at = v_at + chunk_at<D, true>(r, 2 * c + (g >> 2)) + (g & 3) * 4;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[e]) : "r"(at) : "memory");
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t sel = j == 0 ? 0x5140 : 0x7362;
+                        const uint32_t lo2 = __byte_perm(w[0], w[1], sel), hi2 = __byte_perm(w[2], w[3], sel);
+                        const uint32_t b[4] = {f16x2_from_e4m3x2(lo2), f16x2_from_e4m3x2(lo2 >> 16),
+                                               f16x2_from_e4m3x2(hi2), f16x2_from_e4m3x2(hi2 >> 16)};
+#pragma unroll
+                        for (int n = 0; n < kQ; ++n) mma<M>(o[n][2 * c + j], b, pb[n][0], pb[n][1]);
+                    }
+                }
+            }
+        } else {
+            // one key after another, for the rows that see it
+#pragma unroll 1
+            for (int r = 0; r < kUnit; ++r) {
+                const uint32_t j = key + r;
+#pragma unroll
+                for (int n = 0; n < kQ; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float low = __shfl_sync(0xffffffffu, p[n][e], (r & 7) * 4 + t);
+                        const float high = __shfl_sync(0xffffffffu, p[n][e + 2], (r & 7) * 4 + t);
+                        const float pk = r < 8 ? low : high;
+                        if (!(page >= 0 && j < rr[n][e].hi && (j >= rr[n][e].lo || j < rr[n][e].first))) continue;
+#pragma unroll
+                        for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                                o[n][d][2 * x + e] += pk * value_at<T, D, kCodes>(ring + slot * 2 * S::kUnitBytes + S::kUnitBytes,
+                                                                                  r, channel(d, x));
+                    }
+            }
+        }
+        __syncwarp();
+        // this slot's unit is done: the one kStages - 1 ahead goes to the slot before it
+        const uint32_t next = i + S::kStages - 1;
+        if (next < count) load(next, slot == 0 ? S::kStages - 1 : slot - 1);
+        cp_commit();
+        if (++slot == S::kStages) slot = 0;
     }
     cp_wait<0>();
-    if constexpr (kCodes) {
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n)
+    for (int n = 0; n < kQ; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][e] *= v_ref;
-    }
-#pragma unroll
-    for (int i2 = 0; i2 < 2; ++i2) {
-        l[i2] += __shfl_xor_sync(0xffffffffu, l[i2], 1);
-        l[i2] += __shfl_xor_sync(0xffffffffu, l[i2], 2);
-    }
-    auto channel = [&](int n, int e) { return kCodes ? 32 * (n >> 2) + 8 * t + 4 * e + (n & 3) : 8 * n + 2 * t + e; };
+        for (int e = 0; e < 2; ++e) {
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+        }
 
     if constexpr (!kShared) {
         // the warp's own rows: through its ring to whole 16-byte stores
         __syncwarp();
-        T* part = reinterpret_cast<T*>(ring);
+        T* part = reinterpret_cast<T*>(smem + warp * (S::kRings / kWarps));
 #pragma unroll
-        for (int i2 = 0; i2 < 2; ++i2) {
-            const float inv = l[i2] == 0.0f ? 0.0f : 1.0f / l[i2];
+        for (int n = 0; n < kQ; ++n)
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n)
+            for (int e = 0; e < 2; ++e) {
+                const float inv = (l[n][e] == 0.0f ? 0.0f : 1.0f / l[n][e]) * (kCodes ? v_ref : 1.0f);
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    part[(g + 8 * i2) * D + channel(n, e)] = static_cast<T>(o[n][2 * i2 + e] * inv);
-        }
+                for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        part[(8 * n + 2 * t + e) * D + channel(d, x)] = static_cast<T>(o[n][d][2 * x + e] * inv);
+            }
         __syncwarp();
-        for (int x = lane; x < 16 * D / 8; x += 32) {
+        for (int x = lane; x < kRows * D / 8; x += 32) {
             const uint32_t R = row0 + x / (D / 8), c8 = 8 * (x % (D / 8));
             if (R >= rows) continue;
             const uint32_t tok = a.group_div.div(R), head = h * a.group + (R - tok * a.group);
@@ -497,32 +549,36 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a, u
         // join the warps, then the blocks of the cluster
         __syncthreads();  // every ring is done with
         float* parts = reinterpret_cast<float*>(smem);
-        float* mine = parts + warp * (S::kPartFloats + 32);
+        constexpr int kPart = S::kPartFloats + 2 * kRows;
+        float* mine = parts + warp * kPart;
 #pragma unroll
-        for (int i2 = 0; i2 < 2; ++i2) {
+        for (int n = 0; n < kQ; ++n)
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n)
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * n + 2 * t + e;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) mine[(g + 8 * i2) * D + channel(n, e)] = o[n][2 * i2 + e];
-            if (t == 0) {
-                mine[S::kPartFloats + g + 8 * i2] = m[i2];
-                mine[S::kPartFloats + 16 + g + 8 * i2] = l[i2];
+                for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        mine[r * S::kPitch + channel(d, x)] = o[n][d][2 * x + e] * (kCodes ? v_ref : 1.0f);
+                if (g == 0) {
+                    mine[S::kPartFloats + r] = m[n][e];
+                    mine[S::kPartFloats + kRows + r] = l[n][e];
+                }
             }
-        }
         if (split > 1) cg::this_cluster().sync();
         else __syncthreads();
         if (live) {
             // this block finishes every split-th vector of 4 channels
             const uint32_t stride = split * kThreads;
-            for (uint32_t x = rank * kThreads + threadIdx.x; x < 16 * D / 4; x += stride) {
+            for (uint32_t x = rank * kThreads + threadIdx.x; x < kRows * D / 4; x += stride) {
                 const uint32_t r = x / (D / 4), c4 = 4 * (x % (D / 4)), R = row0 + r;
                 if (R >= rows) continue;
                 float top = -INFINITY;
                 for (uint32_t b = 0; b < split; ++b) {
                     const float* p = split > 1 ? cg::this_cluster().map_shared_rank(parts, b) : parts;
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w)
-                        top = fmaxf(top, p[w * (S::kPartFloats + 32) + S::kPartFloats + r]);
+                    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, p[w * kPart + S::kPartFloats + r]);
                 }
                 float sum = 0.0f;
                 float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -530,12 +586,11 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a, u
                     const float* p = split > 1 ? cg::this_cluster().map_shared_rank(parts, b) : parts;
 #pragma unroll
                     for (int w = 0; w < kWarps; ++w) {
-                        const float* pw = p + w * (S::kPartFloats + 32);
-                        const float mw = pw[S::kPartFloats + r];
-                        const float lw = pw[S::kPartFloats + 16 + r];
+                        const float* pw = p + w * kPart;
+                        const float mw = pw[S::kPartFloats + r], lw = pw[S::kPartFloats + kRows + r];
                         if (lw == 0.0f) continue;  // saw nothing
                         const float f = exp2_fast(mw - top);
-                        const float4 ov = *reinterpret_cast<const float4*>(pw + r * D + c4);
+                        const float4 ov = *reinterpret_cast<const float4*>(pw + r * S::kPitch + c4);
                         sum += lw * f;
                         acc.x += ov.x * f;
                         acc.y += ov.y * f;
@@ -553,31 +608,31 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a, u
     }
 }
 
-template <typename T, int D, bool kCodes> cudaError_t launch(const CacheAttnArgs& a, cudaStream_t s) {
-    using S = Shape<D, kCodes>;
-    const uint32_t tiles = (a.c.max_new * a.group + 15) / 16;
+template <typename T, int D, bool kCodes, int kRows> cudaError_t launch(CacheAttnArgs a, cudaStream_t s) {
+    const uint32_t tiles = (a.c.max_new * a.group + kRows - 1) / kRows;
     const uint64_t jobs = static_cast<uint64_t>(a.c.sequences) * a.c.kv_heads * tiles;
+    a.tile_div = FastDiv(tiles);
+    a.kv_div = FastDiv(a.c.kv_heads);
     // keys a row can see
     uint64_t span = a.c.max_length ? a.c.max_length : static_cast<uint64_t>(a.c.table_stride) << a.c.page_shift;
     if (a.window) span = min(span, static_cast<uint64_t>(a.window) * a.frame + a.sinks + a.c.max_new);
     const uint64_t units = (span + kUnit - 1) / kUnit;
-    auto set = [](auto* kernel) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        return e;
-    };
     if (units <= 8 && jobs >= 148 * 4) {
-        const cudaError_t e = set(cache_attn_kernel<T, D, kCodes, false>);
+        using S = Shape<D, kCodes, kRows, false>;
+        auto* kernel = cache_attn_kernel<T, D, kCodes, kRows, false>;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
         if (e != cudaSuccess) return e;
-        cache_attn_kernel<T, D, kCodes, false>
-            <<<static_cast<uint32_t>((jobs + kWarps - 1) / kWarps), kThreads, S::kBytes, s>>>(a, tiles, 1);
+        kernel<<<static_cast<uint32_t>((jobs + kWarps - 1) / kWarps), kThreads, S::kBytes, s>>>(a, tiles, 1);
         return cudaGetLastError();
     }
-    // blocks for two a SM, at least four units a warp
+    // as many blocks a job as fit the GPU at once, at least four units a warp
+    using S = Shape<D, kCodes, kRows, true>;
     uint32_t split = 1;
-    while (split < kMaxSplit && jobs * split < 148 * 2 && units >= static_cast<uint64_t>(split) * 2 * kWarps * 4)
+    while (split < kMaxSplit && jobs * split * 2 <= 148 * S::kBlocks && units >= static_cast<uint64_t>(split) * 2 * kWarps * 4)
         split *= 2;
-    cudaError_t e = set(cache_attn_kernel<T, D, kCodes, true>);
+    auto* kernel = cache_attn_kernel<T, D, kCodes, kRows, true>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<uint32_t>(jobs * split));
@@ -590,14 +645,18 @@ template <typename T, int D, bool kCodes> cudaError_t launch(const CacheAttnArgs
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = split > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, cache_attn_kernel<T, D, kCodes, true>, a, tiles, split);
+    return cudaLaunchKernelEx(&cfg, kernel, a, tiles, split);
+}
+
+template <typename T, int D, bool kCodes> cudaError_t by_rows(const CacheAttnArgs& a, cudaStream_t s) {
+    return a.c.max_new * a.group <= 8 ? launch<T, D, kCodes, 8>(a, s) : launch<T, D, kCodes, 16>(a, s);
 }
 
 template <typename T, bool kCodes> cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t s) {
     switch (a.c.head_dim) {
-        case 32: return launch<T, 32, kCodes>(a, s);
-        case 64: return launch<T, 64, kCodes>(a, s);
-        default: return launch<T, 128, kCodes>(a, s);
+        case 32: return by_rows<T, 32, kCodes>(a, s);
+        case 64: return by_rows<T, 64, kCodes>(a, s);
+        default: return by_rows<T, 128, kCodes>(a, s);
     }
 }
 

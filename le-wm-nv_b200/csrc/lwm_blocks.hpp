@@ -90,6 +90,7 @@ struct CacheAttnArgs {
     int causal;
     uint32_t window, sinks, frame;
     FastDiv group_div, frame_div;
+    FastDiv tile_div, kv_div;  // set by the launch
 };
 // Few query rows a kv head (any head width), and many (head_dim 64 or 128).
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
