@@ -9,7 +9,9 @@
 // of a block and, for long contexts, to the blocks of a cluster; their
 // (maximum, sum, O) are joined in shared memory and over distributed shared
 // memory, so a call needs no workspace and no second kernel and its sums have
-// one order.  Where contexts are short and jobs many, a warp has a job alone.
+// one order.  Where contexts are short and jobs many, a warp has some heads of a
+// sequence alone, their units one stream through its ring: the sequence's
+// lengths and pages are looked up once and no head waits for its first load.
 //
 // Bound: memory (each K and V byte is used by at most 16 rows, 32 flops a
 // byte).  Every warp keeps its own ring of units in flight with cp.async, so
@@ -35,7 +37,6 @@ namespace cg = cooperative_groups;
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kUnit = 16;    // keys a step
-constexpr int kMaxSplit = 16;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
     // a dead row's 16 bytes are filled with zeros, its address is not read
@@ -111,13 +112,14 @@ __device__ __forceinline__ float value_at(const uint8_t* unit, uint32_t key, uin
 // kRows: query rows of a job, 8 or 16.
 template <int D, bool kCodes, int kRows, bool kShared> struct Shape {
     static constexpr int kUnitBytes = kUnit * D * (kCodes ? 1 : 2);  // of K, and of V
-    static constexpr int kStages = kShared ? 3 : 2;
+    static constexpr int kStages = 3;
     static constexpr int kWarpBytes = kStages * 2 * kUnitBytes;
     static constexpr int kPitch = D + 4;                             // floats of a row of O in shared memory
     static constexpr int kPartFloats = kRows * kPitch;               // a warp's O
-    static constexpr int kPartBytes = kShared ? (kPartFloats + 2 * kRows) * 4 : kRows * D * 2;  // maxima and sums too
+    static constexpr int kPartBytes = kShared ? (kPartFloats + 2 * kRows) * 4 : 0;  // maxima and sums too
     static constexpr int kRings = kWarps * (kWarpBytes > kPartBytes ? kWarpBytes : kPartBytes);
-    static constexpr int kBytes = kRings + kWarps * kStages * 16;    // and the units' pages and scales
+    // and the units' pages and scales; alone, a warp's output rows
+    static constexpr int kBytes = kRings + kWarps * kStages * 16 + (kShared ? 0 : kWarps * kRows * D * 2);
     // blocks a SM, by shared memory and registers
     static constexpr int kBySmem = 220 * 1024 / (kBytes + 1024), kByRegs = kRows == 8 ? (D == 128 ? 4 : 5) : (D == 128 ? 3 : 4);
     static constexpr int kBlocks = kBySmem < kByRegs ? kBySmem : kByRegs;
@@ -140,10 +142,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
     constexpr int kSteps = D / 16, kQ = kRows / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    // job: four warps (and `split` blocks) share one, or a warp has its own
+    // job: four warps (and `split` blocks) share one head's, or a warp has `split` heads' (the last: fewer)
     const uint32_t rank = kShared ? blockIdx.x % split : 0;
     const uint32_t job = kShared ? blockIdx.x / split : blockIdx.x * kWarps + warp;
-    const uint32_t hs = a.tile_div.div(job), tile = job - hs * tiles, s = a.kv_div.div(hs), h = hs - s * a.c.kv_heads;
+    const uint32_t hs = a.tile_div.div(job), tile = job - hs * tiles, s = a.kv_div.div(hs);
+    const uint32_t h0 = (hs - s * a.kv_div.d) * (kShared ? 1 : split);
+    const uint32_t h_end = kShared ? h0 + 1 : min(h0 + split, a.c.kv_heads);
     // a short table's row comes along with the lengths
     int entry = -1;
     const bool small_table = !kShared && a.c.table_stride <= 32;
@@ -151,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
     if (s < a.c.sequences) {
         if (small_table && lane < a.c.table_stride)
             entry = a.c.table[static_cast<size_t>(s) * a.c.table_stride + lane];
-        v = sequence(a.c, s, false, h == 0 && tile == 0 && rank == 0 && lane == 0);
+        v = sequence(a.c, s, false, h0 == 0 && tile == 0 && rank == 0 && lane == 0);
     }
     const uint32_t rows = v.n * a.group, row0 = tile * kRows;
     const bool live = row0 < rows;
@@ -177,6 +181,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         lo_min = r0.lo, hi_min = r0.hi;
         lo_max = r1.lo, hi_max = r1.hi;
     }
+    const bool mixed = lo_min != lo_max || hi_min != hi_max;  // rows that differ in what they see
     const uint32_t sinks_end = min(a.sinks, min(lo_min, hi_max));
     const uint32_t sink_units = (sinks_end + kUnit - 1) / kUnit;
     const uint32_t win_unit = max(lo_min / kUnit, sink_units);
@@ -208,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         return __shfl_sync(0xffffffffu, pages_ahead, i & 31);
     };
     UnitNote* notes = reinterpret_cast<UnitNote*>(smem + S::kRings) + warp * S::kStages;
-    auto load = [&](uint32_t i, uint32_t slot) {
+    auto load = [&](uint32_t h, uint32_t i, uint32_t slot) {
         const int page = page_at(i);
         const uint32_t key = key_of(i);
         constexpr int kRowChunks = S::kUnitBytes / kUnit / 16;
@@ -235,66 +240,88 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
             cp_async16(dst + S::kUnitBytes + chunk_at<D, kCodes>(r, ch), vp + c * 512, ok);
         }
     };
-#pragma unroll 1
-    for (uint32_t i = 0; i < S::kStages - 1; ++i) {
-        if (i < count) load(i, i);
+    // the next unit of the stream: of this head, then of the next one
+    uint32_t load_h = count ? h0 : h_end, load_i = 0;
+    auto load_next = [&](uint32_t slot) {
+        if (load_h < h_end) {
+            load(load_h, load_i, slot);
+            if (++load_i == count) load_i = 0, ++load_h;
+        }
         cp_commit();
-    }
+    };
+#pragma unroll 1
+    for (uint32_t i = 0; i < S::kStages - 1; ++i) load_next(i);
 
-    // queries 8 n + g, in the order of the contraction
+    // queries 8 n + g as they lie, in the order of the contraction
+    auto fetch_q = [&](uint32_t h, uint32_t(&raw)[kQ][kSteps][2]) {
+#pragma unroll
+        for (int n = 0; n < kQ; ++n) {
+            const uint32_t R = row0 + 8 * n + g;
+            const T* qr = nullptr;
+            if (live && R < rows) {
+                const uint32_t tok = a.group_div.div(R);
+                qr = static_cast<const T*>(a.q) + (v.start + tok) * a.q_ts + (h * a.group + (R - tok * a.group)) * a.q_hs;
+            }
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                if constexpr (!kCodes) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        raw[n][k][i] = qr ? *reinterpret_cast<const uint32_t*>(qr + 16 * k + 8 * i + 2 * t) : 0u;
+                } else {
+                    constexpr int kRun = D >= 64 ? 16 : 8;  // channels a thread reads of each 4 * kRun
+                    const int ch = (k / (kRun / 4)) * 4 * kRun + t * kRun + (k % (kRun / 4)) * 4;
+                    uint2 w = make_uint2(0, 0);
+                    if (qr) w = *reinterpret_cast<const uint2*>(qr + ch);
+                    raw[n][k][0] = w.x;
+                    raw[n][k][1] = w.y;
+                }
+            }
+        }
+    };
+    uint32_t raw[kQ][kSteps][2];
+    fetch_q(h0, raw);
+    uint32_t slot = 0;
+    auto channel = [&](int d, int half) {  // of row g + 8 half of channel tile d
+        return kCodes ? 32 * (d >> 1) + 4 * g + 2 * (d & 1) + half : 16 * d + 8 * half + g;
+    };
+
+#pragma unroll 1
+    for (uint32_t h = h0; h < h_end; ++h) {
     uint32_t q[kQ][kSteps][2];
     float row_mul[kQ][2];  // of queries 8 n + 2 t + e
 #pragma unroll
     for (int n = 0; n < kQ; ++n) {
-        const uint32_t R = row0 + 8 * n + g;
-        const T* qr = nullptr;
-        if (live && R < rows) {
-            const uint32_t tok = a.group_div.div(R);
-            qr = static_cast<const T*>(a.q) + (v.start + tok) * a.q_ts + (h * a.group + (R - tok * a.group)) * a.q_hs;
-        }
         row_mul[n][0] = row_mul[n][1] = a.scale_log2;
-        if constexpr (!kCodes) {
+        if constexpr (!(kCodes && std::is_same_v<T, bf16>)) {
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) q[n][k][0] = raw[n][k][0], q[n][k][1] = raw[n][k][1];
+        } else {
+            float amax = 0.0f;
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    q[n][k][i] = qr ? *reinterpret_cast<const uint32_t*>(qr + 16 * k + 8 * i + 2 * t) : 0u;
-        } else {
-            constexpr int kRun = D >= 64 ? 16 : 8;  // channels a thread reads of each 4 * kRun
-            float f[kSteps][4], amax = 0.0f;
+                    amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(raw[n][k][i] << 16)),
+                                             fabsf(__uint_as_float(raw[n][k][i] & 0xffff0000u))));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+            if (amax == 0.0f || e == 128) e = 0;
+            e = min(max(e, -126), 126);
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                const int ch = (k / (kRun / 4)) * 4 * kRun + t * kRun + (k % (kRun / 4)) * 4;
-                uint2 w = make_uint2(0, 0);
-                if (qr) w = *reinterpret_cast<const uint2*>(qr + ch);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint16_t x = static_cast<uint16_t>((e < 2 ? w.x : w.y) >> (16 * (e & 1)));
-                    f[k][e] = static_cast<float>(*reinterpret_cast<const T*>(&x));
-                    amax = fmaxf(amax, fabsf(f[k][e]));
-                }
-            }
-            if constexpr (std::is_same_v<T, bf16>) {
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-                if (amax == 0.0f || e == 128) e = 0;
-                e = min(max(e, -126), 126);
-                const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) row_mul[n][i] *= __shfl_sync(0xffffffffu, up, (2 * t + i) * 4);
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) f[k][x] *= down;
-            }
+            for (int i = 0; i < 2; ++i) row_mul[n][i] *= __shfl_sync(0xffffffffu, up, (2 * t + i) * 4);
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) q[n][k][i] = pack2(f[k][2 * i], f[k][2 * i + 1], __half{});
+                for (int i = 0; i < 2; ++i)
+                    q[n][k][i] = pack2(__uint_as_float(raw[n][k][i] << 16) * down,
+                                       __uint_as_float(raw[n][k][i] & 0xffff0000u) * down, __half{});
         }
     }
+    if (!kShared && h + 1 < h_end) fetch_q(h + 1, raw);
 
     // O^T: tile n of queries, tile d of channels; element i is query 2 t + (i & 1), channel of row g + 8 (i >> 1)
     float o[kQ][kSteps][4];
@@ -309,12 +336,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
             for (int e = 0; e < 4; ++e) o[n][d][e] = 0.0f;
     }
     float v_ref = 0.0f;  // 8 bits: O is in units of this value scale
-    auto channel = [&](int d, int half) {  // of row g + 8 half of channel tile d
-        return kCodes ? 32 * (d >> 1) + 4 * g + 2 * (d & 1) + half : 16 * d + 8 * half + g;
-    };
 
     // (not unrolled over the ring: copies of the body missed the instruction cache)
-    uint32_t slot = 0;
 #pragma unroll 1
     for (uint32_t i = 0; i < count; ++i) {
         cp_wait<S::kStages - 2>();
@@ -397,6 +420,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
                     x = fmaxf(x, m[n][e]);
                     const float down = m[n][e] == -INFINITY ? 0.0f : exp2_fast(m[n][e] - x);
                     m[n][e] = x;
+                    if (i == 0) continue;
                     l[n][e] *= down;
 #pragma unroll
                     for (int d = 0; d < kSteps; ++d) {
@@ -407,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         }
         float v_mul = 1.0f;
         if constexpr (kCodes) {
+            if (i == 0 && v_scale > 0.0f) v_ref = v_scale;
             if (v_scale > v_ref) {
                 const float down = v_ref / v_scale;
 #pragma unroll
@@ -438,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         // a key that some rows of the tile see and others do not: zero
         // times an infinity or NaN would reach the others
         bool poison = false;
-        if (!whole) {
+        if (!whole && mixed) {
             constexpr int kVecs = S::kUnitBytes / 16 / 32;
 #pragma unroll
             for (int c = 0; c < kVecs; ++c) {
@@ -507,12 +532,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         }
         __syncwarp();
         // this slot's unit is done: the one kStages - 1 ahead goes to the slot before it
-        const uint32_t next = i + S::kStages - 1;
-        if (next < count) load(next, slot == 0 ? S::kStages - 1 : slot - 1);
-        cp_commit();
+        load_next(slot == 0 ? S::kStages - 1 : slot - 1);
         if (++slot == S::kStages) slot = 0;
     }
-    cp_wait<0>();
 #pragma unroll
     for (int n = 0; n < kQ; ++n)
 #pragma unroll
@@ -523,9 +545,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         }
 
     if constexpr (!kShared) {
-        // the warp's own rows: through its ring to whole 16-byte stores
-        __syncwarp();
-        T* part = reinterpret_cast<T*>(smem + warp * (S::kRings / kWarps));
+        // the warp's own rows: through shared memory to whole 16-byte stores
+        T* part = reinterpret_cast<T*>(smem + S::kRings + kWarps * S::kStages * 16 + warp * kRows * D * 2);
 #pragma unroll
         for (int n = 0; n < kQ; ++n)
 #pragma unroll
@@ -545,8 +566,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
             store8(static_cast<T*>(a.out) + (v.start + tok) * a.o_ts + head * a.o_hs + c8,
                    *reinterpret_cast<const Vec8<T>*>(part + x * 8));
         }
+        __syncwarp();  // the next head's rows go there
     } else {
         // join the warps, then the blocks of the cluster
+        cp_wait<0>();
         __syncthreads();  // every ring is done with
         float* parts = reinterpret_cast<float*>(smem);
         constexpr int kPart = S::kPartFloats + 2 * kRows;
@@ -606,30 +629,37 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         }
         if (split > 1) cg::this_cluster().sync();  // a block's parts stay until all have read them
     }
+    }
 }
 
 template <typename T, int D, bool kCodes, int kRows> cudaError_t launch(CacheAttnArgs a, cudaStream_t s) {
     const uint32_t tiles = (a.c.max_new * a.group + kRows - 1) / kRows;
     const uint64_t jobs = static_cast<uint64_t>(a.c.sequences) * a.c.kv_heads * tiles;
     a.tile_div = FastDiv(tiles);
-    a.kv_div = FastDiv(a.c.kv_heads);
     // keys a row can see
     uint64_t span = a.c.max_length ? a.c.max_length : static_cast<uint64_t>(a.c.table_stride) << a.c.page_shift;
     if (a.window) span = min(span, static_cast<uint64_t>(a.window) * a.frame + a.sinks + a.c.max_new);
     const uint64_t units = (span + kUnit - 1) / kUnit;
     if (units <= 8 && jobs >= 148 * 4) {
         using S = Shape<D, kCodes, kRows, false>;
+        // the heads in as many parts as run at once, evenly
+        const uint64_t lots = static_cast<uint64_t>(a.c.sequences) * tiles, slots = 148 * kWarps * S::kBlocks;
+        uint32_t parts = static_cast<uint32_t>(min(uint64_t{a.c.kv_heads}, max(uint64_t{1}, slots / lots)));
+        const uint32_t heads = (a.c.kv_heads + parts - 1) / parts;
+        parts = (a.c.kv_heads + heads - 1) / heads;
+        a.kv_div = FastDiv(parts);
         auto* kernel = cache_attn_kernel<T, D, kCodes, kRows, false>;
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
         if (e != cudaSuccess) return e;
-        kernel<<<static_cast<uint32_t>((jobs + kWarps - 1) / kWarps), kThreads, S::kBytes, s>>>(a, tiles, 1);
+        const uint64_t warps = lots * parts;
+        kernel<<<static_cast<uint32_t>((warps + kWarps - 1) / kWarps), kThreads, S::kBytes, s>>>(a, tiles, heads);
         return cudaGetLastError();
     }
-    // as many blocks a job as fit the GPU at once, at least four units a warp
+    // as many blocks a job as fit the GPU at once (above 8: 16, a cluster of a whole GPC), at least four units a warp
     using S = Shape<D, kCodes, kRows, true>;
-    uint32_t split = 1;
-    while (split < kMaxSplit && jobs * split * 2 <= 148 * S::kBlocks && units >= static_cast<uint64_t>(split) * 2 * kWarps * 4)
-        split *= 2;
+    a.kv_div = FastDiv(a.c.kv_heads);
+    const uint64_t fit = min(static_cast<uint64_t>(148 * S::kBlocks) / max(jobs, uint64_t{1}), units / (kWarps * 4));
+    const uint32_t split = fit >= 16 ? 16 : fit > 8 ? 8 : fit > 1 ? static_cast<uint32_t>(fit) : 1;
     auto* kernel = cache_attn_kernel<T, D, kCodes, kRows, true>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
