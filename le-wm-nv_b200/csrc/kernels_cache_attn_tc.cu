@@ -24,8 +24,9 @@
 // Producers (a warpgroup): a tile that every row sees comes by TMA, a box of
 // 64 channels for each page; the few tiles at the edges of the masks are
 // gathered row by row with cp.async, rows that no query sees as zeros.
-// 8-bit codes are loaded a tile ahead into registers and become halves
-// (exact) on the way to shared memory.  Their scales stay out of the products: a page's key
+// 8-bit codes are copied tiles ahead (four for 64 channels; shared memory has
+// room for one of 128) and become halves (exact) on the way to the operands;
+// each thread expands what it copied itself.  Their scales stay out of the products: a page's key
 // scale multiplies its 16-key groups' scores, its value scale, relative to
 // the block's largest, enters the exponent of the weight.
 //
@@ -60,6 +61,12 @@ struct TileInfo {
     uint32_t pad[7];
 };
 
+// A tile of codes in flight, by 16-key groups, a copy for each producer warp.
+struct TileNotes {
+    int page[8];
+    float k_scale[8], v_scale[8];
+};
+
 struct Control {
     uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_half[2], o_done[2], info_full[kInfos], drain;
     uint32_t tmem;
@@ -73,8 +80,11 @@ struct Control {
 template <int D, bool kCodes> struct Shape {
     static constexpr int kPanels = D / 64;
     static constexpr int kTileBytes = kPanels * kPanel;
-    static constexpr int kQ = 0, kK = 2 * kTileBytes, kV = kK + 2 * kTileBytes, kControl = kV + 2 * kTileBytes;
-    static constexpr int kBytes = kControl + static_cast<int>(sizeof(Control)) + 1024;  // + alignment
+    static constexpr int kRaw = kCodes ? (D == 64 ? 4 : 1) : 0;      // tiles of codes in flight
+    static constexpr int kRawBytes = kTile * D;                     // of K, and of V
+    static constexpr int kQ = 0, kK = 2 * kTileBytes, kV = kK + 2 * kTileBytes, kCodesAt = kV + 2 * kTileBytes;
+    static constexpr int kControl = kCodesAt + kRaw * 2 * kRawBytes, kNotes = kControl + static_cast<int>(sizeof(Control));
+    static constexpr int kBytes = kNotes + (kCodes ? 4 * (kRaw + 1) * static_cast<int>(sizeof(TileNotes)) : 0) + 1024;  // + alignment
 };
 
 // Called by whole warps; the answer is the warp's, so that its lanes stay together.
@@ -168,6 +178,10 @@ __device__ __forceinline__ uint32_t below(uint32_t end, uint32_t k32) {
     return end <= k32 ? 0u : end - k32 >= 32 ? 0xffffffffu : (1u << (end - k32)) - 1u;
 }
 
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(dst)), "l"(src) : "memory");
+}
+
 // 64 channels of the rows of a box to shared memory (no multicast).
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int channel, int row, int page, uint64_t* bar) {
     asm volatile(
@@ -232,25 +246,35 @@ __device__ __forceinline__ float weights(const float (&x)[64], uint32_t (&p)[32]
         const int group = 4 * half + g;
         const float gm = kCodes ? info.k_scale[group] * mul : mul;
         const float add = kCodes ? sub + info.v_log[group] : sub;
-        uint32_t seen = 0;
+        uint32_t seen = 0xffffu;
         if constexpr (kMasked) {
+            // (rows of a warp mostly see all or none of 16 keys: a frame's rows see alike)
             const uint32_t k16 = key + 16 * group;
-            seen = (ok >> group) & 1 ? below(rr.hi, k16) & (~below(rr.lo, k16) | below(rr.first, k16)) : 0u;
+            seen = (ok >> group) & 1 ? below(rr.hi, k16) & (~below(rr.lo, k16) | below(rr.first, k16)) & 0xffffu : 0u;
+            if (__all_sync(0xffffffffu, seen == 0)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[8 * g + e] = 0u;
+                continue;
+            }
         }
         float2 part = make_float2(0.0f, 0.0f);
+        auto weigh = [&](auto masked) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            float2 y = fma2(make_float2(x[16 * g + e], x[16 * g + e + 1]), make_float2(gm, gm), make_float2(add, add));
-            if constexpr (kMasked) {
-                if (!((seen >> e) & 1)) y.x = -INFINITY;
-                if (!((seen >> (e + 1)) & 1)) y.y = -INFINITY;
+            for (int e = 0; e < 16; e += 2) {
+                float2 y = fma2(make_float2(x[16 * g + e], x[16 * g + e + 1]), make_float2(gm, gm), make_float2(add, add));
+                if constexpr (decltype(masked)::value) {
+                    if (!((seen >> e) & 1)) y.x = -INFINITY;
+                    if (!((seen >> (e + 1)) & 1)) y.y = -INFINITY;
+                }
+                if (e & 2) top1 = max3(top1, y.x, y.y);
+                else top0 = max3(top0, y.x, y.y);
+                y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                part = add2(part, y);
+                p[8 * g + e / 2] = pack2(y.x, y.y, M{});
             }
-            if (e & 2) top1 = max3(top1, y.x, y.y);
-            else top0 = max3(top0, y.x, y.y);
-            y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-            part = add2(part, y);
-            p[8 * g + e / 2] = pack2(y.x, y.y, M{});
-        }
+        };
+        if (!kMasked || __all_sync(0xffffffffu, seen == 0xffffu)) weigh(std::false_type{});
+        else weigh(std::true_type{});
         if constexpr (kCodes) sum = fma2(part, make_float2(info.v_inv[group], info.v_inv[group]), sum);
         else sum = add2(sum, part);
     }
@@ -307,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp < 8) {
         // ---------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kCodes ? 168 : 192));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(192));
         const int tile = warp >> 2, r = threadIdx.x & 127;
         const uint32_t R = row0 + tile * kTile + r;
         if (tile == 0 || two) {
@@ -498,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp < 12) {
         // -------------------------------------------------------- producers
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCodes ? 120 : 72));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(72));
         const int t = threadIdx.x - 256;
         constexpr int kRowChunks = kCodes ? D / 16 : D / 8;  // 16-byte chunks of a cached row
         constexpr int kEach = kTile * kRowChunks / kProducers, kRowStep = kProducers / kRowChunks;
@@ -517,40 +541,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             return static_cast<const uint8_t*>(pool) +
                    (pool_at(a.c, page < 0 ? 0 : page, h, j & (a.c.page_tokens - 1)) * kElem + ch * 16);
         };
-        if constexpr (kCodes) {
-            // the largest value scale of the visible pages
-            float top = 0.0f;
-            for (uint32_t i = t; i < w.tiles * 8; i += kProducers) {
-                const uint32_t j = w.key0(i / 8) + 16 * (i % 8);
-                if (j < w.hi_max && (j + 16 > w.lo_min || j < w.sinks_end)) {
-                    const int p = a.c.table[static_cast<size_t>(s) * a.c.table_stride + (j >> a.c.page_shift)];
-                    if (static_cast<uint32_t>(p) < a.c.pages) {
-                        const float x = a.c.v_scale[static_cast<size_t>(p) * a.c.kv_heads + h];
-                        if (isfinite(x)) top = fmaxf(top, x);
-                    }
+        bool fine = true;
+        int pages = kCodes ? -1 : page_ids(0);
+        // codes in flight: this thread's chunks, and its warp's notes of the tiles
+        TileNotes* notes = reinterpret_cast<TileNotes*>(smem + S::kNotes) + (warp - 8) * (S::kRaw + 1);
+        uint8_t* raw = smem + S::kCodesAt + t * 16;
+        auto note_of = [&](uint32_t i) -> TileNotes& { return notes[i % (S::kRaw + 1)]; };
+        auto copy_notes = [&](uint32_t i) {
+            const int p = page_ids(i);
+            TileNotes& n = note_of(i);
+            if (lane < 8) {
+                n.page[lane] = p;
+                if (p >= 0) {
+                    const size_t at = static_cast<size_t>(p) * a.c.kv_heads + h;
+                    cp_async4(&n.k_scale[lane], a.c.k_scale + at);
+                    cp_async4(&n.v_scale[lane], a.c.v_scale + at);
                 }
             }
+            __syncwarp();
+        };
+        auto copy_codes = [&](uint32_t i, const void* pool, int which) {
+            const TileNotes& n = note_of(i);
+            const uint32_t dst = tc::smem_u32(raw) + ((i % max(S::kRaw, 1)) * 2 + which) * S::kRawBytes;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (lane == 0) ctl->reduce[warp - 8] = top;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            top = fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]), fmaxf(ctl->reduce[2], ctl->reduce[3]));
-            if (top == 0.0f) top = 1.0f;
-            if (t == 0) ctl->v_ref = top;
-        }
-        const float v_ref_inv = kCodes ? 1.0f / fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]),
-                                                      fmaxf(ctl->reduce[2], ctl->reduce[3]))
-                                       : 1.0f;
-        bool fine = true;
-        int pages = page_ids(0);
-        uint4 kc[kCodes ? kEach : 1], vc[kCodes ? kEach : 1];
-        auto fetch = [&](uint4(&to)[kCodes ? kEach : 1], const void* pool, uint32_t i, int ids) {
-#pragma unroll
-            for (int c = 0; c < (kCodes ? kEach : 1); ++c) {
+            for (int c = 0; c < (kCodes ? kEach : 0); ++c) {
                 const uint32_t r = r0 + c * kRowStep, j = w.key0(i) + r;
-                const int page = __shfl_sync(0xffffffffu, ids, r >> 4);
-                to[c] = make_uint4(0, 0, 0, 0);
-                if (page >= 0 && row_live(j)) to[c] = *reinterpret_cast<const uint4*>(source(pool, page, j));
+                const int page = n.page[r >> 4];
+                cp_async16(dst + c * kProducers * 16, source(pool, page, j), page >= 0 && row_live(j));
             }
         };
         // 16 codes to two chunks of halves; NaN codes of a mixed tile are taken out
@@ -576,59 +593,87 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<uint4*>(row + ((((c0 + 1) & 7) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
         };
         if constexpr (kCodes) {
-            if (w.tiles) {
-                fetch(kc, a.c.k, 0, pages);
-                fetch(vc, a.c.v, 0, pages);
+#pragma unroll 1
+            for (uint32_t i = 0; i < S::kRaw; ++i) {
+                if (i < w.tiles) copy_notes(i), copy_codes(i, a.c.k, 0);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (i < w.tiles) copy_codes(i, a.c.v, 1);
+                asm volatile("cp.async.commit_group;" ::: "memory");
             }
         }
+        if constexpr (kCodes) {
+            // the largest value scale of the visible pages
+            float top = 0.0f;
+            for (uint32_t i = t; i < w.tiles * 8; i += kProducers) {
+                const uint32_t j = w.key0(i / 8) + 16 * (i % 8);
+                if (j < w.hi_max && (j + 16 > w.lo_min || j < w.sinks_end)) {
+                    const int p = a.c.table[static_cast<size_t>(s) * a.c.table_stride + (j >> a.c.page_shift)];
+                    if (static_cast<uint32_t>(p) < a.c.pages) {
+                        const float x = a.c.v_scale[static_cast<size_t>(p) * a.c.kv_heads + h];
+                        if (isfinite(x)) top = fmaxf(top, x);
+                    }
+                }
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (lane == 0) ctl->reduce[warp - 8] = top;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            top = fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]), fmaxf(ctl->reduce[2], ctl->reduce[3]));
+            if (top == 0.0f) top = 1.0f;
+            if (t == 0) ctl->v_ref = top;
+        }
+        const float v_ref_inv = kCodes ? 1.0f / fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]),
+                                                      fmaxf(ctl->reduce[2], ctl->reduce[3]))
+                                       : 1.0f;
         for (uint32_t i = 0; i < w.tiles && fine; ++i) {
             const uint32_t st = i & 1, use = (i >> 1) & 1, key = w.key0(i);
             const bool mixed = !w.whole(key);
-            const int next_pages = page_ids(i + 1);
+            const int next_pages = kCodes ? -1 : page_ids(i + 1);
+            if constexpr (kCodes) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(2 * S::kRaw - 1) : "memory");  // K of this tile
+                __syncwarp();
+                pages = lane < 8 ? note_of(i).page[lane] : -1;
+            }
             uint8_t* kd = smem + S::kK + st * S::kTileBytes;
             uint8_t* vd = smem + S::kV + st * S::kTileBytes;
             if (i >= 2 && !wait(&ctl->k_empty[st], use ^ 1, ctl, 20, err, s)) { fine = false; break; }
             // what the softmax needs to know; the ring is four tiles deep, the stages two
-            float v_scale = 1.0f;
-            if (lane < 8) {
+            if (warp == 8 && lane < 8) {
                 TileInfo& info = ctl->info[i % kInfos];
-                if (warp == 8) {
-                    if constexpr (kCodes) {
-                        float ks = 1.0f;
-                        if (pages >= 0) {
-                            const size_t at = static_cast<size_t>(pages) * a.c.kv_heads + h;
-                            ks = a.c.k_scale[at];
-                            v_scale = a.c.v_scale[at];
-                        }
-                        float ratio = isfinite(v_scale) && pages >= 0 ? v_scale * v_ref_inv : 1.0f;
-                        ratio = fmaxf(ratio, 0x1p-60f);  // halves of such weights are zero
-                        info.k_scale[lane] = ks;
-                        info.v_log[lane] = log2f(ratio);
-                        info.v_inv[lane] = 1.0f / ratio;
-                    }
-                    const uint32_t ok = __ballot_sync(0xffu, pages >= 0);
-                    if (lane == 0) info.ok = ok;
-                    tc::mbar_arrive(&ctl->info_full[i % kInfos]);
-                } else if constexpr (kCodes) {
-                    if (pages >= 0) v_scale = a.c.v_scale[static_cast<size_t>(pages) * a.c.kv_heads + h];
+                if constexpr (kCodes) {
+                    const float ks = pages >= 0 ? note_of(i).k_scale[lane] : 1.0f, vs = pages >= 0 ? note_of(i).v_scale[lane] : 1.0f;
+                    float ratio = isfinite(vs) && pages >= 0 ? vs * v_ref_inv : 1.0f;
+                    ratio = fmaxf(ratio, 0x1p-60f);  // halves of such weights are zero
+                    info.k_scale[lane] = ks;
+                    info.v_log[lane] = log2f(ratio);
+                    info.v_inv[lane] = 1.0f / ratio;
                 }
+                const uint32_t ok = __ballot_sync(0xffu, pages >= 0);
+                if (lane == 0) info.ok = ok;
+                tc::mbar_arrive(&ctl->info_full[i % kInfos]);
             }
             if constexpr (kCodes) {
+                const uint8_t* kr = raw + (i % max(S::kRaw, 1)) * 2 * S::kRawBytes;
+                const uint8_t* vr = kr + S::kRawBytes;
 #pragma unroll
-                for (int c = 0; c < kEach; ++c) expand(kd, r0 + c * kRowStep, kc[c], false, false);
+                for (int c = 0; c < kEach; ++c)
+                    expand(kd, r0 + c * kRowStep, *reinterpret_cast<const uint4*>(kr + c * kProducers * 16), false, false);
                 tc::fence_async_smem();
                 tc::mbar_arrive(&ctl->k_full[st]);
-                if (i + 1 < w.tiles) fetch(kc, a.c.k, i + 1, next_pages);
+                if (i + S::kRaw < w.tiles) copy_notes(i + S::kRaw), copy_codes(i + S::kRaw, a.c.k, 0);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                asm volatile("cp.async.wait_group %0;" ::"n"(2 * S::kRaw - 1) : "memory");  // V of this tile
                 if (i >= 2 && !wait(&ctl->v_empty[st], use ^ 1, ctl, 21, err, s)) { fine = false; break; }
 #pragma unroll
                 for (int c = 0; c < kEach; ++c) {
                     const uint32_t r = r0 + c * kRowStep;
-                    const float vs = __shfl_sync(0xffffffffu, v_scale, r >> 4);
-                    expand(vd, r, vc[c], mixed, !isfinite(vs));
+                    const bool nan = note_of(i).page[r >> 4] >= 0 && !isfinite(note_of(i).v_scale[r >> 4]);
+                    expand(vd, r, *reinterpret_cast<const uint4*>(vr + c * kProducers * 16), mixed, nan);
                 }
                 tc::fence_async_smem();
                 tc::mbar_arrive(&ctl->v_full[st]);
-                if (i + 1 < w.tiles) fetch(vc, a.c.v, i + 1, next_pages);
+                if (i + S::kRaw < w.tiles) copy_codes(i + S::kRaw, a.c.v, 1);
+                asm volatile("cp.async.commit_group;" ::: "memory");
             } else if (!mixed && __all_sync(0xffffffffu, lane >= 8 || pages >= 0)) {
                 // (the lookups of all warps agree, so all of them come here)
                 const uint32_t box = min(a.c.page_tokens, static_cast<uint32_t>(kTile));  // rows a box
