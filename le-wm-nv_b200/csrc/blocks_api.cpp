@@ -289,9 +289,9 @@ lwm_status lwm_cache_attention_device(lwm_ctx* ctx, const lwm_paged_cache* cache
     a.frame_div = lwm::FastDiv(a.frame);
     return on_device(ctx, c, "cache attention",
                      [&](cudaStream_t s) {
-                         const bool many = cache->head_dim >= 64 && static_cast<uint64_t>(a.c.max_new) * a.group >= 64;
-                         return many ? lwm::launch_cache_attention_tc(a, cache->dtype, cache->storage, s)
-                                     : lwm::launch_cache_attention(a, cache->dtype, cache->storage, s);
+                         return lwm::cache_attention_many_rows(a)
+                                    ? lwm::launch_cache_attention_tc(a, cache->dtype, cache->storage, s)
+                                    : lwm::launch_cache_attention(a, cache->dtype, cache->storage, s);
                      });
 }
 

@@ -36,6 +36,9 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "lwm_blocks.cuh"
 #include "lwm_cache_attn.cuh"
 #include "lwm_tc.cuh"
@@ -846,6 +849,26 @@ template <typename T, bool kCodes> cudaError_t by_dim(const CacheAttnArgs& a, cu
 }
 
 }  // namespace
+
+// Which kernel is faster, by what each was measured to cost (us, one B200,
+// 16 heads over 8 kv heads, 1 to 256 sequences of 64 to 4096 tokens).  Here:
+// a block of 256 rows costs 6.5 (64 channels) or 9 (128) and 1.25 or 1.6 a
+// tile of 128 keys, half again with two row tiles, one block a SM at a time.
+// The other kernel: 6 a call, and 3100 or 1580 (16 rows x 16 keys) a us, 4 of
+// them lost a job.  E.g. 256 sequences, 128 rows a kv head, 64 channels: 64
+// tokens 50 there and 101 here, 1024 tokens 335 there and 201 here; 16
+// sequences of 4096 tokens, 32 rows 40 and 56, 128 rows 109 and 56.
+bool cache_attention_many_rows(const CacheAttnArgs& a) {
+    if (a.c.head_dim < 64) return false;
+    const bool wide = a.c.head_dim == 128;
+    const double rows = static_cast<double>(a.c.max_new) * a.group, lots = static_cast<double>(a.c.sequences) * a.c.kv_heads;
+    double span = a.c.max_length ? a.c.max_length : static_cast<double>(a.c.table_stride) * a.c.page_tokens;
+    if (a.window) span = std::min(span, static_cast<double>(a.window) * a.frame + a.sinks + a.c.max_new);
+    const double waves = std::max(1.0, lots * std::ceil(rows / 256) / 148);
+    const double here = waves * ((wide ? 9.0 : 6.5) + (wide ? 1.6 : 1.25) * (rows > 128 ? 1.5 : 1.0) * std::ceil(span / 128));
+    const double there = 6.0 + lots * std::ceil(rows / 16) * (std::ceil(span / 16) + 4) / (wide ? 1580.0 : 3100.0);
+    return here < there;
+}
 
 cudaError_t launch_cache_attention_tc(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s) {
     if (storage == LWM_CACHE_E4M3)

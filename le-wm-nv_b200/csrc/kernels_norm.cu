@@ -3,8 +3,8 @@
 //   x' = x + rs * gate * post(y);  u = pre(x') (1 + scale) + shift;
 //   h = LayerNorm(u) or u.
 // Bound: memory; x and y are read once, x' and h written once.  A row lives
-// in registers: 32 threads for widths up to 1024 (8 values a vector, up to
-// four vectors a thread), 256 threads above.  Means first, then squared
+// in registers, 8 values a vector: 32 threads for widths up to 512 (one or two
+// vectors a thread), 128 up to 1024, 256 above.  Means first, then squared
 // differences, both in f32.
 #include "lwm_blocks.cuh"
 
@@ -258,7 +258,7 @@ template <typename R, typename T, typename C> cudaError_t launch_vectors(const G
     const uint32_t v = g.a.width / 8;
     if (v <= 32) return launch_rows<R, T, C, 32, 1>(g, s);
     if (v <= 64) return launch_rows<R, T, C, 32, 2>(g, s);
-    if (v <= 128) return launch_rows<R, T, C, 32, 4>(g, s);
+    if (v <= 128) return launch_rows<R, T, C, 128, 1>(g, s);
     if (v <= 256) return launch_rows<R, T, C, 256, 1>(g, s);
     if (v <= 512) return launch_rows<R, T, C, 256, 2>(g, s);
     return launch_rows<R, T, C, 256, 4>(g, s);

@@ -94,6 +94,7 @@ struct CacheAttnArgs {
 };
 // Few query rows a kv head (any head width), and many (head_dim 64 or 128).
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
+bool cache_attention_many_rows(const CacheAttnArgs& a);  // which of the two
 cudaError_t launch_cache_attention_tc(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
 
 struct GatedNormArgs {
