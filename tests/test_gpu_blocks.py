@@ -434,11 +434,22 @@ def attention_tolerance(out, mass, reach, keys, d, dtype, codes, v_scale):
     return tol + (keys * 2.0 ** -25 * 448 * v_scale if codes else 0.0)
 
 
+# Packed rows (all but the first few behind the last sequence) and a bound on the new tokens of a sequence that
+# make the tensor-core kernel the cheaper one by the library's costs: 20000 / 16 row tiles of the other kernel
+# against 20000 / 256 blocks of its own.
+MANY = 20000
+
+
 def check_attention(ctx, c, news, heads, seed, causal=True, window=0, sinks=0, frame=1, scale=None, q=None,
-                    table=None, lengths=None, **kw):
+                    table=None, lengths=None, many=False, **kw):
     g = gen(seed)
     lengths = c.lengths if lengths is None else lengths
     tokens = sum(news) + 3  # rows behind the last sequence
+    if many:
+        tokens = MANY
+        kw["max_new"] = MANY
+        if q is not None:
+            q = torch.cat([q, q[:1].expand(MANY - q.shape[0], -1, -1)])
     q = randn(g, tokens, heads, c.d, dtype=c.dtype) if q is None else q
     out = torch.full((tokens, heads, c.d), 5.0, device="cuda", dtype=c.dtype)
     b = c.batch(news, lengths=lengths, tokens=tokens, table=table, **kw)
@@ -480,6 +491,7 @@ def test_attention_masks(ctx, dtype, codes, d, window, sinks, frame, causal):
     c = Paged(22, lengths, 32, 2, d, dtype, codes)
     c.fill_random(23)
     check_attention(ctx, c, [1, 31, 17, 40, 1, 0], 6, 24, causal, window, sinks, frame)
+    check_attention(ctx, c, [1, 31, 17, 100, 1, 0], 6, 24, causal, window, sinks, frame, many=True)
 
 
 @pytest.mark.parametrize("dtype,codes", POOLS)
@@ -490,17 +502,19 @@ def test_attention_many_rows(ctx, dtype, codes, d, kv, heads):
     lengths = [127, 128, 129, 255, 257, 700, 1025, 383]
     c = Paged(25, lengths, 64, kv, d, dtype, codes)
     c.fill_random(26)
-    check_attention(ctx, c, [127, 128, 129, 200, 257, 130, 300, 0], heads, 27)
-    check_attention(ctx, c, [127, 128, 129, 200, 257, 130, 300, 64], heads, 28, window=150, sinks=20)
-    check_attention(ctx, c, [1, 128, 0, 200, 257, 130, 300, 383], heads, 29, causal=False)
+    for many in (False, True):
+        check_attention(ctx, c, [127, 128, 129, 200, 257, 130, 300, 0], heads, 27, many=many)
+        check_attention(ctx, c, [127, 128, 129, 200, 257, 130, 300, 64], heads, 28, window=150, sinks=20, many=many)
+        check_attention(ctx, c, [1, 128, 0, 200, 257, 130, 300, 383], heads, 29, causal=False, many=many)
 
 
 @pytest.mark.parametrize("page", [16, 32, 128])
 def test_attention_many_rows_pages(ctx, page):
     for codes in (False, True):
-        c = Paged(30, [300, 511], page, 2, 128, BF16, codes)
-        c.fill_random(31)
-        check_attention(ctx, c, [260, 140], 4, 32)
+        for d in (64, 128):
+            c = Paged(30, [300, 511], page, 2, d, BF16, codes)
+            c.fill_random(31)
+            check_attention(ctx, c, [260, 140], 4, 32, many=True)
 
 
 @pytest.mark.parametrize("dtype,codes", POOLS)
@@ -528,10 +542,11 @@ def test_attention_rows_that_see_nothing(ctx):
     for dtype, codes in POOLS:
         c = Paged(43, [0, 4, 20, 150], 16, 1, 64, dtype, codes)
         c.fill_random(44)
-        out = check_attention(ctx, c, [3, 9, 1, 170], 2, 45)
-        assert (out[:3] == 0).all() and (out[3:8] == 0).all() and (out[13:33] == 0).all()
-        out = check_attention(ctx, c, [200, 9, 1, 170], 2, 46, causal=False)
-        assert (out[:205] == 0).all()
+        for many in (False, True):
+            out = check_attention(ctx, c, [3, 9, 1, 170], 2, 45, many=many)
+            assert (out[:3] == 0).all() and (out[3:8] == 0).all() and (out[13:33] == 0).all()
+            out = check_attention(ctx, c, [200, 9, 1, 170], 2, 46, causal=False, many=many)
+            assert (out[:205] == 0).all()
 
 
 @pytest.mark.parametrize("dtype,codes", POOLS)
@@ -552,7 +567,7 @@ def test_attention_is_not_reached_by_what_it_does_not_see(ctx, dtype, codes, d, 
             pool[int(c.table[s, j // 32]), 0, j % 32, 2::3] = float("nan")
     kpool = c.k.view(torch.uint8) if codes else c.k
     kpool[int(c.table[1, (length - 3) // 32]), 0, (length - 3) % 32] = 0x7f if codes else float("nan")
-    out = check_attention(ctx, c, [n, n], 2, 49, window=100, sinks=2, table=table)
+    out = check_attention(ctx, c, [n, n], 2, 49, window=100, sinks=2, table=table, many=many)
     assert torch.isnan(out[:2 * n]).any() and torch.isfinite(out[:2 * n]).any()
 
 
@@ -568,13 +583,13 @@ def test_attention_extreme_scores(ctx):
                 c.set("k", 0, ramp * sign)
                 q = torch.ones(many + 3, 2, 64, device="cuda", dtype=F16)
                 q[:, 1] = -4
-                check_attention(ctx, c, [many], 2, 53, q=q)
+                check_attention(ctx, c, [many], 2, 53, q=q, many=many > 1)
             c.set("k", 0, torch.full((400, 1, 64), -30.0, device="cuda"))
             q = torch.full((many + 3, 2, 64), 30.0, device="cuda", dtype=F16)
-            check_attention(ctx, c, [many], 2, 54, q=q)
+            check_attention(ctx, c, [many], 2, 54, q=q, many=many > 1)
             c.set("k", 0, randn(g, 400, 1, 64))
-            check_attention(ctx, c, [many], 2, 55, scale=0.0)
-            check_attention(ctx, c, [many], 2, 56, scale=-0.3)
+            check_attention(ctx, c, [many], 2, 55, scale=0.0, many=many > 1)
+            check_attention(ctx, c, [many], 2, 56, scale=-0.3, many=many > 1)
 
 
 def test_attention_small_and_large_queries_on_codes(ctx):
@@ -583,20 +598,21 @@ def test_attention_small_and_large_queries_on_codes(ctx):
     c.fill_random(58)
     g = gen(59)
     for size in (2.0 ** -60, 2.0 ** -20, 2.0 ** 20, 2.0 ** 100):
-        q = (randn(g, 4, 2, 64) * size).to(BF16)
-        check_attention(ctx, c, [1], 2, 60, q=q, scale=0.125 / size)
+        for n in (1, 90):
+            q = (randn(g, n + 3, 2, 64) * size).to(BF16)
+            check_attention(ctx, c, [n], 2, 60, q=q, scale=0.125 / size, many=n > 1)
 
 
 def test_attention_strides_and_in_place(ctx):
     g = gen(61)
     c = Paged(62, [150, 33], 16, 2, 64)
     c.fill_random(63)
-    for news in ([1, 1], [140, 20]):
-        t = sum(news)
+    for news, t in (([1, 1], 2), ([140, 20], 160), ([140, 20], MANY)):
         wide = randn(g, 8, t + 2, 80, dtype=BF16)
         q = wide[1:7, 1:t + 1, 8:72].transpose(0, 1)  # [t, 6, 64], heads first
         want = torch.empty(t, 6, 64, device="cuda", dtype=BF16)
-        b = c.batch(news)
+        b = c.batch(news, tokens=t, max_new=t)
+        want.copy_(q)
         L.cache_attention_device(ctx, c.cache, b, q.contiguous(), want)
         before = wide.clone()
         L.cache_attention_device(ctx, c.cache, b, q, q)
@@ -616,6 +632,9 @@ def test_attention_shared_pages_and_repeated_calls_agree(ctx):
     assert torch.equal(out[:2], out[4:6])
     again = check_attention(ctx, c, [2, 2, 2], 4, 67, q=torch.cat([q, q[:3]]))
     assert torch.equal(out, again)
+    out = check_attention(ctx, c, [2, 2, 2], 4, 67, q=torch.cat([q, q[:3]]), many=True)
+    again = check_attention(ctx, c, [2, 2, 2], 4, 67, q=torch.cat([q, q[:3]]), many=True)
+    assert torch.equal(out[:2], out[4:6]) and torch.equal(out, again)
 
 
 def test_cache_offsets_beyond_32_bits(ctx):
@@ -635,10 +654,11 @@ def test_cache_offsets_beyond_32_bits(ctx):
     ko, vo = torch.empty_like(x), torch.empty_like(y)
     L.cache_gather_device(ctx, cache, b, ko, vo)
     assert torch.equal(ko, x) and torch.equal(vo, y)
-    for n in (1, 300):
-        q = randn(g, n, kv, d, dtype=BF16)
+    for n, t in ((1, 1), (300, MANY)):
+        q = randn(g, t, kv, d, dtype=BF16)
         out = torch.empty_like(q)
-        L.cache_attention_device(ctx, cache, L.CacheBatch(table, ints([0, n]), ints([300]), n), q, out)
+        L.cache_attention_device(ctx, cache, L.CacheBatch(table, ints([0, n]), ints([300]), t, max_new=t), q, out)
+        q, out = q[:n], out[:n]
         parts = attention_64(q.double(), x.double(), y.double(), mask_of(300, n, True, 0, 0, 1), d ** -0.5)
         close(out, parts[0], attention_tolerance(*parts, d, BF16, False, 0.0))
 
@@ -651,14 +671,16 @@ def test_bad_batches_are_skipped_and_reported(ctx, many):
     c = Paged(70, [200, 200, 200], 64, 1, 64, fill=0.0)
     c.fill_random(71)
     g = gen(72)
-    q = randn(g, 3 * n, 2, 64, dtype=BF16)
-    kv = randn(g, 3 * n, 1, 64, dtype=BF16)
+    tokens = MANY if many else 3 * n
+    q = randn(g, tokens, 2, 64, dtype=BF16)
+    kv = randn(g, tokens, 1, 64, dtype=BF16)
     good = torch.empty_like(q)
-    L.cache_attention_device(ctx, c.cache, c.batch([n] * 3), q, good)
+    L.cache_attention_device(ctx, c.cache, c.batch([n] * 3, tokens=tokens, max_new=MANY if many else n), q, good)
     ctx.synchronize()
 
     def broken(what):
-        table, starts, lengths, max_new = c.table.copy(), [0, n, 2 * n, 3 * n], [200, 200, 200], n
+        table, starts, lengths = c.table.copy(), [0, n, 2 * n, 3 * n], [200, 200, 200]
+        max_new = MANY if many else n
         if what == "page":
             table[1, 3] = c.k.shape[0]
         elif what == "negative page":
@@ -666,14 +688,16 @@ def test_bad_batches_are_skipped_and_reported(ctx, many):
         elif what == "starts":
             starts = [0, n, n - 1, n - 1]
         elif what == "rows":
-            starts = [0, n, 3 * n + 1, 3 * n + 1]
+            starts = [0, n, tokens + 1, tokens + 1]
         elif what == "length":
             lengths[1] = 4 * 64 + 1
         elif what == "negative length":
             lengths[1] = -1
         elif what == "new":
             starts, max_new = [0, n - 1, 2 * n, 3 * n], n
-        return L.CacheBatch(ints(table), ints(starts), ints(lengths), 3 * n, max_new=max_new)
+            if many:  # its longest sequence alone; the kernel that looks is the same
+                starts, max_new = [0, 0, MANY, MANY], MANY - 1
+        return L.CacheBatch(ints(table), ints(starts), ints(lengths), tokens, max_new=max_new)
 
     for what, message in (("page", "not in the pool"), ("negative page", "not in the pool"),
                           ("starts", "out of order"), ("rows", "beyond the packed rows"),
@@ -685,8 +709,11 @@ def test_bad_batches_are_skipped_and_reported(ctx, many):
             ctx.synchronize()
         assert e.value.status == "INVALID_ARGUMENT"
         ctx.synchronize()  # reported once
-        if what != "new" and what != "rows":
+        if what not in ("new", "rows"):
             assert torch.equal(out[:n], good[:n]), what
+        if what not in ("page", "negative page"):  # a skipped sequence's rows are zero or as they were
+            rest = out[n:2 * n] if what != "new" else out[max(n - 1, 0):2 * n]
+            assert ((rest == 3.0) | (rest == 0.0)).all() or what == "new", what
         before_k, before_v = c.k.clone(), c.v.clone()
         L.cache_append_device(ctx, c.cache, broken(what), kv, kv)
         with pytest.raises(L.LwmError, match=message):
@@ -897,6 +924,33 @@ def test_captured_step_replays_on_new_lengths(ctx):
                 close(out[s:s + 1], parts[0], attention_tolerance(*parts, 64, BF16, codes, vs))
 
 
+def test_captured_chunk_replays_on_new_lengths(ctx):
+    """A chunk of tokens on the tensor-core kernel, captured once."""
+    for codes in (False, True):
+        c = Paged(97, [300, 200], 64, 2, 128, BF16, codes)
+        c.fill_random(98)
+        q = randn(gen(99), MANY, 4, 128, dtype=BF16)
+        out = torch.zeros_like(q)
+        lengths = ints([300, 200])
+        b = L.CacheBatch(ints(c.table), ints([0, 130, 200]), lengths, MANY, max_new=MANY)
+        ctx.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=ctx.torch_stream()):
+            L.cache_attention_device(ctx, c.cache, b, q, out, window=64, sinks=3)
+        for lens in ([300, 200], [131, 190], [260, 71]):
+            lengths.copy_(ints(lens))
+            graph.replay()
+            got = out.clone()
+            L.cache_attention_device(ctx, c.cache, b, q, out, window=64, sinks=3)
+            assert torch.equal(got, out)
+            c.lengths = lens
+            for s, (a, z) in enumerate(((0, 130), (130, 200))):
+                parts = attention_64(q[a:z].double(), c.dense("k", s), c.dense("v", s),
+                                     mask_of(lens[s], z - a, True, 64, 3, 1), 128 ** -0.5)
+                vs = float(c.vs[c.table[s]].nan_to_num(0).max()) if codes else 0.0
+                close(out[a:z], parts[0], attention_tolerance(*parts, 128, BF16, codes, vs))
+
+
 def test_two_contexts_at_once(ctx):
     """Two contexts' streams run the same calls side by side on shared pages."""
     import threading
@@ -904,17 +958,18 @@ def test_two_contexts_at_once(ctx):
     try:
         c = Paged(94, [3000, 200], 64, 2, 128)
         c.fill_random(95)
-        q = randn(gen(96), 160, 4, 128, dtype=BF16)
+        q = randn(gen(96), MANY, 4, 128, dtype=BF16)
         torch.cuda.synchronize()
         results = {}
 
         def work(name, cx):
             with torch.cuda.stream(cx.torch_stream()):
                 for i in range(20):
-                    for news in ([1, 1], [2, 140]):
-                        out = torch.empty(sum(news), 4, 128, device="cuda", dtype=BF16)
-                        L.cache_attention_device(cx, c.cache, c.batch(news), q[:sum(news)], out)
-                        results[name, i, news[1]] = out
+                    for news, t in (([1, 1], 2), ([2, 140], 142), ([20, 1], MANY)):
+                        out = torch.zeros(t, 4, 128, device="cuda", dtype=BF16)
+                        b = c.batch(news, tokens=t, max_new=max(news) if t < MANY else t)
+                        L.cache_attention_device(cx, c.cache, b, q[:t], out)
+                        results[name, i, t] = out
                 cx.synchronize()
 
         threads = [threading.Thread(target=work, args=(n, x)) for n, x in (("a", ctx), ("b", other))]
