@@ -287,7 +287,7 @@ __device__ __forceinline__ float weights(const float (&x)[64], uint32_t (&p)[32]
 template <typename T, int D, bool kCodes>
 __global__ void __launch_bounds__(kThreads, 1)
     cache_attn_tc_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ CUtensorMap k_map,
-                         const __grid_constant__ CUtensorMap v_map, uint32_t row_blocks) {
+                         const __grid_constant__ CUtensorMap v_map) {
     using M = std::conditional_t<kCodes, __half, T>;
     using S = Shape<D, kCodes>;
     constexpr int kSteps = D / 16;
@@ -295,13 +295,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
     Control* ctl = reinterpret_cast<Control*>(smem + S::kControl);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // the last rows of the sequences first: causal rows there see the most keys
+    // The last rows of the sequences first, where causal rows see the most keys, and blocks counted from the last row,
+    // so that the one that is not full is the shortest and starts last.
     const uint32_t pairs = a.c.sequences * a.c.kv_heads, turn = blockIdx.x / pairs, hs = blockIdx.x - turn * pairs;
     const uint32_t h = hs % a.c.kv_heads, s = hs / a.c.kv_heads;
     const SeqView v = sequence(a.c, s, false, threadIdx.x == 0 && h == 0 && turn == 0);
-    const uint32_t rows = v.n * a.group, row0 = (row_blocks - 1 - turn) * 2 * kTile;
-    if (row0 >= rows) return;
-    const uint32_t last = min(row0 + 2 * kTile, rows) - 1;
+    const uint32_t later = turn * 2 * kTile;
+    if (later >= v.n * a.group) return;
+    const uint32_t rows = v.n * a.group - later;  // the end of this block's
+    const uint32_t row0 = max(rows, 2u * kTile) - 2 * kTile, last = rows - 1;
     const bool two = last >= row0 + kTile;  // the second tile has rows
     const Walk w = walk_of(a, v, row0, last);
 
@@ -395,7 +397,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t t_s = t_lane + tile * kTile, t_o = t_lane + kOCol + tile * D;
             float m = -INFINITY, l = 0.0f;
             bool fine = true;
-            for (uint32_t i = 0; i < w.tiles && fine; ++i) {
+            // a warp without rows leaves its part of P as it is: a row of P enters its own row of O alone
+            const bool idle = row0 + tile * kTile + (warp & 3) * 32 >= rows;
+            for (uint32_t i = 0; i < w.tiles && fine && idle; ++i) {
+                fine = wait(&ctl->s_full[tile], i & 1, ctl, 10 + tile, err, s);
+                if (fine && lane < 2) tc::mbar_arrive(&ctl->p_full[tile][lane]);
+            }
+            for (uint32_t i = 0; i < w.tiles && fine && !idle; ++i) {
                 // (the producers' notes are there long before the scores)
                 const TileInfo& info = ctl->info[i % kInfos];
                 fine = wait(&ctl->info_full[i % kInfos], (i / kInfos) & 1, ctl, 12 + tile, err, s);
@@ -840,7 +848,7 @@ template <typename T, int D, bool kCodes> cudaError_t launch(const CacheAttnArgs
         if (e == cudaSuccess) e = page_map(a.c, a.c.v, std::is_same_v<T, bf16>, &v_map);
     }
     if (e != cudaSuccess) return e;
-    kernel<<<row_blocks * a.c.sequences * a.c.kv_heads, kThreads, S::kBytes, s>>>(a, k_map, v_map, row_blocks);
+    kernel<<<row_blocks * a.c.sequences * a.c.kv_heads, kThreads, S::kBytes, s>>>(a, k_map, v_map);
     return cudaGetLastError();
 }
 
