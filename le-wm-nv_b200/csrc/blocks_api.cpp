@@ -37,6 +37,7 @@ template <class F> lwm_status on_device(lwm_ctx* ctx, const CtxView& c, const ch
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool aligned4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
 // A [rows, heads, head_dim] tensor: aligned, strides in whole vectors.
 lwm_status check_heads(const char* name, const void* p, uint64_t ts, uint64_t hs) {
@@ -73,11 +74,16 @@ lwm_status check_cache(const lwm_paged_cache* c, const lwm_cache_batch* b, lwm::
     if (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128)
         return fail(LWM_UNSUPPORTED, "cache page_tokens " + std::to_string(c->page_tokens) + " is not 16, 32, 64 or 128");
     if (c->kv_heads == 0) return bad("cache kv_heads must be greater than zero");
+    if (c->pages == 0) return bad("cache pages must be greater than zero");
     if (c->pages > 0x7fffffffu || c->kv_heads > 65535) return bad("cache pages or kv_heads out of range");
     if (!c->k || !c->v) return bad("cache pools are null");
     if (!aligned16(c->k) || !aligned16(c->v)) return bad("cache pools are not 16-byte aligned");
     if (c->storage == LWM_CACHE_E4M3 && (!c->k_scale || !c->v_scale)) return bad("an 8-bit cache needs its scales");
+    if (c->storage == LWM_CACHE_E4M3 && (!aligned4(c->k_scale) || !aligned4(c->v_scale)))
+        return bad("cache scales are not 4-byte aligned");
     if (b->sequences && (!b->table || !b->lengths || !b->starts)) return bad("batch arrays are null");
+    if (b->sequences && (!aligned4(b->table) || !aligned4(b->lengths) || !aligned4(b->starts)))
+        return bad("batch arrays are not 4-byte aligned");
     if (b->sequences && b->table_stride == 0) return bad("batch table_stride must be greater than zero");
     if (b->sequences > 0x7ffffffu || b->tokens > 0x7fffffffu || b->max_new > b->tokens)
         return bad("batch sizes out of range (max_new " + std::to_string(b->max_new) + ", tokens " +
@@ -159,6 +165,7 @@ lwm_status lwm_rotary_device(lwm_ctx* ctx, const lwm_rotary* rotary, const lwm_r
         LWM_TRY(check_heads("x", x->x, x->x_token_stride, x->x_head_stride));
         LWM_TRY(check_heads("out", x->out, x->out_token_stride, x->out_head_stride));
         if (!x->positions) return bad("positions are null");
+        if (!aligned4(x->positions)) return bad("positions are not 4-byte aligned");
     }
     CtxView c;
     if (!lwm::ctx_view(ctx, &c)) return bad("null context");
@@ -192,6 +199,7 @@ lwm_status lwm_cache_append_device(lwm_ctx* ctx, const lwm_paged_cache* cache, c
     if (x->q && x->heads == 0) return bad("query heads must be greater than zero");
     if (x->q && x->heads > 65535) return bad("query heads out of range");
     const bool work = a.c.sequences && a.c.max_new;
+    if (!aligned4(x->positions)) return bad("positions are not 4-byte aligned");
     if (work) {
         LWM_TRY(check_heads("k", x->k, x->k_token_stride, x->k_head_stride));
         LWM_TRY(check_heads("v", x->v, x->v_token_stride, x->v_head_stride));
@@ -312,7 +320,7 @@ lwm_status lwm_gated_norm_device(lwm_ctx* ctx, const lwm_gated_norm_args* x) {
         return bad("gated norm eps must be finite and non-negative");
     if (x->out_bias && !x->out_weight) return bad("out_bias needs out_weight");
     if (cond && x->rows_per_cond == 0) return bad("rows_per_cond must be greater than zero");
-    if (!x->x_out && !x->h) return bad("gated norm has no output");
+    if (x->rows && !x->x_out && !x->h) return bad("gated norm has no output");
     if (x->rows && !x->x) return bad("x is null");
     const auto size = [](int32_t d) { return d == LWM_DTYPE_F32 ? 4u : 2u; };
     const auto natural = [](const void* p, unsigned e) { return reinterpret_cast<uintptr_t>(p) % e == 0; };
@@ -323,7 +331,7 @@ lwm_status lwm_gated_norm_device(lwm_ctx* ctx, const lwm_gated_norm_args* x) {
         return bad("gated norm tensors must be aligned to their element size");
     for (const float* p : {x->residual_scale, x->post_weight, x->post_bias, x->pre_weight, x->pre_bias, x->out_weight,
                            x->out_bias})
-        if (!natural(p, 4)) return bad("gated norm weights must be aligned to 4 bytes");
+        if (!aligned4(p)) return bad("gated norm weights must be aligned to 4 bytes");
     CtxView c;
     if (!lwm::ctx_view(ctx, &c)) return bad("null context");
     if (x->rows == 0) return LWM_OK;

@@ -1270,6 +1270,11 @@ def _ints(name: str, t, shape) -> None:
         raise LwmError(1, f"{name} must be a contiguous int32 tensor {list(shape)}, got {t.dtype} {list(t.shape)}")
 
 
+def _u32(name: str, x: int) -> None:
+    if not 0 <= x < 1 << 32:
+        raise LwmError(1, f"{name} must be 0 to 2^32 - 1, got {x}")
+
+
 class PagedCache:
     """lwm_paged_cache over torch tensors: k, v [pages, kv_heads, page_tokens,
     head_dim] in bfloat16 or float16, or 8-bit codes (float8_e4m3fn or uint8)
@@ -1315,13 +1320,16 @@ class CacheBatch:
         _ints("page table", table, tuple(table.shape))
         _ints("starts", starts, (n + 1,))
         _ints("lengths", lengths, (n,))
+        max_new = tokens if max_new is None else max_new
+        for name, x in (("tokens", tokens), ("max_new", max_new), ("max_length", max_length)):
+            _u32(name, x)
         self._keep = (table, starts, lengths)
         self.device, self.device_index = table.device, table.get_device()
         if starts.device != table.device or lengths.device != table.device:
             raise LwmError(1, "batch tensors are on different devices")
         self.tokens = tokens
         self._c = _CacheBatch(table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), n, table.shape[1], tokens,
-                              tokens if max_new is None else max_new, max_length)
+                              max_new, max_length)
         self._ref = C.byref(self._c)
 
 
@@ -1391,6 +1399,9 @@ def cache_attention_device(ctx: Context, cache: PagedCache, batch: CacheBatch, q
     _same_device(ctx, cache, batch)
     if q.dim() != 3:
         raise LwmError(1, f"q must be [tokens, heads, head_dim], got {list(q.shape)}")
+    if not 0 <= (window | sinks | frame_tokens) < 1 << 32:  # any of them
+        for name, x in (("window", window), ("sinks", sinks), ("frame_tokens", frame_tokens)):
+            _u32(name, x)
     heads = q.shape[1]
     shape = (batch.tokens, heads, cache.head_dim)
     qp, qt, qh = _heads(ctx, "q", q, shape, cache.dtype)
@@ -1433,7 +1444,7 @@ class GatedNorm:
 
 def _rows(ctx: Context, name: str, t, x, width: int):
     """(address, row stride) of a tensor shaped like x with contiguous rows."""
-    stride, unit = t.stride()
+    stride, unit = t.stride() if t.dim() == 2 else (0, 0)
     if t.shape != x.shape or (unit != 1 and width > 1):
         raise LwmError(1, f"{name} must be {list(x.shape)} with contiguous rows, got {list(t.shape)}")
     if t.get_device() != ctx.device:
@@ -1470,8 +1481,8 @@ def gated_norm_device(ctx: Context, norm: GatedNorm, x, y=None, x_out=None, h=No
     for i, t in enumerate((gate, shift, scale)):
         if t is None:
             continue
-        stride, unit = t.stride()
-        if rows_per_cond < 1 or t.shape[1] != width or t.shape[0] * rows_per_cond < rows or (unit != 1 and width > 1):
+        stride, unit = t.stride() if t.dim() == 2 else (0, 0)
+        if t.dim() != 2 or rows_per_cond < 1 or t.shape[1] != width or t.shape[0] * rows_per_cond < rows or (unit != 1 and width > 1):
             raise LwmError(1, f"{('gate', 'shift', 'scale')[i]} must be [ceil(rows / rows_per_cond), {width}] with "
                               f"contiguous rows, got {list(t.shape)}")
         if cond_dtype is not None and (t.dtype != cond_dtype or stride != cond_stride):

@@ -66,6 +66,7 @@ def _rotary_args(**kw):
     (dict(out=None), "out is null"),
     (dict(x_head_stride=68), "x strides must be multiples of 8 elements"),
     (dict(positions=None), "positions are null"),
+    (dict(positions=P + 1), "positions are not 4-byte aligned"),
     (dict(), "null context"),
 ])
 def test_rotary_call_refusals(kw, message):
@@ -114,10 +115,13 @@ CACHE_REFUSALS = [
     (dict(page_tokens=24), {}, "cache page_tokens 24 is not 16, 32, 64 or 128"),
     (dict(kv_heads=0), {}, "cache kv_heads must be greater than zero"),
     (dict(pages=1 << 31), {}, "cache pages or kv_heads out of range"),
+    (dict(pages=0), {}, "cache pages must be greater than zero"),
     (dict(v=None), {}, "cache pools are null"),
     (dict(k=P + 4), {}, "cache pools are not 16-byte aligned"),
     (dict(k_scale=None), {}, "an 8-bit cache needs its scales"),
+    (dict(v_scale=P + 2), {}, "cache scales are not 4-byte aligned"),
     ({}, dict(table=None), "batch arrays are null"),
+    ({}, dict(lengths=P + 1), "batch arrays are not 4-byte aligned"),
     ({}, dict(table_stride=0), "batch table_stride must be greater than zero"),
     ({}, dict(max_new=7), "batch sizes out of range (max_new 7, tokens 6)"),
     ({}, {}, "null context"),
@@ -144,6 +148,7 @@ def test_cache_refusals(call, cache, batch, message):
     (dict(v=P + 2), "v is not 16-byte aligned"),
     (dict(k_token_stride=100), "k strides must be multiples of 8 elements"),
     (dict(q_out=None), "q_out is null"),
+    (dict(positions=P + 2), "positions are not 4-byte aligned"),
     (dict(q=None, q_out=None, heads=0), "null context"),
 ])
 def test_append_refusals(kw, message):
@@ -198,6 +203,7 @@ def _norm(**kw):
     (dict(pre_weight=P + 1), "gated norm weights must be aligned to 4 bytes"),
     (dict(), "null context"),
     (dict(rows=0), "null context"),
+    (dict(rows=0, x=None, y=None, x_out=None, h=None), "null context"),
 ])
 def test_gated_norm_refusals(kw, message):
     assert L.lib.lwm_gated_norm_device(None, C.byref(_norm(**kw))) != 0
@@ -225,6 +231,10 @@ def test_python_checks_name_the_tensor():
         L.CacheBatch(table[:, :2], starts, lengths, 0)
     with pytest.raises(L.LwmError, match="lengths must be"):
         L.CacheBatch(table, starts, lengths.long(), 0)
+    with pytest.raises(L.LwmError, match="max_new must be 0 to"):
+        L.CacheBatch(table, starts, lengths, 4, max_new=-1)
+    with pytest.raises(L.LwmError, match="max_length must be 0 to"):
+        L.CacheBatch(table, starts, lengths, 4, max_length=1 << 32)
     with pytest.raises(L.LwmError, match="kinds"):
         L.GatedNorm(pre="batch")
     with pytest.raises(L.LwmError, match="float32"):

@@ -751,9 +751,29 @@ def test_wrong_tensors_are_refused(ctx):
             (lambda: L.cache_append_device(ctx, c.cache, b, kv, kv, q=q), "needs q_out"),
             (lambda: L.rotary_device(ctx, L.Rotary.make([32], [1e4]), q, q, ints([1, 2])), "positions must be"),
             (lambda: L.gated_norm_device(ctx, L.GatedNorm(), q[0], h=q[0], gate=torch.zeros(3, 64, device="cuda")),
-             "gate must be")):
+             "gate must be"),
+            (lambda: L.gated_norm_device(ctx, L.GatedNorm(), q[0], h=q[0], gate=torch.zeros(64, device="cuda")),
+             "gate must be"),
+            (lambda: L.gated_norm_device(ctx, L.GatedNorm(), q[0], h=q), "h must be"),
+            (lambda: L.cache_attention_device(ctx, c.cache, b, q, q, window=-1), "window must be 0 to"),
+            (lambda: L.cache_attention_device(ctx, c.cache, b, q, q, sinks=1 << 32), "sinks must be 0 to")):
         with pytest.raises(L.LwmError, match=message):
             call()
+
+
+def test_empty_batches(ctx):
+    """No rows, no sequences, sequences without new tokens: nothing runs, nothing is reported."""
+    c = Paged(75, [20, 0], 16, 2, 64)
+    q, kv = torch.zeros(0, 4, 64, device="cuda", dtype=BF16), torch.zeros(0, 2, 64, device="cuda", dtype=BF16)
+    none = L.CacheBatch(torch.zeros(0, 2, device="cuda", dtype=torch.int32), ints([0]), ints([]), 0)
+    for b in (c.batch([0, 0]), none):
+        L.cache_append_device(ctx, c.cache, b, kv, kv, L.Rotary.make([64], [1e4]), q=q, q_out=q)
+        L.cache_attention_device(ctx, c.cache, b, q, q)
+        L.cache_gather_device(ctx, c.cache, b, kv, kv)
+    L.rotary_device(ctx, L.Rotary.make([64], [1e4]), q, q, torch.zeros(0, 1, device="cuda", dtype=torch.int32))
+    x = torch.zeros(0, 64, device="cuda", dtype=BF16)
+    L.gated_norm_device(ctx, L.GatedNorm(), x, y=x, x_out=x, h=x, gate=x)
+    ctx.synchronize()
 
 
 # --------------------------------------------------------------- gated norm
