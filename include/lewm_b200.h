@@ -63,7 +63,9 @@ lwm_status lwm_ctx_destroy(lwm_ctx* ctx);
 lwm_status lwm_ctx_stream(lwm_ctx* ctx, void** stream_out);
 /* Waits for the context's stream.  Also reports (LWM_CUDA_ERROR, once) an
  * NV12 preprocessing launch whose source-row copies never completed since
- * the previous call; that launch's output is then incomplete. */
+ * the previous call; that launch's output is then incomplete.  Likewise
+ * (LWM_INVALID_ARGUMENT, once) a batch of the paged cache below whose device
+ * arrays were out of range. */
 lwm_status lwm_ctx_synchronize(lwm_ctx* ctx);
 /* Number of kernels this library has launched on the context so far. */
 lwm_status lwm_ctx_launch_count(lwm_ctx* ctx, uint64_t* out);
@@ -743,9 +745,10 @@ lwm_status lwm_lewm_plan_nv12_device(lwm_planner* planner, lwm_scorer* scorer, c
  *
  * All buffers are the caller's, all work is asynchronous on the context's
  * stream, nothing is allocated and no state is kept between calls, so every
- * call can be captured into a CUDA graph, and graphs or threads share
- * nothing but the buffers that the caller gives them.  The calls leave the
- * calling thread's current device as it was.  16-bit and 32-bit tensors
+ * call can be captured into a CUDA graph (which must not outlive the
+ * context: the kernels hold the address of its error word), and graphs or
+ * threads share nothing else but the buffers that the caller gives them.
+ * The calls leave the calling thread's current device as it was.  16-bit and 32-bit tensors
  * start on 16-byte boundaries and have strides (in elements) that are
  * multiples of 8, with the channels of a head contiguous. */
 typedef enum lwm_dtype {
@@ -793,7 +796,8 @@ lwm_status lwm_rotary_device(lwm_ctx* ctx, const lwm_rotary* rotary, const lwm_r
  * head_dim 32, 64 or 128; page_tokens 16, 32, 64 or 128.  LWM_CACHE_16BIT
  * holds values of `dtype` (bf16 or f16); LWM_CACHE_E4M3 holds 8-bit codes
  * (4-bit exponent, 3-bit mantissa) and one f32 scale for each page and head,
- * k_scale and v_scale [pages, kv_heads]: a value is code * scale. */
+ * k_scale and v_scale [pages, kv_heads]: a value is code * scale.  Scales
+ * are positive and finite, as the append writes them. */
 typedef enum lwm_cache_storage {
     LWM_CACHE_16BIT = 0,
     LWM_CACHE_E4M3 = 1,
@@ -817,8 +821,8 @@ typedef struct lwm_paged_cache {
  * from starts[sequences] on are left as they are), `max_new` at least every
  * n; `max_length` (0: the table's reach) says how long sequences get, for
  * the shape of the launch only.  Sequences may share pages that this call
- * does not append to; entries of pages that no visible token lies in are
- * not read.
+ * does not append to; table entries of pages that no visible token lies in
+ * may hold anything.
  *
  * A sequence whose starts or length are out of order, above max_new, below 0
  * or beyond its table, and a visible token whose page is not in the pool,
@@ -864,7 +868,8 @@ typedef struct lwm_cache_gather_args {
 lwm_status lwm_cache_gather_device(lwm_ctx* ctx, const lwm_paged_cache* cache, const lwm_cache_batch* batch,
                                    const lwm_cache_gather_args* args);
 /* Attention of the batch's tokens over their sequences' cached tokens: out =
- * softmax(scale q . k) v over the visible keys, zero where there is none.
+ * softmax(scale q . k) v over the visible keys, zero where there is none or
+ * every visible score is minus infinity.
  * q, out [tokens, heads, head_dim] of the cache's dtype (out may be q);
  * query head h reads kv head h / (heads / kv_heads).  The token at cache
  * index p of a sequence of length L sees index j when

@@ -9,6 +9,16 @@
 // (page, head): the new tokens' largest value first, then the scale, the
 // earlier tokens' codes where the scale grew, and the new codes, so that no
 // scale is shared between groups.
+//
+// Measured (one B200): 16 sequences x up to 1568 new tokens, 16 heads of 64
+// channels, bf16, queries turned along: 215 MB read and written in 49 us,
+// 4.4 TB/s; gathering 151 MB of them back 24 us, 6.2 TB/s.  8 bits, one token
+// for each of 1024 sequences: 16 to 22 us, the chain lengths -> page ->
+// tokens -> scale -> codes twice over (80 registers: three blocks a SM);
+// gathering 17 tokens of each, 35 MB of codes to 70 MB: 23 us, two thirds of
+// the issue slots.  Left, as they cost more than they gave: more blocks a SM
+// with 64 registers or fewer (spills, +2 %), 16 codes a load in the gather
+// (+6 %), eight loads in flight (+2 %).
 #include "lwm_blocks.cuh"
 
 namespace lwm {

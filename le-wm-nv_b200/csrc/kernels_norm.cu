@@ -6,6 +6,11 @@
 // in registers, 8 values a vector: 32 threads for widths up to 512 (one or two
 // vectors a thread), 128 up to 1024, 256 above.  Means first, then squared
 // differences, both in f32.
+//
+// Measured (one B200): 50176 rows of 1024, f32 stream and bf16 block, 617 MB
+// in 116 us, 5.3 TB/s (a warp a row with four vectors a thread: 138); 1024
+// rows of 192 in f32: 6.4 us, launch and one chain.  One barrier a sum
+// instead of two, and streaming loads or stores, measured the same.
 #include "lwm_blocks.cuh"
 
 namespace lwm {

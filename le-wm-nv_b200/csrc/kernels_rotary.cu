@@ -4,7 +4,9 @@
 // A block takes a few tokens: it computes the cosine and sine of their pairs
 // once into shared memory (64-bit fixed-point angles, see turn_of), then its
 // threads turn the heads' 16-byte vectors.  With halves a thread owns both
-// vectors of 8 pairs, so no value is read twice.
+// vectors of 8 pairs, so no value is read twice.  Measured (one B200): 537 MB
+// of bf16 read and written in 90 us, 6.0 TB/s; 20 MB of f32 8.8 us, most of
+// it launch and ramp.
 #include "lwm_blocks.cuh"
 
 namespace lwm {
