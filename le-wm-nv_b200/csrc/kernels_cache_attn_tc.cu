@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp < 8) {
         // ---------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(192));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(184));
         const int tile = warp >> 2, r = threadIdx.x & 127;
         const uint32_t R = row0 + tile * kTile + r;
         if (tile == 0 || two) {
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp < 12) {
         // -------------------------------------------------------- producers
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(72));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(88));
         const int t = threadIdx.x - 256;
         constexpr int kRowChunks = kCodes ? D / 16 : D / 8;  // 16-byte chunks of a cached row
         constexpr int kEach = kTile * kRowChunks / kProducers, kRowStep = kProducers / kRowChunks;
@@ -565,10 +565,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         // codes in flight: this thread's chunks, and its warp's notes of the tiles
         TileNotes* notes = reinterpret_cast<TileNotes*>(smem + S::kNotes) + (warp - 8) * (S::kRaw + 1);
         uint8_t* raw = smem + S::kCodesAt + t * 16;
-        auto note_of = [&](uint32_t i) -> TileNotes& { return notes[i % (S::kRaw + 1)]; };
-        auto copy_notes = [&](uint32_t i) {
-            const int p = page_ids(i);
-            TileNotes& n = note_of(i);
+        uint32_t note_in = 0, note_out = 0;  // slots of the notes written and read next
+        auto copy_notes = [&](int p) {
+            TileNotes& n = notes[note_in];
+            note_in = note_in == S::kRaw ? 0 : note_in + 1;
             if (lane < 8) {
                 n.page[lane] = p;
                 if (p >= 0) {
@@ -577,16 +577,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     cp_async4(&n.v_scale[lane], a.c.v_scale + at);
                 }
             }
-            __syncwarp();
+        };
+        // where this thread's chunks of tile i lie in either pool (all ones: not to be read), before any is asked for
+        constexpr int kMine = kCodes ? kEach : 1;
+        size_t from[kMine];
+        auto locate = [&](uint32_t i, int p) {
+#pragma unroll
+            for (int c = 0; c < kMine; ++c) {
+                const uint32_t r = r0 + c * kRowStep, j = w.key0(i) + r;
+                const int page = __shfl_sync(0xffffffffu, p, r >> 4);
+                from[c] = page >= 0 && row_live(j) ? pool_at(a.c, page, h, j & (a.c.page_tokens - 1)) + ch * 16 : ~size_t{0};
+            }
         };
         auto copy_codes = [&](uint32_t i, const void* pool, int which) {
-            const TileNotes& n = note_of(i);
             const uint32_t dst = tc::smem_u32(raw) + ((i % max(S::kRaw, 1)) * 2 + which) * S::kRawBytes;
 #pragma unroll
-            for (int c = 0; c < (kCodes ? kEach : 0); ++c) {
-                const uint32_t r = r0 + c * kRowStep, j = w.key0(i) + r;
-                const int page = n.page[r >> 4];
-                cp_async16(dst + c * kProducers * 16, source(pool, page, j), page >= 0 && row_live(j));
+            for (int c = 0; c < kMine; ++c) {
+                const bool live = from[c] != ~size_t{0};
+                cp_async16(dst + c * kProducers * 16, static_cast<const uint8_t*>(pool) + (live ? from[c] : 0), live);
             }
         };
         // 16 codes to two chunks of halves; NaN codes of a mixed tile are taken out
@@ -614,7 +622,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (kCodes) {
 #pragma unroll 1
             for (uint32_t i = 0; i < S::kRaw; ++i) {
-                if (i < w.tiles) copy_notes(i), copy_codes(i, a.c.k, 0);
+                if (i < w.tiles) {
+                    const int p = page_ids(i);
+                    copy_notes(p);
+                    locate(i, p);
+                    copy_codes(i, a.c.k, 0);
+                }
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if (i < w.tiles) copy_codes(i, a.c.v, 1);
                 asm volatile("cp.async.commit_group;" ::: "memory");
@@ -644,33 +657,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float v_ref_inv = kCodes ? 1.0f / fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]),
                                                       fmaxf(ctl->reduce[2], ctl->reduce[3]))
                                        : 1.0f;
+        int ahead = kCodes ? page_ids(S::kRaw) : -1;  // codes: pages of the next tile to copy, looked up a tile earlier
         for (uint32_t i = 0; i < w.tiles && fine; ++i) {
             const uint32_t st = i & 1, use = (i >> 1) & 1, key = w.key0(i);
             const bool mixed = !w.whole(key);
             const int next_pages = kCodes ? -1 : page_ids(i + 1);
+            float k_scale = 1.0f, v_scale = 1.0f;
+            uint32_t nan_groups = 0;
             if constexpr (kCodes) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(2 * S::kRaw - 1) : "memory");  // K of this tile
                 __syncwarp();
-                pages = lane < 8 ? note_of(i).page[lane] : -1;
+                const TileNotes& n = notes[note_out];
+                note_out = note_out == S::kRaw ? 0 : note_out + 1;
+                pages = lane < 8 ? n.page[lane] : -1;
+                if (pages >= 0) k_scale = n.k_scale[lane], v_scale = n.v_scale[lane];
+                nan_groups = __ballot_sync(0xffffffffu, !isfinite(v_scale));
             }
             uint8_t* kd = smem + S::kK + st * S::kTileBytes;
             uint8_t* vd = smem + S::kV + st * S::kTileBytes;
             if (i >= 2 && !wait(&ctl->k_empty[st], use ^ 1, ctl, 20, err, s)) { fine = false; break; }
-            // what the softmax needs to know; the ring is four tiles deep, the stages two
-            if (warp == 8 && lane < 8) {
+            // what the softmax needs to know, a warp in turn; the ring is four tiles deep, the stages two
+            auto inform = [&] {
+                if (warp != 8 + static_cast<int>(i & 3) || lane >= 8) return;
                 TileInfo& info = ctl->info[i % kInfos];
                 if constexpr (kCodes) {
-                    const float ks = pages >= 0 ? note_of(i).k_scale[lane] : 1.0f, vs = pages >= 0 ? note_of(i).v_scale[lane] : 1.0f;
-                    float ratio = isfinite(vs) && pages >= 0 ? vs * v_ref_inv : 1.0f;
+                    float ratio = isfinite(v_scale) && pages >= 0 ? v_scale * v_ref_inv : 1.0f;
                     ratio = fmaxf(ratio, 0x1p-60f);  // halves of such weights are zero
-                    info.k_scale[lane] = ks;
+                    info.k_scale[lane] = k_scale;
                     info.v_log[lane] = log2f(ratio);
                     info.v_inv[lane] = 1.0f / ratio;
                 }
                 const uint32_t ok = __ballot_sync(0xffu, pages >= 0);
                 if (lane == 0) info.ok = ok;
                 tc::mbar_arrive(&ctl->info_full[i % kInfos]);
-            }
+            };
+            if constexpr (!kCodes) inform();
             if constexpr (kCodes) {
                 const uint8_t* kr = raw + (i % max(S::kRaw, 1)) * 2 * S::kRawBytes;
                 const uint8_t* vr = kr + S::kRawBytes;
@@ -679,19 +700,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                     expand(kd, r0 + c * kRowStep, *reinterpret_cast<const uint4*>(kr + c * kProducers * 16), false, false);
                 tc::fence_async_smem();
                 tc::mbar_arrive(&ctl->k_full[st]);
-                if (i + S::kRaw < w.tiles) copy_notes(i + S::kRaw), copy_codes(i + S::kRaw, a.c.k, 0);
+                inform();
+                const bool more = i + S::kRaw < w.tiles;
+                if (more) {
+                    copy_notes(ahead);
+                    locate(i + S::kRaw, ahead);
+                    copy_codes(i + S::kRaw, a.c.k, 0);
+                    ahead = page_ids(i + S::kRaw + 1);
+                }
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 asm volatile("cp.async.wait_group %0;" ::"n"(2 * S::kRaw - 1) : "memory");  // V of this tile
                 if (i >= 2 && !wait(&ctl->v_empty[st], use ^ 1, ctl, 21, err, s)) { fine = false; break; }
+                if (!mixed && nan_groups == 0) {
 #pragma unroll
-                for (int c = 0; c < kEach; ++c) {
-                    const uint32_t r = r0 + c * kRowStep;
-                    const bool nan = note_of(i).page[r >> 4] >= 0 && !isfinite(note_of(i).v_scale[r >> 4]);
-                    expand(vd, r, *reinterpret_cast<const uint4*>(vr + c * kProducers * 16), mixed, nan);
+                    for (int c = 0; c < kEach; ++c)
+                        expand(vd, r0 + c * kRowStep, *reinterpret_cast<const uint4*>(vr + c * kProducers * 16), false, false);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kEach; ++c) {
+                        const uint32_t r = r0 + c * kRowStep;
+                        expand(vd, r, *reinterpret_cast<const uint4*>(vr + c * kProducers * 16), mixed, (nan_groups >> (r >> 4)) & 1);
+                    }
                 }
                 tc::fence_async_smem();
                 tc::mbar_arrive(&ctl->v_full[st]);
-                if (i + S::kRaw < w.tiles) copy_codes(i + S::kRaw, a.c.v, 1);
+                if (more) copy_codes(i + S::kRaw, a.c.v, 1);
                 asm volatile("cp.async.commit_group;" ::: "memory");
             } else if (!mixed && __all_sync(0xffffffffu, lane >= 8 || pages >= 0)) {
                 // (the lookups of all warps agree, so all of them come here)
