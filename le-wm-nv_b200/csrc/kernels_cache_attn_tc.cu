@@ -59,6 +59,7 @@ constexpr int kTile = 128;           // rows of a tile, keys of a step
 constexpr int kHalf = 64;            // keys whose weights go to the product at once
 constexpr int kThreads = 512;        // two softmax warpgroups, producers, MMA issuers
 constexpr int kProducers = 128;
+constexpr int kScaleThreads = 96;    // of the warps beside the MMA issuer
 constexpr int kPanel = kTile * 128;  // bytes of 128 rows x 64 channels
 constexpr int kInfos = 4;
 constexpr uint32_t kOCol = 256;
@@ -547,14 +548,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int kEach = kTile * kRowChunks / kProducers, kRowStep = kProducers / kRowChunks;
         const int ch = t % kRowChunks, r0 = t / kRowChunks;
         constexpr size_t kElem = kCodes ? 1 : 2;
-        auto page_ids = [&](uint32_t i) {  // lane g: the page of group g of tile i, -1: nothing visible or no page
-            int p = -1;
-            if (i < w.tiles && lane < 8) {
-                const uint32_t j = w.key0(i) + 16 * lane;
-                if (j < w.hi_max && (j + 16 > w.lo_min || j < w.sinks_end)) p = page_of(a.c, s, j >> a.c.page_shift);
-            }
-            return p;
+        // the page of group g of tile i, -1: nothing visible or no page
+        auto group_page = [&](uint32_t i, uint32_t g) {
+            const uint32_t j = w.key0(i) + 16 * g;
+            return i < w.tiles && j < w.hi_max && (j + 16 > w.lo_min || j < w.sinks_end) ? page_of(a.c, s, j >> a.c.page_shift) : -1;
         };
+        auto page_ids = [&](uint32_t i) { return lane < 8 ? group_page(i, lane) : -1; };  // lane g: of group g
         auto row_live = [&](uint32_t j) { return j < w.hi_max && (j >= w.lo_min || j < w.sinks_end); };
         auto source = [&](const void* pool, int page, uint32_t j) {
             return static_cast<const uint8_t*>(pool) +
@@ -620,10 +619,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<uint4*>(row + ((((c0 + 1) & 7) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
         };
         if constexpr (kCodes) {
+            const int first = lane < 8 * S::kRaw ? group_page(lane >> 3, lane & 7) : -1;  // of all of them at once
 #pragma unroll 1
             for (uint32_t i = 0; i < S::kRaw; ++i) {
+                const int p = __shfl_sync(0xffffffffu, first, 8 * i + (lane & 7));
                 if (i < w.tiles) {
-                    const int p = page_ids(i);
                     copy_notes(p);
                     locate(i, p);
                     copy_codes(i, a.c.k, 0);
@@ -633,30 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 asm volatile("cp.async.commit_group;" ::: "memory");
             }
         }
-        if constexpr (kCodes) {
-            // the largest value scale of the visible pages
-            float top = 0.0f;
-            for (uint32_t i = t; i < w.tiles * 8; i += kProducers) {
-                const uint32_t j = w.key0(i / 8) + 16 * (i % 8);
-                if (j < w.hi_max && (j + 16 > w.lo_min || j < w.sinks_end)) {
-                    const int p = a.c.table[static_cast<size_t>(s) * a.c.table_stride + (j >> a.c.page_shift)];
-                    if (static_cast<uint32_t>(p) < a.c.pages) {
-                        const float x = a.c.v_scale[static_cast<size_t>(p) * a.c.kv_heads + h];
-                        if (isfinite(x)) top = fmaxf(top, x);
-                    }
-                }
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (lane == 0) ctl->reduce[warp - 8] = top;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            top = fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]), fmaxf(ctl->reduce[2], ctl->reduce[3]));
-            if (top == 0.0f) top = 1.0f;
-            if (t == 0) ctl->v_ref = top;
-        }
-        const float v_ref_inv = kCodes ? 1.0f / fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]),
-                                                      fmaxf(ctl->reduce[2], ctl->reduce[3]))
-                                       : 1.0f;
+        float v_ref_inv = 1.0f;
         int ahead = kCodes ? page_ids(S::kRaw) : -1;  // codes: pages of the next tile to copy, looked up a tile earlier
         for (uint32_t i = 0; i < w.tiles && fine; ++i) {
             const uint32_t st = i & 1, use = (i >> 1) & 1, key = w.key0(i);
@@ -700,6 +677,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     expand(kd, r0 + c * kRowStep, *reinterpret_cast<const uint4*>(kr + c * kProducers * 16), false, false);
                 tc::fence_async_smem();
                 tc::mbar_arrive(&ctl->k_full[st]);
+                if (i == 0) {  // the idle warps' maximum
+                    asm volatile("bar.sync 1, %0;" ::"n"(kProducers + kScaleThreads) : "memory");
+                    float top = fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]), ctl->reduce[2]);
+                    if (top == 0.0f) top = 1.0f;
+                    v_ref_inv = 1.0f / top;
+                    if (t == 0) ctl->v_ref = top;
+                }
                 inform();
                 const bool more = i + S::kRaw < w.tiles;
                 if (more) {
@@ -847,6 +831,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::commit_w(&ctl->drain);
             tc::mbar_wait_landing(&ctl->drain, 0);
             tc::fence_before();
+        } else if (kCodes && w.tiles) {
+            // ------------------- the largest value scale of the visible pages
+            float top = 0.0f;
+            for (uint32_t i = threadIdx.x - 13 * 32; i < w.tiles * 8; i += kScaleThreads) {
+                const uint32_t j = w.key0(i / 8) + 16 * (i % 8);
+                if (j < w.hi_max && (j + 16 > w.lo_min || j < w.sinks_end)) {
+                    const int p = a.c.table[static_cast<size_t>(s) * a.c.table_stride + (j >> a.c.page_shift)];
+                    if (static_cast<uint32_t>(p) < a.c.pages) {
+                        const float x = a.c.v_scale[static_cast<size_t>(p) * a.c.kv_heads + h];
+                        if (isfinite(x)) top = fmaxf(top, x);
+                    }
+                }
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (lane == 0) ctl->reduce[warp - 13] = top;
+            __syncwarp();
+            asm volatile("bar.arrive 1, %0;" ::"n"(kProducers + kScaleThreads) : "memory");
         }
     }
     tc::fence_before();
