@@ -21,8 +21,12 @@
 // channels, causal, bf16: 370 us, 966 TFLOP/s, tensor pipe 48 %, issue slots
 // 41 %: bound by a tile's chain of scores, softmax and product.  8 sequences
 // of 394 new tokens over 1700 visible ones, 12 heads of 64 channels, 8-bit
-// codes: 86 us; 192 blocks on 148 SMs, most of their 14 steps at edges of the
-// masks, and the expansion of the codes (61 us with a 16-bit cache).
+// codes: 67 us; 192 blocks on 148 SMs, a third of their 16 steps at edges of
+// the masks (a 16-bit cache: 61).  The producers of codes bounded a tile (4800
+// cycles) until they located their chunks once for K and V, looked pages up a
+// tile ahead and kept the test for NaN scales out of the plain expansion: 86.
+// Left: three buffers of scores for 64 channels (16-bit cache 7 % faster,
+// codes 2 %, but 128 channels 5 % slower).
 //
 // TMEM: S (and P) of tile t at column 128 t, O at 256 and 256 + D.  Shared
 // memory: Q, two stages of K and of V, all rows of 64 channels (128 bytes,
@@ -34,9 +38,10 @@
 // gathered row by row with cp.async, rows that no query sees as zeros.
 // 8-bit codes are copied tiles ahead (four for 64 channels; shared memory has
 // room for one of 128) and become halves (exact) on the way to the operands;
-// each thread expands what it copied itself.  Their scales stay out of the products: a page's key
-// scale multiplies its 16-key groups' scores, its value scale, relative to
-// the block's largest, enters the exponent of the weight.
+// each thread expands what it copied itself.  Their scales stay out of the
+// products: a page's key scale multiplies its 16-key groups' scores, its value
+// scale, relative to the block's largest (which the warps beside the issuer
+// find meanwhile), enters the exponent of the weight.
 //
 // O is rescaled only when a score passes a row's maximum by more than kRaise
 // (a factor of 2^8).
