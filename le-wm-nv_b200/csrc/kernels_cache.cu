@@ -89,7 +89,15 @@ __device__ __forceinline__ void head_unit(const lwm_rotary& r, uint32_t pairs, c
 
 template <int kLanes> __device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-    for (int o = kLanes / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = min(kLanes, 32) / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if constexpr (kLanes > 32) {  // the block
+        __shared__ float parts[kThreads / 32];
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) v = fmaxf(v, parts[w]);
+    }
     return v;
 }
 __device__ __forceinline__ float finite_abs(float v) { return isfinite(v) ? fabsf(v) : 0.0f; }
@@ -147,7 +155,8 @@ __device__ __forceinline__ void append_codes(const AppendArgs& a, const PagePart
                      });
     }
     // every lane of the group has read the old scale
-    __syncwarp(kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u) << ((threadIdx.x & 31) / kLanes * kLanes));
+    if constexpr (kLanes > 32) __syncthreads();
+    else __syncwarp(kLanes == 32 ? 0xffffffffu : ((1u << (kLanes & 31)) - 1u) << ((threadIdx.x & 31) / kLanes * kLanes));
     if (lane == 0) *scale_at = scale;
 }
 
@@ -165,12 +174,13 @@ __device__ __forceinline__ void part_angles(const AppendArgs& a, const PagePart&
 
 // Turns heads [0, heads) of the part's tokens: queries, then (16 bits) keys.
 // Both vectors of a unit are read before either is written: q_out may be q.
+// The work of the part's blocks (blockIdx.y) is dealt out by loads in flight.
 template <typename T>
 __device__ __forceinline__ void turn_heads(const AppendArgs& a, const CacheDivs& d, const PagePart& p, uint32_t q_heads,
                                            uint32_t heads, const float2* trig) {
     const HeadUnits hu(a.pairs, a.r.interleaved, a.c.head_dim);
     const uint32_t work = p.count * heads * hu.count;
-    for (uint32_t base = threadIdx.x; base < work; base += 4 * kThreads) {
+    for (uint32_t base = blockIdx.y * 4 * kThreads + threadIdx.x; base < work; base += gridDim.y * 4 * kThreads) {
         Vec8<T> x[4], y[4];
         T* dst[4];
         uint32_t apart[4], pair[4], at[4];
@@ -248,8 +258,9 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 }
 
 // 8 bits; kLanes lanes a (page, head): 8 when a call brings a token or two a
-// sequence (a head's units fill no more), a warp otherwise.  blockIdx.y:
-// parts of the heads, where the pages alone are too few blocks.
+// sequence (a head's units fill no more), the whole block when pages are few
+// and full, a warp otherwise.  blockIdx.y: parts of the heads, where the
+// pages alone are too few blocks.
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(kThreads) append_codes_kernel(const __grid_constant__ AppendArgs a, const CacheDivs d,
                                                                 uint32_t pages) {
@@ -259,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) append_codes_kernel(const __grid_con
     const PagePart p = page_part(a.c, v, s, ordinal, a.c.page_shift);
     if (p.page < 0) return;
     part_angles(a, p, trig);
-    if (a.q && blockIdx.y == 0) turn_heads<T>(a, d, p, a.heads, a.heads, trig);
+    if (a.q) turn_heads<T>(a, d, p, a.heads, a.heads, trig);
     const uint32_t kv = a.c.kv_heads, group = threadIdx.x / kLanes, groups = kThreads / kLanes;
     const uint32_t stride = groups * gridDim.y, rounds = (2 * kv + stride - 1) / stride;
     for (uint32_t i = 0; i < rounds; ++i) {
@@ -336,13 +347,15 @@ template <typename T> cudaError_t append(const AppendArgs& a, bool codes, cudaSt
         return cudaGetLastError();
     }
     const bool few = a.c.max_new <= 2;
-    auto* kernel = few ? append_codes_kernel<T, 8> : append_codes_kernel<T, 32>;
+    // a block a (page, head) where a warp each would leave SMs idle
+    const bool block = !few && static_cast<uint64_t>(blocks) * 2 * a.c.kv_heads < 148 * 16;
+    auto* kernel = few ? append_codes_kernel<T, 8> : block ? append_codes_kernel<T, kThreads> : append_codes_kernel<T, 32>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
         if (e != cudaSuccess) return e;
     }
     // heads in parts until there are four blocks a SM, or a group has one head
-    const uint32_t groups = kThreads / (few ? 8 : 32);
+    const uint32_t groups = kThreads / (few ? 8 : block ? kThreads : 32);
     uint32_t parts = 1;
     while (parts < 64 && static_cast<uint64_t>(blocks) * parts < 148 * 4 && 2 * a.c.kv_heads > groups * parts) parts *= 2;
     kernel<<<dim3(blocks, parts), kThreads, smem, s>>>(a, divs_of(a.c, hu.count, q_heads, runs), runs);

@@ -3,7 +3,8 @@
 // tcgen05 tensor cores.
 //
 // A block takes 256 query rows (tokens x heads of the group) of one sequence
-// and kv head as two tiles of 128, and walks the visible keys 128 at a time.
+// and kv head as two tiles of 128 (or one, where that fills more SMs), and
+// walks the visible keys 128 at a time.
 // S = Q K^T goes to TMEM, a softmax warpgroup a tile (one row a thread, so no
 // shuffles) reads it, writes P back over it in the operands' type, and O +=
 // P V accumulates in TMEM with P as the A operand there.  The two tiles
@@ -301,7 +302,7 @@ __device__ __forceinline__ float weights(const float (&x)[64], uint32_t (&p)[32]
 template <typename T, int D, bool kCodes>
 __global__ void __launch_bounds__(kThreads, 1)
     cache_attn_tc_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ CUtensorMap k_map,
-                         const __grid_constant__ CUtensorMap v_map) {
+                         const __grid_constant__ CUtensorMap v_map, uint32_t block_rows) {
     using M = std::conditional_t<kCodes, __half, T>;
     using S = Shape<D, kCodes>;
     constexpr int kSteps = D / 16;
@@ -314,10 +315,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t pairs = a.c.sequences * a.c.kv_heads, turn = blockIdx.x / pairs, hs = blockIdx.x - turn * pairs;
     const uint32_t h = hs % a.c.kv_heads, s = hs / a.c.kv_heads;
     const SeqView v = sequence(a.c, s, false, threadIdx.x == 0 && h == 0 && turn == 0);
-    const uint32_t later = turn * 2 * kTile;
+    const uint32_t later = turn * block_rows;
     if (later >= v.n * a.group) return;
     const uint32_t rows = v.n * a.group - later;  // the end of this block's
-    const uint32_t row0 = max(rows, 2u * kTile) - 2 * kTile, last = rows - 1;
+    const uint32_t row0 = max(rows, block_rows) - block_rows, last = rows - 1;
     const bool two = last >= row0 + kTile;  // the second tile has rows
     const Walk w = walk_of(a, v, row0, last);
 
@@ -884,10 +885,38 @@ cudaError_t page_map(const CacheArgs& c, void* pool, bool is_bf16, CUtensorMap* 
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// Which kernel is faster, and whether a block here takes one row tile or two,
+// by what each was measured to cost (us, one B200, 16 heads over 8 kv heads,
+// 1 to 256 sequences of 64 to 4096 tokens).  Here: a block costs 6.5 (64
+// channels) or 9 (128) and 1.25 or 1.6 a tile of 128 keys, half again with
+// two row tiles, one block a SM at a time: two tiles share what is loaded,
+// one a block fills the SMs where rows are few.  The other kernel: 6 a call,
+// and 3100 or 1580 (16 rows x 16 keys) a us, 4 of them lost a job.  E.g. 256
+// sequences, 128 rows a kv head, 64 channels: 64 tokens 50 there and 101
+// here, 1024 tokens 335 there and 201 here; 16 sequences of 4096 tokens, 32
+// rows 40 and 56, 128 rows 109 and 56.
+struct Costs {
+    double here, there;
+    uint32_t rows;  // of a block here
+};
+Costs costs_of(const CacheAttnArgs& a) {
+    const bool wide = a.c.head_dim == 128;
+    const double rows = static_cast<double>(a.c.max_new) * a.group, lots = static_cast<double>(a.c.sequences) * a.c.kv_heads;
+    double span = a.c.max_length ? a.c.max_length : static_cast<double>(a.c.table_stride) * a.c.page_tokens;
+    if (a.window) span = std::min(span, static_cast<double>(a.window) * a.frame + a.sinks + a.c.max_new);
+    const auto blocks_cost = [&](double block, double factor) {
+        const double waves = std::max(1.0, lots * std::ceil(rows / block) / 148);
+        return waves * ((wide ? 9.0 : 6.5) + (wide ? 1.6 : 1.25) * factor * std::ceil(span / kTile));
+    };
+    const double one = blocks_cost(kTile, 1.0), both = blocks_cost(2 * kTile, rows > kTile ? 1.5 : 1.0);
+    const double there = 6.0 + lots * std::ceil(rows / 16) * (std::ceil(span / 16) + 4) / (wide ? 1580.0 : 3100.0);
+    return {std::min(one, both), there, one < both ? kTile : 2u * kTile};
+}
+
 template <typename T, int D, bool kCodes> cudaError_t launch(const CacheAttnArgs& a, cudaStream_t s) {
     using S = Shape<D, kCodes>;
     static_assert(S::kBytes <= 227 * 1024, "shared memory");
-    const uint32_t row_blocks = (a.c.max_new * a.group + 2 * kTile - 1) / (2 * kTile);
+    const uint32_t block_rows = costs_of(a).rows, row_blocks = (a.c.max_new * a.group + block_rows - 1) / block_rows;
     auto* kernel = cache_attn_tc_kernel<T, D, kCodes>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
     CUtensorMap k_map{}, v_map{};
@@ -896,7 +925,7 @@ template <typename T, int D, bool kCodes> cudaError_t launch(const CacheAttnArgs
         if (e == cudaSuccess) e = page_map(a.c, a.c.v, std::is_same_v<T, bf16>, &v_map);
     }
     if (e != cudaSuccess) return e;
-    kernel<<<row_blocks * a.c.sequences * a.c.kv_heads, kThreads, S::kBytes, s>>>(a, k_map, v_map);
+    kernel<<<row_blocks * a.c.sequences * a.c.kv_heads, kThreads, S::kBytes, s>>>(a, k_map, v_map, block_rows);
     return cudaGetLastError();
 }
 
@@ -906,24 +935,10 @@ template <typename T, bool kCodes> cudaError_t by_dim(const CacheAttnArgs& a, cu
 
 }  // namespace
 
-// Which kernel is faster, by what each was measured to cost (us, one B200,
-// 16 heads over 8 kv heads, 1 to 256 sequences of 64 to 4096 tokens).  Here:
-// a block of 256 rows costs 6.5 (64 channels) or 9 (128) and 1.25 or 1.6 a
-// tile of 128 keys, half again with two row tiles, one block a SM at a time.
-// The other kernel: 6 a call, and 3100 or 1580 (16 rows x 16 keys) a us, 4 of
-// them lost a job.  E.g. 256 sequences, 128 rows a kv head, 64 channels: 64
-// tokens 50 there and 101 here, 1024 tokens 335 there and 201 here; 16
-// sequences of 4096 tokens, 32 rows 40 and 56, 128 rows 109 and 56.
 bool cache_attention_many_rows(const CacheAttnArgs& a) {
     if (a.c.head_dim < 64) return false;
-    const bool wide = a.c.head_dim == 128;
-    const double rows = static_cast<double>(a.c.max_new) * a.group, lots = static_cast<double>(a.c.sequences) * a.c.kv_heads;
-    double span = a.c.max_length ? a.c.max_length : static_cast<double>(a.c.table_stride) * a.c.page_tokens;
-    if (a.window) span = std::min(span, static_cast<double>(a.window) * a.frame + a.sinks + a.c.max_new);
-    const double waves = std::max(1.0, lots * std::ceil(rows / 256) / 148);
-    const double here = waves * ((wide ? 9.0 : 6.5) + (wide ? 1.6 : 1.25) * (rows > 128 ? 1.5 : 1.0) * std::ceil(span / 128));
-    const double there = 6.0 + lots * std::ceil(rows / 16) * (std::ceil(span / 16) + 4) / (wide ? 1580.0 : 3100.0);
-    return here < there;
+    const Costs c = costs_of(a);
+    return c.here < c.there;
 }
 
 cudaError_t launch_cache_attention_tc(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s) {
