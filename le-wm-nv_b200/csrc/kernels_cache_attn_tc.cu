@@ -29,6 +29,9 @@
 // Left: three buffers of scores for 64 channels (16-bit cache 7 % faster,
 // codes 2 %, but 128 channels 5 % slower).
 //
+// 32 channels run as 64 whose upper half is zero (by TMA's fill beyond the
+// tensor, or copies of no bytes): the softmax bounds them all the same.
+//
 // TMEM: S (and P) of tile t at column 128 t, O at 256 and 256 + D.  Shared
 // memory: Q, two stages of K and of V, all rows of 64 channels (128 bytes,
 // 128-byte swizzle); K is a K-major operand, V the transposed (N-major) one
@@ -371,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t Rk = row0 + tile * kTile + (warp & 3) * 32 + k * kAtOnce + lane / kLanes;
                     const uint32_t tk = Rk < rows ? a.group_div.div(Rk) : 0;
                     x[k].a = make_uint4(0, 0, 0, 0);
-                    if (Rk < rows)
+                    if (Rk < rows && 8u * c < a.c.head_dim)
                         x[k] = load8(static_cast<const T*>(a.q) + (v.start + tk) * a.q_ts +
                                      (h * a.group + (Rk - tk * a.group)) * a.q_hs + 8 * c);
                 }
@@ -485,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // rows go through the tile's Q, which no product reads any more, and out in whole 16-byte runs
             uint8_t* stage = smem + S::kQ + tile * S::kTileBytes;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
+            for (int c = 0; c < static_cast<int>(a.c.head_dim); c += 16) {
                 float o[16];
                 if (w.tiles) {
                     tc::tmem_ld16(t_o + c, o);
@@ -538,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int k = 0; k < kLanes; ++k) {
                     const int rk = (warp & 3) * 32 + k * kAtOnce + lane / kLanes;
                     const uint32_t Rk = row0 + tile * kTile + rk;
-                    if (Rk >= rows) continue;
+                    if (Rk >= rows || 8u * c >= a.c.head_dim) continue;
                     const uint32_t tk = a.group_div.div(Rk);
                     *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (v.start + tk) * a.o_ts +
                                               (h * a.group + (Rk - tk * a.group)) * a.o_hs + 8 * c) =
@@ -554,13 +557,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int kEach = kTile * kRowChunks / kProducers, kRowStep = kProducers / kRowChunks;
         const int ch = t % kRowChunks, r0 = t / kRowChunks;
         constexpr size_t kElem = kCodes ? 1 : 2;
+        const bool inside = ch * 16 < static_cast<int>(a.c.head_dim * kElem);  // (32 channels: half of a row)
         // the page of group g of tile i, -1: nothing visible or no page
         auto group_page = [&](uint32_t i, uint32_t g) {
             const uint32_t j = w.key0(i) + 16 * g;
             return i < w.tiles && j < w.hi_max && (j + 16 > w.lo_min || j < w.sinks_end) ? page_of(a.c, s, j >> a.c.page_shift) : -1;
         };
         auto page_ids = [&](uint32_t i) { return lane < 8 ? group_page(i, lane) : -1; };  // lane g: of group g
-        auto row_live = [&](uint32_t j) { return j < w.hi_max && (j >= w.lo_min || j < w.sinks_end); };
+        auto row_live = [&](uint32_t j) { return inside && j < w.hi_max && (j >= w.lo_min || j < w.sinks_end); };
         auto source = [&](const void* pool, int page, uint32_t j) {
             return static_cast<const uint8_t*>(pool) +
                    (pool_at(a.c, page < 0 ? 0 : page, h, j & (a.c.page_tokens - 1)) * kElem + ch * 16);
@@ -889,12 +893,14 @@ cudaError_t page_map(const CacheArgs& c, void* pool, bool is_bf16, CUtensorMap* 
 // by what each was measured to cost (us, one B200, 16 heads over 8 kv heads,
 // 1 to 256 sequences of 64 to 4096 tokens).  Here: a block costs 6.5 (64
 // channels) or 9 (128) and 1.25 or 1.6 a tile of 128 keys, half again with
-// two row tiles, one block a SM at a time: two tiles share what is loaded,
-// one a block fills the SMs where rows are few.  The other kernel: 6 a call,
-// and 3100 or 1580 (16 rows x 16 keys) a us, 4 of them lost a job.  E.g. 256
-// sequences, 128 rows a kv head, 64 channels: 64 tokens 50 there and 101
-// here, 1024 tokens 335 there and 201 here; 16 sequences of 4096 tokens, 32
-// rows 40 and 56, 128 rows 109 and 56.
+// two row tiles, one block a SM at a time (32 channels cost what 64 do): two
+// tiles share what is loaded, one a block fills the SMs where rows are few.
+// The other kernel: 6 a call, and 1580, 3100 or (32 channels) 3700 (16 rows x
+// 16 keys) a us, 4 of them lost a job.  E.g. 256 sequences, 128 rows a kv
+// head, 64 channels: 64 tokens 50 there and 101 here, 1024 tokens 335 there
+// and 201 here; 16 sequences of 4096 tokens, 32 rows 40 and 56, 128 rows 109
+// and 56; 32 channels: 256 sequences of 640 tokens, 256 rows 355 and 195, 32
+// rows of 1024 tokens 83 and 190.
 struct Costs {
     double here, there;
     uint32_t rows;  // of a block here
@@ -909,7 +915,8 @@ Costs costs_of(const CacheAttnArgs& a) {
         return waves * ((wide ? 9.0 : 6.5) + (wide ? 1.6 : 1.25) * factor * std::ceil(span / kTile));
     };
     const double one = blocks_cost(kTile, 1.0), both = blocks_cost(2 * kTile, rows > kTile ? 1.5 : 1.0);
-    const double there = 6.0 + lots * std::ceil(rows / 16) * (std::ceil(span / 16) + 4) / (wide ? 1580.0 : 3100.0);
+    const double there = 6.0 + lots * std::ceil(rows / 16) * (std::ceil(span / 16) + 4) /
+                                   (wide ? 1580.0 : a.c.head_dim == 64 ? 3100.0 : 3700.0);
     return {std::min(one, both), there, one < both ? kTile : 2u * kTile};
 }
 
@@ -930,13 +937,12 @@ template <typename T, int D, bool kCodes> cudaError_t launch(const CacheAttnArgs
 }
 
 template <typename T, bool kCodes> cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t s) {
-    return a.c.head_dim == 64 ? launch<T, 64, kCodes>(a, s) : launch<T, 128, kCodes>(a, s);
+    return a.c.head_dim == 128 ? launch<T, 128, kCodes>(a, s) : launch<T, 64, kCodes>(a, s);
 }
 
 }  // namespace
 
 bool cache_attention_many_rows(const CacheAttnArgs& a) {
-    if (a.c.head_dim < 64) return false;
     const Costs c = costs_of(a);
     return c.here < c.there;
 }

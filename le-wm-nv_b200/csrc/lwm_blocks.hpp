@@ -92,7 +92,7 @@ struct CacheAttnArgs {
     FastDiv group_div, frame_div;
     FastDiv tile_div, kv_div;  // set by the launch
 };
-// Few query rows a kv head (any head width), and many (head_dim 64 or 128).
+// Few query rows a kv head, and many.
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
 bool cache_attention_many_rows(const CacheAttnArgs& a);  // which of the two
 cudaError_t launch_cache_attention_tc(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);

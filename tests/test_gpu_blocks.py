@@ -495,7 +495,7 @@ def test_attention_masks(ctx, dtype, codes, d, window, sinks, frame, causal):
 
 
 @pytest.mark.parametrize("dtype,codes", POOLS)
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("kv,heads", [(1, 1), (1, 3), (2, 8), (3, 3), (1, 16)])
 def test_attention_many_rows(ctx, dtype, codes, d, kv, heads):
     """Whole histories and chunks behind a history, at lengths around the tiles' borders."""
@@ -550,7 +550,7 @@ def test_attention_rows_that_see_nothing(ctx):
 
 
 @pytest.mark.parametrize("dtype,codes", POOLS)
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("many", [False, True])
 def test_attention_is_not_reached_by_what_it_does_not_see(ctx, dtype, codes, d, many):
     """NaN and infinities in later tokens, behind the window, in unused slots; pages that nobody sees are not looked up."""
