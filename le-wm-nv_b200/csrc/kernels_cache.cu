@@ -161,13 +161,14 @@ __device__ __forceinline__ void append_codes(const AppendArgs& a, const PagePart
 }
 
 // cos and sin of the part's tokens.
-__device__ __forceinline__ void part_angles(const AppendArgs& a, const PagePart& p, float2* trig) {
+__device__ __forceinline__ void part_angles(const AppendArgs& a, const PagePart& p, const PairTurns& turns, float2* trig) {
+    __syncthreads();  // turns
     for (uint32_t i = threadIdx.x; i < p.count * a.pairs; i += kThreads) {
         const uint32_t t = i / a.pairs, pr = i - t * a.pairs;
         const int32_t pos = a.positions
-                                ? a.positions[static_cast<size_t>(p.row + t) * a.axes + axis_of(a.r, pr)]
+                                ? a.positions[static_cast<size_t>(p.row + t) * a.axes + turns.axis[pr]]
                                 : static_cast<int32_t>(p.index + t);
-        trig[i] = turn_of(pos, a.r.turn[pr]);
+        trig[i] = turn_of(pos, turns.turn[pr]);
     }
     __syncthreads();
 }
@@ -231,11 +232,13 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a, const CacheDivs d,
                                                           uint32_t runs) {
     extern __shared__ float2 trig[];  // [16][pairs]
+    __shared__ PairTurns turns;
+    fill_turns(a.r, a.pairs, turns);
     const uint32_t s = d.ordinals.div(blockIdx.x), ordinal = blockIdx.x - s * runs;
     const SeqView v = sequence(a.c, s, true, threadIdx.x == 0 && ordinal == 0);
     const PagePart p = page_part(a.c, v, s, ordinal, 4);
     if (p.page < 0) return;
-    part_angles(a, p, trig);
+    part_angles(a, p, turns, trig);
     const uint32_t kv = a.c.kv_heads, vecs = a.c.head_dim / 8, q_heads = a.q ? a.heads : 0;
     turn_heads<T>(a, d, p, q_heads, q_heads + kv, trig);
     const uint32_t work = p.count * kv * vecs;
@@ -265,11 +268,13 @@ template <typename T, int kLanes>
 __global__ void __launch_bounds__(kThreads) append_codes_kernel(const __grid_constant__ AppendArgs a, const CacheDivs d,
                                                                 uint32_t pages) {
     extern __shared__ float2 trig[];  // [page_tokens][pairs]
+    __shared__ PairTurns turns;
+    fill_turns(a.r, a.pairs, turns);
     const uint32_t s = d.ordinals.div(blockIdx.x), ordinal = blockIdx.x - s * pages;
     const SeqView v = sequence(a.c, s, true, threadIdx.x == 0 && ordinal == 0 && blockIdx.y == 0);
     const PagePart p = page_part(a.c, v, s, ordinal, a.c.page_shift);
     if (p.page < 0) return;
-    part_angles(a, p, trig);
+    part_angles(a, p, turns, trig);
     if (a.q) turn_heads<T>(a, d, p, a.heads, a.heads, trig);
     const uint32_t kv = a.c.kv_heads, group = threadIdx.x / kLanes, groups = kThreads / kLanes;
     const uint32_t stride = groups * gridDim.y, rounds = (2 * kv + stride - 1) / stride;

@@ -19,11 +19,14 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, uint32_t block_tokens, FastDiv units_div,
                                                           FastDiv heads_div, FastDiv pairs_div) {
     extern __shared__ float2 trig[];  // [block_tokens][pairs]
+    __shared__ PairTurns turns;
+    fill_turns(a.r, a.pairs, turns);
+    __syncthreads();
     const uint32_t t0 = blockIdx.x * block_tokens, nt = min(block_tokens, a.tokens - t0);
     const HeadUnits hu(a.pairs, a.r.interleaved, a.head_dim);
     for (uint32_t i = threadIdx.x; i < nt * a.pairs; i += kThreads) {
         const uint32_t t = pairs_div.div(i), p = i - t * a.pairs;
-        float2 cs = turn_of(a.positions[static_cast<size_t>(t0 + t) * a.r.axes + axis_of(a.r, p)], a.r.turn[p]);
+        float2 cs = turn_of(a.positions[static_cast<size_t>(t0 + t) * a.r.axes + turns.axis[p]], turns.turn[p]);
         if (a.inverse) cs.y = -cs.y;
         trig[i] = cs;
     }

@@ -126,6 +126,20 @@ __device__ __forceinline__ uint32_t axis_of(const lwm_rotary& r, uint32_t pair) 
     while (pair >= end) end += r.dims[++a] / 2;
     return a;
 }
+// A launch's frequencies and axes by pair, in shared memory: in the kernel's
+// parameters they are constants, which a warp reads one address at a time
+// (61316 tokens of one head: 24 us so, 9 from shared memory).
+struct PairTurns {
+    uint64_t turn[LWM_ROTARY_MAX_PAIRS];
+    uint8_t axis[LWM_ROTARY_MAX_PAIRS];
+};
+// (the caller synchronises the block)
+__device__ __forceinline__ void fill_turns(const lwm_rotary& r, uint32_t pairs, PairTurns& to) {
+    for (uint32_t p = threadIdx.x; p < pairs; p += blockDim.x) {
+        to.turn[p] = r.turn[p];
+        to.axis[p] = static_cast<uint8_t>(axis_of(r, p));
+    }
+}
 
 // A head as units of work: with halves, unit u < pairs / 8 is two vectors,
 // channels [c, c + 8) and [c + n/2, c + n/2 + 8) of an axis with n channels;
