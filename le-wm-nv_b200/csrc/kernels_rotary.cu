@@ -5,8 +5,8 @@
 // once into shared memory (64-bit fixed-point angles, see turn_of), then its
 // threads turn the heads' 16-byte vectors.  With halves a thread owns both
 // vectors of 8 pairs, so no value is read twice.  Measured (one B200): 537 MB
-// of bf16 read and written in 90 us, 6.0 TB/s; 20 MB of f32 8.8 us, most of
-// it launch and ramp.
+// of bf16 read and written in 88 us, 6.1 TB/s; 20 MB of f32 8.2 us, most of
+// it launch and ramp.  Smaller blocks, of threads or tokens, measured the same.
 #include "lwm_blocks.cuh"
 
 namespace lwm {

@@ -128,7 +128,7 @@ __device__ __forceinline__ uint32_t axis_of(const lwm_rotary& r, uint32_t pair) 
 }
 // A launch's frequencies and axes by pair, in shared memory: in the kernel's
 // parameters they are constants, which a warp reads one address at a time
-// (61316 tokens of one head: 24 us so, 9 from shared memory).
+// (61316 tokens of one head: 24 us so, 15.5 from shared memory).
 struct PairTurns {
     uint64_t turn[LWM_ROTARY_MAX_PAIRS];
     uint8_t axis[LWM_ROTARY_MAX_PAIRS];
