@@ -649,7 +649,9 @@ template <typename T, int D, bool kCodes, int kRows> cudaError_t launch(CacheAtt
     uint64_t span = a.c.max_length ? a.c.max_length : static_cast<uint64_t>(a.c.table_stride) << a.c.page_shift;
     if (a.window) span = min(span, static_cast<uint64_t>(a.window) * a.frame + a.sinks + a.c.max_new);
     const uint64_t units = (span + kUnit - 1) / kUnit;
-    if (units <= 8 && jobs >= 148 * 4) {
+    // A warp alone or four a job (bf16, 1024 sequences, 16 heads of 64 channels, one new token; us with the events
+    // around them): 16-bit pools, 192 tokens 109 and 140, 400 tokens 201 and 195; codes 138 and 132, 260 and 186.
+    if (units <= (kCodes ? 8 : 16) && jobs >= 148 * 4) {
         using S = Shape<D, kCodes, kRows, false>;
         // the heads in as many parts as run at once, evenly
         const uint64_t lots = static_cast<uint64_t>(a.c.sequences) * tiles, slots = 148 * kWarps * S::kBlocks;
