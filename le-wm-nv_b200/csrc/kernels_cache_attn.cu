@@ -645,9 +645,7 @@ template <typename T, int D, bool kCodes, int kRows> cudaError_t launch(CacheAtt
     const uint32_t tiles = (a.c.max_new * a.group + kRows - 1) / kRows;
     const uint64_t jobs = static_cast<uint64_t>(a.c.sequences) * a.c.kv_heads * tiles;
     a.tile_div = FastDiv(tiles);
-    // keys a row can see
-    uint64_t span = a.c.max_length ? a.c.max_length : static_cast<uint64_t>(a.c.table_stride) << a.c.page_shift;
-    if (a.window) span = min(span, static_cast<uint64_t>(a.window) * a.frame + a.sinks + a.c.max_new);
+    const uint64_t span = visible_span(a, kRows);
     const uint64_t units = (span + kUnit - 1) / kUnit;
     // A warp alone or four a job (bf16, 1024 sequences, 16 heads of 64 channels, one new token; us with the events
     // around them): 16-bit pools, 192 tokens 109 and 140, 400 tokens 201 and 195; codes 138 and 132, 260 and 186.

@@ -908,14 +908,13 @@ struct Costs {
 Costs costs_of(const CacheAttnArgs& a) {
     const bool wide = a.c.head_dim == 128;
     const double rows = static_cast<double>(a.c.max_new) * a.group, lots = static_cast<double>(a.c.sequences) * a.c.kv_heads;
-    double span = a.c.max_length ? a.c.max_length : static_cast<double>(a.c.table_stride) * a.c.page_tokens;
-    if (a.window) span = std::min(span, static_cast<double>(a.window) * a.frame + a.sinks + a.c.max_new);
-    const auto blocks_cost = [&](double block, double factor) {
+    const auto blocks_cost = [&](uint32_t block, double factor) {
         const double waves = std::max(1.0, lots * std::ceil(rows / block) / 148);
-        return waves * ((wide ? 9.0 : 6.5) + (wide ? 1.6 : 1.25) * factor * std::ceil(span / kTile));
+        const double tiles = std::ceil(static_cast<double>(visible_span(a, block)) / kTile);
+        return waves * ((wide ? 9.0 : 6.5) + (wide ? 1.6 : 1.25) * factor * tiles);
     };
     const double one = blocks_cost(kTile, 1.0), both = blocks_cost(2 * kTile, rows > kTile ? 1.5 : 1.0);
-    const double there = 6.0 + lots * std::ceil(rows / 16) * (std::ceil(span / 16) + 4) /
+    const double there = 6.0 + lots * std::ceil(rows / 16) * (std::ceil(static_cast<double>(visible_span(a, 16)) / 16) + 4) /
                                    (wide ? 1580.0 : a.c.head_dim == 64 ? 3100.0 : 3700.0);
     return {std::min(one, both), there, one < both ? kTile : 2u * kTile};
 }

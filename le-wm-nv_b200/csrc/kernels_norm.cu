@@ -195,39 +195,45 @@ __global__ void __launch_bounds__(256) gated_norm_kernel(GatedNormArgs g) {
     }
 }
 
-// Any width and alignment: a block a row, the row's values in shared memory.
-__device__ void norm_smem(float* v, int kind, const float* w, const float* b, float eps, uint32_t width, float* red) {
+// Any width and alignment: a warp or a block a row, the row's values in shared
+// memory.  us with the events around them: 20490 rows of 193, a warp each 51,
+// a block each 103; of 1001, 139 and 190; but 100 rows of 1001, 35 and 23.
+template <int kRow>
+__device__ __forceinline__ void norm_smem(float* v, int kind, const float* w, const float* b, float eps, uint32_t width,
+                                          uint32_t lane, float* red) {
     if (kind == LWM_NORM_NONE) return;
     const float inv_n = 1.0f / static_cast<float>(width);
     float mean = 0.0f;
     if (kind == LWM_NORM_LAYER) {
         float s = 0.0f;
-        for (uint32_t i = threadIdx.x; i < width; i += 256) s += v[i];
-        mean = row_sum<256>(s, red) * inv_n;
+        for (uint32_t i = lane; i < width; i += kRow) s += v[i];
+        mean = row_sum<kRow>(s, red) * inv_n;
     }
     float s = 0.0f;
-    for (uint32_t i = threadIdx.x; i < width; i += 256) {
+    for (uint32_t i = lane; i < width; i += kRow) {
         const float c = v[i] - mean;
         s += c * c;
     }
-    const float r = 1.0f / sqrtf(row_sum<256>(s, red) * inv_n + eps);
-    for (uint32_t i = threadIdx.x; i < width; i += 256) {
+    const float r = 1.0f / sqrtf(row_sum<kRow>(s, red) * inv_n + eps);
+    for (uint32_t i = lane; i < width; i += kRow) {
         float t = (v[i] - mean) * (w ? r * w[i] : r);
         if (b) t += b[i];
         v[i] = t;
     }
 }
-__global__ void __launch_bounds__(256) gated_norm_any_kernel(GatedNormArgs g) {
-    extern __shared__ float row[];  // [width], each thread touches its own elements only
+template <int kRow> __global__ void __launch_bounds__(256) gated_norm_any_kernel(GatedNormArgs g) {
+    extern __shared__ float rows[];  // [rows of the block][width], each thread touches its own elements only
     __shared__ float red[8];
     const lwm_gated_norm_args& a = g.a;
-    const uint32_t r = blockIdx.x;
+    const uint32_t lane = threadIdx.x % kRow, r = blockIdx.x * (256 / kRow) + threadIdx.x / kRow;
+    if (r >= a.rows) return;  // whole warps, or (kRow 256) never
+    float* row = rows + threadIdx.x / kRow * a.width;
     const size_t cond = static_cast<size_t>(g.cond_div.div(r)) * a.cond_stride;
     if (a.y) {
-        for (uint32_t i = threadIdx.x; i < a.width; i += 256) row[i] = load_one(a.y, r * a.y_stride + i, a.dtype);
-        norm_smem(row, a.post_kind, a.post_weight, a.post_bias, a.post_eps, a.width, red);
+        for (uint32_t i = lane; i < a.width; i += kRow) row[i] = load_one(a.y, r * a.y_stride + i, a.dtype);
+        norm_smem<kRow>(row, a.post_kind, a.post_weight, a.post_bias, a.post_eps, a.width, lane, red);
     }
-    for (uint32_t i = threadIdx.x; i < a.width; i += 256) {
+    for (uint32_t i = lane; i < a.width; i += kRow) {
         float x = load_one(a.x, r * a.x_stride + i, a.residual_dtype);
         if (a.y) {
             float y = row[i];
@@ -239,15 +245,15 @@ __global__ void __launch_bounds__(256) gated_norm_any_kernel(GatedNormArgs g) {
         if (a.x_out) store_one(a.x_out, r * a.x_out_stride + i, a.residual_dtype, x);
     }
     if (!a.h) return;
-    norm_smem(row, a.pre_kind, a.pre_weight, a.pre_bias, a.pre_eps, a.width, red);
-    for (uint32_t i = threadIdx.x; i < a.width; i += 256) {
+    norm_smem<kRow>(row, a.pre_kind, a.pre_weight, a.pre_bias, a.pre_eps, a.width, lane, red);
+    for (uint32_t i = lane; i < a.width; i += kRow) {
         float u = row[i];
         if (a.scale) u *= 1.0f + load_one(a.scale, cond + i, a.cond_dtype);
         if (a.shift) u += load_one(a.shift, cond + i, a.cond_dtype);
         row[i] = u;
     }
-    if (g.out_norm) norm_smem(row, LWM_NORM_LAYER, a.out_weight, a.out_bias, a.out_eps, a.width, red);
-    for (uint32_t i = threadIdx.x; i < a.width; i += 256) store_one(a.h, r * a.h_stride + i, a.dtype, row[i]);
+    if (g.out_norm) norm_smem<kRow>(row, LWM_NORM_LAYER, a.out_weight, a.out_bias, a.out_eps, a.width, lane, red);
+    for (uint32_t i = lane; i < a.width; i += kRow) store_one(a.h, r * a.h_stride + i, a.dtype, row[i]);
 }
 
 bool aligned(const void* p, uint64_t stride, size_t elem) {
@@ -300,7 +306,10 @@ cudaError_t launch_gated_norm(const GatedNormArgs& g, cudaStream_t s) {
             if (rt && ct) return launch_vectors<__half, __half, __half>(g, s);
         }
     }
-    gated_norm_any_kernel<<<a.rows, 256, a.width * sizeof(float), s>>>(g);
+    if (a.width <= 256 || (a.width <= 1024 && a.rows >= 148 * 16))
+        gated_norm_any_kernel<32><<<(a.rows + 7) / 8, 256, 8 * a.width * sizeof(float), s>>>(g);
+    else
+        gated_norm_any_kernel<256><<<a.rows, 256, a.width * sizeof(float), s>>>(g);
     return cudaGetLastError();
 }
 

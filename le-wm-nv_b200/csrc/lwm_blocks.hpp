@@ -92,6 +92,16 @@ struct CacheAttnArgs {
     FastDiv group_div, frame_div;
     FastDiv tile_div, kv_div;  // set by the launch
 };
+// Keys that a tile of query rows can see, by the sizes that the host knows.
+inline uint64_t visible_span(const CacheAttnArgs& a, uint32_t tile_rows) {
+    const uint64_t reach = a.c.max_length ? a.c.max_length : static_cast<uint64_t>(a.c.table_stride) << a.c.page_shift;
+    if (!a.window) return reach;
+    // the window of the tile's first token, up to the end of its last one's frame (or of the sequence)
+    const uint64_t tokens = static_cast<uint64_t>(tile_rows) / a.group + 1 + a.frame;
+    const uint64_t beyond = a.causal && tokens < a.c.max_new ? tokens : a.c.max_new;
+    const uint64_t keys = static_cast<uint64_t>(a.window) * a.frame + a.sinks + beyond;
+    return keys < reach ? keys : reach;
+}
 // Few query rows a kv head, and many.
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
 bool cache_attention_many_rows(const CacheAttnArgs& a);  // which of the two
