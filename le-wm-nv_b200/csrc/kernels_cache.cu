@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 
 // 8 bits; kLanes lanes a (page, head): 8 when a call brings a token or two a
 // sequence (a head's units fill no more), the whole block when pages are few
-// and full, a warp otherwise.  blockIdx.y: parts of the heads, where the
+// and full, else a warp.  blockIdx.y: parts of the heads, where the
 // pages alone are too few blocks.
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(kThreads) append_codes_kernel(const __grid_constant__ AppendArgs a, const CacheDivs d,
@@ -352,8 +352,11 @@ template <typename T> cudaError_t append(const AppendArgs& a, bool codes, cudaSt
         return cudaGetLastError();
     }
     const bool few = a.c.max_new <= 2;
-    // a block a (page, head) where a warp each would leave SMs idle
-    const bool block = !few && static_cast<uint64_t>(blocks) * 2 * a.c.kv_heads < 148 * 16;
+    // A block a (page, head) where pages are full enough for all its threads and too few for the GPU's warps; us with
+    // the events around them, a block and a warp each: 413 tokens of 3 sequences, 8 heads of 128, pages of 128, 42 and
+    // 86; 316 of 23, 16 of 64, 128, 72 and 94; 1024 of 64, 16 of 64, 128, 327 and 301; 19 of 146, 8 of 32, 32, 38 and 30.
+    const bool block = !few && min(tokens, a.c.max_new) * hu.count >= kThreads &&
+                       static_cast<uint64_t>(blocks) * 2 * a.c.kv_heads < 148 * 32;
     auto* kernel = few ? append_codes_kernel<T, 8> : block ? append_codes_kernel<T, kThreads> : append_codes_kernel<T, 32>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
