@@ -363,6 +363,24 @@ def test_append_8_bit_step_by_step(ctx, page, kv, d, dtype):
         have = lens
 
 
+@pytest.mark.parametrize("page,kv,d", [(128, 2, 64), (64, 8, 32), (16, 3, 64), (32, 1, 128)])
+@pytest.mark.parametrize("news", [[300, 0, 65, 1], [1, 2, 0, 1]])
+def test_append_8_bit_turns_queries_too(ctx, page, kv, d, news):
+    """q_out is what the rotary gives for the tokens' indexes, however the call deals out its heads; rows behind stay."""
+    lens = [n + 7 for n in news]
+    c = Paged(12, lens, page, kv, d, BF16, codes=True, fill=1.0)
+    g, tokens, r = gen(13), sum(news) + 2, L.Rotary.make([d], [1e4])
+    q, k, v = randn(g, tokens, 5, d), randn(g, tokens, kv, d), randn(g, tokens, kv, d)
+    q, k, v = q.to(BF16), k.to(BF16), v.to(BF16)
+    out, want = torch.full_like(q, 5.0), torch.empty_like(q)
+    L.cache_append_device(ctx, c.cache, c.batch(news, lengths=lens, tokens=tokens, max_new=max(news)), k, v, rotary=r, q=q,
+                          q_out=out)
+    index = np.concatenate([np.arange(n - m, n) for n, m in zip(lens, news)] + [np.zeros(2, int)])
+    L.rotary_device(ctx, r, q, want, ints(index)[:, None].contiguous())
+    ctx.synchronize()
+    assert torch.equal(out[:-2], want[:-2]) and (out[-2:] == 5.0).all()
+
+
 def test_append_8_bit_keeps_what_it_cannot_hold_visible(ctx):
     c = Paged(11, [3], 16, 1, 32, BF16, codes=True, fill=1.0)
     v = torch.ones(3, 1, 32, device="cuda", dtype=BF16) * 448
