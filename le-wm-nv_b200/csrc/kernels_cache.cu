@@ -358,7 +358,7 @@ template <typename T> cudaError_t append(const AppendArgs& a, bool codes, cudaSt
     const bool block = !few && min(tokens, a.c.max_new) * hu.count >= kThreads &&
                        static_cast<uint64_t>(blocks) * 2 * a.c.kv_heads < 148 * 32;
     auto* kernel = few ? append_codes_kernel<T, 8> : block ? append_codes_kernel<T, kThreads> : append_codes_kernel<T, 32>;
-    if (smem > 48 * 1024) {
+    if (smem > 40 * 1024) {  // with the static part beyond the 48 KB that need no leave
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
         if (e != cudaSuccess) return e;
     }

@@ -363,8 +363,8 @@ def test_append_8_bit_step_by_step(ctx, page, kv, d, dtype):
         have = lens
 
 
-@pytest.mark.parametrize("page,kv,d", [(128, 2, 64), (64, 8, 32), (16, 3, 64), (32, 1, 128)])
-@pytest.mark.parametrize("news", [[300, 0, 65, 1], [1, 2, 0, 1]])
+@pytest.mark.parametrize("page,kv,d", [(128, 2, 64), (64, 8, 32), (16, 3, 64), (32, 1, 128), (128, 2, 128)])
+@pytest.mark.parametrize("news", [[300, 0, 65, 1], [1, 2, 0, 1], [96, 3], [95, 80], [81]])
 def test_append_8_bit_turns_queries_too(ctx, page, kv, d, news):
     """q_out is what the rotary gives for the tokens' indexes, however the call deals out its heads; rows behind stay."""
     lens = [n + 7 for n in news]
