@@ -30,9 +30,17 @@
 // contraction's order is free, so a thread's 16 bytes of a key are the four
 // channels each of four k-steps, and Q is loaded in the same order; V's
 // bytes are interleaved by key pairs with byte permutes.  The key scale
-// multiplies the scores; the value scales are kept relative to the largest
-// so far, which multiplies O once at the end.  bf16 queries are brought to
-// fp16 by a power of two a row, exactly down to 2^-17 of the row's largest.
+// multiplies the scores.  A value scale 2^e f (f in [1, 2)) goes into the
+// weight before it is rounded: a row keeps, beside its maximum m and sum, the
+// power of two E of its largest weighted scale, and its weights for the
+// product are exp2(score - m + e - E) f, at most 2^9 and near one for the page
+// that counts most, whatever the scales of the others.  So a weight has two
+// exponentials, one for the sum and one for the product (one, times the row's
+// power of two, measured the same or slower; the ratio of the scales on the
+// finished weight, 0 to 8 % faster, loses what lies 2^14 below the largest
+// scale).  bf16 queries are
+// brought to fp16 by a power of two a row, exactly down to 2^-17 of the row's
+// largest.
 #include <cooperative_groups.h>
 
 #include "lwm_blocks.cuh"
@@ -125,7 +133,8 @@ template <int D, bool kCodes, int kRows, bool kShared> struct Shape {
     static constexpr int kWarpBytes = kStages * 2 * kUnitBytes;
     static constexpr int kPitch = D + 4;                             // floats of a row of O in shared memory
     static constexpr int kPartFloats = kRows * kPitch;               // a warp's O
-    static constexpr int kPartBytes = kShared ? (kPartFloats + 2 * kRows) * 4 : 0;  // maxima and sums too
+    static constexpr int kPart = kPartFloats + (kCodes ? 3 : 2) * kRows;  // maxima, sums (and powers of two) too
+    static constexpr int kPartBytes = kShared ? kPart * 4 : 0;
     static constexpr int kRings = kWarps * (kWarpBytes > kPartBytes ? kWarpBytes : kPartBytes);
     // and the units' pages and scales; alone, a warp's output rows
     static constexpr int kBytes = kRings + kWarps * kStages * 16 + (kShared ? 0 : kWarps * kRows * D * 2);
@@ -133,6 +142,11 @@ template <int D, bool kCodes, int kRows, bool kShared> struct Shape {
     static constexpr int kBySmem = 220 * 1024 / (kBytes + 1024), kByRegs = kRows == 8 ? (D == 128 ? 4 : 5) : (D == 128 ? 3 : 4);
     static constexpr int kBlocks = kBySmem < kByRegs ? kBySmem : kByRegs;
 };
+
+// 2^e of a whole number in [-126, 127] (any other: the nearer end).
+__device__ __forceinline__ float power_of_two(float e) {
+    return __uint_as_float(static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(e, -126.0f), 127.0f)) + 127) << 23);
+}
 
 // A unit in flight: its page (-1: none) and, of codes, the page's scales.
 struct UnitNote {
@@ -344,7 +358,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][d][e] = 0.0f;
     }
-    float v_ref = 0.0f;  // 8 bits: O is in units of this value scale
+    float vx[kQ][2];  // 8 bits: O is in units of 2^vx (a whole number) times the weights' 2^m
+#pragma unroll
+    for (int n = 0; n < kQ; ++n) vx[n][0] = vx[n][1] = INFINITY;  // (no key yet)
 
     // (not unrolled over the ring: copies of the body missed the instruction cache)
 #pragma unroll 1
@@ -354,11 +370,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         const int page = notes[slot].page;
         const uint32_t key = key_of(i);
         const uint32_t k_at = ring_a + slot * 2 * S::kUnitBytes, v_at = k_at + S::kUnitBytes;
-        float k_scale = 1.0f, v_scale = 1.0f;
+        float k_scale = 1.0f, v_exp = 0.0f, v_frac = 1.0f;
         if constexpr (kCodes) {
             k_scale = notes[slot].k_scale;
-            v_scale = page < 0 ? 1.0f : notes[slot].v_scale;
+            float v_scale = page < 0 ? 1.0f : notes[slot].v_scale;
             if (!isfinite(v_scale)) v_scale = __int_as_float(0x7fc00000);
+            const int e = min(max(static_cast<int>((__float_as_uint(v_scale) >> 23) & 255) - 127, -126), 126);
+            v_exp = static_cast<float>(e);
+            v_frac = v_scale * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
         }
         // scores: element e is key g + 8 (e >> 1), query 2 t + (e & 1); two chains of products
         float sc[kQ][4], odd[kQ][4];
@@ -413,10 +432,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
             for (int e = 0; e < 4; ++e) {
                 sc[n][e] = (sc[n][e] + odd[n][e]) * (k_scale * row_mul[n][e & 1]);
                 if (!whole && !sees(n, e)) sc[n][e] = -INFINITY;
-                above |= sc[n][e] > m[n][e & 1] + kRaise;
+                const float lift = kCodes ? fmaxf(v_exp - vx[n][e & 1], 0.0f) : 0.0f;
+                above |= sc[n][e] > m[n][e & 1] + (kRaise - lift);
             }
-        // the maximum moves only when a score passes it by kRaise: until
-        // then exp2(score - m) stays below 2^kRaise
+        // the maximum (of the scores, and of them with their scales) moves
+        // only when a score passes it by kRaise: until then exp2(score - m),
+        // scaled or not, stays below 2^kRaise
         if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
             for (int n = 0; n < kQ; ++n)
@@ -426,32 +447,27 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    const float here = x;  // this unit's largest
                     x = fmaxf(x, m[n][e]);
-                    const float down = m[n][e] == -INFINITY ? 0.0f : exp2_fast(m[n][e] - x);
+                    const bool first = m[n][e] == -INFINITY;
+                    const float down = first ? 0.0f : exp2_fast(m[n][e] - x);
+                    float o_down = down;
+                    if constexpr (kCodes) {
+                        // (m - x and the powers of two are differences of near numbers, so nothing is lost far from zero)
+                        const float kept = first ? -INFINITY : (m[n][e] - x) + vx[n][e];
+                        const float to = x == -INFINITY ? INFINITY : ceilf(fmaxf(kept, (here - x) + v_exp));
+                        o_down = first ? 0.0f : exp2_fast(kept - to);
+                        vx[n][e] = to;
+                    }
                     m[n][e] = x;
                     if (i == 0) continue;
                     l[n][e] *= down;
 #pragma unroll
                     for (int d = 0; d < kSteps; ++d) {
-                        o[n][d][e] *= down;
-                        o[n][d][e + 2] *= down;
+                        o[n][d][e] *= o_down;
+                        o[n][d][e + 2] *= o_down;
                     }
                 }
-        }
-        float v_mul = 1.0f;
-        if constexpr (kCodes) {
-            if (i == 0 && v_scale > 0.0f) v_ref = v_scale;
-            if (v_scale > v_ref) {
-                const float down = v_ref / v_scale;
-#pragma unroll
-                for (int n = 0; n < kQ; ++n)
-#pragma unroll
-                    for (int d = 0; d < kSteps; ++d)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[n][d][e] *= down;
-                v_ref = v_scale;
-            }
-            v_mul = v_scale == v_ref ? 1.0f : v_scale == 0.0f ? 0.0f : v_scale / v_ref;
         }
         // P in the operands' type: 2^-9 (bf16) or 2^-12 (fp16) of itself,
         // no more than rounding the output costs
@@ -461,10 +477,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         for (int n = 0; n < kQ; ++n) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float top = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
-                p[n][e] = exp2_fast(sc[n][e] - top);
+                const float over = sc[n][e] - (m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1]);
+                p[n][e] = exp2_fast(over);
                 l[n][e & 1] += p[n][e];
-                if constexpr (kCodes) p[n][e] *= v_mul;
+                if constexpr (kCodes) p[n][e] = exp2_fast(over + (v_exp - vx[n][e & 1])) * v_frac;
             }
             pb[n][0] = turn_over(pack2(p[n][0], p[n][1], M{}));
             pb[n][1] = turn_over(pack2(p[n][2], p[n][3], M{}));
@@ -484,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
 #pragma unroll
                 for (int e = 0; e < 4; ++e) poison |= any_not_finite<T, kCodes>(w[e]);
             }
-            poison |= kCodes && v_scale != v_scale;
+            poison |= kCodes && v_frac != v_frac;
             poison = __any_sync(0xffffffffu, poison);
         }
         if (!poison) {
@@ -560,12 +576,13 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         for (int n = 0; n < kQ; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float inv = (l[n][e] == 0.0f ? 0.0f : 1.0f / l[n][e]) * (kCodes ? v_ref : 1.0f);
+                const float inv = l[n][e] == 0.0f ? 0.0f : 1.0f / l[n][e];
+                const float unit = kCodes ? power_of_two(vx[n][e]) : 1.0f;
 #pragma unroll
                 for (int d = 0; d < kSteps; ++d)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        part[(8 * n + 2 * t + e) * D + channel(d, x)] = static_cast<T>(o[n][d][2 * x + e] * inv);
+                        part[(8 * n + 2 * t + e) * D + channel(d, x)] = static_cast<T>(o[n][d][2 * x + e] * inv * unit);
             }
         __syncwarp();
         for (int x = lane; x < kRows * D / 8; x += 32) {
@@ -581,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         cp_wait<0>();
         __syncthreads();  // every ring is done with
         float* parts = reinterpret_cast<float*>(smem);
-        constexpr int kPart = S::kPartFloats + 2 * kRows;
+        constexpr int kPart = S::kPart;
         float* mine = parts + warp * kPart;
 #pragma unroll
         for (int n = 0; n < kQ; ++n)
@@ -592,10 +609,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
                 for (int d = 0; d < kSteps; ++d)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        mine[r * S::kPitch + channel(d, x)] = o[n][d][2 * x + e] * (kCodes ? v_ref : 1.0f);
+                        mine[r * S::kPitch + channel(d, x)] = o[n][d][2 * x + e];
                 if (g == 0) {
                     mine[S::kPartFloats + r] = m[n][e];
                     mine[S::kPartFloats + kRows + r] = l[n][e];
+                    if constexpr (kCodes) mine[S::kPartFloats + 2 * kRows + r] = vx[n][e];
                 }
             }
         if (split > 1) cg::this_cluster().sync();
@@ -612,6 +630,18 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
 #pragma unroll
                     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, p[w * kPart + S::kPartFloats + r]);
                 }
+                float unit = -INFINITY;  // 8 bits: the power of two of the joined O
+                if constexpr (kCodes) {
+                    for (uint32_t b = 0; b < split; ++b) {
+                        const float* p = split > 1 ? cg::this_cluster().map_shared_rank(parts, b) : parts;
+#pragma unroll
+                        for (int w = 0; w < kWarps; ++w) {
+                            const float* pw = p + w * kPart + S::kPartFloats + r;
+                            if (pw[kRows] != 0.0f) unit = fmaxf(unit, (pw[0] - top) + pw[2 * kRows]);
+                        }
+                    }
+                    unit = ceilf(unit);
+                }
                 float sum = 0.0f;
                 float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 for (uint32_t b = 0; b < split; ++b) {
@@ -621,18 +651,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
                         const float* pw = p + w * kPart;
                         const float mw = pw[S::kPartFloats + r], lw = pw[S::kPartFloats + kRows + r];
                         if (lw == 0.0f) continue;  // saw nothing
-                        const float f = exp2_fast(mw - top);
+                        const float lf = exp2_fast(mw - top);
+                        const float f = kCodes ? exp2_fast((mw - top) + (pw[S::kPartFloats + 2 * kRows + r] - unit)) : lf;
                         const float4 ov = *reinterpret_cast<const float4*>(pw + r * S::kPitch + c4);
-                        sum += lw * f;
+                        sum += lw * lf;
                         acc.x += ov.x * f;
                         acc.y += ov.y * f;
                         acc.z += ov.z * f;
                         acc.w += ov.w * f;
                     }
                 }
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, up = kCodes ? power_of_two(unit) : 1.0f;
                 const uint32_t tok = a.group_div.div(R), head = h * a.group + (R - tok * a.group);
-                uint2 w2 = make_uint2(pack2(acc.x * inv, acc.y * inv, T{}), pack2(acc.z * inv, acc.w * inv, T{}));
+                uint2 w2 = make_uint2(pack2(acc.x * inv * up, acc.y * inv * up, T{}), pack2(acc.z * inv * up, acc.w * inv * up, T{}));
                 *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (v.start + tok) * a.o_ts + head * a.o_hs + c4) = w2;
             }
         }
