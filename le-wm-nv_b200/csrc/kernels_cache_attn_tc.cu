@@ -45,7 +45,13 @@
 // each thread expands what it copied itself.  Their scales stay out of the
 // products: a page's key scale multiplies its 16-key groups' scores, its value
 // scale, relative to the block's largest (which the warps beside the issuer
-// find meanwhile), enters the exponent of the weight.
+// find meanwhile), enters the exponent of the weight, before a row's maximum m
+// is taken.  The row's sum takes it out again, by a factor for each 16 keys;
+// where a page lies more than 2^60 below the largest (kFar) its weights may
+// vanish although the softmax gives them all, so their sum is taken from the
+// scores once more, against a maximum of its own that is never below m.  Only
+// a block that sees such pages runs that form of the loop (frames on codes:
+// 67.7 us; one loop for both, with more registers alive, 69.7).
 //
 // O is rescaled only when a score passes a row's maximum by more than kRaise
 // (a factor of 2^8).
@@ -72,14 +78,16 @@ constexpr int kScaleThreads = 96;    // of the warps beside the MMA issuer
 constexpr int kPanel = kTile * 128;  // bytes of 128 rows x 64 channels
 constexpr int kInfos = 4;
 constexpr uint32_t kOCol = 256;
+constexpr float kFar = 0x1p-60f;     // ratio of a value scale to the largest below which its sum goes by itself
 
 // What the softmax needs of a key tile, by 16-key groups.
 struct TileInfo {
     float k_scale[8];  // codes: key scales
     float v_log[8];    // log2 of the value scale relative to the block's
-    float v_inv[8];    // its reciprocal
+    float v_inv[8];    // that ratio's reciprocal, 0 below kFar
     uint32_t ok;       // groups whose page is in the pool
-    uint32_t pad[7];
+    uint32_t far;      // groups below kFar
+    uint32_t pad[6];
 };
 
 // A tile of codes in flight, by 16-key groups, a copy for each producer warp.
@@ -94,7 +102,8 @@ struct Control {
     int dead;        // a wait gave up
     int poisoned;    // infinities or NaN were taken out of a V tile
     float v_ref;     // codes: the largest value scale of the visible pages
-    float reduce[4];
+    int wide;        // codes: some visible page lies below kFar of it
+    float high[3], low[3];
     TileInfo info[kInfos];
 };
 
@@ -255,8 +264,8 @@ template <typename T> __device__ __forceinline__ bool take_out(uint4& x) {
 }
 
 // The weights exp2(score - maximum) of a row's 64 keys, packed for the
-// product, their sum (the value scales taken out again) and the largest
-// exponent.  kMasked: only the keys that the row sees.
+// product, their sum (the value scales taken out again, far groups left out)
+// and the largest exponent.  kMasked: only the keys that the row sees.
 template <typename M, bool kCodes, bool kMasked>
 __device__ __forceinline__ float weights(const float (&x)[64], uint32_t (&p)[32], float2& sum, const TileInfo& info,
                                          int half, float mul, float sub, const VisibleRange& rr, uint32_t key, uint32_t ok) {
@@ -302,6 +311,32 @@ __device__ __forceinline__ float weights(const float (&x)[64], uint32_t (&p)[32]
     return fmaxf(top0, top1);
 }
 
+// Adds the far groups' weights of a row's 64 keys (scores at `t_scores`) to
+// l, which is in units of 2^ml.
+__device__ __forceinline__ void far_sum(uint32_t t_scores, const TileInfo& info, int half, float mul, const VisibleRange& rr,
+                                     uint32_t key, float& l, float& ml) {
+#pragma unroll 1
+    for (int g = 0; g < 4; ++g) {
+        const int group = 4 * half + g;
+        if (!((info.far >> group) & 1)) continue;
+        float x[16];
+        tc::tmem_ld16(t_scores + 16 * g, x);
+        tc::tmem_ld_wait();
+        const uint32_t k16 = key + 16 * group, seen = below(rr.hi, k16) & (~below(rr.lo, k16) | below(rr.first, k16));
+        const float gm = info.k_scale[group] * mul;
+        float top = ml;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            x[e] = (seen >> e) & 1 ? x[e] * gm : -INFINITY;
+            top = fmaxf(top, x[e]);
+        }
+        if (top > ml) l *= exp2_fast(ml - top), ml = top;
+        const float sub = ml == -INFINITY ? 0.0f : ml;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) l += exp2_fast(x[e] - sub);
+    }
+}
+
 template <typename T, int D, bool kCodes>
 __global__ void __launch_bounds__(kThreads, 1)
     cache_attn_tc_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ CUtensorMap k_map,
@@ -343,6 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ctl->dead = 0;
         ctl->poisoned = 0;
         ctl->v_ref = 1.0f;
+        ctl->wide = 0;
         tc::mbar_fence_init();
     }
     if (warp == 12) tc::tmem_alloc(&ctl->tmem, 512);
@@ -421,7 +457,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fine = wait(&ctl->s_full[tile], i & 1, ctl, 10 + tile, err, s);
                 if (fine && lane < 2) tc::mbar_arrive(&ctl->p_full[tile][lane]);
             }
-            for (uint32_t i = 0; i < w.tiles && fine && !idle; ++i) {
+            // the tiles one after another; returns the root of O's unit over l's
+            auto walk = [&](auto far_apart) {
+            constexpr bool kWide = decltype(far_apart)::value;
+            float ml = -INFINITY;  // wide: l is in units of 2^ml, ml >= m
+            for (uint32_t i = 0; i < w.tiles && fine; ++i) {
                 // (the producers' notes are there long before the scores)
                 const TileInfo& info = ctl->info[i % kInfos];
                 fine = wait(&ctl->info_full[i % kInfos], (i / kInfos) & 1, ctl, 12 + tile, err, s);
@@ -450,7 +490,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         again = true;
                         const float up = first ? top : fmaxf(top, 0.0f), down = first ? 0.0f : exp2_fast(-up);
                         m = first ? top : m + up;
-                        l *= down;
+                        if constexpr (kWide) {
+                            if (m > ml) l *= exp2_fast(ml - m), ml = m;
+                        } else {
+                            l *= down;
+                        }
                         if (i > 0 || half) {  // O holds every product up to here once the last one is done
                             fine = half ? wait(&ctl->o_half[tile], i & 1, ctl, 14 + tile, err, s)
                                         : wait(&ctl->o_done[tile], (i - 1) & 1, ctl, 14 + tile, err, s);
@@ -471,7 +515,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc::tmem_ld_wait();
                     }
                     if (!fine) break;
-                    l += sum.x + sum.y;
+                    if constexpr (kWide) {
+                        l += (sum.x + sum.y) * (m == ml ? 1.0f : exp2_fast(m - ml));
+                        if ((info.far >> (4 * half)) & 0xfu) far_sum(t_s + kHalf * half, info, half, mul, rr, key, l, ml);
+                    } else {
+                        l += sum.x + sum.y;
+                    }
 #pragma unroll
                     for (int c = 0; c < 32; c += 8)
                         tc::tmem_st8u(t_s + 32 * half + c, reinterpret_cast<const uint32_t(&)[8]>(p[c]));
@@ -481,9 +530,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) tc::mbar_arrive(&ctl->p_full[tile][half]);
                 }
             }
+            // (twice the root of 2^(m - ml), as the whole may be below the smallest float)
+            return kWide && m != ml ? exp2_fast(0.5f * (m - ml)) : 1.0f;
+            };
+            float root = 1.0f;
+            if constexpr (kCodes) {
+                bool wide = false;
+                if (w.tiles && !idle) {
+                    fine = wait(&ctl->info_full[0], 0, ctl, 12 + tile, err, s);
+                    wide = fine && ctl->wide != 0;
+                }
+                if (wide) root = walk(std::true_type{});
+                else if (!idle) walk(std::false_type{});
+            } else if (!idle) {
+                walk(std::false_type{});
+            }
             if (fine && w.tiles) fine = wait(&ctl->o_done[tile], (w.tiles - 1) & 1, ctl, 16 + tile, err, s);
             tc::fence_after();
-            const float inv = l == 0.0f ? 0.0f : (kCodes ? ctl->v_ref : 1.0f) / l;
+            const float inv = l == 0.0f ? 0.0f : (kCodes ? ctl->v_ref * root : 1.0f) / l;
             const bool poisoned = *static_cast<volatile int*>(&ctl->poisoned) != 0;
             // rows go through the tile's Q, which no product reads any more, and out in whole 16-byte runs
             uint8_t* stage = smem + S::kQ + tile * S::kTileBytes;
@@ -495,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc::tmem_ld_wait();
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = l == 0.0f ? 0.0f : o[e] * inv;
+                for (int e = 0; e < 16; ++e) o[e] = l == 0.0f ? 0.0f : kCodes ? o[e] * inv * root : o[e] * inv;
                 if (poisoned && live) {
                     // a value that is not finite, in a tile where rows differ in what they see: its weight is
                     // positive, so it decides its channel for the rows that see it
@@ -668,11 +732,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (warp != 8 + static_cast<int>(i & 3) || lane >= 8) return;
                 TileInfo& info = ctl->info[i % kInfos];
                 if constexpr (kCodes) {
-                    float ratio = isfinite(v_scale) && pages >= 0 ? v_scale * v_ref_inv : 1.0f;
-                    ratio = fmaxf(ratio, 0x1p-60f);  // halves of such weights are zero
+                    const float ratio = isfinite(v_scale) && pages >= 0 ? v_scale * v_ref_inv : 1.0f;
+                    const bool is_far = ratio < kFar;
+                    const uint32_t far = __ballot_sync(0xffu, is_far);
                     info.k_scale[lane] = k_scale;
                     info.v_log[lane] = log2f(ratio);
-                    info.v_inv[lane] = 1.0f / ratio;
+                    info.v_inv[lane] = is_far ? 0.0f : 1.0f / ratio;
+                    if (is_far) info.v_log[lane] = log2f(v_scale) + log2f(v_ref_inv);  // (the ratio may vanish)
+                    if (lane == 0) info.far = far;
                 }
                 const uint32_t ok = __ballot_sync(0xffu, pages >= 0);
                 if (lane == 0) info.ok = ok;
@@ -689,10 +756,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::mbar_arrive(&ctl->k_full[st]);
                 if (i == 0) {  // the idle warps' maximum
                     asm volatile("bar.sync 1, %0;" ::"n"(kProducers + kScaleThreads) : "memory");
-                    float top = fmaxf(fmaxf(ctl->reduce[0], ctl->reduce[1]), ctl->reduce[2]);
+                    float top = fmaxf(fmaxf(ctl->high[0], ctl->high[1]), ctl->high[2]);
+                    const float low = fminf(fminf(ctl->low[0], ctl->low[1]), ctl->low[2]);
                     if (top == 0.0f) top = 1.0f;
                     v_ref_inv = 1.0f / top;
-                    if (t == 0) ctl->v_ref = top;
+                    if (t == 0) ctl->v_ref = top, ctl->wide = low * v_ref_inv < kFar;
                 }
                 inform();
                 const bool more = i + S::kRaw < w.tiles;
@@ -842,21 +910,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::mbar_wait_landing(&ctl->drain, 0);
             tc::fence_before();
         } else if (kCodes && w.tiles) {
-            // ------------------- the largest value scale of the visible pages
-            float top = 0.0f;
+            // ------- the largest and smallest value scale of the visible pages
+            float top = 0.0f, low = INFINITY;
             for (uint32_t i = threadIdx.x - 13 * 32; i < w.tiles * 8; i += kScaleThreads) {
                 const uint32_t j = w.key0(i / 8) + 16 * (i % 8);
                 if (j < w.hi_max && (j + 16 > w.lo_min || j < w.sinks_end)) {
                     const int p = a.c.table[static_cast<size_t>(s) * a.c.table_stride + (j >> a.c.page_shift)];
                     if (static_cast<uint32_t>(p) < a.c.pages) {
                         const float x = a.c.v_scale[static_cast<size_t>(p) * a.c.kv_heads + h];
-                        if (isfinite(x)) top = fmaxf(top, x);
+                        if (isfinite(x)) top = fmaxf(top, x), low = fminf(low, x);
                     }
                 }
             }
 #pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (lane == 0) ctl->reduce[warp - 13] = top;
+            for (int o = 16; o; o >>= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+            }
+            if (lane == 0) ctl->high[warp - 13] = top, ctl->low[warp - 13] = low;
             __syncwarp();
             asm volatile("bar.arrive 1, %0;" ::"n"(kProducers + kScaleThreads) : "memory");
         }

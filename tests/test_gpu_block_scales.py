@@ -109,6 +109,13 @@ def test_scales_apart_on_many_rows(ctx, exponents, marked, dtype, d):
     check_far_apart(ctx, exponents, marked, dtype, d, [60, 1, 130], True)
 
 
+@pytest.mark.parametrize("exponents,marked", FAR)
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_scales_far_apart_on_many_rows(ctx, exponents, marked, d):
+    """Pages more than 2^60 below the block's largest: their weights vanish from its products, not from its sums."""
+    check_far_apart(ctx, exponents, marked, BF16, d, [60, 1, 130], True)
+
+
 def check_outside_the_window(ctx, exponents, marked, many):
     """Rows of one tile, some of which see the large pages and some not: each row as if it were alone."""
     c = filled(203, [400, 333], 32, 1, 64, BF16, exponents, marked)
@@ -124,6 +131,21 @@ def test_large_scales_outside_the_window(ctx, exponents, marked):
 @pytest.mark.parametrize("exponents,marked", [SPREADS[0], SPREADS[3]])
 def test_large_scales_outside_the_window_on_many_rows(ctx, exponents, marked):
     check_outside_the_window(ctx, exponents, marked, True)
+
+
+@pytest.mark.parametrize("exponents,marked", FAR)
+def test_far_scales_outside_the_window_on_many_rows(ctx, exponents, marked):
+    check_outside_the_window(ctx, exponents, marked, True)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_far_scales_come_and_go(ctx, d):
+    """Large pages before, after and between small ones over several key tiles, rows that begin with either."""
+    for exponents, marked in (([-100] * 5 + [60], [5]), ([60] + [-100] * 8, [0]), ([-110, -110, 0, 100], [2, 3]),
+                              ([-120] * 9 + [119], [9])):
+        c = filled(218, [700, 257], 64, 1, d, BF16, exponents, marked)
+        check(ctx, c, [400, 257], 2, 219, offsets_of(exponents), True)
+        check(ctx, c, [300, 130], 2, 220, offsets_of(exponents), True, window=150, sinks=30)
 
 
 @pytest.mark.parametrize("exponents,marked", [SPREADS[1], FAR[0], FAR[2]])
@@ -153,7 +175,7 @@ def test_scales_far_apart_in_many_short_sequences(ctx):
 @pytest.mark.parametrize("many", [False, True])
 def test_a_row_does_not_depend_on_scales_it_does_not_see(ctx, many):
     """The same rows over a window of small pages, with and without large pages before it: equal to one rounding."""
-    n, large = (140, 30) if many else (3, 100)
+    n, large = (140, 100) if many else (3, 100)
     c = filled(212, [600], 32, 1, 64, BF16, [-30], [0])
     want = check(ctx, c, [n], 2, 213, [0.0], many, window=160 if many else 100)[:n].double()
     for j in range((600 - n - (160 if many else 100)) // 32):
