@@ -3,6 +3,7 @@
 // gated-norm kernels.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <string>
@@ -338,7 +339,7 @@ lwm_status lwm_gated_norm_device(lwm_ctx* ctx, const lwm_gated_norm_args* x) {
     lwm::GatedNormArgs a{};
     a.a = *x;
     a.out_norm = x->out_weight != nullptr;
-    a.cond_div = lwm::FastDiv(cond ? x->rows_per_cond : 1);
+    a.cond_div = lwm::FastDiv(cond ? std::min(x->rows_per_cond, x->rows) : 1);  // (more rows than there are: one for all)
     return on_device(ctx, c, "gated norm", [&](cudaStream_t s) { return lwm::launch_gated_norm(a, s); });
 }
 

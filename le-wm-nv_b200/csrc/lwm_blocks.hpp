@@ -12,7 +12,8 @@
 namespace lwm {
 
 // Division by a launch constant: q = (n * mul) >> 32 >> shift, exact for
-// n < 2^31 (mul = ceil(2^(32 + shift) / d), shift = ceil(log2 d)).
+// n < 2^31 and 0 < d <= 2^31 (mul = ceil(2^(32 + shift) / d) - 2^32, shift =
+// ceil(log2 d), which is 32 for larger d and no shift of 32 bits).
 struct FastDiv {
     uint32_t d = 1, mul = 0, shift = 0;
     FastDiv() = default;

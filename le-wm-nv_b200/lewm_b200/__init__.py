@@ -1275,6 +1275,13 @@ def _u32(name: str, x: int) -> None:
         raise LwmError(1, f"{name} must be 0 to 2^32 - 1, got {x}")
 
 
+def _sizes(name: str, shape) -> None:
+    """Sizes go into 32-bit fields, which would cut them; a stride of zero makes a tensor of any size."""
+    for n in shape:
+        if n >> 32:
+            raise LwmError(1, f"{name} must have sizes below 2^32, got {list(shape)}")
+
+
 class PagedCache:
     """lwm_paged_cache over torch tensors: k, v [pages, kv_heads, page_tokens,
     head_dim] in bfloat16 or float16, or 8-bit codes (float8_e4m3fn or uint8)
@@ -1317,6 +1324,7 @@ class CacheBatch:
         if table.dim() != 2:
             raise LwmError(1, "page table must be [sequences, pages]")
         n = table.shape[0]
+        _sizes("page table", table.shape)
         _ints("page table", table, tuple(table.shape))
         _ints("starts", starts, (n + 1,))
         _ints("lengths", lengths, (n,))
@@ -1343,6 +1351,8 @@ def rotary_device(ctx: Context, rotary: Rotary, x, out, positions, inverse: bool
     if x.dim() != 3:
         raise LwmError(1, f"x must be [tokens, heads, head_dim], got {list(x.shape)}")
     tokens, heads, d = shape = x.shape
+    if (tokens | heads | d) >> 32:  # any of them
+        _sizes("x", shape)
     _ints("positions", positions, (tokens, rotary.axes))
     xp, xt, xh = _heads(ctx, "x", x, shape, x.dtype)
     op, ot, oh = _heads(ctx, "out", out, shape, x.dtype)
@@ -1371,6 +1381,8 @@ def cache_append_device(ctx: Context, cache: PagedCache, batch: CacheBatch, k, v
             raise LwmError(1, "q [tokens, heads, head_dim] needs q_out")
         heads = q.shape[1]
         shape = (n, heads, cache.head_dim)
+        if heads >> 32:
+            _sizes("q", q.shape)
         qp, qt, qh = _heads(ctx, "q", q, shape, dtype)
         op, ot, oh = _heads(ctx, "q_out", q_out, shape, dtype)
         a = _CacheAppendArgs(qp, op, kp, vp, qt, qh, ot, oh, kt, kh, vt, vh, pos, heads)
@@ -1403,6 +1415,8 @@ def cache_attention_device(ctx: Context, cache: PagedCache, batch: CacheBatch, q
         for name, x in (("window", window), ("sinks", sinks), ("frame_tokens", frame_tokens)):
             _u32(name, x)
     heads = q.shape[1]
+    if heads >> 32:
+        _sizes("q", q.shape)
     shape = (batch.tokens, heads, cache.head_dim)
     qp, qt, qh = _heads(ctx, "q", q, shape, cache.dtype)
     op, ot, oh = _heads(ctx, "out", out, shape, cache.dtype)
@@ -1460,6 +1474,9 @@ def gated_norm_device(ctx: Context, norm: GatedNorm, x, y=None, x_out=None, h=No
     if x.dim() != 2:
         raise LwmError(1, f"x must be [rows, width], got {list(x.shape)}")
     rows, width = x.shape
+    if (rows | width | rows_per_cond) >> 32:  # any of them
+        _sizes("x", x.shape)
+        _u32("rows_per_cond", rows_per_cond)
     if norm.width is not None and (norm.width != width or norm.device_index != ctx.device):
         raise LwmError(1, f"gated norm weights are [{norm.width}] on {norm.device}, x is {list(x.shape)} on {x.device}")
     xp, xs = _rows(ctx, "x", x, x, width)

@@ -242,3 +242,43 @@ def test_python_checks_name_the_tensor():
     with pytest.raises(L.LwmError, match="width or device"):
         L.GatedNorm(pre_weight=torch.ones(8), pre_bias=torch.ones(9))
     assert L.GatedNorm(pre_weight=torch.ones(8)).width == 8
+
+
+def _huge(*shape, dtype=torch.bfloat16):
+    """A tensor of any shape without memory; its device counts as -1, which is what the context below says."""
+    return torch.empty(shape, device="meta", dtype=dtype)
+
+
+class _NoContext:
+    device, handle = -1, None
+
+
+TOO_MANY = (1 << 32) + 1  # one, when cut to 32 bits
+
+
+@pytest.mark.parametrize("rows_per_cond", [TOO_MANY, 1 << 32, 1 << 63, -1, 0])
+def test_rows_per_cond_is_not_cut_to_32_bits(rows_per_cond):
+    """Cut, it would be 1, and row r would read conditioning row r of a table with one row."""
+    x = torch.zeros(4, 8)
+    with pytest.raises(L.LwmError, match="rows_per_cond must be 0 to" if rows_per_cond else "gate must be"):
+        L.gated_norm_device(_NoContext, L.GatedNorm(), x, h=x, gate=torch.zeros(1, 8), rows_per_cond=rows_per_cond)
+
+
+def test_sizes_are_not_cut_to_32_bits():
+    r, n = L.Rotary.make([64], [1e4]), TOO_MANY
+    cache = L.PagedCache(_huge(4, 2, 16, 64), _huge(4, 2, 16, 64))
+    i32 = torch.int32
+    batch = L.CacheBatch(torch.zeros(1, 2, dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(1, dtype=i32), 1)
+    pos, q, kv, x = _huge(1, 1, dtype=i32), _huge(1, n, 64), _huge(1, 2, 64), _huge(n, 1, 64)
+    for name, call in (
+            ("x", lambda: L.rotary_device(_NoContext, r, x, x, _huge(n, 1, dtype=i32))),
+            ("x", lambda: L.rotary_device(_NoContext, r, q, q, pos)),
+            ("x", lambda: L.rotary_device(_NoContext, r, _huge(1, 1, n), _huge(1, 1, n), pos)),
+            ("q", lambda: L.cache_append_device(_NoContext, cache, batch, kv, kv, q=q, q_out=q)),
+            ("q", lambda: L.cache_attention_device(_NoContext, cache, batch, q, q)),
+            ("x", lambda: L.gated_norm_device(_NoContext, L.GatedNorm(), x[:, 0], h=x[:, 0])),
+            ("x", lambda: L.gated_norm_device(_NoContext, L.GatedNorm(), q[:, :, 0], h=q[:, :, 0])),
+            ("page table", lambda: L.CacheBatch(_huge(n, 2, dtype=i32), _huge(n + 1, dtype=i32), _huge(n, dtype=i32), 1)),
+            ("page table", lambda: L.CacheBatch(_huge(1, n, dtype=i32), _huge(2, dtype=i32), _huge(1, dtype=i32), 1))):
+        with pytest.raises(L.LwmError, match=f"{name} must have sizes below"):
+            call()
