@@ -389,12 +389,18 @@ def _lib():
         if "le-wm-nv_b200" not in sys.path:
             sys.path.insert(0, "le-wm-nv_b200")
         import lewm_b200
-        _context = (lewm_b200, lewm_b200.Context(0))
+        ctx = lewm_b200.Context(0)
+        # The calls run on the context's own stream.  A program that uses them works on it throughout, as a callback
+        # scorer does, and waits once for what it had in hand before.
+        stream = ctx.torch_stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(stream)
+        _context = (lewm_b200, ctx, stream, torch.accelerator.current_stream(), torch.cuda.Event(), torch.cuda.Event())
     return _context
 
 
 def _own(st):
-    L, ctx = _lib()
+    L, ctx, stream, usual, ready, done = _lib()
     case, op = st["case"], st["case"]["op"]
     plan = st.get("plan")
     if plan is None:  # what a program lays out once for a model and a batch
@@ -425,6 +431,20 @@ def _own(st):
             plan["gate"] = t[:, :w] if case["gate"] else None
             plan["shift"] = t[:, w:2 * w] if case["modulate"] else None
             plan["scale"] = t[:, 2 * w:] if case["modulate"] else None
+    if torch.accelerator.current_stream() == usual:
+        return _call(L, ctx, st, plan)
+    # on any other stream: after what it has in hand, and before what it does next
+    here = torch.cuda.current_stream()
+    ready.record(here)
+    stream.wait_event(ready)
+    out = _call(L, ctx, st, plan)
+    done.record(stream)
+    here.wait_event(done)
+    return out
+
+
+def _call(L, ctx, st, plan):
+    case, op = st["case"], st["case"]["op"]
     if op == "rotary":
         L.rotary_device(ctx, plan["rotary"], st["x"], st["out"], st["positions"], inverse=case["inverse"])
         return st["out"]
