@@ -154,8 +154,8 @@ struct lwm_ctx {
     int* media_err_dev = nullptr;
     // error word of the paged-cache kernels (same kind of memory, made with
     // the context so that a first call may be captured)
-    int* cache_err = nullptr;
-    int* cache_err_dev = nullptr;
+    uint64_t* cache_err = nullptr;
+    uint64_t* cache_err_dev = nullptr;
     lwm_test_faults faults{};  // fault injection for tests (lwm_ctx_set_test_faults)
     // kernel timing (lwm_ctx_set_kernel_timing): events around the last
     // SkyJEPA rollout launch
@@ -1074,9 +1074,9 @@ lwm_status lwm_ctx_create(int device, lwm_ctx** out) {
         delete ctx;
         return fail(LWM_CUDA_ERROR, std::string("cudaStreamCreate failed: ") + cudaGetErrorString(e));
     }
-    e = cudaHostAlloc(reinterpret_cast<void**>(&ctx->cache_err), 4 * sizeof(int), cudaHostAllocMapped);
+    e = cudaHostAlloc(reinterpret_cast<void**>(&ctx->cache_err), sizeof(uint64_t), cudaHostAllocMapped);
     if (e == cudaSuccess) {
-        for (int i = 0; i < 4; ++i) ctx->cache_err[i] = 0;
+        *ctx->cache_err = 0;
         e = cudaHostGetDevicePointer(reinterpret_cast<void**>(&ctx->cache_err_dev), ctx->cache_err, 0);
     }
     if (e != cudaSuccess) {
@@ -1121,11 +1121,12 @@ lwm_status lwm_ctx_synchronize(lwm_ctx* ctx) {
         return fail(LWM_CUDA_ERROR, "image preprocessing: a source-row copy never completed (" + where +
                                         "); that launch's output is incomplete");
     }
-    if (const int code = static_cast<volatile int*>(ctx->cache_err)[0]) {
-        const std::string seq = "paged cache: sequence " + std::to_string(ctx->cache_err[1]);
-        const std::string at = std::to_string(ctx->cache_err[2]);
-        for (int i = 0; i < 4; ++i) ctx->cache_err[i] = 0;
-        switch (code) {
+    if (const uint64_t word = *static_cast<volatile uint64_t*>(ctx->cache_err)) {
+        const lwm::CacheReport r = lwm::cache_report_of(word);
+        const std::string seq = "paged cache: sequence " + std::to_string(r.sequence);
+        const std::string at = std::to_string(r.detail);
+        *ctx->cache_err = 0;
+        switch (r.code) {
             case lwm::kCacheErrStarts: return fail(LWM_INVALID_ARGUMENT, seq + ": starts are out of order or beyond the packed rows (" + at + ")");
             case lwm::kCacheErrNew: return fail(LWM_INVALID_ARGUMENT, seq + ": more new tokens (" + at + ") than max_new or its length");
             case lwm::kCacheErrLength: return fail(LWM_INVALID_ARGUMENT, seq + ": length " + at + " is negative or beyond its page table");

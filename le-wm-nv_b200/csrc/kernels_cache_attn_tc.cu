@@ -118,7 +118,7 @@ template <int D, bool kCodes> struct Shape {
 };
 
 // Called by whole warps; the answer is the warp's, so that its lanes stay together.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Control* c, int site, int* err, uint32_t seq) {
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Control* c, int site, uint64_t* err, uint32_t seq) {
     bool done = tc::mbar_try(bar, parity);
     for (uint32_t i = 0; i < tc::kWaitLimit && !done; ++i) {
         done = tc::mbar_try(bar, parity);
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = ctl->tmem;
-    int* const err = a.c.err;
+    uint64_t* const err = a.c.err;
 
     if (warp < 8) {
         // ---------------------------------------------------------- softmax

@@ -193,12 +193,8 @@ __device__ __forceinline__ void turn_pairs(float (&a)[8], const float2* cs) {
 
 // ------------------------------------------------------- paged sequences
 
-__device__ __forceinline__ void cache_report(int* err, int code, uint32_t seq, int detail) {
-    volatile int* e = err;
-    e[1] = static_cast<int>(seq);
-    e[2] = detail;
-    __threadfence_system();
-    e[0] = code;
+__device__ __forceinline__ void cache_report(uint64_t* err, int code, uint32_t seq, int detail) {
+    *static_cast<volatile uint64_t*>(err) = cache_report_word({code, seq, detail});
 }
 
 struct SeqView {

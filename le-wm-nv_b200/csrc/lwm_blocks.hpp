@@ -32,8 +32,24 @@ struct FastDiv {
     }
 };
 
-// Codes of the paged-cache kernels' error word: [code, sequence, detail, 0].
+// Codes of the paged-cache kernels' error word.  It is one 64-bit store (code
+// above 27 bits of sequence above 32 of detail), so that of many threads that
+// report at once one is read whole, not one's page with another's sequence.
 constexpr int kCacheErrStarts = 1, kCacheErrNew = 2, kCacheErrLength = 3, kCacheErrPage = 4, kCacheErrWait = 5;
+constexpr uint32_t kCacheErrSequences = 1u << 27;  // more than a batch may have
+struct CacheReport {
+    int code;
+    uint32_t sequence;
+    int detail;
+};
+__host__ __device__ inline uint64_t cache_report_word(const CacheReport& r) {
+    return static_cast<uint64_t>(r.code) << 59 | static_cast<uint64_t>(r.sequence & (kCacheErrSequences - 1)) << 32 |
+           static_cast<uint32_t>(r.detail);
+}
+inline CacheReport cache_report_of(uint64_t word) {
+    return {static_cast<int>(word >> 59), static_cast<uint32_t>(word >> 32) & (kCacheErrSequences - 1),
+            static_cast<int>(static_cast<uint32_t>(word))};
+}
 
 struct RotaryArgs {
     lwm_rotary r;
@@ -58,7 +74,7 @@ struct CacheArgs {
     const int32_t* lengths;
     const int32_t* starts;
     uint32_t sequences, table_stride, tokens, max_new, max_length;
-    int* err;
+    uint64_t* err;
 };
 struct AppendArgs {
     CacheArgs c;

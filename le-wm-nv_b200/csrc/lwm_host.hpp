@@ -18,7 +18,7 @@ lwm_status set_last_error(lwm_status status, const std::string& message);
 struct CtxView {
     int device = 0;
     void* stream = nullptr;   // cudaStream_t
-    int* cache_err = nullptr; // the paged-cache kernels' error word (device address, 4 ints)
+    uint64_t* cache_err = nullptr; // the paged-cache kernels' error word (device address)
 };
 bool ctx_view(lwm_ctx* ctx, CtxView* out);
 void ctx_add_launches(lwm_ctx* ctx, uint64_t n);

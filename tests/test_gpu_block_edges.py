@@ -22,3 +22,34 @@ def test_one_conditioning_row_for_all(ctx, per, width):
     x2, h2 = torch.empty_like(x_out), torch.empty_like(h)
     L.gated_norm_device(ctx, norm, x, y, x2, h2, gate=gate, shift=shift, scale=scale, rows_per_cond=per)
     assert torch.equal(x2, x_out) and torch.equal(h2, h)
+
+
+@pytest.mark.parametrize("call", ["append", "gather", "attention", "many rows"])
+@pytest.mark.parametrize("what", ["page", "length", "both"])
+def test_a_report_names_one_sequence_of_many(ctx, call, what):
+    """Thousands of sequences are wrong at once, each in its own way: the report belongs to one of them."""
+    n, kv, d = 3000, 2, 64
+    c = Paged(230, [16], 16, kv, d, fill=0.0)
+    table, lengths = np.arange(n)[:, None] + 10 ** 6, np.full(n, 16)
+    if what != "page":
+        lengths[:: 1 if what == "length" else 2] = -1000 - np.arange(n)[:: 1 if what == "length" else 2]
+    rows = 2 * MANY if call == "many rows" else n
+    b = L.CacheBatch(ints(table), ints(np.arange(n + 1)), ints(lengths), rows, max_new=MANY if call == "many rows" else 1)
+    x, q = torch.zeros(rows, kv, d, device="cuda", dtype=BF16), torch.zeros(rows, 4, d, device="cuda", dtype=BF16)
+    for _ in range(5):
+        if call == "append":
+            L.cache_append_device(ctx, c.cache, b, x, x)
+        elif call == "gather":
+            L.cache_gather_device(ctx, c.cache, b, x, x)
+        else:
+            L.cache_attention_device(ctx, c.cache, b, q, q)
+        with pytest.raises(L.LwmError) as e:
+            ctx.synchronize()
+        m = re.search(r"sequence (\d+): (?:page (\d+) is not|length (-\d+) is)", e.value.message)
+        assert m, e.value.message
+        s, page, length = int(m[1]), m[2], m[3]
+        if length:
+            assert what != "page" and int(length) == lengths[s], e.value.message
+        else:
+            assert what != "length" and int(page) == 10 ** 6 + s and lengths[s] == 16, e.value.message
+        ctx.synchronize()  # reported once
