@@ -576,13 +576,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         for (int n = 0; n < kQ; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float inv = l[n][e] == 0.0f ? 0.0f : 1.0f / l[n][e];
+                const bool none = l[n][e] == 0.0f;  // nothing weighs, not even against infinities in O
+                const float inv = none ? 0.0f : 1.0f / l[n][e];
                 const float unit = kCodes ? power_of_two(vx[n][e]) : 1.0f;
 #pragma unroll
                 for (int d = 0; d < kSteps; ++d)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        part[(8 * n + 2 * t + e) * D + channel(d, x)] = static_cast<T>(o[n][d][2 * x + e] * inv * unit);
+                        part[(8 * n + 2 * t + e) * D + channel(d, x)] = static_cast<T>(none ? 0.0f : o[n][d][2 * x + e] * inv * unit);
             }
         __syncwarp();
         for (int x = lane; x < kRows * D / 8; x += 32) {

@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[e] = l == 0.0f ? 0.0f : kCodes ? o[e] * inv * root : o[e] * inv;
-                if (poisoned && live) {
+                if (poisoned && live && l != 0.0f) {
                     // a value that is not finite, in a tile where rows differ in what they see: its weight is
                     // positive, so it decides its channel for the rows that see it
                     for (uint32_t i = 0; i < w.tiles; ++i) {

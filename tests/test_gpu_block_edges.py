@@ -53,3 +53,25 @@ def test_a_report_names_one_sequence_of_many(ctx, call, what):
         else:
             assert what != "length" and int(page) == 10 ** 6 + s and lengths[s] == 16, e.value.message
         ctx.synchronize()  # reported once
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("lengths,news,kw", [
+    ([40, 1, 300], [1, 1, 1], {}), ([40, 1, 300], [3, 1, 12], dict(window=20)), ([4000], [1], {}),
+    ([40] * 600, [1] * 600, dict(max_length=40)), ([300, 260], [140, 260], {}), ([700], [300], dict(window=160, sinks=3))])
+def test_rows_whose_scores_are_all_minus_infinity_are_zero(ctx, dtype, d, lengths, news, kw):
+    """Nothing weighs, also where the values are infinities or NaN."""
+    many = max(news) > 100
+    c = Paged(231, lengths, 16, 1, d, dtype, fill=0.0)
+    c.fill_random(232)
+    c.k[..., 0] = -float("inf")
+    c.v[..., 1::5], c.v[..., 2::5] = float("inf"), float("nan")
+    rows = MANY if many else sum(news)
+    q = randn(gen(233), rows, 2, d, dtype=dtype)
+    q[..., 0] = 1.0
+    out = torch.full_like(q, 5.0)
+    kw = dict(kw)
+    b = c.batch(news, tokens=rows, max_length=kw.pop("max_length", 0), **(dict(max_new=MANY) if many else {}))
+    L.cache_attention_device(ctx, c.cache, b, q, out, **kw)
+    assert (out[:sum(news)] == 0).all() and (out[sum(news):] == 5.0).all()
