@@ -199,6 +199,7 @@ lwm_status lwm_cache_append_device(lwm_ctx* ctx, const lwm_paged_cache* cache, c
     }
     if (x->q && x->heads == 0) return bad("query heads must be greater than zero");
     if (x->q && x->heads > 65535) return bad("query heads out of range");
+    if (!x->q && x->q_out) return bad("q_out needs q");
     const bool work = a.c.sequences && a.c.max_new;
     if (!aligned4(x->positions)) return bad("positions are not 4-byte aligned");
     if (work) {

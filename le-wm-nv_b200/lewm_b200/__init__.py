@@ -1386,6 +1386,8 @@ def cache_append_device(ctx: Context, cache: PagedCache, batch: CacheBatch, k, v
         qp, qt, qh = _heads(ctx, "q", q, shape, dtype)
         op, ot, oh = _heads(ctx, "q_out", q_out, shape, dtype)
         a = _CacheAppendArgs(qp, op, kp, vp, qt, qh, ot, oh, kt, kh, vt, vh, pos, heads)
+    elif q_out is not None:
+        raise LwmError(1, "q_out needs q")
     else:
         a = _CacheAppendArgs(None, None, kp, vp, 0, 0, 0, 0, kt, kh, vt, vh, pos, 0)
     _check(lib.lwm_cache_append_device(ctx.handle, cache._ref, batch._ref,

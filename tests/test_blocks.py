@@ -282,3 +282,13 @@ def test_sizes_are_not_cut_to_32_bits():
             ("page table", lambda: L.CacheBatch(_huge(1, n, dtype=i32), _huge(2, dtype=i32), _huge(1, dtype=i32), 1))):
         with pytest.raises(L.LwmError, match=f"{name} must have sizes below"):
             call()
+
+
+def test_append_refuses_an_output_without_its_queries():
+    status = L.lib.lwm_cache_append_device(None, C.byref(_cache()), C.byref(_batch()), None, C.byref(_append(q=None)))
+    assert status != 0 and _message() == "q_out needs q"
+    cache = L.PagedCache(_huge(4, 2, 16, 64), _huge(4, 2, 16, 64))
+    i32 = torch.int32
+    batch = L.CacheBatch(torch.zeros(1, 2, dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(1, dtype=i32), 1)
+    with pytest.raises(L.LwmError, match="q_out needs q"):
+        L.cache_append_device(_NoContext, cache, batch, _huge(1, 2, 64), _huge(1, 2, 64), q_out=_huge(1, 4, 64))
