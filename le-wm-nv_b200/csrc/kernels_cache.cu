@@ -228,6 +228,7 @@ __device__ __forceinline__ void turn_heads(const AppendArgs& a, const CacheDivs&
     }
 }
 
+// (80 registers a thread are three blocks a SM; at 81, two blocks, 215 MB and the gather took 84 us, not 79)
 template <typename T>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a, const CacheDivs d,
                                                           uint32_t runs) {
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 // and full, else a warp.  blockIdx.y: parts of the heads, where the
 // pages alone are too few blocks.
 template <typename T, int kLanes>
-__global__ void __launch_bounds__(kThreads) append_codes_kernel(const __grid_constant__ AppendArgs a, const CacheDivs d,
+__global__ void __launch_bounds__(kThreads, 3) append_codes_kernel(const __grid_constant__ AppendArgs a, const CacheDivs d,
                                                                 uint32_t pages) {
     extern __shared__ float2 trig[];  // [page_tokens][pairs]
     __shared__ PairTurns turns;

@@ -194,7 +194,11 @@ __device__ __forceinline__ void turn_pairs(float (&a)[8], const float2* cs) {
 // ------------------------------------------------------- paged sequences
 
 __device__ __forceinline__ void cache_report(uint64_t* err, int code, uint32_t seq, int detail) {
-    *static_cast<volatile uint64_t*>(err) = cache_report_word({code, seq, detail});
+    const uint64_t word = cache_report_word({code, seq, detail});
+    const uint32_t lo = static_cast<uint32_t>(word), hi = static_cast<uint32_t>(word >> 32);
+    // (joined here: as a 64-bit operand it cost the append's kernels the register that their third block a SM needs)
+    asm volatile("{\n\t.reg .b64 w;\n\tmov.b64 w, {%1, %2};\n\tst.volatile.global.u64 [%0], w;\n\t}" ::"l"(err), "r"(lo), "r"(hi)
+                 : "memory");
 }
 
 struct SeqView {

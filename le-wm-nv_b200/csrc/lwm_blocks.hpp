@@ -36,19 +36,19 @@ struct FastDiv {
 // above 27 bits of sequence above 32 of detail), so that of many threads that
 // report at once one is read whole, not one's page with another's sequence.
 constexpr int kCacheErrStarts = 1, kCacheErrNew = 2, kCacheErrLength = 3, kCacheErrPage = 4, kCacheErrWait = 5;
-constexpr uint32_t kCacheErrSequences = 1u << 27;  // more than a batch may have
+constexpr uint32_t kCacheErrSequences = 1u << 27;  // as many as a batch may have
 struct CacheReport {
     int code;
     uint32_t sequence;
     int detail;
 };
 __host__ __device__ inline uint64_t cache_report_word(const CacheReport& r) {
-    return static_cast<uint64_t>(r.code) << 59 | static_cast<uint64_t>(r.sequence & (kCacheErrSequences - 1)) << 32 |
-           static_cast<uint32_t>(r.detail);
+    const uint32_t high = static_cast<uint32_t>(r.code) * kCacheErrSequences + r.sequence;
+    return static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(r.detail);
 }
 inline CacheReport cache_report_of(uint64_t word) {
-    return {static_cast<int>(word >> 59), static_cast<uint32_t>(word >> 32) & (kCacheErrSequences - 1),
-            static_cast<int>(static_cast<uint32_t>(word))};
+    const uint32_t high = static_cast<uint32_t>(word >> 32);
+    return {static_cast<int>(high / kCacheErrSequences), high % kCacheErrSequences, static_cast<int>(static_cast<uint32_t>(word))};
 }
 
 struct RotaryArgs {
