@@ -744,7 +744,9 @@ lwm_status lwm_lewm_plan_nv12_device(lwm_planner* planner, lwm_scorer* scorer, c
  * history keeps a cache, whose pages all candidates of a vehicle share.
  *
  * All buffers are the caller's, all work is asynchronous on the context's
- * stream, nothing is allocated and no state is kept between calls, so every
+ * stream (lwm_ctx_stream; no other stream waits for it: inputs are ready
+ * there before the call, outputs are read there or after an event that is
+ * recorded there), nothing is allocated and no state is kept between calls, so every
  * call can be captured into a CUDA graph (which must not outlive the
  * context: the kernels hold the address of its error word), and graphs or
  * threads share nothing else but the buffers that the caller gives them.
@@ -819,8 +821,11 @@ typedef struct lwm_paged_cache {
  * starts[s + 1]), its newest tokens, at cache indices lengths[s] - n ..
  * lengths[s] - 1.  `tokens` is the row count of the packed tensors (rows
  * from starts[sequences] on are left as they are), `max_new` at least every
- * n; `max_length` (0: the table's reach) says how long sequences get, for
- * the shape of the launch only.  Sequences may share pages that this call
+ * n, and no more than it if the call is to be quick: launches are sized,
+ * and the attention's kernel is chosen, as if every sequence had that many
+ * (a batch of single tokens wants 1, not `tokens`); `max_length` (0: the
+ * table's reach) says how long sequences get, for the shape of the launch
+ * only.  Sequences may share pages that this call
  * does not append to; table entries of pages that no visible token lies in
  * may hold anything.
  *
@@ -836,8 +841,8 @@ typedef struct lwm_cache_batch {
 } lwm_cache_batch;
 /* Appends keys and values, turned on the way (rotary NULL: as they are).  k,
  * v [tokens, kv_heads, head_dim] and, optionally, q [tokens, heads,
- * head_dim] with q_out (which may be q) of the cache's dtype; only keys and
- * queries are turned.  positions [tokens, axes] int32, or NULL: a token's
+ * head_dim] with q_out (which may be q; without q it is refused) of the
+ * cache's dtype; only keys and queries are turned.  positions [tokens, axes] int32, or NULL: a token's
  * cache index on every axis.
  *
  * LWM_CACHE_E4M3: the scale of a page and head becomes the least power of
@@ -878,7 +883,14 @@ lwm_status lwm_cache_gather_device(lwm_ctx* ctx, const lwm_paged_cache* cache, c
  * with f = frame_tokens (0: 1): tokens of a frame see each other, the window
  * counts frames (tokens when f is 1), the first `sinks` tokens stay visible.
  * Tokens before the first cached one (n > length) see nothing.  What a token
- * does not see does not reach it, not even as infinities or NaN. */
+ * does not see does not reach it, not even as infinities or NaN, nor as the
+ * scales of its pages, which may lie any distance apart.
+ *
+ * Scores, maxima and sums are held in 32 bits.  The weights are rounded to
+ * the cache's dtype for the product with v, to f16 on an 8-bit cache (there
+ * with their page's scale, relative to the row's largest such weight); their
+ * sum is taken before that.  bf16 queries on an 8-bit cache become f16 over a
+ * power of two of the row: channels below 2^-17 of its largest lose bits. */
 typedef struct lwm_cache_attention_args {
     const void* q;
     void* out;
@@ -899,7 +911,8 @@ lwm_status lwm_cache_attention_device(lwm_ctx* ctx, const lwm_paged_cache* cache
  * post and pre are LWM_NORM_LAYER, LWM_NORM_RMS or LWM_NORM_NONE, with f32
  * weights and biases [width] or NULL.  gate, shift, scale: [ceil(rows /
  * rows_per_cond), width] of cond_dtype with row stride cond_stride (e.g. one
- * modulation table's column ranges), or NULL; residual_scale f32 [width] or
+ * modulation table's column ranges; rows_per_cond from `rows` up: one row for
+ * all), or NULL; residual_scale f32 [width] or
  * NULL.  x, x_out [rows, width] of residual_dtype, y, h of dtype, each with
  * its row stride; x_out may be x or NULL, h may be y or NULL (x_out: y too,
  * when the types agree).  width 1 to 8192; rows of any alignment.  Sums and

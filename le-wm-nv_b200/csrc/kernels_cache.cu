@@ -11,9 +11,10 @@
 // scale is shared between groups.
 //
 // Measured (one B200): 16 sequences x up to 1568 new tokens, 16 heads of 64
-// channels, bf16, queries turned along: 215 MB read and written in 49 us,
-// 4.4 TB/s; gathering 151 MB of them back 24 us, 6.2 TB/s.  8 bits, one token
-// for each of 1024 sequences: 16 to 22 us, the chain lengths -> page ->
+// channels, bf16, queries turned along: 215 MB read and written in 49 us, 165
+// MB of them in DRAM; gathering 151 MB back 24 us, 99 MB of them in DRAM (the
+// rest hit the L2, which the append before has filled).  8 bits, one token
+// for each of 1024 sequences: 16 to 24 us, the chain lengths -> page ->
 // tokens -> scale -> codes twice over (80 registers: three blocks a SM);
 // gathering 17 tokens of each, 35 MB of codes to 70 MB: 23 us, two thirds of
 // the issue slots.  Left, as they cost more than they gave: more blocks a SM

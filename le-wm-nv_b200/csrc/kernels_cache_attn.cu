@@ -18,7 +18,7 @@
 // no barrier stands between a load and its use.  Measured (one B200, DRAM
 // bytes as ncu counts them): four sequences of up to 65536 tokens, 8 kv heads
 // of 128 channels, bf16: 910 MB in 146 us, 6.2 TB/s; 48 sequences, windows
-// of 4096 tokens in 8-bit codes: 178 MB in 43 us, 4.1 TB/s, half of the issue
+// of 4096 tokens in 8-bit codes: 178 MB in 42 us, 4.2 TB/s, half of the issue
 // slots in use for the codes; 1024 sequences of 34 tokens, 16 heads of 64
 // channels: 50 MB in 33 us, bound by instructions and by the chain lengths ->
 // page -> keys -> scores of a sequence, not by memory; one sequence of 37
@@ -38,9 +38,8 @@
 // exponentials, one for the sum and one for the product (one, times the row's
 // power of two, measured the same or slower; the ratio of the scales on the
 // finished weight, 0 to 8 % faster, loses what lies 2^14 below the largest
-// scale).  bf16 queries are
-// brought to fp16 by a power of two a row, exactly down to 2^-17 of the row's
-// largest.
+// scale).  bf16 queries are brought to fp16 by a power of two a row, exactly
+// down to 2^-17 of the row's largest.
 #include <cooperative_groups.h>
 
 #include "lwm_blocks.cuh"

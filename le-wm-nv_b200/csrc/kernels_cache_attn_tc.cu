@@ -19,13 +19,15 @@
 // scores, 379 in one); part of the exponentials as polynomials (375 to 381).
 //
 // Measured: 2 sequences of 8192 tokens, 16 heads over 4 kv heads of 128
-// channels, causal, bf16: 370 us, 966 TFLOP/s, tensor pipe 48 %, issue slots
-// 41 %: bound by a tile's chain of scores, softmax and product.  8 sequences
-// of 394 new tokens over 1700 visible ones, 12 heads of 64 channels, 8-bit
-// codes: 67 us; 192 blocks on 148 SMs, a third of their 16 steps at edges of
-// the masks (a 16-bit cache: 61).  The producers of codes bounded a tile (4800
-// cycles) until they located their chunks once for K and V, looked pages up a
-// tile ahead and kept the test for NaN scales out of the plain expansion: 86.
+// channels, causal, bf16: 398 us a call one after another, 897 TFLOP/s (373
+// with pauses between, as the alternatives above were timed), tensor pipe 47
+// %, issue slots 41 %: bound by a tile's chain of scores, softmax and product.
+// 8 sequences of 394 new tokens over 1700 visible ones, 12 heads of 64
+// channels, 8-bit codes: 68 us; 192 blocks on 148 SMs, a third of their 16
+// steps at edges of the masks (a 16-bit cache: 61).  The producers of codes
+// bounded a tile (4800 cycles) until they located their chunks once for K and
+// V, looked pages up a tile ahead and kept the test for NaN scales out of the
+// plain expansion: 86.
 // Left: three buffers of scores for 64 channels (16-bit cache 7 % faster,
 // codes 2 %, but 128 channels 5 % slower).
 //

@@ -1229,6 +1229,11 @@ def preprocess_nv12_device(ctx: Context, y_plane, uv_plane, batch: int, height: 
 #
 # Operators of a world model that the caller runs itself (in a CallbackScorer,
 # or around a planner), on torch CUDA tensors and the context's stream.
+#
+# The calls below return before their kernels have run, and torch's stream does
+# not wait for the context's: work under torch.cuda.stream(ctx.torch_stream()),
+# as a callback scorer does, or order the two with events, before the call for
+# its inputs and after it for its outputs.  Tensors stay alive until then.
 
 DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
 _dtype_codes: dict = {}  # the same by torch dtype, as they are met
@@ -1318,7 +1323,9 @@ class CacheBatch:
     """lwm_cache_batch: the page table [sequences, pages], starts [sequences +
     1] and lengths [sequences] (int32 device tensors, read when the kernels
     run), the packed rows `tokens`, and bounds of a sequence's new tokens and
-    length."""
+    length.  `max_new` None is `tokens`, which is right for one sequence; give
+    it for more (1 for a batch of single tokens): launches are sized, and the
+    attention's kernel is chosen, by it."""
 
     def __init__(self, table, starts, lengths, tokens: int, max_new: Optional[int] = None, max_length: int = 0):
         if table.dim() != 2:
@@ -1347,7 +1354,8 @@ def _same_device(ctx: Context, cache: PagedCache, batch: CacheBatch) -> None:
 
 
 def rotary_device(ctx: Context, rotary: Rotary, x, out, positions, inverse: bool = False) -> None:
-    """out = x [tokens, heads, head_dim] turned by positions [tokens, axes] int32 (`inverse`: turned back)."""
+    """out = x [tokens, heads, head_dim] turned by positions [tokens, axes]
+    int32 (`inverse`: turned back).  `out` is ready on the context's stream."""
     if x.dim() != 3:
         raise LwmError(1, f"x must be [tokens, heads, head_dim], got {list(x.shape)}")
     tokens, heads, d = shape = x.shape
@@ -1365,7 +1373,8 @@ def cache_append_device(ctx: Context, cache: PagedCache, batch: CacheBatch, k, v
                         positions=None, q=None, q_out=None) -> None:
     """Appends k, v [tokens, kv_heads, head_dim] to the batch's sequences, the
     keys (and q [tokens, heads, head_dim] into q_out) turned by `positions`
-    [tokens, axes] (None: each token's cache index)."""
+    [tokens, axes] (None: each token's cache index).  Pages and q_out are
+    ready on the context's stream."""
     _same_device(ctx, cache, batch)
     n, dtype, shape = batch.tokens, cache.dtype, (batch.tokens, cache.kv_heads, cache.head_dim)
     pos = None
@@ -1395,7 +1404,8 @@ def cache_append_device(ctx: Context, cache: PagedCache, batch: CacheBatch, k, v
 
 
 def cache_gather_device(ctx: Context, cache: PagedCache, batch: CacheBatch, k_out, v_out) -> None:
-    """The batch's cached tokens as values: k_out, v_out [tokens, kv_heads, head_dim] of the cache's dtype."""
+    """The batch's cached tokens as values: k_out, v_out [tokens, kv_heads,
+    head_dim] of the cache's dtype, ready on the context's stream."""
     _same_device(ctx, cache, batch)
     shape = (batch.tokens, cache.kv_heads, cache.head_dim)
     kp, kt, kh = _heads(ctx, "k_out", k_out, shape, cache.dtype)
@@ -1409,7 +1419,7 @@ def cache_attention_device(ctx: Context, cache: PagedCache, batch: CacheBatch, q
     """out = attention of q [tokens, heads, head_dim] over the sequences'
     cached tokens (scale None: head_dim ** -0.5); `window` frames of
     `frame_tokens` tokens and the first `sinks` tokens are visible, window 0:
-    everything before."""
+    everything before.  `out` is ready on the context's stream."""
     _same_device(ctx, cache, batch)
     if q.dim() != 3:
         raise LwmError(1, f"q must be [tokens, heads, head_dim], got {list(q.shape)}")
@@ -1472,7 +1482,8 @@ def gated_norm_device(ctx: Context, norm: GatedNorm, x, y=None, x_out=None, h=No
                       rows_per_cond: int = 1) -> None:
     """One pass over the rows of x [rows, width] and y (None: x' = x); gate,
     shift, scale [ceil(rows / rows_per_cond), width] of one type and row
-    stride; writes x' to x_out and the normed rows to h (either may be None)."""
+    stride; writes x' to x_out and the normed rows to h (either may be None),
+    ready on the context's stream."""
     if x.dim() != 2:
         raise LwmError(1, f"x must be [rows, width], got {list(x.shape)}")
     rows, width = x.shape

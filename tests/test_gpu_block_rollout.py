@@ -2,12 +2,14 @@
 scales and codes against the keys and values that went in, each attention
 against 64 bits over the tokens that the pages then stand for, so that a stale
 scale, a wrong window or page shows at once, not only in a score."""
+import os
+
 import numpy as np
 import pytest
 
 import lewm_b200 as L
 from test_gpu_block_scales import tolerance
-from test_gpu_blocks import (BF16, F8, WorldModel, attention_64, close, gen, ints, mask_of, need_scale,  # noqa: F401
+from test_gpu_blocks import (BF16, F8, WorldModel, attention_64, attention_tolerance, close, gen, ints, mask_of, need_scale,  # noqa: F401
                              on_context_stream, randn, turned)
 
 torch = pytest.importorskip("torch")
@@ -123,3 +125,19 @@ def test_8_bit_rollout_step_by_step(ctx, H, windows):
         x = x + acts[:, t] @ m.embed
         x = forward(x.clone(), acts[:, t].contiguous(), m.positions([H + t], n), table, [H + t + 1] * n, [1] * n)
     assert torch.isfinite(x).all()
+
+
+def test_the_guides_example(ctx):
+    """The integration guide's program, and its last attention against 64 bits."""
+    guide = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
+    program = [b.split("```")[0] for b in guide.split("```python\n")[1:] if "PagedCache" in b.split("```")[0]]
+    assert len(program) == 1
+    names = dict(ctx=ctx, L=L)
+    exec(program[0], names)
+    q, out, dim, S = names["q"], names["out"], names["dim"], names["S"]
+    k, v = (p[[0, 1]].double() for p in names["pool"])
+    for s in range(S):
+        dense = [torch.cat([whole, p[3 + s][None].double()]).transpose(1, 2).reshape(-1, names["kv"], dim)[:41]
+                 for whole, p in zip((k, v), names["pool"])]
+        parts = attention_64(q[s:s + 1].double(), *dense, mask_of(41, 1, True, 0, 0, 1), dim ** -0.5)
+        close(out[s:s + 1], parts[0], attention_tolerance(*parts, dim, BF16, False, 0.0))
