@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     asm volatile("bar.sync 1, %0;" ::"n"(kProducers + kScaleThreads) : "memory");
                     float top = fmaxf(fmaxf(ctl->high[0], ctl->high[1]), ctl->high[2]);
                     const float low = fminf(fminf(ctl->low[0], ctl->low[1]), ctl->low[2]);
-                    if (top == 0.0f) top = 1.0f;
+                    top = fmaxf(top, 0x1p-126f);  // (zero, or so small that its reciprocal is infinite)
                     v_ref_inv = 1.0f / top;
                     if (t == 0) ctl->v_ref = top, ctl->wide = low * v_ref_inv < kFar;
                 }

@@ -185,6 +185,15 @@ def test_a_row_does_not_depend_on_scales_it_does_not_see(ctx, many):
     assert ((got - want).abs() <= 2 * rounded(BF16, want)).all()
 
 
+@pytest.mark.parametrize("exponents,marked", [([-127], [0]), ([-133], [0]), ([-140, -149], [0]), ([-128, -60], [1]),
+                                              ([-149, 30], [1])])
+@pytest.mark.parametrize("news,many", [([1, 5, 3], False), ([60, 1, 130], True)])
+def test_scales_below_the_smallest_normal(ctx, exponents, marked, news, many):
+    """Positive and finite is all that a scale has to be."""
+    c = filled(221, [130, 70, 300], 16, 2, 64, BF16, exponents, marked)
+    check(ctx, c, news, 6, 222, offsets_of(exponents), many)
+
+
 @pytest.mark.parametrize("many", [False, True])
 def test_zero_and_broken_scales(ctx, many):
     """A scale of zero is a page of zeros; of infinity or NaN, NaN for the rows that see it and for no other."""
