@@ -888,8 +888,9 @@ lwm_status lwm_cache_gather_device(lwm_ctx* ctx, const lwm_paged_cache* cache, c
  *
  * Scores, maxima and sums are held in 32 bits.  The weights are rounded to
  * the cache's dtype for the product with v, to f16 on an 8-bit cache (there
- * with their page's scale, relative to the row's largest such weight); their
- * sum is taken before that.  bf16 queries on an 8-bit cache become f16 over a
+ * with their page's scale, relative to the row's largest such weight); f16
+ * ones far below the row's largest lose at most 2^-29 of it each; their sum
+ * is taken before that.  bf16 queries on an 8-bit cache become f16 over a
  * power of two of the row: channels below 2^-17 of its largest lose bits. */
 typedef struct lwm_cache_attention_args {
     const void* q;

@@ -468,15 +468,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
                     }
                 }
         }
-        // P in the operands' type: 2^-9 (bf16) or 2^-12 (fp16) of itself,
-        // no more than rounding the output costs
+        // P in the operands' type: 2^-9 (bf16) or 2^-12 (fp16) of itself, no
+        // more than rounding the output costs.  Halves end at 2^-25, so theirs
+        // are 2^kLift times as large (below 2^15): what a weight can lose, 2^-32
+        // (codes 2^-29) of the row's largest, stays below that rounding in sums
+        // of 2^18 keys too
+        constexpr float kLift = !std::is_same_v<M, __half> ? 0.0f : kCodes ? 5.0f : 7.0f;
         float p[kQ][4];
         uint32_t pb[kQ][2];
 #pragma unroll
         for (int n = 0; n < kQ; ++n) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float over = sc[n][e] - (m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1]);
+                const float over = sc[n][e] - (m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1] - kLift);
                 p[n][e] = exp2_fast(over);
                 l[n][e & 1] += p[n][e];
                 if constexpr (kCodes) p[n][e] = exp2_fast(over + (v_exp - vx[n][e & 1])) * v_frac;

@@ -56,7 +56,9 @@
 // 67.7 us; one loop for both, with more registers alive, 69.7).
 //
 // O is rescaled only when a score passes a row's maximum by more than kRaise
-// (a factor of 2^8).
+// (a factor of 2^8).  Weights that become halves are 2^kLift times as large, at
+// most 2^15: halves end at 2^-25, so a weight loses 2^-32 of the row's largest
+// at most, less than rounding the output costs in sums of 2^18 keys too.
 // Every wait is bounded: one that gives up marks the block, which unwinds.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -314,9 +316,9 @@ __device__ __forceinline__ float weights(const float (&x)[64], uint32_t (&p)[32]
 }
 
 // Adds the far groups' weights of a row's 64 keys (scores at `t_scores`) to
-// l, which is in units of 2^ml.
+// l, which is in units of 2^(ml - lift).
 __device__ __forceinline__ void far_sum(uint32_t t_scores, const TileInfo& info, int half, float mul, const VisibleRange& rr,
-                                     uint32_t key, float& l, float& ml) {
+                                     uint32_t key, float& l, float& ml, float lift) {
 #pragma unroll 1
     for (int g = 0; g < 4; ++g) {
         const int group = 4 * half + g;
@@ -333,7 +335,7 @@ __device__ __forceinline__ void far_sum(uint32_t t_scores, const TileInfo& info,
             top = fmaxf(top, x[e]);
         }
         if (top > ml) l *= exp2_fast(ml - top), ml = top;
-        const float sub = ml == -INFINITY ? 0.0f : ml;
+        const float sub = ml == -INFINITY ? 0.0f : ml - lift;
 #pragma unroll
         for (int e = 0; e < 16; ++e) l += exp2_fast(x[e] - sub);
     }
@@ -346,6 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using M = std::conditional_t<kCodes, __half, T>;
     using S = Shape<D, kCodes>;
     constexpr int kSteps = D / 16;
+    constexpr float kLift = std::is_same_v<M, __half> ? 7.0f : 0.0f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
     Control* ctl = reinterpret_cast<Control*>(smem + S::kControl);
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the tiles one after another; returns the root of O's unit over l's
             auto walk = [&](auto far_apart) {
             constexpr bool kWide = decltype(far_apart)::value;
-            float ml = -INFINITY;  // wide: l is in units of 2^ml, ml >= m
+            float ml = -INFINITY;  // wide: l is in units of 2^(ml - kLift), O in those of 2^(m - kLift), ml >= m
             for (uint32_t i = 0; i < w.tiles && fine; ++i) {
                 // (the producers' notes are there long before the scores)
                 const TileInfo& info = ctl->info[i % kInfos];
@@ -485,12 +488,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     bool again = false;
                     while (true) {
                         const bool first = m == -INFINITY;
-                        const float sub = first ? 0.0f : -m;
+                        const float sub = first ? 0.0f : kLift - m;
                         const float top = whole ? weights<M, kCodes, false>(x, p, sum, info, half, mul, sub, rr, key, ok)
                                                 : weights<M, kCodes, true>(x, p, sum, info, half, mul, sub, rr, key, ok);
-                        if (again || !__any_sync(0xffffffffu, top > (first ? -INFINITY : kRaise))) break;
+                        if (again || !__any_sync(0xffffffffu, top > (first ? -INFINITY : kRaise + kLift))) break;
                         again = true;
-                        const float up = first ? top : fmaxf(top, 0.0f), down = first ? 0.0f : exp2_fast(-up);
+                        const float up = first ? top : fmaxf(top - kLift, 0.0f), down = first ? 0.0f : exp2_fast(-up);
                         m = first ? top : m + up;
                         if constexpr (kWide) {
                             if (m > ml) l *= exp2_fast(ml - m), ml = m;
@@ -519,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!fine) break;
                     if constexpr (kWide) {
                         l += (sum.x + sum.y) * (m == ml ? 1.0f : exp2_fast(m - ml));
-                        if ((info.far >> (4 * half)) & 0xfu) far_sum(t_s + kHalf * half, info, half, mul, rr, key, l, ml);
+                        if ((info.far >> (4 * half)) & 0xfu) far_sum(t_s + kHalf * half, info, half, mul, rr, key, l, ml, kLift);
                     } else {
                         l += sum.x + sum.y;
                     }
@@ -549,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (fine && w.tiles) fine = wait(&ctl->o_done[tile], (w.tiles - 1) & 1, ctl, 16 + tile, err, s);
             tc::fence_after();
-            const float inv = l == 0.0f ? 0.0f : (kCodes ? ctl->v_ref * root : 1.0f) / l;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l, v_ref = ctl->v_ref;
             const bool poisoned = *static_cast<volatile int*>(&ctl->poisoned) != 0;
             // rows go through the tile's Q, which no product reads any more, and out in whole 16-byte runs
             uint8_t* stage = smem + S::kQ + tile * S::kTileBytes;
@@ -561,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc::tmem_ld_wait();
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = l == 0.0f ? 0.0f : kCodes ? o[e] * inv * root : o[e] * inv;
+                for (int e = 0; e < 16; ++e) o[e] = l == 0.0f ? 0.0f : kCodes ? o[e] * inv * root * v_ref * root : o[e] * inv;
                 if (poisoned && live && l != 0.0f) {
                     // a value that is not finite, in a tile where rows differ in what they see: its weight is
                     // positive, so it decides its channel for the rows that see it

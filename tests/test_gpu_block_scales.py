@@ -212,3 +212,34 @@ def test_zero_and_broken_scales(ctx, many):
         j = (512 - n) // 32
         hit = (index >= 32 * j) & (index - window + 1 < 32 * (j + 1))
         assert torch.isnan(out[:n][hit]).all() and torch.isfinite(out[:n][~hit]).all()
+
+
+@pytest.mark.parametrize("dtype,codes", [(F16, False), (BF16, True), (F16, True), (BF16, False)])
+@pytest.mark.parametrize("length,n,power", [(50000, 1, 25.5), (50000, 1, 27.0), (700, 1, 24.5), (16000, 60, 25.2),
+                                            (30000, 20, 26.0)])
+def test_small_weights_add_up(ctx, dtype, codes, length, n, power):
+    """One key outweighs each of the others by 2^power and has small values: the others, each less than the halves'
+    last step beside it, still count.  Lost: 2^-29 of the largest weight for each key at most, beside the weights' own
+    rounding."""
+    many = n > 1
+    c = Paged(223, [length], 64, 1, 64, dtype, codes)
+    g = gen(224)
+    k, v = torch.zeros(length, 1, 64, device="cuda"), randn(g, length, 1, 64).abs()
+    k[..., 1], k[1, 0, 0], v[1] = 1.0, 1.0, 2.0 ** -6  # (channel 1, which no query has, gives each page a scale)
+    c.set("k", 0, k)
+    c.set("v", 0, v)
+    if codes:
+        c.vs[:] = 2.0 ** -7
+    q = torch.zeros(MANY if many else n, 2, 64, device="cuda", dtype=dtype)
+    keys, values = c.dense("k", 0), c.dense("v", 0)
+    q[..., 0] = power * math.log(2) * 8 / float(keys[1, 0, 0])
+    out = torch.empty_like(q)
+    b = c.batch([n], tokens=q.shape[0], max_new=q.shape[0])
+    L.cache_attention_device(ctx, c.cache, b, q, out)
+    assert torch.isfinite(keys).all() and torch.isfinite(values).all()
+    seen = mask_of(length, n, True, 0, 0, 1)
+    want, mass, reach, count = attention_64(q[:n].double(), keys, values, seen, 0.125)
+    each = E32 * 70 * reach * 1.5 + 2.0 ** -21
+    top = 1 / (1 + length * 2.0 ** -power)
+    tol = mass * (U(F16 if codes else dtype) + 2 * each + 2 * (count + 16) * E32) + rounded(dtype, want)
+    close(out[:n], want, tol + count * 2.0 ** -29 * float(values.max()) * top)
