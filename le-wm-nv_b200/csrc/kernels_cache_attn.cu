@@ -33,13 +33,13 @@
 // multiplies the scores.  A value scale 2^e f (f in [1, 2)) goes into the
 // weight before it is rounded: a row keeps, beside its maximum m and sum, the
 // power of two E of its largest weighted scale, and its weights for the
-// product are exp2(score - m + e - E) f, at most 2^9 and near one for the page
-// that counts most, whatever the scales of the others.  So a weight has two
-// exponentials, one for the sum and one for the product (one, times the row's
-// power of two, measured the same or slower; the ratio of the scales on the
-// finished weight, 0 to 8 % faster, loses what lies 2^14 below the largest
-// scale).  bf16 queries are brought to fp16 by a power of two a row, exactly
-// down to 2^-17 of the row's largest.
+// product are exp2(score - m + e - E) f, at most 2^9 (2^14 as rounded, see
+// kLift) and near one for the page that counts most, whatever the scales of
+// the others.  So a weight has two exponentials, one for the sum and one for
+// the product (one, times the row's power of two, measured the same or slower;
+// the ratio of the scales on the finished weight, 0 to 8 % faster, loses what
+// lies 2^14 below the largest scale).  bf16 queries are brought to fp16 by a
+// power of two a row, exactly down to 2^-17 of the row's largest.
 #include <cooperative_groups.h>
 
 #include "lwm_blocks.cuh"
