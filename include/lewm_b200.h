@@ -904,6 +904,99 @@ typedef struct lwm_cache_attention_args {
 lwm_status lwm_cache_attention_device(lwm_ctx* ctx, const lwm_paged_cache* cache, const lwm_cache_batch* batch,
                                       const lwm_cache_attention_args* args);
 
+/* Linear attention with a decay for each head: with lambda = exp(log_decay
+ * of the head), over a sequence's tokens in order,
+ *   S = lambda S + k v^T,   out = scale q S,
+ * S [head_dim, head_dim] (key channel, value channel) the head's state, in 32
+ * bits.  A model of that kind needs no cache: its history is one state of
+ * fixed size, from which any number of candidates may go on.
+ *
+ * states [slots, heads, head_dim, head_dim] f32, head_dim 32, 64 or 128.
+ * Device arrays: starts [sequences + 1] (ascending from 0: sequence s owns
+ * packed rows [starts[s], starts[s + 1]), at most max_new of them; rows from
+ * starts[sequences] on are left as they are), source [sequences] (slot of the
+ * state before a sequence's first token, below 0: zero), target [sequences]
+ * (slot that its state after the last one goes to, below 0: nowhere); NULL: slot s
+ * for sequence s.  Sequences may share a source; a target may be its own
+ * sequence's source, but no other's and no other's target (which of two states
+ * a slot then holds, or whether a sequence starts from the old state, is
+ * undefined).  A sequence without tokens hands its state on.  Launches are
+ * sized by max_new: with up to 8 new tokens the state is read and written
+ * once and the tokens follow each other; longer sequences go by chunks of 64
+ * on tensor cores.
+ *
+ * q, out [tokens, heads, head_dim], k, v [tokens, kv_heads, head_dim] of
+ * `dtype` (bf16 or f16; out may be q); query head h and its state use kv head
+ * h / (heads / kv_heads).  log_decay [heads] f32, natural logarithms, zero
+ * (nothing fades) or below; minus infinity: every token starts afresh.
+ * In chunks, the weights q.k lambda^n are rounded to dtype for their product
+ * with v, the state is rounded to bf16 (f16: to 11 bits of any range) for the
+ * product with q, and keys times their decay enter the state with 16 bits
+ * (f16: 22).  Infinities and NaN reach later tokens of their sequence and
+ * head only.
+ *
+ * A sequence whose starts are out of order or above max_new, or whose slots
+ * are beyond the pool, is skipped; the next lwm_ctx_synchronize returns
+ * LWM_INVALID_ARGUMENT naming one, once. */
+typedef struct lwm_state_batch {
+    float* states;
+    const int32_t* starts;
+    const int32_t* source;
+    const int32_t* target;
+    uint32_t slots, heads, head_dim, sequences, tokens, max_new;
+} lwm_state_batch;
+typedef struct lwm_linear_attention_args {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    uint64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    uint64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+    const float* log_decay;
+    uint32_t kv_heads;
+    int32_t dtype;
+    float scale;
+} lwm_linear_attention_args;
+lwm_status lwm_linear_attention_device(lwm_ctx* ctx, const lwm_state_batch* batch, const lwm_linear_attention_args* args);
+
+/* Draws a token from each row of logits [rows, vocab] with the random number
+ * that the caller gives for it (as the planners take injected noise): with
+ * weights w = exp((logit - largest) / temperature), tokens ordered by logit
+ * and, among equals, by index,
+ *   top_k  keeps the first top_k (0, or vocab and more: all),
+ *   top_p  keeps the shortest run of first tokens whose weights are at least
+ *          top_p of the sum of those that top_k keeps (1: all),
+ *   min_p  keeps those with w >= min_p (0: all),
+ * a token has to pass all three, and the one drawn is the token of lowest
+ * index with sum of kept weights up to it > uniform * sum of kept weights.
+ * temperature 0 takes the largest logit.  Minus infinity and NaN are never
+ * drawn; where there are plus infinities, they share the row alike.  A row
+ * without any other logit gives token -1, log-probability minus infinity.
+ * log_probs (or NULL): log of the drawn token's share of the kept weights.
+ *
+ * logits: rows `stride` elements apart (any alignment of the type; whole
+ * 16-byte rows load faster), vocab up to 2^18; uniform [rows] f32 in [0, 1)
+ * (others count as the nearest); tokens [rows] int32.  Parameters of each row, f32
+ * (top_ks int32) [rows] device arrays or NULL for the one value: there,
+ * temperatures not above 0 take the largest logit, top_ks below 1 and top_ps
+ * from 1 on (or NaN) keep all, min_ps not above 0 too.  Weights have a relative error
+ * below 1e-13 and are summed exactly in units of 2^-43. */
+typedef struct lwm_sample_tokens_args {
+    const void* logits;
+    uint64_t stride;
+    const float* uniform;
+    int32_t* tokens;
+    float* log_probs;
+    const float* temperatures;
+    const int32_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    double temperature, top_p, min_p;
+    uint32_t top_k, rows, vocab;
+    int32_t dtype;
+} lwm_sample_tokens_args;
+lwm_status lwm_sample_tokens_device(lwm_ctx* ctx, const lwm_sample_tokens_args* args);
+
 /* The end of one residual block and the norm that opens the next
  * (ConditionalBlock, src/models/lewm/modules.rs:275-330, as one row pass):
  *   x' = x + residual_scale * gate * post(y)        (y NULL: x' = x)

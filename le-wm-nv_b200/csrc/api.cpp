@@ -1126,11 +1126,19 @@ lwm_status lwm_ctx_synchronize(lwm_ctx* ctx) {
         const std::string seq = "paged cache: sequence " + std::to_string(r.sequence);
         const std::string at = std::to_string(r.detail);
         *ctx->cache_err = 0;
+        const std::string state = "linear attention: sequence " + std::to_string(r.sequence);
         switch (r.code) {
             case lwm::kCacheErrStarts: return fail(LWM_INVALID_ARGUMENT, seq + ": starts are out of order or beyond the packed rows (" + at + ")");
             case lwm::kCacheErrNew: return fail(LWM_INVALID_ARGUMENT, seq + ": more new tokens (" + at + ") than max_new or its length");
             case lwm::kCacheErrLength: return fail(LWM_INVALID_ARGUMENT, seq + ": length " + at + " is negative or beyond its page table");
             case lwm::kCacheErrPage: return fail(LWM_INVALID_ARGUMENT, seq + ": page " + at + " is not in the pool");
+            case lwm::kCacheErrGroup:
+                return fail(LWM_INVALID_ARGUMENT, "paged cache: group " + std::to_string(r.sequence) +
+                                                      ": its sequences or its prefix are out of order, above their bounds or beyond the page table (" + at + ")");
+            case lwm::kCacheErrShared: return fail(LWM_INVALID_ARGUMENT, seq + ": new tokens reach into the shared prefix (length " + at + ")");
+            case lwm::kStateErrStarts: return fail(LWM_INVALID_ARGUMENT, state + ": starts are out of order or beyond the packed rows (" + at + ")");
+            case lwm::kStateErrNew: return fail(LWM_INVALID_ARGUMENT, state + ": more new tokens (" + at + ") than max_new");
+            case lwm::kStateErrSlot: return fail(LWM_INVALID_ARGUMENT, state + ": state slot " + at + " is not in the pool");
             default: return fail(LWM_CUDA_ERROR, seq + ": a pipeline wait of the attention kernel gave up (site " + at + ")");
         }
     }

@@ -1,6 +1,6 @@
 // blocks_api.cpp — the C ABI of the transformer blocks (include/lewm_b200.h):
-// argument checks and launches of the rotary, paged-cache, attention and
-// gated-norm kernels.
+// argument checks and launches of the rotary, paged-cache, attention,
+// linear-attention, sampling and gated-norm kernels.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -342,6 +342,87 @@ lwm_status lwm_gated_norm_device(lwm_ctx* ctx, const lwm_gated_norm_args* x) {
     a.out_norm = x->out_weight != nullptr;
     a.cond_div = lwm::FastDiv(cond ? std::min(x->rows_per_cond, x->rows) : 1);  // (more rows than there are: one for all)
     return on_device(ctx, c, "gated norm", [&](cudaStream_t s) { return lwm::launch_gated_norm(a, s); });
+}
+
+lwm_status lwm_linear_attention_device(lwm_ctx* ctx, const lwm_state_batch* b, const lwm_linear_attention_args* x) {
+    if (!b || !x) return bad("null argument");
+    if (x->dtype != LWM_DTYPE_BF16 && x->dtype != LWM_DTYPE_F16) return bad("linear attention dtype must be bf16 or f16");
+    if (b->head_dim != 32 && b->head_dim != 64 && b->head_dim != 128)
+        return fail(LWM_UNSUPPORTED, "state head_dim " + std::to_string(b->head_dim) + " is not 32, 64 or 128");
+    if (b->heads == 0 || b->heads > 65535) return bad("state heads must be 1 to 65535");
+    if (x->kv_heads == 0 || b->heads % x->kv_heads)
+        return bad("state heads " + std::to_string(b->heads) + " must be a positive multiple of kv_heads " + std::to_string(x->kv_heads));
+    if (!std::isfinite(x->scale)) return bad("attention scale must be finite");
+    if (b->slots > 0x7fffffffu) return bad("state slots out of range");
+    if (b->sequences > 0x7ffffffu || b->tokens > 0x7fffffffu || b->max_new > b->tokens)
+        return bad("batch sizes out of range (max_new " + std::to_string(b->max_new) + ", tokens " + std::to_string(b->tokens) + ")");
+    if (static_cast<uint64_t>(b->sequences) * b->heads > 0x7ffffffull) return fail(LWM_UNSUPPORTED, "batch is too large for one call");
+    if (b->sequences) {
+        if (!b->states) return bad("states are null");
+        if (!aligned16(b->states)) return bad("states are not 16-byte aligned");
+        if (!b->starts) return bad("batch arrays are null");
+        if (!aligned4(b->starts) || !aligned4(b->source) || !aligned4(b->target)) return bad("batch arrays are not 4-byte aligned");
+        if ((!b->source || !b->target) && b->sequences > b->slots)
+            return bad("sequences " + std::to_string(b->sequences) + " need as many state slots, or source and target");
+        if (!x->log_decay) return bad("log_decay is null");
+        if (!aligned4(x->log_decay)) return bad("log_decay is not 4-byte aligned");
+    }
+    if (b->sequences && b->max_new) {
+        LWM_TRY(check_heads("q", x->q, x->q_token_stride, x->q_head_stride));
+        LWM_TRY(check_heads("k", x->k, x->k_token_stride, x->k_head_stride));
+        LWM_TRY(check_heads("v", x->v, x->v_token_stride, x->v_head_stride));
+        LWM_TRY(check_heads("out", x->out, x->out_token_stride, x->out_head_stride));
+    }
+    CtxView c;
+    if (!lwm::ctx_view(ctx, &c)) return bad("null context");
+    if (b->sequences == 0) return LWM_OK;
+    lwm::LinearArgs a{};
+    a.q = x->q, a.k = x->k, a.v = x->v, a.out = x->out;
+    a.q_ts = x->q_token_stride, a.q_hs = x->q_head_stride;
+    a.k_ts = x->k_token_stride, a.k_hs = x->k_head_stride;
+    a.v_ts = x->v_token_stride, a.v_hs = x->v_head_stride;
+    a.o_ts = x->out_token_stride, a.o_hs = x->out_head_stride;
+    a.states = b->states;
+    a.log_decay = x->log_decay;
+    a.starts = b->starts, a.source = b->source, a.target = b->target;
+    a.slots = b->slots, a.sequences = b->sequences, a.tokens = b->tokens, a.max_new = b->max_new;
+    a.heads = b->heads, a.head_dim = b->head_dim;
+    a.scale = x->scale;
+    a.head_div = lwm::FastDiv(b->heads);
+    a.group_div = lwm::FastDiv(b->heads / x->kv_heads);
+    a.err = c.cache_err;
+    return on_device(ctx, c, "linear attention", [&](cudaStream_t s) { return lwm::launch_linear_attention(a, x->dtype, s); });
+}
+
+lwm_status lwm_sample_tokens_device(lwm_ctx* ctx, const lwm_sample_tokens_args* x) {
+    if (!x) return bad("null argument");
+    if (x->dtype < LWM_DTYPE_F32 || x->dtype > LWM_DTYPE_F16) return bad("unknown dtype");
+    if (x->vocab == 0) return bad("vocabulary must be greater than zero");
+    if (x->vocab > lwm::kSampleVocab)
+        return fail(LWM_UNSUPPORTED, "vocabulary " + std::to_string(x->vocab) + " is above " + std::to_string(lwm::kSampleVocab));
+    if (x->rows > 0x7ffffffu) return bad("rows out of range");
+    if (!x->temperatures && !(std::isfinite(x->temperature) && x->temperature >= 0.0))
+        return bad("temperature must be finite and non-negative");
+    if (!x->top_ps && !(x->top_p > 0.0 && x->top_p <= 1.0)) return bad("top_p must be above 0 and at most 1");
+    if (!x->min_ps && !(x->min_p >= 0.0 && x->min_p <= 1.0)) return bad("min_p must be 0 to 1");
+    if (x->rows) {
+        if (!x->logits) return bad("logits are null");
+        if (reinterpret_cast<uintptr_t>(x->logits) % (x->dtype == LWM_DTYPE_F32 ? 4 : 2)) return bad("logits must be aligned to their element size");
+        if (!x->uniform || !x->tokens) return bad("uniform or tokens are null");
+        for (const void* p : {static_cast<const void*>(x->uniform), static_cast<const void*>(x->tokens), static_cast<const void*>(x->log_probs),
+                              static_cast<const void*>(x->temperatures), static_cast<const void*>(x->top_ks),
+                              static_cast<const void*>(x->top_ps), static_cast<const void*>(x->min_ps)})
+            if (!aligned4(p)) return bad("row arrays must be aligned to 4 bytes");
+    }
+    CtxView c;
+    if (!lwm::ctx_view(ctx, &c)) return bad("null context");
+    if (x->rows == 0) return LWM_OK;
+    lwm::TokenArgs a{};
+    a.logits = x->logits, a.stride = x->stride, a.uniform = x->uniform, a.tokens = x->tokens, a.log_probs = x->log_probs;
+    a.temperatures = x->temperatures, a.top_ks = x->top_ks, a.top_ps = x->top_ps, a.min_ps = x->min_ps;
+    a.temperature = x->temperature, a.top_p = x->top_p, a.min_p = x->min_p, a.top_k = x->top_k;
+    a.rows = x->rows, a.vocab = x->vocab;
+    return on_device(ctx, c, "token sampling", [&](cudaStream_t s) { return lwm::launch_sample_tokens(a, x->dtype, s); });
 }
 
 }  // extern "C"

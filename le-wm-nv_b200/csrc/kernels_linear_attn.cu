@@ -1,0 +1,416 @@
+// kernels_linear_attn.cu — linear attention with a decay for each head
+// (lwm_linear_attention_device):
+//   S_t = lambda S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,
+// S one f32 [head_dim, head_dim] state a head.
+//
+// A few tokens a sequence (linear_step_kernel): the state is read once, kept
+// in registers over the tokens, and written once.
+//
+// Whole histories (linear_chunk_kernel): chunks of 64 tokens,
+//   O = lambda^(i+1) Q S + (Q K^T . lambda^(i-j), j <= i) V,
+//   S' = lambda^m S + sum_j lambda^(m-1-j) k_j v_j^T   (m tokens),
+// all four products on mma.sync with the state in the accumulators' registers.
+#include <algorithm>
+
+#include "lwm_blocks.cuh"
+#include "lwm_linear_attn.cuh"
+
+namespace lwm {
+
+namespace {
+
+// -------------------------------------------------------------- few tokens
+
+// A block takes (sequence, head): thread (r, c) keeps rows r, r + kRowGroups,
+// ... of the state at value channels 4 c .. 4 c + 3.
+template <int D> struct StepShape {
+    static constexpr int kCols = D / 4, kThreads = D == 128 ? 256 : D == 64 ? 128 : 64;
+    static constexpr int kRowGroups = kThreads / kCols, kRows = D / kRowGroups;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(StepShape<D>::kThreads) linear_step_kernel(const __grid_constant__ LinearArgs a) {
+    using S = StepShape<D>;
+    __shared__ float q_s[D], k_s[D], v_s[D];
+    __shared__ float4 part[S::kRowGroups][S::kCols];
+    const uint32_t s = a.head_div.div(blockIdx.x), h = blockIdx.x - s * a.heads;
+    const StateView v = state_view(a, s, h == 0 && threadIdx.x == 0);
+    if (!v.ok) return;
+    const int c = threadIdx.x % S::kCols, r = threadIdx.x / S::kCols;
+    float4 st[S::kRows];
+    const size_t size = static_cast<size_t>(D) * D;
+    const float* from = a.states + (static_cast<size_t>(v.source < 0 ? 0 : v.source) * a.heads + h) * size + 4 * c;
+#pragma unroll
+    for (int i = 0; i < S::kRows; ++i)
+        st[i] = v.source < 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                             : *reinterpret_cast<const float4*>(from + (r + i * S::kRowGroups) * D);
+    const float lambda = expf(a.log_decay[h]);
+    const uint32_t hk = a.group_div.div(h);
+    for (uint32_t i = 0; i < v.n; ++i) {
+        const size_t tok = v.start + i;
+        for (int e = threadIdx.x; e < 3 * D; e += S::kThreads) {
+            const int w = e / D, ch = e % D;
+            const T* src = w == 0 ? static_cast<const T*>(a.q) + tok * a.q_ts + h * a.q_hs
+                           : w == 1 ? static_cast<const T*>(a.k) + tok * a.k_ts + hk * a.k_hs
+                                    : static_cast<const T*>(a.v) + tok * a.v_ts + hk * a.v_hs;
+            (w == 0 ? q_s : w == 1 ? k_s : v_s)[ch] = static_cast<float>(src[ch]);
+        }
+        __syncthreads();
+        const float4 x = *reinterpret_cast<const float4*>(v_s + 4 * c);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < S::kRows; ++j) {
+            const float k = k_s[r + j * S::kRowGroups], q = q_s[r + j * S::kRowGroups];
+            st[j].x = fmaf(lambda, st[j].x, k * x.x), o.x = fmaf(q, st[j].x, o.x);
+            st[j].y = fmaf(lambda, st[j].y, k * x.y), o.y = fmaf(q, st[j].y, o.y);
+            st[j].z = fmaf(lambda, st[j].z, k * x.z), o.z = fmaf(q, st[j].z, o.z);
+            st[j].w = fmaf(lambda, st[j].w, k * x.w), o.w = fmaf(q, st[j].w, o.w);
+        }
+        part[r][c] = o;
+        __syncthreads();
+        for (int e = threadIdx.x; e < D; e += S::kThreads) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < S::kRowGroups; ++j) sum += reinterpret_cast<const float*>(part[j])[e];
+            static_cast<T*>(a.out)[tok * a.o_ts + h * a.o_hs + e] = static_cast<T>(sum * a.scale);
+        }
+    }
+    if (v.target < 0) return;
+    float* to = a.states + (static_cast<size_t>(v.target) * a.heads + h) * size + 4 * c;
+#pragma unroll
+    for (int i = 0; i < S::kRows; ++i) *reinterpret_cast<float4*>(to + (r + i * S::kRowGroups) * D) = st[i];
+}
+
+// --------------------------------------------------------- whole histories
+
+constexpr int kChunk = 64;
+
+template <typename T, int D> struct ChunkShape {
+    static constexpr bool kHalf = std::is_same_v<T, __half>;
+    static constexpr int kWarps = D == 128 ? 8 : 4, kThreads = kWarps * 32;
+    static constexpr int kSplit = kWarps / 4;        // warps that share 16 tokens, each with its value channels
+    static constexpr int kTile = kChunk * D * 2;     // bytes of a chunk of Q, K or V
+    static constexpr int kPitch = D + 4;             // floats of a row of an f32 state
+    static constexpr int kState = kHalf ? D * kPitch * 4 : D * D * 2;
+    static constexpr int kBytes = 6 * kTile + kState;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(ChunkShape<T, D>::kThreads)
+    linear_chunk_kernel(const __grid_constant__ LinearArgs a) {
+    using S = ChunkShape<T, D>;
+    constexpr int kSteps = D / 16, kTiles = D / 8, kCols = kTiles / S::kSplit;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float power[kChunk + 1];  // lambda^i
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t s = a.head_div.div(blockIdx.x), h = blockIdx.x - s * a.heads;
+    const StateView v = state_view(a, s, h == 0 && threadIdx.x == 0);
+    if (!v.ok) return;
+    const uint32_t hk = a.group_div.div(h);
+    float decay = a.log_decay[h];
+    if (decay < -200.0f) decay = -200.0f;  // (e^-200 is zero; minus infinity times zero would be NaN)
+    for (int i = threadIdx.x; i <= kChunk; i += S::kThreads) power[i] = expf(decay * i);
+
+    const uint32_t smem_a = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    uint8_t* const state_s = smem + 6 * S::kTile;
+    const uint32_t state_a = smem_a + 6 * S::kTile;
+    const uint32_t chunks = (v.n + kChunk - 1) / kChunk;
+    constexpr int kRowChunks = D / 8, kEach = kChunk * kRowChunks / S::kThreads;
+    auto load = [&](uint32_t i) {
+        if (i < chunks) {
+            const uint32_t dst = smem_a + (i & 1) * 3 * S::kTile;
+            const T* src[3] = {static_cast<const T*>(a.q) + h * a.q_hs, static_cast<const T*>(a.k) + hk * a.k_hs,
+                               static_cast<const T*>(a.v) + hk * a.v_hs};
+            const size_t ts[3] = {a.q_ts, a.k_ts, a.v_ts};
+#pragma unroll
+            for (int w = 0; w < 3; ++w)
+#pragma unroll
+                for (int c = 0; c < kEach; ++c) {
+                    const uint32_t x = c * S::kThreads + threadIdx.x, r = x / kRowChunks, ch = x % kRowChunks;
+                    const uint32_t tok = i * kChunk + r;
+                    const bool live = tok < v.n;
+                    cp_async16(dst + w * S::kTile + tile_at<D>(r, ch), src[w] + (v.start + (live ? tok : 0)) * ts[w] + 8 * ch, live);
+                }
+        }
+        cp_commit();
+    };
+    load(0);
+
+    // state: row 16 warp + g (+ 8), channels 8 n + 2 t (+ 1)
+    float st[kTiles][4];
+    const bool holds = warp < kSteps;
+    const size_t at = static_cast<size_t>(16 * warp + g) * D + 2 * t;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) st[n][0] = st[n][1] = st[n][2] = st[n][3] = 0.0f;
+    if (holds && v.source >= 0) {
+        const float* from = a.states + (static_cast<size_t>(v.source) * a.heads + h) * D * D + at;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+            const float2 x = *reinterpret_cast<const float2*>(from + 8 * n), y = *reinterpret_cast<const float2*>(from + 8 * D + 8 * n);
+            st[n][0] = x.x, st[n][1] = x.y, st[n][2] = y.x, st[n][3] = y.y;
+        }
+    }
+    const int tile = warp / S::kSplit, col0 = (warp % S::kSplit) * kCols;  // this warp's tokens and value channels
+
+#pragma unroll 1
+    for (uint32_t i = 0; i < chunks; ++i) {
+        // the state before the chunk, for the product with Q
+        if (holds) {
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = 16 * warp + g + 8 * r;
+                    if constexpr (S::kHalf)
+                        *reinterpret_cast<uint2*>(state_s + (row * S::kPitch + 8 * n + 2 * t) * 4) =
+                            make_uint2(to_tf32(st[n][2 * r]), to_tf32(st[n][2 * r + 1]));
+                    else
+                        *reinterpret_cast<uint32_t*>(state_s + tile_at<D>(row, n) + 4 * t) = pack2(st[n][2 * r], st[n][2 * r + 1], T{});
+                }
+        }
+        load(i + 1);
+        cp_wait<1>();
+        const uint8_t* const base = smem + (i & 1) * 3 * S::kTile;
+        const uint32_t q_a = smem_a + (i & 1) * 3 * S::kTile, k_a = q_a + S::kTile, v_a = k_a + S::kTile;
+        // infinities and NaN among the values must not reach earlier tokens as zero times them
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < kEach; ++c) {
+            const uint32_t x = c * S::kThreads + threadIdx.x;
+            const uint4 w = *reinterpret_cast<const uint4*>(base + 2 * S::kTile + tile_at<D>(x / kRowChunks, x % kRowChunks));
+            bad |= not_finite2<T>(w.x) | not_finite2<T>(w.y) | not_finite2<T>(w.z) | not_finite2<T>(w.w);
+        }
+        bad = __syncthreads_or(bad);
+        const uint32_t m = min(static_cast<uint32_t>(kChunk), v.n - i * kChunk);
+
+        if (16u * tile < m) {
+            // scores of tokens 16 tile + g (+ 8) with keys up to their own
+            float p[8][4], o[kCols][4];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) p[n][0] = p[n][1] = p[n][2] = p[n][3] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                uint32_t q[4];
+                ldsm4(q, q_a + tile_at<D>(16 * tile + (lane & 15), 2 * k + (lane >> 4)));
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    if (n > tile) continue;
+                    uint32_t b[4];  // keys 16 n + 0-7 at both halves of the channels, then keys 8-15
+                    ldsm4(b, k_a + tile_at<D>(16 * n + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                    mma<T>(p[2 * n], q, b[0], b[1]);
+                    mma<T>(p[2 * n + 1], q, b[2], b[3]);
+                }
+                if constexpr (!S::kHalf) {
+#pragma unroll
+                    for (int n = 0; n < kCols; n += 2) {
+                        uint32_t b[4];  // state rows 16 k + 0-15 at 8 channels, then at the next 8
+                        ldsm4t(b, state_a + tile_at<D>(16 * k + (lane & 15), col0 + n + (lane >> 4)));
+                        mma<T>(o[n], q, b[0], b[1]);
+                        mma<T>(o[n + 1], q, b[2], b[3]);
+                    }
+                } else {
+                    // halves have no room for a state's range: tf32, exact for q, with f16's precision for the state
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float2 r0 = half2_at(q[2 * e]), r1 = half2_at(q[2 * e + 1]);
+                        const uint32_t x[4] = {__float_as_uint(r0.x), __float_as_uint(r1.x), __float_as_uint(r0.y),
+                                               __float_as_uint(r1.y)};
+                        const float* rows = reinterpret_cast<const float*>(state_s) + (16 * k + 8 * e + 2 * t) * S::kPitch + 8 * col0 + g;
+#pragma unroll
+                        for (int n = 0; n < kCols; ++n)
+                            mma_tf32(o[n], x, __float_as_uint(rows[8 * n]), __float_as_uint(rows[S::kPitch + 8 * n]));
+                    }
+                }
+            }
+            // decays; what a token does not see is zero
+            float up[2] = {1.0f, 1.0f};
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = 16 * tile + g + 8 * r;
+                float top = 0.0f;
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = 8 * n + 2 * t + e;
+                        float& x = p[n][2 * r + e];
+                        x = key <= row && n <= 2 * tile + 1 ? x * power[max(row - key, 0)] : 0.0f;
+                        top = fmaxf(top, fabsf(x));
+                    }
+                float down = 1.0f;
+                if constexpr (S::kHalf) {
+                    // weights become halves below 2^15, by a power of two a row
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const float2 f = row_scale(top);
+                    down = f.x, up[r] = f.y;
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) p[n][2 * r] *= down, p[n][2 * r + 1] *= down;
+                }
+                const float grow = power[row + 1] * down;
+#pragma unroll
+                for (int n = 0; n < kCols; ++n) o[n][2 * r] *= grow, o[n][2 * r + 1] *= grow;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (k > tile) continue;
+                const uint32_t x[4] = {pack2(p[2 * k][0], p[2 * k][1], T{}), pack2(p[2 * k][2], p[2 * k][3], T{}),
+                                       pack2(p[2 * k + 1][0], p[2 * k + 1][1], T{}), pack2(p[2 * k + 1][2], p[2 * k + 1][3], T{})};
+#pragma unroll
+                for (int n = 0; n < kCols; n += 2) {
+                    uint32_t b[4];
+                    ldsm4t(b, v_a + tile_at<D>(16 * k + (lane & 15), col0 + n + (lane >> 4)));
+                    if (bad) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) b[e] = finite2<T>(b[e]);
+                    }
+                    mma<T>(o[n], x, b[0], b[1]);
+                    mma<T>(o[n + 1], x, b[2], b[3]);
+                }
+            }
+            if (bad) {
+                // the values that were left out, one by one, for the tokens that see them
+#pragma unroll 1
+                for (int r = 0; r < 2; ++r) {
+                    const int row = 16 * tile + g + 8 * r;
+#pragma unroll 1
+                    for (int key = 0; key <= row && key < static_cast<int>(m); ++key) {
+                        float dot = 0.0f;
+#pragma unroll 1
+                        for (int ch = 0; ch < D; ++ch)
+                            dot = fmaf(tile_value<T, D>(base, row, ch), tile_value<T, D>(base + S::kTile, key, ch), dot);
+                        dot *= power[row - key];
+#pragma unroll
+                        for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float x = tile_value<T, D>(base + 2 * S::kTile, key, 8 * (col0 + n) + 2 * t + e);
+                                if (!isfinite(x)) o[n][r ? 2 + e : e] += dot * x;
+                            }
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const uint32_t row = 16 * tile + g + 8 * r;
+                if (row >= m) continue;
+                T* to = static_cast<T*>(a.out) + (v.start + i * kChunk + row) * a.o_ts + h * a.o_hs + 8 * col0 + 2 * t;
+                const float f = a.scale * up[r];
+#pragma unroll
+                for (int n = 0; n < kCols; ++n)
+                    *reinterpret_cast<uint32_t*>(to + 8 * n) = pack2(o[n][2 * r] * f, o[n][2 * r + 1] * f, T{});
+            }
+        }
+        if (holds) {
+            // S' : rows of K turned over, times lambda^(m - 1 - j) and split in two parts, so that the state keeps
+            // 16 (f16: 22) bits of each of them
+            const float fade = expm1f(decay * m);
+            float scale[2] = {1.0f, 1.0f}, back[2] = {1.0f, 1.0f};
+            uint32_t raw[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                ldsm4t(raw[k], k_a + tile_at<D>(16 * k + (lane & 7) + ((lane >> 4) << 3), 2 * warp + ((lane >> 3) & 1)));
+            float w[4][4];  // weights of tokens 16 k + 2 t, + 1, + 8, + 9
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int left = static_cast<int>(m) - 1 - (16 * k + 2 * t + (e & 1) + 8 * (e >> 1));
+                    w[k][e] = left >= 0 ? power[left] : 0.0f;
+                }
+            if constexpr (S::kHalf) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float2 x = half2_at(raw[k][r + 2 * e]);
+                            top = fmaxf(top, fmaxf(fabsf(x.x) * w[k][2 * e], fabsf(x.y) * w[k][2 * e + 1]));
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const float2 f = row_scale(top);
+                    scale[r] = f.x, back[r] = f.y;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    st[n][e] = fmaf(st[n][e], fade, st[n][e]);
+                    if constexpr (S::kHalf) st[n][e] *= scale[e >> 1];
+                }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // register e: row g + 8 (e & 1), tokens 2 t (+ 1) + 8 (e >> 1)
+                    const float2 x = pair_at<T>(raw[k][e]);
+                    const float x0 = x.x * w[k][2 * (e >> 1)] * scale[e & 1], x1 = x.y * w[k][2 * (e >> 1) + 1] * scale[e & 1];
+                    hi[e] = pack2(x0, x1, T{});
+                    const float2 y = pair_at<T>(hi[e]);
+                    lo[e] = pack2(x0 - y.x, x1 - y.y, T{});
+                }
+#pragma unroll
+                for (int n = 0; n < kTiles; n += 2) {
+                    uint32_t b[4];
+                    ldsm4t(b, v_a + tile_at<D>(16 * k + (lane & 15), n + (lane >> 4)));
+                    mma<T>(st[n], hi, b[0], b[1]);
+                    mma<T>(st[n + 1], hi, b[2], b[3]);
+                    mma<T>(st[n], lo, b[0], b[1]);
+                    mma<T>(st[n + 1], lo, b[2], b[3]);
+                }
+            }
+            if constexpr (S::kHalf) {
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) st[n][e] *= back[e >> 1];
+            }
+        }
+        __syncthreads();  // the tiles and the state in shared memory are done with
+    }
+    if (holds && v.target >= 0) {
+        float* to = a.states + (static_cast<size_t>(v.target) * a.heads + h) * D * D + at;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+            *reinterpret_cast<float2*>(to + 8 * n) = make_float2(st[n][0], st[n][1]);
+            *reinterpret_cast<float2*>(to + 8 * D + 8 * n) = make_float2(st[n][2], st[n][3]);
+        }
+    }
+    cp_wait<0>();
+}
+
+template <typename T, int D> cudaError_t launch(const LinearArgs& a, cudaStream_t s) {
+    const uint32_t blocks = a.sequences * a.heads;
+    if (a.max_new <= kStepTokens) {
+        linear_step_kernel<T, D><<<blocks, StepShape<D>::kThreads, 0, s>>>(a);
+        return cudaGetLastError();
+    }
+    using S = ChunkShape<T, D>;
+    auto* kernel = linear_chunk_kernel<T, D>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (e != cudaSuccess) return e;
+    kernel<<<blocks, S::kThreads, S::kBytes, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T> cudaError_t by_dim(const LinearArgs& a, cudaStream_t s) {
+    switch (a.head_dim) {
+        case 32: return launch<T, 32>(a, s);
+        case 64: return launch<T, 64>(a, s);
+        default: return launch<T, 128>(a, s);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_linear_attention(const LinearArgs& a, int dtype, cudaStream_t s) {
+    return dtype == LWM_DTYPE_BF16 ? by_dim<bf16>(a, s) : by_dim<__half>(a, s);
+}
+
+}  // namespace lwm

@@ -36,6 +36,8 @@ struct FastDiv {
 // above 27 bits of sequence above 32 of detail), so that of many threads that
 // report at once one is read whole, not one's page with another's sequence.
 constexpr int kCacheErrStarts = 1, kCacheErrNew = 2, kCacheErrLength = 3, kCacheErrPage = 4, kCacheErrWait = 5;
+constexpr int kCacheErrGroup = 6, kCacheErrShared = 7;                      // groups that share a prefix
+constexpr int kStateErrStarts = 8, kStateErrNew = 9, kStateErrSlot = 10;    // linear attention
 constexpr uint32_t kCacheErrSequences = 1u << 27;  // as many as a batch may have
 struct CacheReport {
     int code;
@@ -123,6 +125,42 @@ inline uint64_t visible_span(const CacheAttnArgs& a, uint32_t tile_rows) {
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
 bool cache_attention_many_rows(const CacheAttnArgs& a);  // which of the two
 cudaError_t launch_cache_attention_tc(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
+
+// Linear attention: packed tokens, the state slots, the error word.
+struct LinearArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    size_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
+    float* states;  // [slots, heads, head_dim, head_dim]
+    const float* log_decay;
+    const int32_t* starts;
+    const int32_t* source;  // NULL: the sequence's own index
+    const int32_t* target;
+    uint32_t slots, sequences, tokens, max_new, heads, head_dim;
+    float scale;
+    FastDiv head_div, group_div;  // by heads, by heads a kv head
+    uint64_t* err;
+};
+constexpr uint32_t kStepTokens = 8;  // up to here the recurrent kernel
+cudaError_t launch_linear_attention(const LinearArgs& a, int dtype, cudaStream_t s);
+
+struct TokenArgs {
+    const void* logits;
+    size_t stride;
+    const float* uniform;
+    int32_t* tokens;
+    float* log_probs;
+    const float* temperatures;
+    const int32_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    double temperature, top_p, min_p;
+    uint32_t top_k, rows, vocab;
+};
+constexpr uint32_t kSampleVocab = 1u << 18;  // the largest
+cudaError_t launch_sample_tokens(const TokenArgs& a, int dtype, cudaStream_t s);
 
 struct GatedNormArgs {
     lwm_gated_norm_args a;

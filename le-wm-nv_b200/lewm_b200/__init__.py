@@ -333,6 +333,25 @@ class _GatedNormArgs(C.Structure):
                 ("pre_weight", VP), ("pre_bias", VP), ("out_weight", VP), ("out_bias", VP)]
 
 
+class _StateBatch(C.Structure):
+    _fields_ = [("states", VP), ("starts", VP), ("source", VP), ("target", VP), ("slots", U32), ("heads", U32),
+                ("head_dim", U32), ("sequences", U32), ("tokens", U32), ("max_new", U32)]
+
+
+class _LinearAttentionArgs(C.Structure):
+    _fields_ = [("q", VP), ("k", VP), ("v", VP), ("out", VP), ("q_token_stride", U64), ("q_head_stride", U64),
+                ("k_token_stride", U64), ("k_head_stride", U64), ("v_token_stride", U64), ("v_head_stride", U64),
+                ("out_token_stride", U64), ("out_head_stride", U64), ("log_decay", VP), ("kv_heads", U32),
+                ("dtype", I32), ("scale", F)]
+
+
+class _SampleTokensArgs(C.Structure):
+    _fields_ = [("logits", VP), ("stride", U64), ("uniform", VP), ("tokens", VP), ("log_probs", VP),
+                ("temperatures", VP), ("top_ks", VP), ("top_ps", VP), ("min_ps", VP), ("temperature", C.c_double),
+                ("top_p", C.c_double), ("min_p", C.c_double), ("top_k", U32), ("rows", U32), ("vocab", U32),
+                ("dtype", I32)]
+
+
 class Rotary(C.Structure):
     """lwm_rotary: rotary positions with one to four axes (include/lewm_b200.h)."""
     _fields_ = [("axes", U32), ("dims", U32 * 4), ("interleaved", I32), ("turn", U64 * 64)]
@@ -463,6 +482,8 @@ _sig("lwm_lewm_plan_nv12_device", C.c_int, VP, VP, VP, VP, U32, U32, U32, U32, I
      C.POINTER(_PlanDeviceResult))
 _sig("lwm_rotary_init", C.c_int, U32, C.POINTER(U32), C.POINTER(C.c_double), I32, C.POINTER(Rotary))
 _sig("lwm_rotary_device", C.c_int, VP, C.POINTER(Rotary), C.POINTER(_RotaryArgs))
+_sig("lwm_linear_attention_device", C.c_int, VP, C.POINTER(_StateBatch), C.POINTER(_LinearAttentionArgs))
+_sig("lwm_sample_tokens_device", C.c_int, VP, C.POINTER(_SampleTokensArgs))
 _sig("lwm_cache_append_device", C.c_int, VP, C.POINTER(_PagedCache), C.POINTER(_CacheBatch), C.POINTER(Rotary),
      C.POINTER(_CacheAppendArgs))
 _sig("lwm_cache_gather_device", C.c_int, VP, C.POINTER(_PagedCache), C.POINTER(_CacheBatch),
@@ -1435,6 +1456,105 @@ def cache_attention_device(ctx: Context, cache: PagedCache, batch: CacheBatch, q
     a = _CacheAttentionArgs(qp, op, qt, qh, ot, oh, heads, cache.head_dim ** -0.5 if scale is None else scale,
                             int(causal), window, sinks, frame_tokens)
     _check(lib.lwm_cache_attention_device(ctx.handle, cache._ref, batch._ref, C.byref(a)))
+
+
+class StateBatch:
+    """lwm_state_batch over torch tensors: states [slots, heads, head_dim,
+    head_dim] float32, starts [sequences + 1], source and target [sequences]
+    (int32 device tensors, read when the kernels run; None: slot s for sequence
+    s; below 0: from zero, not kept), the packed rows `tokens`, and a bound of a
+    sequence's new tokens (None: `tokens`)."""
+
+    def __init__(self, states, starts, tokens: int, max_new: Optional[int] = None, source=None, target=None):
+        if states.dim() != 4 or states.shape[2] != states.shape[3] or str(states.dtype) != "torch.float32":
+            raise LwmError(1, "states must be a [slots, heads, head_dim, head_dim] float32 tensor")
+        if not states.is_contiguous():
+            raise LwmError(1, "states must be contiguous")
+        if starts.dim() != 1 or starts.shape[0] < 1:
+            raise LwmError(1, "starts must be [sequences + 1]")
+        n = starts.shape[0] - 1
+        _sizes("states", states.shape)
+        _sizes("starts", starts.shape)
+        _ints("starts", starts, (n + 1,))
+        max_new = tokens if max_new is None else max_new
+        _u32("tokens", tokens)
+        _u32("max_new", max_new)
+        for name, t in (("source", source), ("target", target)):
+            if t is not None:
+                _ints(name, t, (n,))
+        self._keep = (states, starts, source, target)
+        if any(t is not None and t.device != states.device for t in self._keep):
+            raise LwmError(1, "state tensors are on different devices")
+        self.device, self.device_index = states.device, states.get_device()
+        self.tokens, self.heads, self.head_dim = tokens, states.shape[1], states.shape[2]
+        at = [None if t is None else t.data_ptr() for t in self._keep]
+        self._c = _StateBatch(*at, *states.shape[:3], n, tokens, max_new)
+        self._ref = C.byref(self._c)
+
+
+def linear_attention_device(ctx: Context, batch: StateBatch, q, k, v, out, log_decay, scale: Optional[float] = None) -> None:
+    """out = linear attention of q [tokens, heads, head_dim] over k, v [tokens,
+    kv_heads, head_dim] and the batch's states, which go on to their targets;
+    log_decay [heads] float32 (scale None: head_dim ** -0.5).  `out` and the
+    states are ready on the context's stream."""
+    if batch.device_index != ctx.device:
+        raise LwmError(1, f"states must be on cuda:{ctx.device}, got {batch.device}")
+    if k.dim() != 3:
+        raise LwmError(1, f"k must be [tokens, kv_heads, head_dim], got {list(k.shape)}")
+    n, heads, d = batch.tokens, batch.heads, batch.head_dim
+    kv = k.shape[1]
+    if kv >> 32:
+        _sizes("k", k.shape)
+    dtype = q.dtype
+    qp, qt, qh = _heads(ctx, "q", q, (n, heads, d), dtype)
+    kp, kt, kh = _heads(ctx, "k", k, (n, kv, d), dtype)
+    vp, vt, vh = _heads(ctx, "v", v, (n, kv, d), dtype)
+    op, ot, oh = _heads(ctx, "out", out, (n, heads, d), dtype)
+    if log_decay.shape != (heads,) or str(log_decay.dtype) != "torch.float32" or not log_decay.is_contiguous():
+        raise LwmError(1, f"log_decay must be a contiguous float32 tensor [{heads}], got {log_decay.dtype} {list(log_decay.shape)}")
+    a = _LinearAttentionArgs(qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, _on(ctx, "log_decay", log_decay), kv,
+                             _dtype(q, "q"), d ** -0.5 if scale is None else scale)
+    _check(lib.lwm_linear_attention_device(ctx.handle, batch._ref, C.byref(a)))
+
+
+def sample_tokens_device(ctx: Context, logits, uniform, tokens, log_probs=None, temperature=1.0, top_k=0, top_p=1.0,
+                         min_p=0.0) -> None:
+    """tokens [rows] int32 = a token of each row of logits [rows, vocab], drawn
+    with the random numbers uniform [rows] float32 in [0, 1) from what top_k,
+    top_p and min_p keep; log_probs [rows] float32 its log-probability there.
+    Each parameter is a number or a [rows] tensor (float32, top_k int32).
+    Outputs are ready on the context's stream."""
+    if logits.dim() != 2:
+        raise LwmError(1, f"logits must be [rows, vocab], got {list(logits.shape)}")
+    rows, vocab = logits.shape
+    if (rows | vocab) >> 32:
+        _sizes("logits", logits.shape)
+    stride, unit = logits.stride()
+    if unit != 1 and vocab > 1:
+        raise LwmError(1, "logits need contiguous rows")
+    at = []
+    for name, t, kind in (("uniform", uniform, "float32"), ("tokens", tokens, "int32"), ("log_probs", log_probs, "float32")):
+        if t is None and name == "log_probs":
+            at.append(None)
+            continue
+        if t.shape != (rows,) or str(t.dtype) != "torch." + kind or not t.is_contiguous():
+            raise LwmError(1, f"{name} must be a contiguous {kind} tensor [{rows}], got {t.dtype} {list(t.shape)}")
+        at.append(_on(ctx, name, t))
+    values, arrays = [], []
+    for name, x, kind, usual in (("temperature", temperature, "float32", 1.0), ("top_k", top_k, "int32", 0),
+                                 ("top_p", top_p, "float32", 1.0), ("min_p", min_p, "float32", 0.0)):
+        if hasattr(x, "data_ptr"):
+            if x.shape != (rows,) or str(x.dtype) != "torch." + kind or not x.is_contiguous():
+                raise LwmError(1, f"{name} must be a number or a contiguous {kind} tensor [{rows}]")
+            arrays.append(_on(ctx, name, x))
+            x = usual
+        else:
+            arrays.append(None)
+        values.append(x)
+    _u32("top_k", values[1])
+    a = _SampleTokensArgs(_on(ctx, "logits", logits), stride, *at, *arrays, values[0], values[2], values[3], values[1],
+                          rows, vocab, _dtype(logits, "logits"))
+    _check(lib.lwm_sample_tokens_device(ctx.handle, C.byref(a)))
 
 
 class GatedNorm:
