@@ -904,6 +904,44 @@ typedef struct lwm_cache_attention_args {
 lwm_status lwm_cache_attention_device(lwm_ctx* ctx, const lwm_paged_cache* cache, const lwm_cache_batch* batch,
                                       const lwm_cache_attention_args* args);
 
+/* The same attention for sequences that share their first tokens, such as the
+ * candidates that continue one vehicle's history: the prefix's keys and values
+ * are read once for all rows of a group, not once a sequence.
+ * Device arrays: groups [count + 1] (ascending sequence indices: group g is
+ * sequences [groups[g], groups[g + 1]); sequences of no group are attended by
+ * themselves), lengths [count] (tokens of the group's prefix, its cached
+ * tokens 0 .. lengths[g] - 1, in whole pages or not).  The page tables of a
+ * group's sequences name pages that hold the same tokens there (the same pages
+ * as a rule, and for a page that the prefix ends in a copy of each sequence's
+ * own); a call may read them from the first sequence's.  New tokens lie behind
+ * the prefix.  max_tokens is at least the packed rows of any group,
+ * max_length (0: the table's reach) and max_tail (0: the batch's max_length
+ * less this one, if both are given) say how long prefixes and what follows
+ * them get, for the shape of the launch only.
+ *
+ * workspace: 16-byte aligned, at least as many bytes as
+ * lwm_cache_attention_shared_workspace says for the same arguments (tensors
+ * may be null there; none are needed, 0, where the sequences are so few or the prefix
+ * so short that lwm_cache_attention_device costs less; it runs then).  It holds
+ * nothing between calls; calls in flight at once need one each.
+ *
+ * A group whose sequences or rows are out of order or above max_tokens, or
+ * whose prefix is beyond the table, is skipped with the sequences that it
+ * names, as is a sequence whose new tokens reach into its prefix; the next
+ * lwm_ctx_synchronize names one (not where lwm_cache_attention_device runs,
+ * which does not look at the groups). */
+typedef struct lwm_shared_prefix {
+    const int32_t* groups;
+    const int32_t* lengths;
+    uint32_t count, max_tokens, max_length, max_tail;
+} lwm_shared_prefix;
+lwm_status lwm_cache_attention_shared_workspace(const lwm_paged_cache* cache, const lwm_cache_batch* batch,
+                                                const lwm_shared_prefix* prefix, const lwm_cache_attention_args* args,
+                                                uint64_t* bytes);
+lwm_status lwm_cache_attention_shared_device(lwm_ctx* ctx, const lwm_paged_cache* cache, const lwm_cache_batch* batch,
+                                             const lwm_shared_prefix* prefix, const lwm_cache_attention_args* args,
+                                             void* workspace, uint64_t workspace_bytes);
+
 /* Linear attention with a decay for each head: with lambda = exp(log_decay
  * of the head), over a sequence's tokens in order,
  *   S = lambda S + k v^T,   out = scale q S,

@@ -118,6 +118,80 @@ lwm_status check_run_blocks(const lwm::CacheArgs& a) {
     return LWM_OK;
 }
 
+// An attention call's arguments; `work`: there is something to do.
+lwm_status check_attention(const lwm_paged_cache* cache, const lwm_cache_batch* batch, const lwm_cache_attention_args* x,
+                           lwm::CacheAttnArgs* out, bool* work, bool tensors = true) {
+    if (!x) return bad("null argument");
+    lwm::CacheAttnArgs a{};
+    LWM_TRY(check_cache(cache, batch, &a.c));
+    if (x->heads == 0 || x->heads % cache->kv_heads || x->heads > 65535)
+        return bad("query heads " + std::to_string(x->heads) + " must be a positive multiple of kv_heads " +
+                   std::to_string(cache->kv_heads));
+    if (!std::isfinite(x->scale)) return bad("attention scale must be finite");
+    if (x->frame_tokens > (1u << 30)) return bad("frame_tokens out of range");
+    a.heads = x->heads;
+    a.group = x->heads / cache->kv_heads;
+    if (static_cast<uint64_t>(a.c.max_new) * a.group > 0x7fffffffull)
+        return fail(LWM_UNSUPPORTED, "batch is too large for one call");
+    const uint64_t jobs = static_cast<uint64_t>(a.c.sequences) * cache->kv_heads *
+                          ((static_cast<uint64_t>(a.c.max_new) * a.group + 15) / 16);
+    if (jobs > (0x7fffffffull >> 4)) return fail(LWM_UNSUPPORTED, "batch is too large for one call");
+    *work = a.c.sequences && a.c.max_new;
+    if (*work && tensors) {
+        LWM_TRY(check_heads("q", x->q, x->q_token_stride, x->q_head_stride));
+        LWM_TRY(check_heads("out", x->out, x->out_token_stride, x->out_head_stride));
+    }
+    a.q = x->q;
+    a.out = x->out;
+    a.q_ts = x->q_token_stride;
+    a.q_hs = x->q_head_stride;
+    a.o_ts = x->out_token_stride;
+    a.o_hs = x->out_head_stride;
+    a.scale_log2 = x->scale * 1.4426950408889634f;
+    a.causal = x->causal != 0;
+    a.window = x->window;
+    a.sinks = x->sinks;
+    a.frame = x->frame_tokens ? x->frame_tokens : 1;
+    a.group_div = lwm::FastDiv(a.group);
+    a.frame_div = lwm::FastDiv(a.frame);
+    *out = a;
+    return LWM_OK;
+}
+
+cudaError_t launch_attention(const lwm::CacheAttnArgs& a, const lwm_paged_cache* cache, cudaStream_t s) {
+    return lwm::cache_attention_many_rows(a) ? lwm::launch_cache_attention_tc(a, cache->dtype, cache->storage, s)
+                                             : lwm::launch_cache_attention(a, cache->dtype, cache->storage, s);
+}
+
+// The groups of a call that shares prefixes, and how it is to run: no parts
+// (splits 0) where every sequence for itself costs less.
+lwm_status check_shared(const lwm_shared_prefix* p, const lwm_cache_batch* b, lwm::CacheAttnArgs* a, lwm::SharedPlan* plan) {
+    if (!p) return bad("null argument");
+    if (p->count > b->sequences) return bad("groups " + std::to_string(p->count) + " are more than the sequences");
+    if (p->count && (!p->groups || !p->lengths)) return bad("group arrays are null");
+    if (!aligned4(p->groups) || !aligned4(p->lengths)) return bad("group arrays are not 4-byte aligned");
+    if (p->max_tokens > b->tokens) return bad("max_tokens " + std::to_string(p->max_tokens) + " is above the batch's tokens " + std::to_string(b->tokens));
+    a->groups = p->groups;
+    a->shared = p->lengths;
+    a->group_count = p->count;
+    a->max_tokens = p->max_tokens;
+    a->max_tail = p->max_tail;
+    if (!a->max_tail && p->max_length && b->max_length > p->max_length) a->max_tail = b->max_length - p->max_length;
+    plan->splits = 0;
+    const uint64_t rows = static_cast<uint64_t>(p->max_tokens) * a->group;
+    if (rows > 0x7fffffffull || (rows / 128 + 1) * p->count * a->c.kv_heads > (0x7fffffffull >> 6))
+        return fail(LWM_UNSUPPORTED, "batch is too large for one call");
+    if (!p->count || !p->max_tokens) return LWM_OK;
+    lwm::CacheAttnArgs prefix = *a;
+    prefix.c.max_length = p->max_length;
+    const lwm::SharedPlan best = lwm::shared_plan(prefix, 64);
+    if (best.cost + lwm::shared_tail_cost(*a) < lwm::cache_attention_cost(*a)) *plan = best;
+    return LWM_OK;
+}
+uint64_t shared_bytes(const lwm::CacheAttnArgs& a, const lwm::SharedPlan& plan) {
+    return static_cast<uint64_t>(plan.splits) * a.c.tokens * a.heads * (a.c.head_dim + 1) * sizeof(float);
+}
+
 }  // namespace
 
 extern "C" {
@@ -260,49 +334,54 @@ lwm_status lwm_cache_gather_device(lwm_ctx* ctx, const lwm_paged_cache* cache, c
 
 lwm_status lwm_cache_attention_device(lwm_ctx* ctx, const lwm_paged_cache* cache, const lwm_cache_batch* batch,
                                       const lwm_cache_attention_args* x) {
-    if (!x) return bad("null argument");
     lwm::CacheAttnArgs a{};
-    LWM_TRY(check_cache(cache, batch, &a.c));
-    if (x->heads == 0 || x->heads % cache->kv_heads || x->heads > 65535)
-        return bad("query heads " + std::to_string(x->heads) + " must be a positive multiple of kv_heads " +
-                   std::to_string(cache->kv_heads));
-    if (!std::isfinite(x->scale)) return bad("attention scale must be finite");
-    if (x->frame_tokens > (1u << 30)) return bad("frame_tokens out of range");
-    a.heads = x->heads;
-    a.group = x->heads / cache->kv_heads;
-    if (static_cast<uint64_t>(a.c.max_new) * a.group > 0x7fffffffull)
-        return fail(LWM_UNSUPPORTED, "batch is too large for one call");
-    const uint64_t jobs = static_cast<uint64_t>(a.c.sequences) * cache->kv_heads *
-                          ((static_cast<uint64_t>(a.c.max_new) * a.group + 15) / 16);
-    if (jobs > (0x7fffffffull >> 4)) return fail(LWM_UNSUPPORTED, "batch is too large for one call");
-    const bool work = a.c.sequences && a.c.max_new;
-    if (work) {
-        LWM_TRY(check_heads("q", x->q, x->q_token_stride, x->q_head_stride));
-        LWM_TRY(check_heads("out", x->out, x->out_token_stride, x->out_head_stride));
-    }
+    bool work = false;
+    LWM_TRY(check_attention(cache, batch, x, &a, &work));
     CtxView c;
     if (!lwm::ctx_view(ctx, &c)) return bad("null context");
     if (!work) return LWM_OK;
     a.c.err = c.cache_err;
-    a.q = x->q;
-    a.out = x->out;
-    a.q_ts = x->q_token_stride;
-    a.q_hs = x->q_head_stride;
-    a.o_ts = x->out_token_stride;
-    a.o_hs = x->out_head_stride;
-    a.scale_log2 = x->scale * 1.4426950408889634f;
-    a.causal = x->causal != 0;
-    a.window = x->window;
-    a.sinks = x->sinks;
-    a.frame = x->frame_tokens ? x->frame_tokens : 1;
-    a.group_div = lwm::FastDiv(a.group);
-    a.frame_div = lwm::FastDiv(a.frame);
-    return on_device(ctx, c, "cache attention",
-                     [&](cudaStream_t s) {
-                         return lwm::cache_attention_many_rows(a)
-                                    ? lwm::launch_cache_attention_tc(a, cache->dtype, cache->storage, s)
-                                    : lwm::launch_cache_attention(a, cache->dtype, cache->storage, s);
-                     });
+    return on_device(ctx, c, "cache attention", [&](cudaStream_t s) { return launch_attention(a, cache, s); });
+}
+
+lwm_status lwm_cache_attention_shared_workspace(const lwm_paged_cache* cache, const lwm_cache_batch* batch,
+                                                const lwm_shared_prefix* prefix, const lwm_cache_attention_args* x,
+                                                uint64_t* bytes) {
+    if (!bytes) return bad("null argument");
+    lwm::CacheAttnArgs a{};
+    bool work = false;
+    lwm::SharedPlan plan;
+    LWM_TRY(check_attention(cache, batch, x, &a, &work, false));
+    LWM_TRY(check_shared(prefix, batch, &a, &plan));
+    *bytes = work ? shared_bytes(a, plan) : 0;
+    return LWM_OK;
+}
+
+lwm_status lwm_cache_attention_shared_device(lwm_ctx* ctx, const lwm_paged_cache* cache, const lwm_cache_batch* batch,
+                                             const lwm_shared_prefix* prefix, const lwm_cache_attention_args* x,
+                                             void* workspace, uint64_t workspace_bytes) {
+    lwm::CacheAttnArgs a{};
+    bool work = false;
+    lwm::SharedPlan plan;
+    LWM_TRY(check_attention(cache, batch, x, &a, &work));
+    LWM_TRY(check_shared(prefix, batch, &a, &plan));
+    const uint64_t need = work ? shared_bytes(a, plan) : 0;
+    if (need && workspace_bytes < need)
+        return bad("workspace has " + std::to_string(workspace_bytes) + " bytes, the call needs " + std::to_string(need));
+    if (need && !workspace) return bad("workspace is null");
+    if (need && !aligned16(workspace)) return bad("workspace is not 16-byte aligned");
+    CtxView c;
+    if (!lwm::ctx_view(ctx, &c)) return bad("null context");
+    if (!work) return LWM_OK;
+    a.c.err = c.cache_err;
+    if (!need) return on_device(ctx, c, "cache attention", [&](cudaStream_t s) { return launch_attention(a, cache, s); });
+    a.splits = plan.splits;
+    a.part_out = static_cast<float*>(workspace);
+    a.part_log = a.part_out + static_cast<size_t>(a.splits) * a.c.tokens * a.heads * a.c.head_dim;
+    LWM_TRY(on_device(ctx, c, "shared attention's prefix",
+                      [&](cudaStream_t s) { return lwm::launch_cache_attention_prefix(a, plan.rows, cache->dtype, cache->storage, s); }));
+    return on_device(ctx, c, "shared attention's tails",
+                     [&](cudaStream_t s) { return lwm::launch_cache_attention_tail(a, cache->dtype, cache->storage, s); });
 }
 
 lwm_status lwm_gated_norm_device(lwm_ctx* ctx, const lwm_gated_norm_args* x) {

@@ -156,7 +156,7 @@ struct UnitNote {
 // Visible keys of one row: [0, first) and [lo, hi).
 struct RowRange { uint32_t lo, hi, first; };
 
-template <typename T, int D, bool kCodes, int kRows, bool kShared>
+template <typename T, int D, bool kCodes, int kRows, bool kShared, int kKeys>
 __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kBlocks)
     cache_attn_kernel(const __grid_constant__ CacheAttnArgs a, uint32_t tiles, uint32_t split) {
     using M = std::conditional_t<kCodes, __half, T>;  // the operands' type
@@ -179,9 +179,31 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
             entry = a.c.table[static_cast<size_t>(s) * a.c.table_stride + lane];
         v = sequence(a.c, s, false, h0 == 0 && tile == 0 && rank == 0 && lane == 0);
     }
+    // A tail: what lies behind the prefix that the sequence's group shares (no group: everything).
+    constexpr bool kTail = kKeys == kTailKeys;
+    uint32_t shared = 0;
+    bool joined = false;  // with the prefix's parts
+    if constexpr (kTail) {
+        if (v.ok && a.group_count && static_cast<int>(s) >= a.groups[0]) {
+            const uint32_t g = last_at_most(a.groups, 0, a.group_count, static_cast<int>(s));
+            if (static_cast<int>(s) < a.groups[g + 1]) {
+                const GroupView group = group_view(a, g, false);
+                // (the prefix's rows are the group's)
+                joined = group.ok && v.start >= group.start && v.start + v.n <= group.start + group.n;
+                shared = group.shared;
+                const bool reaches = joined && v.n && static_cast<uint64_t>(v.n) + shared > v.length;
+                if (reaches && h0 == 0 && tile == 0 && rank == 0 && lane == 0) cache_report(a.c.err, kCacheErrShared, s, shared);
+                if (!joined || reaches) v.n = 0;
+            }
+        }
+    }
     const uint32_t rows = v.n * a.group, row0 = tile * kRows;
     const bool live = row0 < rows;
-    if (!live && (!kShared || split == 1)) return;  // uniform over what waits together
+    if (!live && (!kShared || split == 1)) {  // uniform over what waits together
+        // (this grid is not done before the prefix's is)
+        if constexpr (kTail) asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
 
     // the keys that this thread's queries 8 n + 2 t + e see, and the tile's union
     RowRange rr[kQ][2];
@@ -195,18 +217,20 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
                 rr[n][e] = {0, 0, 0};
                 if (R < rows) {
                     const VisibleRange vr = visible(a, v, a.group_div.div(R));
-                    rr[n][e] = {vr.lo, vr.hi, vr.first};
+                    rr[n][e] = {kTail ? max(vr.lo, shared) : vr.lo, vr.hi, vr.first};
                 }
             }
         const uint32_t tok0 = a.group_div.div(row0), tok1 = a.group_div.div(min(row0 + kRows - 1, rows - 1));
         const VisibleRange r0 = visible(a, v, tok0), r1 = visible(a, v, tok1);
         lo_min = r0.lo, hi_min = r0.hi;
         lo_max = r1.lo, hi_max = r1.hi;
+        if (kTail) lo_min = max(lo_min, shared), lo_max = max(lo_max, shared);
     }
     const bool mixed = lo_min != lo_max || hi_min != hi_max;  // rows that differ in what they see
     const uint32_t sinks_end = min(a.sinks, min(lo_min, hi_max));
-    const uint32_t sink_units = (sinks_end + kUnit - 1) / kUnit;
-    const uint32_t win_unit = max(lo_min / kUnit, sink_units);
+    const uint32_t sink0 = kTail ? min(shared, sinks_end) / kUnit : 0;  // (a tail's first unit may hold keys of the prefix)
+    const uint32_t sink_units = kTail && sinks_end <= shared ? 0 : (sinks_end + kUnit - 1) / kUnit - sink0;
+    const uint32_t win_unit = max(lo_min / kUnit, sink_units ? sink0 + sink_units : 0);
     const uint32_t win_units = hi_max > win_unit * kUnit ? (hi_max - win_unit * kUnit + kUnit - 1) / kUnit : 0;
     const uint32_t units = sink_units + win_units;
     // this warp's units: walk, walk + step, ... below end
@@ -220,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
     const uint32_t count = walk < end ? (end - walk + step - 1) / step : 0;
     auto key_of = [&](uint32_t i) {
         const uint32_t u = walk + i * step;
-        return (u < sink_units ? u : u - sink_units + win_unit) * kUnit;
+        return (u < sink_units ? u + sink0 : u - sink_units + win_unit) * kUnit;
     };
     // page of the warp's unit i: from the table's row, or looked up 32 units at a time
     int pages_ahead = -1;
@@ -252,12 +276,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
         const uint8_t* kp = static_cast<const uint8_t*>(a.c.k) + base + lane * 16;
         const uint8_t* vp = static_cast<const uint8_t*>(a.c.v) + base + lane * 16;
         // rows that no query sees come as zeros
-        const bool all = page >= 0 && key + kUnit <= hi_max && (key >= lo_min || key + kUnit <= sinks_end);
+        const bool all = page >= 0 && key + kUnit <= hi_max && (key >= lo_min || (key + kUnit <= sinks_end && key >= shared));
 #pragma unroll
         for (int c = 0; c < kUnit * kRowChunks / 32; ++c) {
             const uint32_t x = c * 32 + lane, r = x / kRowChunks, ch = x % kRowChunks;
             const uint32_t j = key + r;
-            const bool ok = all || (page >= 0 && j < hi_max && (j >= lo_min || j < sinks_end));
+            const bool ok = all || (page >= 0 && j < hi_max && (j >= lo_min || (j < sinks_end && j >= shared)));
             cp_async16(dst + chunk_at<D, kCodes>(r, ch), kp + c * 512, ok);
             cp_async16(dst + S::kUnitBytes + chunk_at<D, kCodes>(r, ch), vp + c * 512, ok);
         }
@@ -419,10 +443,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
             }
         }
         // in units of log2, masked where a query does not see the key
-        const bool whole = page >= 0 && (key >= lo_max || key + kUnit <= sinks_end) && key + kUnit <= hi_min;
+        const bool whole = page >= 0 && (key >= lo_max || (key + kUnit <= sinks_end && key >= shared)) && key + kUnit <= hi_min;
         auto sees = [&](int n, int e) {
             const uint32_t j = key + g + 8 * (e >> 1);
-            return page >= 0 && j < rr[n][e & 1].hi && (j >= rr[n][e & 1].lo || j < rr[n][e & 1].first);
+            return page >= 0 && j < rr[n][e & 1].hi && (j >= rr[n][e & 1].lo || (j < rr[n][e & 1].first && j >= shared));
         };
         bool above = false;
 #pragma unroll
@@ -548,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
                         const float low = __shfl_sync(0xffffffffu, p[n][e], (r & 7) * 4 + t);
                         const float high = __shfl_sync(0xffffffffu, p[n][e + 2], (r & 7) * 4 + t);
                         const float pk = r < 8 ? low : high;
-                        if (!(page >= 0 && j < rr[n][e].hi && (j >= rr[n][e].lo || j < rr[n][e].first))) continue;
+                        if (!(page >= 0 && j < rr[n][e].hi && (j >= rr[n][e].lo || (j < rr[n][e].first && j >= shared)))) continue;
 #pragma unroll
                         for (int d = 0; d < kSteps; ++d)
 #pragma unroll
@@ -572,6 +596,37 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
             l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
         }
 
+    constexpr float kUnitLog = !std::is_same_v<M, __half> ? 0.0f : kCodes ? 5.0f : 7.0f;  // (the weights' kLift)
+    if constexpr (kTail) asm volatile("griddepcontrol.wait;" ::: "memory");  // the prefix's parts are there
+    // a row's share of each part: the sum of weights behind it, relative to the whole (`tail` its own log2, and its
+    // share when it returns); parts are read one after another
+    auto part_row = [&](uint32_t R, uint32_t hh) {
+        const uint32_t tok = a.group_div.div(R);
+        return (static_cast<size_t>(v.start) + tok) * a.heads + hh * a.group + (R - tok * a.group);
+    };
+    const size_t part_rows = static_cast<size_t>(a.c.tokens) * a.heads;
+    auto join = [&](size_t row, float& tail, float& top) {
+        top = tail;
+        bool nan = tail != tail;
+        if (joined)
+            for (uint32_t x = 0; x < a.splits; ++x) {
+                const float log = a.part_log[x * part_rows + row];
+                top = fmaxf(top, log);
+                nan |= log != log;
+            }
+        if (top == -INFINITY && !nan) {
+            tail = 0.0f;
+            return 0.0f;
+        }
+        if (nan) top = __int_as_float(0x7fc00000);
+        float sum = tail = exp2_fast(tail - top);
+        if (joined)
+            for (uint32_t x = 0; x < a.splits; ++x) sum += exp2_fast(a.part_log[x * part_rows + row] - top);
+        const float inv = 1.0f / sum;
+        tail *= inv;
+        return inv;
+    };
+
     if constexpr (!kShared) {
         // the warp's own rows: through shared memory to whole 16-byte stores
         T* part = reinterpret_cast<T*>(smem + S::kRings + kWarps * S::kStages * 16 + warp * kRows * D * 2);
@@ -582,11 +637,38 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
                 const bool none = l[n][e] == 0.0f;  // nothing weighs, not even against infinities in O
                 const float inv = none ? 0.0f : 1.0f / l[n][e];
                 const float unit = kCodes ? power_of_two(vx[n][e]) : 1.0f;
+                if constexpr (kTail) {
+                    const uint32_t R = row0 + 8 * n + 2 * t + e;
+                    float tail = none ? -INFINITY : m[n][e] - kUnitLog + log2f(l[n][e]), top = -INFINITY, all = 0.0f;
+                    const size_t row = R < rows ? part_row(R, h) : 0;
+                    if (R < rows) all = join(row, tail, top);
+#pragma unroll
+                    for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) o[n][d][2 * x + e] = none ? 0.0f : o[n][d][2 * x + e] * inv * unit * tail;
+                    if (R < rows && joined) {
+                        for (uint32_t y = 0; y < a.splits; ++y) {
+                            const float w = all == 0.0f ? 0.0f : exp2_fast(a.part_log[y * part_rows + row] - top) * all;
+                            if (w == 0.0f) continue;
+                            const float* from = a.part_out + (y * part_rows + row) * D;
+#pragma unroll
+                            for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+                                for (int x = 0; x < 2; ++x) o[n][d][2 * x + e] += w * from[channel(d, x)];
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            part[(8 * n + 2 * t + e) * D + channel(d, x)] = static_cast<T>(o[n][d][2 * x + e]);
+                } else {
 #pragma unroll
                 for (int d = 0; d < kSteps; ++d)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
                         part[(8 * n + 2 * t + e) * D + channel(d, x)] = static_cast<T>(none ? 0.0f : o[n][d][2 * x + e] * inv * unit);
+                }
             }
         __syncwarp();
         for (int x = lane; x < kRows * D / 8; x += 32) {
@@ -665,7 +747,24 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
                         acc.w += ov.w * f;
                     }
                 }
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, up = kCodes ? power_of_two(unit) : 1.0f;
+                float inv = sum == 0.0f ? 0.0f : 1.0f / sum, up = kCodes ? power_of_two(unit) : 1.0f;
+                if constexpr (kTail) {
+                    float tail = sum == 0.0f ? -INFINITY : top - kUnitLog + log2f(sum), high = -INFINITY;
+                    const size_t row = part_row(R, h);
+                    const float all = join(row, tail, high);
+                    if (sum == 0.0f) acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    acc.x = acc.x * inv * up * tail, acc.y = acc.y * inv * up * tail;
+                    acc.z = acc.z * inv * up * tail, acc.w = acc.w * inv * up * tail;
+                    if (joined) {
+                        for (uint32_t y = 0; y < a.splits; ++y) {
+                            const float w = all == 0.0f ? 0.0f : exp2_fast(a.part_log[y * part_rows + row] - high) * all;
+                            if (w == 0.0f) continue;
+                            const float4 x = *reinterpret_cast<const float4*>(a.part_out + (y * part_rows + row) * D + c4);
+                            acc.x += w * x.x, acc.y += w * x.y, acc.z += w * x.z, acc.w += w * x.w;
+                        }
+                    }
+                    inv = up = 1.0f;
+                }
                 const uint32_t tok = a.group_div.div(R), head = h * a.group + (R - tok * a.group);
                 uint2 w2 = make_uint2(pack2(acc.x * inv * up, acc.y * inv * up, T{}), pack2(acc.z * inv * up, acc.w * inv * up, T{}));
                 *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (v.start + tok) * a.o_ts + head * a.o_hs + c4) = w2;
@@ -676,11 +775,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
     }
 }
 
-template <typename T, int D, bool kCodes, int kRows> cudaError_t launch(CacheAttnArgs a, cudaStream_t s) {
+// The tails' kernel may start while the prefix's runs: it waits for that one before it reads its parts.
+cudaLaunchAttribute beside_the_prefix() {
+    cudaLaunchAttribute x{};
+    x.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    x.val.programmaticStreamSerializationAllowed = 1;
+    return x;
+}
+
+template <typename T, int D, bool kCodes, int kRows, int kKeys> cudaError_t launch(CacheAttnArgs a, cudaStream_t s) {
     const uint32_t tiles = (a.c.max_new * a.group + kRows - 1) / kRows;
     const uint64_t jobs = static_cast<uint64_t>(a.c.sequences) * a.c.kv_heads * tiles;
     a.tile_div = FastDiv(tiles);
-    const uint64_t span = visible_span(a, kRows);
+    const uint64_t span = kKeys == kTailKeys && a.max_tail ? min(visible_span(a, kRows), uint64_t{a.max_tail}) : visible_span(a, kRows);
     const uint64_t units = (span + kUnit - 1) / kUnit;
     // A warp alone or four a job (bf16, 1024 sequences, 16 heads of 64 channels, one new token; us with the events
     // around them): 16-bit pools, 192 tokens 109 and 140, 400 tokens 201 and 195; codes 138 and 132, 260 and 186.
@@ -692,11 +799,23 @@ template <typename T, int D, bool kCodes, int kRows> cudaError_t launch(CacheAtt
         const uint32_t heads = (a.c.kv_heads + parts - 1) / parts;
         parts = (a.c.kv_heads + heads - 1) / heads;
         a.kv_div = FastDiv(parts);
-        auto* kernel = cache_attn_kernel<T, D, kCodes, kRows, false>;
+        auto* kernel = cache_attn_kernel<T, D, kCodes, kRows, false, kKeys>;
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
         if (e != cudaSuccess) return e;
         const uint64_t warps = lots * parts;
-        kernel<<<static_cast<uint32_t>((warps + kWarps - 1) / kWarps), kThreads, S::kBytes, s>>>(a, tiles, heads);
+        const uint32_t blocks = static_cast<uint32_t>((warps + kWarps - 1) / kWarps);
+        if constexpr (kKeys == kTailKeys) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(blocks);
+            cfg.blockDim = dim3(kThreads);
+            cfg.dynamicSmemBytes = S::kBytes;
+            cfg.stream = s;
+            cudaLaunchAttribute early = beside_the_prefix();
+            cfg.attrs = &early;
+            cfg.numAttrs = 1;
+            return cudaLaunchKernelEx(&cfg, kernel, a, tiles, heads);
+        }
+        kernel<<<blocks, kThreads, S::kBytes, s>>>(a, tiles, heads);
         return cudaGetLastError();
     }
     // as many blocks a job as fit the GPU at once (above 8: 16, a cluster of a whole GPC), at least four units a warp
@@ -704,7 +823,7 @@ template <typename T, int D, bool kCodes, int kRows> cudaError_t launch(CacheAtt
     a.kv_div = FastDiv(a.c.kv_heads);
     const uint64_t fit = min(static_cast<uint64_t>(148 * S::kBlocks) / max(jobs, uint64_t{1}), units / (kWarps * 4));
     const uint32_t split = fit >= 16 ? 16 : fit > 8 ? 8 : fit > 1 ? static_cast<uint32_t>(fit) : 1;
-    auto* kernel = cache_attn_kernel<T, D, kCodes, kRows, true>;
+    auto* kernel = cache_attn_kernel<T, D, kCodes, kRows, true, kKeys>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
@@ -713,33 +832,51 @@ template <typename T, int D, bool kCodes, int kRows> cudaError_t launch(CacheAtt
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = S::kBytes;
     cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = split;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = split > 1 ? 1 : 0;
+    cudaLaunchAttribute attr[2] = {};
+    cfg.attrs = attr;
+    if (split > 1) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = split;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.numAttrs = 1;
+    }
+    if (kKeys == kTailKeys) attr[cfg.numAttrs++] = beside_the_prefix();
     return cudaLaunchKernelEx(&cfg, kernel, a, tiles, split);
 }
 
-template <typename T, int D, bool kCodes> cudaError_t by_rows(const CacheAttnArgs& a, cudaStream_t s) {
-    return a.c.max_new * a.group <= 8 ? launch<T, D, kCodes, 8>(a, s) : launch<T, D, kCodes, 16>(a, s);
+template <int kKeys, typename T, int D, bool kCodes> cudaError_t by_rows(const CacheAttnArgs& a, cudaStream_t s) {
+    return a.c.max_new * a.group <= 8 ? launch<T, D, kCodes, 8, kKeys>(a, s) : launch<T, D, kCodes, 16, kKeys>(a, s);
 }
 
-template <typename T, bool kCodes> cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t s) {
+template <int kKeys, typename T, bool kCodes> cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t s) {
     switch (a.c.head_dim) {
-        case 32: return by_rows<T, 32, kCodes>(a, s);
-        case 64: return by_rows<T, 64, kCodes>(a, s);
-        default: return by_rows<T, 128, kCodes>(a, s);
+        case 32: return by_rows<kKeys, T, 32, kCodes>(a, s);
+        case 64: return by_rows<kKeys, T, 64, kCodes>(a, s);
+        default: return by_rows<kKeys, T, 128, kCodes>(a, s);
     }
+}
+
+template <int kKeys> cudaError_t by_type(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s) {
+    if (storage == LWM_CACHE_E4M3)
+        return dtype == LWM_DTYPE_BF16 ? by_dim<kKeys, bf16, true>(a, s) : by_dim<kKeys, __half, true>(a, s);
+    return dtype == LWM_DTYPE_BF16 ? by_dim<kKeys, bf16, false>(a, s) : by_dim<kKeys, __half, false>(a, s);
 }
 
 }  // namespace
 
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s) {
-    if (storage == LWM_CACHE_E4M3)
-        return dtype == LWM_DTYPE_BF16 ? by_dim<bf16, true>(a, s) : by_dim<__half, true>(a, s);
-    return dtype == LWM_DTYPE_BF16 ? by_dim<bf16, false>(a, s) : by_dim<__half, false>(a, s);
+    return by_type<kAllKeys>(a, dtype, storage, s);
+}
+
+cudaError_t launch_cache_attention_tail(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s) {
+    return by_type<kTailKeys>(a, dtype, storage, s);
+}
+
+// What the tails cost here, by the measured rates of this kernel (us); where nothing is said of them, as 128 tokens.
+double shared_tail_cost(const CacheAttnArgs& a) {
+    const double jobs = static_cast<double>(a.c.sequences) * a.c.kv_heads * ((static_cast<double>(a.c.max_new) * a.group + 15) / 16);
+    const uint64_t span = min(visible_span(a, 16), uint64_t{a.max_tail ? a.max_tail : 128});
+    return 4.0 + jobs * (static_cast<double>((span + 15) / 16) + 4) / (a.c.head_dim == 128 ? 1580.0 : a.c.head_dim == 64 ? 3100.0 : 3700.0);
 }
 
 }  // namespace lwm

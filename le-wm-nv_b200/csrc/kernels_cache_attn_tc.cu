@@ -105,6 +105,7 @@ struct Control {
     uint32_t tmem;
     int dead;        // a wait gave up
     int poisoned;    // infinities or NaN were taken out of a V tile
+    uint32_t lo_min, lo_max;  // a prefix: first keys in the window of the block's rows
     float v_ref;     // codes: the largest value scale of the visible pages
     int wide;        // codes: some visible page lies below kFar of it
     float high[3], low[3];
@@ -234,9 +235,24 @@ template <typename M> __device__ __forceinline__ constexpr uint32_t idesc(uint32
 
 // The keys a block walks: tiles [0, sink_tiles) and from win_tile on.
 struct Walk {
-    uint32_t lo_min, lo_max, hi_min, hi_max, sinks_end, sink_tiles, win_tile, tiles;
+    uint32_t lo_min, lo_max, hi_min, hi_max, sinks_end, sink_tiles, win_tile, tiles, skip = 0;
     __device__ __forceinline__ uint32_t key0(uint32_t i) const {
-        return (i < sink_tiles ? i : i - sink_tiles + win_tile) * kTile;
+        return (i < sink_tiles ? i + skip : i - sink_tiles + win_tile) * kTile;
+    }
+    __device__ __forceinline__ void count(uint32_t sinks) {
+        sinks_end = min(sinks, min(lo_min, hi_max));
+        sink_tiles = (sinks_end + kTile - 1) / kTile;
+        win_tile = max(lo_min / kTile, sink_tiles);
+        tiles = sink_tiles + (hi_max > win_tile * kTile ? (hi_max - win_tile * kTile + kTile - 1) / kTile : 0);
+    }
+    // only the share-th of so many parts of the tiles
+    __device__ __forceinline__ void cut(uint32_t share, uint32_t shares) {
+        const uint32_t per = (tiles + shares - 1) / shares, first = min(share * per, tiles);
+        const uint32_t sink = min(first, sink_tiles);
+        tiles = min(per, tiles - first);
+        skip = sink;
+        win_tile += first - sink;
+        sink_tiles -= sink;
     }
     // whether every row sees all 128 keys from `key`
     __device__ __forceinline__ bool whole(uint32_t key) const {
@@ -247,10 +263,7 @@ __device__ __forceinline__ Walk walk_of(const CacheAttnArgs& a, const SeqView& v
     const VisibleRange r0 = visible(a, v, a.group_div.div(row0)), r1 = visible(a, v, a.group_div.div(last));
     Walk w;
     w.lo_min = r0.lo, w.lo_max = r1.lo, w.hi_min = r0.hi, w.hi_max = r1.hi;
-    w.sinks_end = min(a.sinks, min(w.lo_min, w.hi_max));
-    w.sink_tiles = (w.sinks_end + kTile - 1) / kTile;
-    w.win_tile = max(w.lo_min / kTile, w.sink_tiles);
-    w.tiles = w.sink_tiles + (w.hi_max > w.win_tile * kTile ? (w.hi_max - w.win_tile * kTile + kTile - 1) / kTile : 0);
+    w.count(a.sinks);
     return w;
 }
 
@@ -341,7 +354,7 @@ __device__ __forceinline__ void far_sum(uint32_t t_scores, const TileInfo& info,
     }
 }
 
-template <typename T, int D, bool kCodes>
+template <typename T, int D, bool kCodes, int kKeys>
 __global__ void __launch_bounds__(kThreads, 1)
     cache_attn_tc_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map, uint32_t block_rows) {
@@ -353,17 +366,49 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
     Control* ctl = reinterpret_cast<Control*>(smem + S::kControl);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (the tails' kernel may start when every block has)
+    if constexpr (kKeys == kPrefixKeys) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // The last rows of the sequences first, where causal rows see the most keys, and blocks counted from the last row,
     // so that the one that is not full is the shortest and starts last.
-    const uint32_t pairs = a.c.sequences * a.c.kv_heads, turn = blockIdx.x / pairs, hs = blockIdx.x - turn * pairs;
-    const uint32_t h = hs % a.c.kv_heads, s = hs / a.c.kv_heads;
-    const SeqView v = sequence(a.c, s, false, threadIdx.x == 0 && h == 0 && turn == 0);
+    // A prefix: a group's rows as one sequence, over a part of the keys, which its first sequence's table names.
+    constexpr bool kPrefix = kKeys == kPrefixKeys;
+    const uint32_t lots = kPrefix ? a.group_count * a.splits : a.c.sequences;
+    const uint32_t pairs = lots * a.c.kv_heads, turn = blockIdx.x / pairs, hs = blockIdx.x - turn * pairs;
+    const uint32_t h = hs % a.c.kv_heads, lot = hs / a.c.kv_heads, share = kPrefix ? lot % a.splits : 0;
+    SeqView v;
+    GroupView group;
+    uint32_t s = lot;
+    if constexpr (kPrefix) {
+        group = group_view(a, lot / a.splits, threadIdx.x == 0 && h == 0 && turn == 0 && share == 0);
+        s = group.first;
+        v.start = group.start, v.n = group.ok ? group.n : 0, v.length = group.shared, v.ok = group.ok;
+    } else {
+        v = sequence(a.c, s, false, threadIdx.x == 0 && h == 0 && turn == 0);
+    }
     const uint32_t later = turn * block_rows;
     if (later >= v.n * a.group) return;
     const uint32_t rows = v.n * a.group - later;  // the end of this block's
     const uint32_t row0 = max(rows, block_rows) - block_rows, last = rows - 1;
     const bool two = last >= row0 + kTile;  // the second tile has rows
-    const Walk w = walk_of(a, v, row0, last);
+    Walk w;
+    if constexpr (kPrefix) {
+        // rows of many sequences: the ends of what they see, over the block
+        if (threadIdx.x == 0) ctl->lo_min = a.window ? v.length : 0u, ctl->lo_max = 0u;
+        if (a.window) {
+            __syncthreads();
+            if (threadIdx.x < 256 && row0 + threadIdx.x < rows) {
+                const uint32_t lo = visible_prefix(a, group, a.group_div.div(row0 + threadIdx.x)).lo;
+                atomicMin(&ctl->lo_min, lo);
+                atomicMax(&ctl->lo_max, lo);
+            }
+        }
+        __syncthreads();
+        w.lo_min = ctl->lo_min, w.lo_max = ctl->lo_max, w.hi_min = w.hi_max = v.length;
+        w.count(a.sinks);
+        w.cut(share, a.splits);
+    } else {
+        w = walk_of(a, v, row0, last);
+    }
 
     if (threadIdx.x == 0) {
         const int softmax = two ? 256 : 128;
@@ -403,7 +448,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t tok = live ? a.group_div.div(R) : 0;
             VisibleRange rr = {0, 0, 0};
             float mul = a.scale_log2;
-            if (live) rr = visible(a, v, tok);
+            if (live) {
+                if constexpr (kPrefix) rr = visible_prefix(a, group, tok);
+                else rr = visible(a, v, tok);
+            }
             // Q: the warp's 32 rows into the swizzled tile, whole rows at a time
             {
                 constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;  // lanes a row, rows a load
@@ -451,10 +499,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::fence_async_smem();
                 tc::mbar_arrive(&ctl->q_full);
             }
-            const Walk mine = walk_of(a, v, row0 + tile * kTile, min(row0 + (tile + 1) * kTile - 1, last));
+            Walk mine = w;
+            if constexpr (!kPrefix) mine = walk_of(a, v, row0 + tile * kTile, min(row0 + (tile + 1) * kTile - 1, last));
             const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
             const uint32_t t_s = t_lane + tile * kTile, t_o = t_lane + kOCol + tile * D;
             float m = -INFINITY, l = 0.0f;
+            float ml_end = -INFINITY;  // wide: what l is in units of, at the end
             bool fine = true;
             // a warp without rows leaves its part of P as it is: a row of P enters its own row of O alone
             const bool idle = row0 + tile * kTile + (warp & 3) * 32 >= rows;
@@ -535,6 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) tc::mbar_arrive(&ctl->p_full[tile][half]);
                 }
             }
+            if (kPrefix) ml_end = kWide ? ml : m;
             // (twice the root of 2^(m - ml), as the whole may be below the smallest float)
             return kWide && m != ml ? exp2_fast(0.5f * (m - ml)) : 1.0f;
             };
@@ -593,6 +644,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
+                if constexpr (kPrefix) {
+                    // a part: in 32 bits, joined with the others where the tails are read
+                    if (live && fine) {
+                        const size_t row = (static_cast<size_t>(share) * a.c.tokens + v.start + tok) * a.heads + h * a.group + (R - tok * a.group);
+                        float4* to = reinterpret_cast<float4*>(a.part_out + row * a.c.head_dim + c);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        if (c == 0) a.part_log[row] = l == 0.0f ? -INFINITY : ml_end - kLift + log2f(l);
+                    }
+                } else {
                 float f[8];
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
@@ -601,9 +662,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int ch = c / 8 + b;
                     *reinterpret_cast<uint4*>(stage + (ch >> 3) * kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = pack<T>(f).a;
                 }
+                }
             }
             __syncwarp();
-            if (fine) {
+            if (!kPrefix && fine) {
                 constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
                 const int c = lane % kLanes;
 #pragma unroll
@@ -995,11 +1057,13 @@ Costs costs_of(const CacheAttnArgs& a) {
     return {std::min(one, both), there, one < both ? kTile : 2u * kTile};
 }
 
-template <typename T, int D, bool kCodes> cudaError_t launch(const CacheAttnArgs& a, cudaStream_t s) {
+template <typename T, int D, bool kCodes, int kKeys>
+cudaError_t launch(const CacheAttnArgs& a, uint32_t block_rows, cudaStream_t s) {
     using S = Shape<D, kCodes>;
     static_assert(S::kBytes <= 227 * 1024, "shared memory");
-    const uint32_t block_rows = costs_of(a).rows, row_blocks = (a.c.max_new * a.group + block_rows - 1) / block_rows;
-    auto* kernel = cache_attn_tc_kernel<T, D, kCodes>;
+    const uint32_t most = kKeys == kPrefixKeys ? a.max_tokens : a.c.max_new, row_blocks = (most * a.group + block_rows - 1) / block_rows;
+    const uint32_t lots = kKeys == kPrefixKeys ? a.group_count * a.splits : a.c.sequences;
+    auto* kernel = cache_attn_tc_kernel<T, D, kCodes, kKeys>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
     CUtensorMap k_map{}, v_map{};
     if constexpr (!kCodes) {
@@ -1007,12 +1071,17 @@ template <typename T, int D, bool kCodes> cudaError_t launch(const CacheAttnArgs
         if (e == cudaSuccess) e = page_map(a.c, a.c.v, std::is_same_v<T, bf16>, &v_map);
     }
     if (e != cudaSuccess) return e;
-    kernel<<<row_blocks * a.c.sequences * a.c.kv_heads, kThreads, S::kBytes, s>>>(a, k_map, v_map, block_rows);
+    kernel<<<row_blocks * lots * a.c.kv_heads, kThreads, S::kBytes, s>>>(a, k_map, v_map, block_rows);
     return cudaGetLastError();
 }
 
-template <typename T, bool kCodes> cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t s) {
-    return a.c.head_dim == 128 ? launch<T, 128, kCodes>(a, s) : launch<T, 64, kCodes>(a, s);
+template <int kKeys, typename T, bool kCodes> cudaError_t by_dim(const CacheAttnArgs& a, uint32_t rows, cudaStream_t s) {
+    return a.c.head_dim == 128 ? launch<T, 128, kCodes, kKeys>(a, rows, s) : launch<T, 64, kCodes, kKeys>(a, rows, s);
+}
+template <int kKeys> cudaError_t by_type(const CacheAttnArgs& a, uint32_t rows, int dtype, int storage, cudaStream_t s) {
+    if (storage == LWM_CACHE_E4M3)
+        return dtype == LWM_DTYPE_BF16 ? by_dim<kKeys, bf16, true>(a, rows, s) : by_dim<kKeys, __half, true>(a, rows, s);
+    return dtype == LWM_DTYPE_BF16 ? by_dim<kKeys, bf16, false>(a, rows, s) : by_dim<kKeys, __half, false>(a, rows, s);
 }
 
 }  // namespace
@@ -1022,10 +1091,38 @@ bool cache_attention_many_rows(const CacheAttnArgs& a) {
     return c.here < c.there;
 }
 
+double cache_attention_cost(const CacheAttnArgs& a) {
+    const Costs c = costs_of(a);
+    return std::min(c.here, c.there);
+}
+
 cudaError_t launch_cache_attention_tc(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s) {
-    if (storage == LWM_CACHE_E4M3)
-        return dtype == LWM_DTYPE_BF16 ? by_dim<bf16, true>(a, s) : by_dim<__half, true>(a, s);
-    return dtype == LWM_DTYPE_BF16 ? by_dim<bf16, false>(a, s) : by_dim<__half, false>(a, s);
+    return by_type<kAllKeys>(a, costs_of(a).rows, dtype, storage, s);
+}
+
+// The prefix's blocks by the same costs: row tiles a block, and parts of the
+// keys, each of which writes 32-bit results that the tails' kernel reads.
+SharedPlan shared_plan(const CacheAttnArgs& a, uint32_t most_splits) {
+    const bool wide = a.c.head_dim == 128;
+    const uint64_t rows = static_cast<uint64_t>(a.max_tokens) * a.group;
+    uint64_t span = a.c.max_length ? a.c.max_length : static_cast<uint64_t>(a.c.table_stride) << a.c.page_shift;
+    if (a.window)  // rows of several lengths: as if they were as far apart as their tails allow
+        span = std::min(span, static_cast<uint64_t>(a.window) * a.frame + a.sinks + (a.max_tail ? a.max_tail : 128));
+    const uint64_t tiles = std::max<uint64_t>(1, (span + kTile - 1) / kTile);
+    const double part = static_cast<double>(a.c.tokens) * a.heads * a.c.head_dim * 8 / 4e6;  // written and read, us
+    SharedPlan best;
+    for (uint32_t block = kTile; block <= 2 * kTile; block += kTile)
+        for (uint32_t splits = 1; splits <= std::min<uint64_t>(std::min<uint64_t>(tiles, most_splits), 64); ++splits) {
+            const double blocks = static_cast<double>(a.group_count) * a.c.kv_heads * ((rows + block - 1) / block) * splits;
+            const double factor = block > kTile && rows > kTile ? 1.5 : 1.0, steps = static_cast<double>((tiles + splits - 1) / splits);
+            const double cost = std::ceil(blocks / 148) * ((wide ? 9.0 : 6.5) + (wide ? 1.6 : 1.25) * factor * steps) + part * splits;
+            if (best.cost == 0.0 || cost < best.cost) best = {block, splits, cost};
+        }
+    return best;
+}
+
+cudaError_t launch_cache_attention_prefix(const CacheAttnArgs& a, uint32_t block_rows, int dtype, int storage, cudaStream_t s) {
+    return by_type<kPrefixKeys>(a, block_rows, dtype, storage, s);
 }
 
 }  // namespace lwm

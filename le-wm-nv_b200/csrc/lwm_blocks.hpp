@@ -110,7 +110,17 @@ struct CacheAttnArgs {
     uint32_t window, sinks, frame;
     FastDiv group_div, frame_div;
     FastDiv tile_div, kv_div;  // set by the launch
+    // Groups of sequences that share a prefix: group g is sequences [groups[g], groups[g + 1]), shared[g] tokens long.
+    const int32_t* groups;
+    const int32_t* shared;
+    uint32_t group_count, max_tokens, max_tail;  // packed rows of a group, tokens behind its prefix
+    float* part_out;  // [splits, tokens, heads, head_dim]: what the prefix gives, each split of its keys by itself
+    float* part_log;  // [splits, tokens, heads]: log2 of its sum of weights
+    uint32_t splits;
 };
+// Which keys a launch of the attention's kernels is for: all, a group's
+// prefix (as parts), or what follows it (joined with those parts).
+constexpr int kAllKeys = 0, kPrefixKeys = 1, kTailKeys = 2;
 // Keys that a tile of query rows can see, by the sizes that the host knows.
 inline uint64_t visible_span(const CacheAttnArgs& a, uint32_t tile_rows) {
     const uint64_t reach = a.c.max_length ? a.c.max_length : static_cast<uint64_t>(a.c.table_stride) << a.c.page_shift;
@@ -161,6 +171,17 @@ struct TokenArgs {
 };
 constexpr uint32_t kSampleVocab = 1u << 18;  // the largest
 cudaError_t launch_sample_tokens(const TokenArgs& a, int dtype, cudaStream_t s);
+
+// The prefix of every group against its sequences' rows, then their tails.
+struct SharedPlan {
+    uint32_t rows = 256, splits = 1;  // of a block; parts of the keys
+    double cost = 0.0;                // us
+};
+SharedPlan shared_plan(const CacheAttnArgs& a, uint32_t most_splits);
+double shared_tail_cost(const CacheAttnArgs& a);
+double cache_attention_cost(const CacheAttnArgs& a);
+cudaError_t launch_cache_attention_prefix(const CacheAttnArgs& a, uint32_t block_rows, int dtype, int storage, cudaStream_t s);
+cudaError_t launch_cache_attention_tail(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
 
 struct GatedNormArgs {
     lwm_gated_norm_args a;

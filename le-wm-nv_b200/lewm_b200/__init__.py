@@ -324,6 +324,11 @@ class _CacheAttentionArgs(C.Structure):
                 ("sinks", U32), ("frame_tokens", U32)]
 
 
+class _SharedPrefix(C.Structure):
+    _fields_ = [("groups", VP), ("lengths", VP), ("count", U32), ("max_tokens", U32), ("max_length", U32),
+                ("max_tail", U32)]
+
+
 class _GatedNormArgs(C.Structure):
     _fields_ = [("x", VP), ("y", VP), ("x_out", VP), ("h", VP), ("x_stride", U64), ("y_stride", U64),
                 ("x_out_stride", U64), ("h_stride", U64), ("rows", U32), ("width", U32), ("residual_dtype", I32),
@@ -482,6 +487,10 @@ _sig("lwm_lewm_plan_nv12_device", C.c_int, VP, VP, VP, VP, U32, U32, U32, U32, I
      C.POINTER(_PlanDeviceResult))
 _sig("lwm_rotary_init", C.c_int, U32, C.POINTER(U32), C.POINTER(C.c_double), I32, C.POINTER(Rotary))
 _sig("lwm_rotary_device", C.c_int, VP, C.POINTER(Rotary), C.POINTER(_RotaryArgs))
+_sig("lwm_cache_attention_shared_workspace", C.c_int, C.POINTER(_PagedCache), C.POINTER(_CacheBatch),
+     C.POINTER(_SharedPrefix), C.POINTER(_CacheAttentionArgs), C.POINTER(U64))
+_sig("lwm_cache_attention_shared_device", C.c_int, VP, C.POINTER(_PagedCache), C.POINTER(_CacheBatch),
+     C.POINTER(_SharedPrefix), C.POINTER(_CacheAttentionArgs), VP, U64)
 _sig("lwm_linear_attention_device", C.c_int, VP, C.POINTER(_StateBatch), C.POINTER(_LinearAttentionArgs))
 _sig("lwm_sample_tokens_device", C.c_int, VP, C.POINTER(_SampleTokensArgs))
 _sig("lwm_cache_append_device", C.c_int, VP, C.POINTER(_PagedCache), C.POINTER(_CacheBatch), C.POINTER(Rotary),
@@ -1456,6 +1465,80 @@ def cache_attention_device(ctx: Context, cache: PagedCache, batch: CacheBatch, q
     a = _CacheAttentionArgs(qp, op, qt, qh, ot, oh, heads, cache.head_dim ** -0.5 if scale is None else scale,
                             int(causal), window, sinks, frame_tokens)
     _check(lib.lwm_cache_attention_device(ctx.handle, cache._ref, batch._ref, C.byref(a)))
+
+
+class SharedPrefix:
+    """lwm_shared_prefix: groups [count + 1] (sequences [groups[g], groups[g +
+    1]) share their first tokens) and lengths [count] of those prefixes, int32
+    device tensors; bounds of a group's packed rows (None: the batch's), of a
+    prefix and of what follows it (0: not known)."""
+
+    def __init__(self, groups, lengths, max_tokens: Optional[int] = None, max_length: int = 0, max_tail: int = 0):
+        if groups.dim() != 1 or groups.shape[0] < 1:
+            raise LwmError(1, "groups must be [count + 1]")
+        n = groups.shape[0] - 1
+        _sizes("groups", groups.shape)
+        _ints("groups", groups, (n + 1,))
+        _ints("lengths", lengths, (n,))
+        for name, x in (("max_tokens", max_tokens or 0), ("max_length", max_length), ("max_tail", max_tail)):
+            _u32(name, x)
+        if lengths.device != groups.device:
+            raise LwmError(1, "group tensors are on different devices")
+        self._keep = (groups, lengths)
+        self.device, self.device_index = groups.device, groups.get_device()
+        self.max_tokens = max_tokens
+        self._c = _SharedPrefix(groups.data_ptr(), lengths.data_ptr(), n, max_tokens or 0, max_length, max_tail)
+        self._ref = C.byref(self._c)
+
+    def _of(self, batch: CacheBatch):
+        if self.max_tokens is not None:
+            return self._ref
+        c = _SharedPrefix.from_buffer_copy(self._c)
+        c.max_tokens = batch.tokens
+        return C.byref(c)
+
+
+def shared_attention_workspace(cache: PagedCache, batch: CacheBatch, prefix: SharedPrefix, heads: int, causal: bool = True,
+                               window: int = 0, sinks: int = 0, frame_tokens: int = 1) -> int:
+    """Bytes of workspace that cache_attention_shared_device needs for such a
+    call (0: none)."""
+    for name, x in (("heads", heads), ("window", window), ("sinks", sinks), ("frame_tokens", frame_tokens)):
+        _u32(name, x)
+    a = _CacheAttentionArgs(None, None, 0, 0, 0, 0, heads, 1.0, int(causal), window, sinks, frame_tokens)
+    n = U64()
+    _check(lib.lwm_cache_attention_shared_workspace(cache._ref, batch._ref, prefix._of(batch), C.byref(a), C.byref(n)))
+    return n.value
+
+
+def cache_attention_shared_device(ctx: Context, cache: PagedCache, batch: CacheBatch, prefix: SharedPrefix, q, out,
+                                  workspace=None, scale: Optional[float] = None, causal: bool = True, window: int = 0,
+                                  sinks: int = 0, frame_tokens: int = 1) -> None:
+    """cache_attention_device for sequences that share prefixes, each of which
+    is read once for its group.  workspace: a contiguous tensor of at least
+    shared_attention_workspace bytes for the same arguments, used by no other
+    call in flight.  `out` is ready on the context's stream."""
+    _same_device(ctx, cache, batch)
+    if prefix.device_index != ctx.device:
+        raise LwmError(1, f"groups must be on cuda:{ctx.device}, got {prefix.device}")
+    if q.dim() != 3:
+        raise LwmError(1, f"q must be [tokens, heads, head_dim], got {list(q.shape)}")
+    if not 0 <= (window | sinks | frame_tokens) < 1 << 32:  # any of them
+        for name, x in (("window", window), ("sinks", sinks), ("frame_tokens", frame_tokens)):
+            _u32(name, x)
+    heads = q.shape[1]
+    if heads >> 32:
+        _sizes("q", q.shape)
+    shape = (batch.tokens, heads, cache.head_dim)
+    qp, qt, qh = _heads(ctx, "q", q, shape, cache.dtype)
+    op, ot, oh = _heads(ctx, "out", out, shape, cache.dtype)
+    at, size = None, 0
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise LwmError(1, "workspace must be contiguous")
+        at, size = _on(ctx, "workspace", workspace), workspace.numel() * workspace.element_size()
+    a = _CacheAttentionArgs(qp, op, qt, qh, ot, oh, heads, cache.head_dim ** -0.5 if scale is None else scale,
+                            int(causal), window, sinks, frame_tokens)
+    _check(lib.lwm_cache_attention_shared_device(ctx.handle, cache._ref, batch._ref, prefix._of(batch), C.byref(a), at, size))
 
 
 class StateBatch:

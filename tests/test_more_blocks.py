@@ -97,7 +97,77 @@ def test_sampling_refusals(kw, message):
     assert _message() == message
 
 
+def _cache(**kw):
+    d = dict(k=P, v=P, k_scale=P, v_scale=P, pages=4, kv_heads=2, page_tokens=16, head_dim=64, dtype=1, storage=1)
+    d.update(kw)
+    return L._PagedCache(**d)
+
+
+def _batch(**kw):
+    d = dict(table=P, lengths=P, starts=P, sequences=64, table_stride=4000, tokens=64, max_new=1, max_length=0)
+    d.update(kw)
+    return L._CacheBatch(**d)
+
+
+def _prefix(**kw):
+    d = dict(groups=P, lengths=P, count=1, max_tokens=64, max_length=50000, max_tail=30)
+    d.update(kw)
+    return L._SharedPrefix(**d)
+
+
+def _attention(**kw):
+    d = dict(q=P, out=P, q_token_stride=256, q_head_stride=64, out_token_stride=256, out_head_stride=64, heads=4,
+             scale=0.125, causal=1, window=0, sinks=0, frame_tokens=1)
+    d.update(kw)
+    return L._CacheAttentionArgs(**d)
+
+
+def _bytes(cache, batch, prefix, args):
+    n = C.c_uint64(99)
+    status = L.lib.lwm_cache_attention_shared_workspace(C.byref(cache), C.byref(batch), C.byref(prefix), C.byref(args), C.byref(n))
+    return status, n.value
+
+
+def test_shared_attention_says_what_workspace_it_needs():
+    status, n = _bytes(_cache(), _batch(), _prefix(), _attention(q=None, out=None))
+    assert status == 0 and n > 0 and n % (64 * 4 * 65 * 4) == 0  # [splits, tokens, heads, head_dim + 1] f32
+    for batch, prefix in ((dict(sequences=0, tokens=0, max_new=0), dict(count=0, max_tokens=0)), ({}, dict(count=0)),
+                          (dict(sequences=2, tokens=2, table_stride=4), dict(max_tokens=2, max_length=40))):
+        assert _bytes(_cache(), _batch(**batch), _prefix(**prefix), _attention()) == (0, 0)
+
+
+@pytest.mark.parametrize("batch,prefix,args,work,message", [
+    ({}, dict(count=65), {}, {}, "groups 65 are more than the sequences"),
+    ({}, dict(groups=None), {}, {}, "group arrays are null"),
+    ({}, dict(lengths=P + 2), {}, {}, "group arrays are not 4-byte aligned"),
+    ({}, dict(max_tokens=65), {}, {}, "max_tokens 65 is above the batch's tokens 64"),
+    (dict(max_new=65), {}, {}, {}, "batch sizes out of range (max_new 65, tokens 64)"),
+    ({}, {}, dict(heads=3), {}, "query heads 3 must be a positive multiple of kv_heads 2"),
+    ({}, {}, dict(q=None), {}, "q is null"),
+    ({}, {}, dict(out_head_stride=63), {}, "out strides must be multiples of 8 elements"),
+    ({}, {}, {}, dict(workspace=None), "workspace is null"),
+    ({}, {}, {}, dict(workspace=P + 8), "workspace is not 16-byte aligned"),
+    ({}, {}, {}, {}, "null context"),
+])
+def test_shared_attention_refusals(batch, prefix, args, work, message):
+    c, b, p, a = _cache(), _batch(**batch), _prefix(**prefix), _attention(**args)
+    at, size = work.get("workspace", P), work.get("size", 1 << 40)
+    assert L.lib.lwm_cache_attention_shared_device(None, C.byref(c), C.byref(b), C.byref(p), C.byref(a), at, size) != 0
+    assert _message() == message
+
+
+def test_shared_attention_refuses_a_small_workspace():
+    c, b, p, a = _cache(), _batch(), _prefix(), _attention()
+    _, n = _bytes(c, b, p, a)
+    assert L.lib.lwm_cache_attention_shared_device(None, C.byref(c), C.byref(b), C.byref(p), C.byref(a), P, n - 1) != 0
+    assert _message() == f"workspace has {n - 1} bytes, the call needs {n}"
+    assert L.lib.lwm_cache_attention_shared_device(None, C.byref(c), C.byref(b), C.byref(p), C.byref(a), P, n) != 0
+    assert _message() == "null context"
+
+
 def test_null_arguments():
+    assert L.lib.lwm_cache_attention_shared_device(None, C.byref(_cache()), C.byref(_batch()), None, C.byref(_attention()), P, 0) != 0
+    assert _message() == "null argument"
     assert L.lib.lwm_linear_attention_device(None, None, None) != 0 and _message() == "null argument"
     assert L.lib.lwm_sample_tokens_device(None, None) != 0 and _message() == "null argument"
 
