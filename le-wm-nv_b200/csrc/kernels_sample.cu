@@ -9,12 +9,19 @@
 // Which token a random number falls on depends on sums over the whole row, so
 // those are exact: a weight exp((x - max) / temperature) is computed in 64 bits
 // (relative error below 1e-13) and rounded to a multiple of 2^-43, and sums are
-// integers, which have no order.  Thresholds are found by bisection on the
-// logit with 32-bit sums, decided by exact ones where those are too near; the
-// last few hundred candidates of a threshold are sorted.
+// integers, which have no order.  A threshold (the last token that top_k or
+// top_p keeps) is found by a histogram over the logits, in 256 steps of a
+// power of 2^(1/5.7) of the weight: counts, or masses in 16 bits of each bin's
+// own scale.  The bin that a rough sum points at is proved, or changed, by
+// exact sums; its tokens are sorted and walked, or, where they are more than
+// the list takes, binned again by their keys, down to one logit if need be.
+// With top_k up to the list's length all that is kept is in the list, and the
+// rest of the call works on that alone.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cfloat>
+#include <type_traits>
 
 #include "lwm_blocks.cuh"
 
@@ -26,7 +33,9 @@ namespace cg = cooperative_groups;
 
 constexpr int kList = 1024;     // candidates that are sorted
 constexpr int kMaxSplit = 16;   // blocks of a row
-constexpr float kNear = 1e-5f;  // more than a 32-bit sum of weights can be off
+constexpr int kBins = 256;
+constexpr uint32_t kMaxSlice = 32768;  // logits of a block
+constexpr float kSpan = 45.0f;  // powers of two that the bins span: weights end there
 
 // Order of logits: larger ones have larger keys; 0 for what is never drawn
 // (minus infinity, NaN).
@@ -54,9 +63,8 @@ __device__ __forceinline__ double widen(float x) {
 }
 // round(2^43 exp((x - top) / temperature)).  2^(n / 64) comes from a table,
 // the rest, below 2^-7, from five terms of the series.
-__device__ __forceinline__ uint64_t weight(const Weights& w, const double* table, uint32_t key) {
-    if (key == 0) return 0;
-    const float x = value_of(key);
+__device__ __forceinline__ uint64_t weight(const Weights& w, const double* table, float x) {
+    if (x == -INFINITY) return 0;
     if (w.infinite) return x == INFINITY ? 1ull << 43 : 0;
     const double y = (widen(x) - w.top) * w.rate;  // 64ths of a power of two
     if (y < -2900.0) return 0;                     // below 2^-45
@@ -92,42 +100,54 @@ template <int kThreads> struct Shared {
     double table[64];
     uint64_t sums[2][kMaxSplit * kWarps];
     uint32_t counts[2][kMaxSplit * kWarps];
+};
+struct Filter {  // of a kernel with thresholds
+    uint32_t bins[kBins];  // of the row, in every block
+    uint32_t mine[kBins];  // of this block
     uint64_t list[kList];
     uint64_t mass[kList];
     uint64_t found;
-    uint32_t listed;
+    uint32_t listed, picked;
 };
 
-template <typename T, int kThreads, int kVals>
-__global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : 1)
-    sample_kernel(const __grid_constant__ TokenArgs a, uint32_t split, int vectors) {
-    constexpr int kWarps = kThreads / 32, kRounds = kVals / 8;
+// kFilter: top_k or top_p may be on.
+template <typename T, int kThreads, bool kFilter>
+__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ TokenArgs a, uint32_t split, uint32_t slice, int vectors) {
+    constexpr int kWarps = kThreads / 32;
+    extern __shared__ __align__(16) float x[];  // the slice's logits; minus infinity: never drawn
     using S = Shared<kThreads>;
     __shared__ S sh;
+    __shared__ std::conditional_t<kFilter, Filter, char> filter_s;
     const uint32_t rank = blockIdx.x % split, row = blockIdx.x / split;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Params par = params_of(a, row);
-    // elements 8 threadIdx.x + e of run j
-    const uint32_t base = rank * kThreads * kVals + threadIdx.x * 8;
-    auto index_of = [&](int j, int e) { return base + j * kThreads * 8 + e; };
-    uint32_t key[kVals];
+    const uint32_t base = rank * slice, count = base < a.vocab ? min(slice, a.vocab - base) : 0;
+    // A thread's logits: a run of odd length, so that the threads of a warp read different banks, in order of index.
+    const uint32_t each = ((count + kThreads - 1) / kThreads) | 1u;
+    const uint32_t run0 = min(threadIdx.x * each, count), run1 = min(run0 + each, count);
+    float top = -INFINITY;
     {
-        const T* src = static_cast<const T*>(a.logits) + row * a.stride;
-#pragma unroll
-        for (int j = 0; j < kRounds; ++j) {
-            const uint32_t i = index_of(j, 0);
+        const T* src = static_cast<const T*>(a.logits) + row * a.stride + base;
+        auto clean = [&](float v) {
+            v = v == v ? v + 0.0f : -INFINITY;  // (minus zero is zero)
+            top = fmaxf(top, v);
+            return v;
+        };
+        const uint32_t whole = vectors ? count / 8 : 0;
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < whole; i += kThreads) {
             float f[8];
-            if (vectors && i + 8 <= a.vocab) {
-                unpack(load8(src + i), f);
-            } else {
+            unpack(load8(src + 8 * i), f);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = i + e < a.vocab ? static_cast<float>(src[i + e]) : -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) key[8 * j + e] = key_of(f[e]);
+            for (int e = 0; e < 8; ++e) f[e] = clean(f[e]);
+            store8(x + 8 * i, pack<float>(f));
         }
+#pragma unroll 4
+        for (uint32_t i = 8 * whole + threadIdx.x; i < count; i += kThreads) x[i] = clean(static_cast<float>(src[i]));
     }
     for (int i = threadIdx.x; i < 64; i += kThreads) sh.table[i] = exp2(i / 64.0);
+    if constexpr (kFilter)
+        for (int i = threadIdx.x; i < kBins; i += kThreads) filter_s.bins[i] = filter_s.mine[i] = 0;
 
     if (split > 1) cg::this_cluster().sync();  // every block runs before another writes to it
     int turn = 0;
@@ -135,374 +155,435 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 2 : 1)
         if (split > 1) cg::this_cluster().sync();
         else __syncthreads();
     };
-    // Sums over the row, the same in every thread: one barrier each, the buffers alternate.
-    auto share = [&](uint64_t x, uint32_t c) {
+    auto block_of = [&](auto* p, uint32_t b) { return split > 1 ? cg::this_cluster().map_shared_rank(p, b) : p; };
+    // Sums of a warp's values to every block: one barrier, the buffers alternate.
+    auto share = [&](uint64_t v, uint32_t c) {
         const uint32_t slot = rank * kWarps + warp;
-        if (split == 1) {
-            if (lane == 0) sh.sums[turn][slot] = x, sh.counts[turn][slot] = c;
-        } else if (lane < split) {
-            S* to = cg::this_cluster().map_shared_rank(&sh, lane);
-            to->sums[turn][slot] = x, to->counts[turn][slot] = c;
+        if (lane < split) {
+            S* to = block_of(&sh, lane);
+            to->sums[turn][slot] = v, to->counts[turn][slot] = c;
         }
         meet();
     };
-    auto sum_all = [&](uint64_t x, uint32_t c, uint64_t& x_all, uint32_t& c_all) {
+    auto warp_sum = [&](uint64_t v) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        c = __reduce_add_sync(0xffffffffu, c);
-        share(x, c);
-        x = 0, c = 0;
-        for (uint32_t i = lane; i < split * kWarps; i += 32) x += sh.sums[turn][i], c += sh.counts[turn][i];
-#pragma unroll
-        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        x_all = x, c_all = __reduce_add_sync(0xffffffffu, c);
-        turn ^= 1;
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
     };
-    // the same with a 32-bit float sum
-    auto sum_rough = [&](float x, uint32_t c, float& x_all, uint32_t& c_all) {
-#pragma unroll
-        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        c = __reduce_add_sync(0xffffffffu, c);
-        share(__float_as_uint(x), c);
-        x = 0.0f, c = 0;
-        for (uint32_t i = lane; i < split * kWarps; i += 32)
-            x += __uint_as_float(static_cast<uint32_t>(sh.sums[turn][i])), c += sh.counts[turn][i];
-#pragma unroll
-        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        x_all = x, c_all = __reduce_add_sync(0xffffffffu, c);
+    auto sum_all = [&](uint64_t v, uint32_t c, uint64_t& v_all, uint32_t& c_all) {
+        share(warp_sum(v), __reduce_add_sync(0xffffffffu, c));
+        v = 0, c = 0;
+        for (uint32_t i = lane; i < split * kWarps; i += 32) v += sh.sums[turn][i], c += sh.counts[turn][i];
+        v_all = warp_sum(v), c_all = __reduce_add_sync(0xffffffffu, c);
         turn ^= 1;
     };
 
     // the largest logit
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < kVals; ++i) top = max(top, key[i]);
-    top = __reduce_max_sync(0xffffffffu, top);
-    share(0, top);
-    for (uint32_t i = lane; i < split * kWarps; i += 32) top = max(top, sh.counts[turn][i]);
-    top = __reduce_max_sync(0xffffffffu, top);
-    turn ^= 1;
-    if (top == 0) {  // nothing can be drawn
-        if (rank == 0 && threadIdx.x == 0) {
-            a.tokens[row] = -1;
-            if (a.log_probs) a.log_probs[row] = -INFINITY;
-        }
-        if (split > 1) cg::this_cluster().sync();
-        return;
-    }
     Weights w;
-    w.top32 = value_of(top);
-    w.infinite = w.top32 == INFINITY;
-    w.top = widen(w.top32);
-    w.rate = 92.332482616893657 / par.temperature;  // 64 log2(e)
-    w.rate32 = static_cast<float>(1.4426950408889634 / par.temperature);
-    auto rough = [&](uint32_t k) {
-        float r;
-        const float x = value_of(k);
-        const float y = w.infinite ? (x == INFINITY ? 0.0f : -INFINITY) : (x - w.top32) * w.rate32;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
-        return r;
+    {
+        uint32_t k = __reduce_max_sync(0xffffffffu, key_of(top));
+        share(0, k);
+        for (uint32_t i = lane; i < split * kWarps; i += 32) k = max(k, sh.counts[turn][i]);
+        k = __reduce_max_sync(0xffffffffu, k);
+        turn ^= 1;
+        if (k == 0) {  // nothing can be drawn
+            if (rank == 0 && threadIdx.x == 0) {
+                a.tokens[row] = -1;
+                if (a.log_probs) a.log_probs[row] = -INFINITY;
+            }
+            if (split > 1) cg::this_cluster().sync();
+            return;
+        }
+        w.top32 = value_of(k);
+        w.infinite = w.top32 == INFINITY;
+        w.top = widen(w.top32);
+        w.rate = 92.332482616893657 / par.temperature;  // 64 log2(e)
+        w.rate32 = static_cast<float>(1.4426950408889634 / par.temperature);
+    }
+    const uint64_t least = par.min_p > 0.0 ? static_cast<uint64_t>(ceil(par.min_p * 8796093022208.0)) : 1;  // 2^43 min_p
+    const float u = a.uniform[row];
+    // the point on the sum `all` of kept weights that the random number stands for: the first sum above it is drawn
+    auto point_of = [&](uint64_t all) {
+        const double at = (u > 0.0f ? static_cast<double>(fminf(u, 1.0f)) : 0.0) * static_cast<double>(all);
+        return min(static_cast<uint64_t>(at), all - 1);
     };
-    // Tokens in order: larger logits first, then smaller indices.  A threshold is the last token kept, as
-    // key << 32 | ~index; those not below it are kept.
-    auto place = [&](uint32_t k, uint32_t i) { return static_cast<uint64_t>(k) << 32 | (0xffffffffu - i); };
-    uint64_t border = static_cast<uint64_t>(1) << 32;  // every key but 0
+    auto answer = [&](uint32_t token, uint64_t mass, uint64_t all) {
+        a.tokens[row] = static_cast<int32_t>(token);
+        if (a.log_probs) a.log_probs[row] = static_cast<float>(log(static_cast<double>(mass) / static_cast<double>(all)));
+    };
 
-    // The threshold of a filter: kByMass, the first token with which the mass of the kept ones (those not below
-    // `border`) reaches `want`; else the want-th.
-    auto threshold = [&](auto by_mass, double want_mass, uint32_t want_count) {
-        constexpr bool kByMass = decltype(by_mass)::value;
-        uint32_t lo = max(static_cast<uint32_t>(border >> 32), 1u), hi = top + 1, above_count = 0;  // keys [lo, hi) hold it
-        if (kByMass && !w.infinite) lo = max(lo, key_of(w.top32 - 32.0f / w.rate32));  // (weights end at 2^-45)
-        uint64_t above = 0;  // mass and count of the keys from hi on
-        uint32_t inside = 0xffffffffu;
-        bool exact = true;   // `above` is
-        for (int step = 0; hi - lo > 1; ++step) {
-            uint32_t mid = lo + (hi - lo) / 2;
-            if (!(step & 1)) {  // halfway between the logits, then between the keys: one of them soon gets there
-                const float x = 0.5f * value_of(lo) + 0.5f * value_of(hi - 1);
-                const uint32_t k = key_of(x);
-                if (k > lo && k < hi) mid = k;
-            }
-            float m = 0.0f;
-            uint32_t n = 0, below = 0;
-#pragma unroll
-            for (int i = 0; i < kVals; ++i) {
-                const bool kept = place(key[i], index_of(i >> 3, i & 7)) >= border;
-                if (kept && key[i] >= mid) {
-                    ++n;
-                    if (kByMass) m += rough(key[i]);
-                } else if (kept && key[i] >= lo) {
-                    ++below;
-                }
-            }
-            float m_all;
-            uint32_t both;
-            uint32_t n_all, below_all;
-            sum_rough(m, n, m_all, n_all);
-            sum_rough(0.0f, below, m, both);
-            below_all = both;
-            bool up;  // the threshold is at or above mid
-            if constexpr (kByMass) {
-                const double rough_mass = static_cast<double>(m_all) * 8796093022208.0;  // 2^43
-                if (rough_mass > want_mass * (1.0 + kNear)) {
-                    up = true;
-                } else if (rough_mass < want_mass * (1.0 - kNear)) {
-                    up = false;
-                    exact = false;
-                } else {
-                    uint64_t x = 0, x_all;
-                    uint32_t c;
-#pragma unroll
-                    for (int i = 0; i < kVals; ++i)
-                        if (key[i] >= mid && place(key[i], index_of(i >> 3, i & 7)) >= border) x += weight(w, sh.table, key[i]);
-                    sum_all(x, 0, x_all, c);
-                    up = static_cast<double>(x_all) >= want_mass;
-                    if (!up) above = x_all, exact = true;
-                }
-            } else {
-                up = n_all >= want_count;
-            }
-            if (up) {
-                lo = mid;
-                inside = n_all - above_count;
-            } else {
-                hi = mid;
-                above_count = n_all;
-                inside = below_all;
-            }
-            if (inside <= kList) break;
-        }
-        if (kByMass && !exact) {
-            uint64_t x = 0;
-            uint32_t c;
-#pragma unroll
-            for (int i = 0; i < kVals; ++i)
-                if (key[i] >= hi && place(key[i], index_of(i >> 3, i & 7)) >= border) x += weight(w, sh.table, key[i]);
-            sum_all(x, 0, above, c);
-        }
-        if (hi - lo > 1 || inside <= kList) {
-            // few: listed in every block, sorted, and walked
-            if (threadIdx.x == 0) sh.listed = 0;
-            for (int i = threadIdx.x; i < kList; i += kThreads) sh.list[i] = 0;
+    // Tokens in order: larger logits first, then smaller indices; those up to (edge, edge_index) are kept.
+    float edge = -FLT_MAX;
+    uint32_t edge_index = 0xffffffffu;
+    auto kept = [&](float v, uint32_t i) { return v > edge || (v == edge && i <= edge_index); };
+
+    if constexpr (kFilter) {
+        Filter& f = filter_s;
+        auto place = [&](float v, uint32_t i) { return static_cast<uint64_t>(key_of(v)) << 32 | (0xffffffffu - i); };
+        auto index_at = [](uint64_t p) { return 0xffffffffu - static_cast<uint32_t>(p); };
+        // The tokens for which `which` holds, sorted, in block 0 (where the number of them is at most kList); the
+        // other blocks pass through.
+        auto sorted = [&](auto which) {
+            if (threadIdx.x == 0) f.listed = 0;
             meet();
-#pragma unroll
-            for (int i = 0; i < kVals; ++i) {
-                const uint64_t p = place(key[i], index_of(i >> 3, i & 7));
-                if (key[i] >= lo && key[i] < hi && p >= border) {
-                    for (uint32_t b = 0; b < split; ++b) {
-                        S* to = split > 1 ? cg::this_cluster().map_shared_rank(&sh, b) : &sh;
+            Filter* to = block_of(&f, 0);
+#pragma unroll 4
+            for (uint32_t i = run0; i < run1; ++i)
+                    if (which(x[i], base + i)) {
                         const uint32_t at = atomicAdd(&to->listed, 1u);
-                        if (at < kList) to->list[at] = p;
+                        if (at < kList) to->list[at] = place(x[i], base + i);
                     }
-                }
-            }
             meet();
-            const int n = min(sh.listed, static_cast<uint32_t>(kList));
+            if (rank) return 0;
+            const int n = min(f.listed, static_cast<uint32_t>(kList));
             int size = 2;
             while (size < n) size *= 2;
+            for (int i = n + threadIdx.x; i < size; i += kThreads) f.list[i] = 0;
+            __syncthreads();
             for (int k = 2; k <= size; k *= 2)
                 for (int j = k / 2; j > 0; j /= 2) {
-                    for (int i = threadIdx.x; i < size; i += kThreads) {
-                        const int o = i ^ j;
-                        if (o > i) {
-                            const uint64_t x = sh.list[i], y = sh.list[o];
-                            if ((x < y) == ((i & k) == 0)) sh.list[i] = y, sh.list[o] = x;  // descending
-                        }
+                    for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+                        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+                        const uint64_t p = f.list[lo], q = f.list[hi];
+                        if ((p < q) == ((lo & k) == 0)) f.list[lo] = q, f.list[hi] = p;  // descending
                     }
                     __syncthreads();
                 }
-            if constexpr (kByMass) {
-                for (int i = threadIdx.x; i < size; i += kThreads) sh.mass[i] = i < n ? weight(w, sh.table, static_cast<uint32_t>(sh.list[i] >> 32)) : 0;
-                __syncthreads();
-                if (warp == 0) {
-                    uint64_t before = above;
-                    for (int i = 0; i < n; i += 32) {
-                        uint64_t x = i + lane < n ? sh.mass[i + lane] : 0;
-#pragma unroll
-                        for (int o = 1; o < 32; o *= 2) {
-                            const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
-                            if (lane >= o) x += y;
-                        }
-                        const bool there = i + lane < n && (static_cast<double>(before + x) >= want_mass || i + lane == n - 1);
-                        const uint32_t who = __ballot_sync(0xffffffffu, there);
-                        if (who) {
-                            if (lane == 0) sh.found = sh.list[i + __ffs(who) - 1];
-                            break;
-                        }
-                        before += __shfl_sync(0xffffffffu, x, 31);
-                    }
-                }
-                __syncthreads();
-                border = sh.found;
-            } else {
-                border = sh.list[min(want_count - above_count, static_cast<uint32_t>(n)) - 1];
-            }
-            meet();
-        } else {
-            // many tokens of one logit: the first so many of them
-            uint32_t need;
-            if constexpr (kByMass) {
-                const double each = static_cast<double>(weight(w, sh.table, lo));
-                const double c = ceil((want_mass - static_cast<double>(above)) / fmax(each, 1.0));
-                need = static_cast<uint32_t>(fmin(fmax(c, 1.0), 4e9));
-            } else {
-                need = want_count - above_count;
-            }
-            // the need-th in order of index: by runs of every block, then by threads
-            uint32_t mine[kRounds];
-            bool done = false;
-            uint32_t seen = 0;
-            if (threadIdx.x == 0) sh.found = 0;
-#pragma unroll
-            for (int j = 0; j < kRounds; ++j) {
-                mine[j] = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    mine[j] += key[8 * j + e] == lo && place(lo, index_of(j, e)) >= border;
-            }
-            // (runs of a block are in order, and blocks are)
-            uint32_t of_block = 0;
-#pragma unroll
-            for (int j = 0; j < kRounds; ++j) of_block += mine[j];
-            of_block = __reduce_add_sync(0xffffffffu, of_block);
-            share(0, of_block);
-            uint32_t total = 0;
-            for (uint32_t i = 0; i < split * kWarps; ++i) {
-                if (i / kWarps < rank) seen += sh.counts[turn][i];
-                total += sh.counts[turn][i];
-            }
-            turn ^= 1;
-            need = min(need, total);
-#pragma unroll
-            for (int j = 0; j < kRounds; ++j) {
-                // prefix over the block's threads
-                uint32_t x = mine[j];
-#pragma unroll
-                for (int o = 1; o < 32; o *= 2) {
-                    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-                    if (lane >= o) x += y;
-                }
-                if (lane == 31) sh.mass[j * kWarps + warp] = x;
-                __syncthreads();
-                uint32_t run = 0, prefix = 0;
-                for (int i = 0; i < kWarps; ++i) {
-                    if (i < warp) prefix += static_cast<uint32_t>(sh.mass[j * kWarps + i]);
-                    run += static_cast<uint32_t>(sh.mass[j * kWarps + i]);
-                }
-                const uint32_t before = seen + prefix + x - mine[j];
-                if (!done && before < need && before + mine[j] >= need) {
-                    uint32_t left = need - before;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (left && key[8 * j + e] == lo && place(lo, index_of(j, e)) >= border && --left == 0) {
-                            for (uint32_t b = 0; b < split; ++b)
-                                (split > 1 ? cg::this_cluster().map_shared_rank(&sh, b) : &sh)->found = place(lo, index_of(j, e));
-                        }
-                    done = true;
-                }
-                seen += run;
-            }
-            meet();
-            border = sh.found;
-            meet();
-        }
-    };
+            return n;
+        };
+        auto weight_at = [&](int i) { return weight(w, sh.table, value_of(static_cast<uint32_t>(f.list[i] >> 32))); };
 
-    if (par.top_k && par.top_k < a.vocab) {
-        uint32_t n = 0, n_all;
-        float none;
+        // The bin of a logit, 0 for the largest; the last takes all that is left.
+        const float per_bin = kBins / kSpan * w.rate32;
+        auto bin0 = [&](float v) {
+            if (w.infinite) return v == INFINITY ? 0 : kBins - 1;
+            return static_cast<int>(fminf((w.top32 - v) * per_bin, kBins - 1.0f));
+        };
+        // The last token of the first `want_count`, or of the first whose mass is at least `share_of` of the kept ones'.
+        // Returns false where the kept tokens are all wanted.
+        auto threshold = [&](auto by_mass, double share_of, uint32_t want_count) {
+            constexpr bool kByMass = decltype(by_mass)::value;
+            uint32_t lo = 0, hi = 0, shift = 0;  // keys (lo, hi] after the first time round
+            bool first = true;
+            uint64_t above = 0;      // exact mass, or count, of what lies above the bins
+            double want = kByMass ? 0.0 : want_count;
+            auto inside = [&](float v, uint32_t i) {
+                if (v == -INFINITY || !kept(v, i)) return false;
+                const uint32_t k = key_of(v);
+                return first || (k > lo && k <= hi);
+            };
+            auto bin = [&](float v) { return first ? bin0(v) : static_cast<int>((hi - key_of(v)) >> shift); };
+            while (true) {
+                // weights in 15 bits of the largest that a bin can hold
+#pragma unroll 4
+                for (uint32_t i = run0; i < run1; ++i) {
+                        const float v = x[i];
+                        if (!inside(v, base + i)) continue;
+                        const int b = bin(v);
+                        uint32_t m = 1;
+                        if constexpr (kByMass) {
+                            if (first && b == kBins - 1) continue;  // (no weight, or next to none)
+                            const float d = w.infinite ? 0.0f : (w.top32 - v) * w.rate32 - (first ? b * (kSpan / kBins) : 0.0f);
+                            float y;
+                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(first ? -d : (w.infinite ? 0.0f : (v - value_of(hi)) * w.rate32)));
+                            m = __float2uint_rn(fminf(y, 1.0f) * 32768.0f);
+                        }
+                        atomicAdd(&f.mine[b], m);
+                    }
+                __syncthreads();
+                if (split > 1) {
+                    for (int i = threadIdx.x; i < kBins; i += kThreads)
+                        if (f.mine[i])
+                            for (uint32_t b = 0; b < split; ++b) atomicAdd(&block_of(&f, b)->bins[i], f.mine[i]);
+                    meet();
+                }
+                const uint32_t* bins = split > 1 ? f.bins : f.mine;
+                // the bin that the sums point at
+                if (warp == 0) {
+                    double here[kBins / 32], sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kVals; ++i) n += key[i] != 0;
-        sum_rough(0.0f, n, none, n_all);
-        if (n_all > par.top_k) threshold(std::false_type{}, 0.0, par.top_k);
-    }
-    if (par.top_p < 1.0) {
-        uint64_t x = 0, all;
-        uint32_t c;
+                    for (int i = 0; i < kBins / 32; ++i) {
+                        const int b = lane * (kBins / 32) + i;
+                        here[i] = bins[b];
+                        if (kByMass && first) here[i] *= exp2f(-b * (kSpan / kBins));
+                        sum += here[i];
+                    }
+                    double upto = sum;
 #pragma unroll
-        for (int i = 0; i < kVals; ++i)
-            if (key[i] && place(key[i], index_of(i >> 3, i & 7)) >= border) x += weight(w, sh.table, key[i]);
-        sum_all(x, 0, all, c);
-        threshold(std::true_type{}, fmax(par.top_p, 0.0) * static_cast<double>(all), 0);
-    }
-    // the draw: sums of the kept tokens by runs of 8
-    const uint64_t least = par.min_p > 0.0 ? static_cast<uint64_t>(ceil(par.min_p * 8796093022208.0)) : 1;
-    uint64_t run[kRounds];
+                    for (int o = 1; o < 32; o *= 2) {
+                        const double y = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += y;
+                    }
+                    const double total = __shfl_sync(0xffffffffu, upto, 31);
+                    double goal = want - static_cast<double>(above);
+                    if constexpr (kByMass) goal = first ? share_of * total : goal / (8796093022208.0 / 32768.0) * exp2f((w.top32 - value_of(hi)) * w.rate32);
+                    double before = upto - sum;
+                    int mine = -1, any = -1;
 #pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
-        run[j] = 0;
+                    for (int i = 0; i < kBins / 32; ++i) {
+                        if (here[i] > 0.0) {
+                            any = lane * (kBins / 32) + i;
+                            if (mine < 0 && before + here[i] >= goal) mine = any;
+                        }
+                        before += here[i];
+                    }
+                    const uint32_t has = __ballot_sync(0xffffffffu, mine >= 0), some = __ballot_sync(0xffffffffu, any >= 0);
+                    const int b = has ? __shfl_sync(0xffffffffu, mine, __ffs(has) - 1) : __shfl_sync(0xffffffffu, any, 31 - __clz(some));
+                    if (lane == 0) f.picked = b;
+                }
+                __syncthreads();
+                int b = f.picked;
+                // exact sums: all of them the first time, those above the bin, those in it
+                uint64_t over, in;
+                uint32_t n;
+                if constexpr (kByMass) {
+                    while (true) {
+                        uint64_t s_all = 0, s_over = 0, s_in = 0;
+                        uint32_t c_in = 0;
+#pragma unroll 4
+                        for (uint32_t i = run0; i < run1; ++i) {
+                                const float v = x[i];
+                                if (!inside(v, base + i)) continue;
+                                const int c = bin(v);
+                                if (!first && c > b) continue;
+                                const uint64_t m = weight(w, sh.table, v);
+                                s_all += m;
+                                if (c < b) s_over += m;
+                                else if (c == b) s_in += m, ++c_in;
+                            }
+                        uint64_t all;
+                        uint32_t none;
+                        if (first) {
+                            sum_all(s_all, 0, all, none);
+                            want = share_of * static_cast<double>(all);
+                        }
+                        sum_all(s_over, 0, over, none);
+                        sum_all(s_in, c_in, in, n);
+                        // (a rough sum may have missed by a bin that holds next to nothing)
+                        int next = b;
+                        if (static_cast<double>(above + over) >= want) {
+                            for (next = b - 1; next > 0 && !bins[next]; --next) {}
+                            if (next < 0) next = b;
+                        } else if (static_cast<double>(above + over + in) < want) {
+                            for (next = b + 1; next < kBins && !bins[next] && !(first && next == kBins - 1); ++next) {}
+                            if (next == kBins) next = b;
+                        }
+                        if (next == b) break;
+                        b = next;
+                    }
+                } else {
+                    uint64_t c_over = 0;
+                    for (int i = lane; i < b; i += 32) c_over += bins[i];
+                    over = warp_sum(c_over);
+                    n = bins[b];
+                    in = n;
+                }
+                above += over;
+                if (n <= kList) {
+                    const int found = sorted([&](float v, uint32_t i) { return inside(v, i) && bin(v) == b; });
+                    if (rank == 0) {
+                        if constexpr (kByMass) {
+                            for (int i = threadIdx.x; i < found; i += kThreads) f.mass[i] = weight_at(i);
+                            __syncthreads();
+                            if (warp == 0) {
+                                uint64_t before = above;
+                                for (int i = 0; i < found; i += 32) {
+                                    uint64_t y = i + lane < found ? f.mass[i + lane] : 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t k = key[8 * j + e];
-            if (k == 0 || place(k, index_of(j, e)) < border) continue;
-            const uint64_t x = weight(w, sh.table, k);
-            if (x >= least) run[j] += x;
+                                    for (int o = 1; o < 32; o *= 2) {
+                                        const uint64_t z = __shfl_up_sync(0xffffffffu, y, o);
+                                        if (lane >= o) y += z;
+                                    }
+                                    const bool there = i + lane < found && (static_cast<double>(before + y) >= want || i + lane == found - 1);
+                                    const uint32_t who = __ballot_sync(0xffffffffu, there);
+                                    if (who) {
+                                        if (lane < split) block_of(&f, lane)->found = f.list[i + __ffs(who) - 1];
+                                        break;
+                                    }
+                                    before += __shfl_sync(0xffffffffu, y, 31);
+                                }
+                            }
+                        } else if (threadIdx.x < split) {
+                            block_of(&f, threadIdx.x)->found = f.list[max(1, min(static_cast<int>(want_count - above), found)) - 1];
+                        }
+                    }
+                    meet();
+                    edge = value_of(static_cast<uint32_t>(f.found >> 32));
+                    edge_index = index_at(f.found);
+                    return;
+                }
+                // too many: their keys
+                uint32_t least_key = 0xffffffffu, most_key = 0;
+#pragma unroll 4
+                for (uint32_t i = run0; i < run1; ++i)
+                        if (inside(x[i], base + i) && bin(x[i]) == b) {
+                            const uint32_t k = key_of(x[i]);
+                            least_key = min(least_key, k), most_key = max(most_key, k);
+                        }
+                least_key = __reduce_min_sync(0xffffffffu, least_key);
+                most_key = __reduce_max_sync(0xffffffffu, most_key);
+                share(least_key, most_key);
+                for (uint32_t i = 0; i < split * kWarps; ++i) {
+                    least_key = min(least_key, static_cast<uint32_t>(sh.sums[turn][i]));
+                    most_key = max(most_key, sh.counts[turn][i]);
+                }
+                turn ^= 1;
+                if (least_key == most_key) {
+                    // many tokens of one logit: the first so many of them, in order of index
+                    const float v = value_of(least_key);
+                    uint32_t need = want_count - static_cast<uint32_t>(above);
+                    if constexpr (kByMass) {
+                        const double each = static_cast<double>(weight(w, sh.table, v));
+                        need = static_cast<uint32_t>(fmin(fmax(ceil((want - static_cast<double>(above)) / fmax(each, 1.0)), 1.0), 4e9));
+                    }
+                    need = min(need, n);
+                    uint32_t mine = 0;
+                    for (uint32_t i = run0; i < run1; ++i) mine += x[i] == v && kept(v, base + i);
+                    uint32_t y = mine;
+#pragma unroll
+                    for (int o = 1; o < 32; o *= 2) {
+                        const uint32_t z = __shfl_up_sync(0xffffffffu, y, o);
+                        if (lane >= o) y += z;
+                    }
+                    share(0, __shfl_sync(0xffffffffu, y, 31));
+                    uint32_t before = y - mine;
+                    for (uint32_t i = 0; i < rank * kWarps + warp; ++i) before += sh.counts[turn][i];
+                    turn ^= 1;
+                    if (before < need && before + mine >= need) {
+                        uint32_t left = need - before;
+                        for (uint32_t i = run0; left; ++i)
+                            if (x[i] == v && kept(v, base + i) && --left == 0)
+                                for (uint32_t o = 0; o < split; ++o) block_of(&f, o)->found = place(v, base + i);
+                    }
+                    meet();
+                    edge = v;
+                    edge_index = index_at(f.found);
+                    return;
+                }
+                lo = least_key - 1, hi = most_key;
+                shift = 0;
+                while ((most_key - least_key) >> shift >= kBins) ++shift;
+                first = false;
+                meet();
+                for (int i = threadIdx.x; i < kBins; i += kThreads) f.bins[i] = f.mine[i] = 0;
+                meet();
+            }
+        };
+
+        bool count_on = par.top_k && par.top_k < a.vocab;
+        if (count_on) {
+            uint32_t n = 0, n_all;
+            uint64_t none;
+#pragma unroll 4
+            for (uint32_t i = run0; i < run1; ++i) n += x[i] != -INFINITY;
+            sum_all(0, n, none, n_all);
+            count_on = n_all > par.top_k;
+        }
+        if (count_on) threshold(std::false_type{}, 0.0, par.top_k);
+        if (count_on && par.top_k <= kList) {
+            // all that is kept: a list
+            const int n = sorted([&](float v, uint32_t i) { return v != -INFINITY && kept(v, i); });
+            if (rank) return;  // (no other block writes to this one any more)
+            for (int i = threadIdx.x; i < n; i += kThreads) f.mass[i] = weight_at(i);
+            __syncthreads();
+            // how many top_p and min_p keep, and their mass
+            if (warp == 0) {
+                uint64_t all = 0;
+                for (int i = lane; i < n; i += 32) all += f.mass[i];
+                all = warp_sum(all);
+                const double want = par.top_p < 1.0 ? fmax(par.top_p, 0.0) * static_cast<double>(all) : INFINITY;
+                uint64_t before = 0;
+                int m = 0;
+                for (int i = 0; i < n; i += 32) {
+                    const uint64_t own = i + lane < n ? f.mass[i + lane] : 0;
+                    uint64_t y = own;
+#pragma unroll
+                    for (int o = 1; o < 32; o *= 2) {
+                        const uint64_t z = __shfl_up_sync(0xffffffffu, y, o);
+                        if (lane >= o) y += z;
+                    }
+                    const bool keep = i + lane < n && own >= least && (i + lane == 0 || static_cast<double>(before + y - own) < want);
+                    const uint32_t who = __ballot_sync(0xffffffffu, keep);
+                    m += __popc(who);
+                    if (who != 0xffffffffu) {
+                        before += who ? __shfl_sync(0xffffffffu, y, 31 - __clz(who)) : 0;
+                        break;
+                    }
+                    before += __shfl_sync(0xffffffffu, y, 31);
+                }
+                if (lane == 0) f.listed = m, f.found = before;
+            }
+            __syncthreads();
+            const int m = f.listed;
+            const uint64_t all = f.found, point = point_of(all);
+            // each kept token: the sum of those of lower index
+            for (int i = threadIdx.x; i < m; i += kThreads) {
+                const uint32_t mine = index_at(f.list[i]);
+                uint64_t sum = 0;
+                for (int j = 0; j < m; ++j) sum += index_at(f.list[j]) < mine ? f.mass[j] : 0;
+                if (sum <= point && point < sum + f.mass[i]) answer(mine, f.mass[i], all);
+            }
+            return;
+        }
+        if (par.top_p < 1.0) {
+            if (count_on) {
+                meet();
+                for (int i = threadIdx.x; i < kBins; i += kThreads) f.bins[i] = f.mine[i] = 0;
+                meet();
+            }
+            threshold(std::true_type{}, fmax(par.top_p, 0.0), 0);
         }
     }
-    uint64_t mine = 0, all;
+
+    // the draw: sums of the kept tokens, thread by thread
+    uint64_t mine = 0, all = 0;
+#pragma unroll 4
+    for (uint32_t i = run0; i < run1; ++i) {
+        if (!kept(x[i], base + i)) continue;
+        const uint64_t m = weight(w, sh.table, x[i]);
+        if (m >= least) mine += m;
+    }
+    uint64_t y = mine;
 #pragma unroll
-    for (int j = 0; j < kRounds; ++j) mine += run[j];
-    uint64_t in_block = mine;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) in_block += __shfl_xor_sync(0xffffffffu, in_block, o);
-    share(in_block, 0);
-    uint64_t before = 0;  // of the blocks before this one
-    all = 0;
+    for (int o = 1; o < 32; o *= 2) {
+        const uint64_t z = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) y += z;
+    }
+    share(__shfl_sync(0xffffffffu, y, 31), 0);
+    uint64_t sum = y - mine;
     for (uint32_t i = 0; i < split * kWarps; ++i) {
-        if (i / kWarps < rank) before += sh.sums[turn][i];
+        if (i < rank * kWarps + warp) sum += sh.sums[turn][i];
         all += sh.sums[turn][i];
     }
     turn ^= 1;
-    const float u = a.uniform[row];
-    const double at = (u > 0.0f ? static_cast<double>(fminf(u, 1.0f)) : 0.0) * static_cast<double>(all);
-    const uint64_t point = min(static_cast<uint64_t>(at), all - 1);  // the first token whose sum passes it
-    uint64_t* const parts = sh.mass;
-#pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
-        uint64_t x = run[j];
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        if (lane == 31) parts[j * kWarps + warp] = x;
-        __syncthreads();
-        uint64_t total = 0, prefix = 0;
-        for (int i = 0; i < kWarps; ++i) {
-            if (i < warp) prefix += parts[j * kWarps + i];
-            total += parts[j * kWarps + i];
-        }
-        uint64_t sum = before + prefix + x - run[j];
-        if (sum <= point && point < sum + run[j]) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t k = key[8 * j + e];
-                if (k == 0 || place(k, index_of(j, e)) < border) continue;
-                const uint64_t y = weight(w, sh.table, k);
-                if (y < least) continue;
-                if (sum <= point && point < sum + y) {
-                    a.tokens[row] = static_cast<int32_t>(index_of(j, e));
-                    if (a.log_probs) a.log_probs[row] = static_cast<float>(log(static_cast<double>(y) / static_cast<double>(all)));
-                }
-                sum += y;
+    const uint64_t point = point_of(all);
+    if (sum <= point && point < sum + mine) {
+        for (uint32_t i = run0; i < run1; ++i) {
+            if (!kept(x[i], base + i)) continue;
+            const uint64_t m = weight(w, sh.table, x[i]);
+            if (m < least) continue;
+            if (point < sum + m) {
+                answer(base + i, m, all);
+                break;
             }
+            sum += m;
         }
-        before += total;
     }
     if (split > 1) cg::this_cluster().sync();  // (no block ends while another writes to it)
 }
 
-template <typename T, int kThreads, int kVals> cudaError_t launch(const TokenArgs& a, uint32_t split, cudaStream_t s) {
-    auto* kernel = sample_kernel<T, kThreads, kVals>;
+template <typename T, int kThreads, bool kFilter> cudaError_t launch(const TokenArgs& a, uint32_t split, cudaStream_t s) {
+    auto* kernel = sample_kernel<T, kThreads, kFilter>;
     const int vectors = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.stride * sizeof(T) % 16 == 0;
-    if (split > 8) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-    }
+    const uint32_t slice = ((a.vocab + split - 1) / split + 7) / 8 * 8;
+    cudaError_t e = cudaSuccess;
+    if (split > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && slice * 4 > 16384) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice * 4);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.rows * split);
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = slice * 4;
     cfg.stream = s;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -510,23 +591,29 @@ template <typename T, int kThreads, int kVals> cudaError_t launch(const TokenArg
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = split > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, a, split, vectors);
+    return cudaLaunchKernelEx(&cfg, kernel, a, split, slice, vectors);
 }
 
-template <typename T> cudaError_t by_vocab(const TokenArgs& a, cudaStream_t s) {
-    if (a.vocab <= 1024) return launch<T, 128, 8>(a, 1, s);
-    if (a.vocab <= 4096) return launch<T, 128, 32>(a, 1, s);
-    const uint32_t slices = (a.vocab + 16383) / 16384;
+template <typename T, bool kFilter> cudaError_t by_vocab(const TokenArgs& a, cudaStream_t s) {
+    if (a.vocab <= 1024) return launch<T, 32, kFilter>(a, 1, s);
+    if (a.vocab <= 8192) return launch<T, 128, kFilter>(a, 1, s);
     uint32_t split = 1;
-    while (split < slices) split *= 2;
-    return launch<T, 512, 32>(a, split, s);
+    while (split * kMaxSlice < a.vocab) split *= 2;
+    // few rows: more blocks each, down to 8192 logits
+    while (a.rows * split * 2 <= 148 && split < 8 && split * 2 * 8192 <= a.vocab) split *= 2;
+    return launch<T, 512, kFilter>(a, split, s);
+}
+
+template <typename T> cudaError_t by_filter(const TokenArgs& a, cudaStream_t s) {
+    const bool filter = a.top_ks || a.top_ps || a.temperatures || a.top_k || a.top_p < 1.0 || !(a.temperature > 0.0);
+    return filter ? by_vocab<T, true>(a, s) : by_vocab<T, false>(a, s);
 }
 
 }  // namespace
 
 cudaError_t launch_sample_tokens(const TokenArgs& a, int dtype, cudaStream_t s) {
-    if (dtype == LWM_DTYPE_F32) return by_vocab<float>(a, s);
-    return dtype == LWM_DTYPE_BF16 ? by_vocab<bf16>(a, s) : by_vocab<__half>(a, s);
+    if (dtype == LWM_DTYPE_F32) return by_filter<float>(a, s);
+    return dtype == LWM_DTYPE_BF16 ? by_filter<bf16>(a, s) : by_filter<__half>(a, s);
 }
 
 }  // namespace lwm
