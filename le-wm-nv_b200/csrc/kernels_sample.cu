@@ -53,7 +53,6 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 struct Weights {
     double top, rate;  // largest logit, 64 log2(e) / temperature
     float top32, rate32;
-    bool infinite;     // the largest logit is plus infinity: all such tokens weigh the same
 };
 constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number in the low bits
 // A float as a double, without the conversion unit (subnormals may become any tiny number).
@@ -64,17 +63,16 @@ __device__ __forceinline__ double widen(float x) {
 // round(2^43 exp((x - top) / temperature)).  2^(n / 64) comes from a table,
 // the rest, below 2^-7, from five terms of the series.
 __device__ __forceinline__ uint64_t weight(const Weights& w, const double* table, float x) {
-    if (x == -INFINITY) return 0;
-    if (w.infinite) return x == INFINITY ? 1ull << 43 : 0;
     const double y = (widen(x) - w.top) * w.rate;  // 64ths of a power of two
-    if (y < -2900.0) return 0;                     // below 2^-45
     const double t = y + kMagic, n = t - kMagic;
     const int i = __double2loint(t);
     const double r = (y - n) * 0.010830424696249145;  // ln 2 / 64
-    const double p = fma(fma(fma(fma(1.0 / 24.0, r, 1.0 / 6.0), r, 0.5), r, 1.0), r, 1.0);
+    const double r2 = r * r;
+    const double p = fma(fma(1.0 / 24.0, r2, 0.5), r2, 1.0) + fma(1.0 / 6.0, r2, 1.0) * r;  // the series to r^4
     const double f = table[i & 63] * p;  // [2^-1/128, 2)
     const double scaled = __hiloint2double(__double2hiint(f) + (((i >> 6) + 43) << 20), __double2loint(f));
-    return __double_as_longlong(scaled + kMagic) - __double_as_longlong(kMagic);
+    const uint64_t m = __double_as_longlong(scaled + kMagic) - __double_as_longlong(kMagic);
+    return static_cast<uint32_t>(__double2hiint(y)) < 0xc0a6a800u ? m : 0;  // (y > -2900: below that it is 2^-45 and less)
 }
 
 struct Params {
@@ -106,7 +104,7 @@ struct Filter {  // of a kernel with thresholds
     uint32_t mine[kBins];  // of this block
     uint64_t list[kList];
     uint64_t mass[kList];
-    uint64_t found;
+    uint64_t found, most;
     uint32_t listed, picked;
 };
 
@@ -125,7 +123,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     // A thread's logits: a run of odd length, so that the threads of a warp read different banks, in order of index.
     const uint32_t each = ((count + kThreads - 1) / kThreads) | 1u;
     const uint32_t run0 = min(threadIdx.x * each, count), run1 = min(run0 + each, count);
-    float top = -INFINITY;
+    float top = -INFINITY;  // of the logits that this thread loads
     {
         const T* src = static_cast<const T*>(a.logits) + row * a.stride + base;
         auto clean = [&](float v) {
@@ -178,6 +176,15 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         turn ^= 1;
     };
 
+    // The thread's logits four at a time, so that their chains run side by side.
+    auto by_four = [&](auto what) {
+        for (uint32_t i = run0; i < run1; i += 4) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = i + e < run1 ? x[i + e] : -INFINITY;
+            what(v, base + i);
+        }
+    };
     // the largest logit
     Weights w;
     {
@@ -195,7 +202,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
             return;
         }
         w.top32 = value_of(k);
-        w.infinite = w.top32 == INFINITY;
+        if (w.top32 == INFINITY) {  // infinities share the row: as if they were zero, and nothing else there
+            for (uint32_t i = run0; i < run1; ++i) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+            top = top == INFINITY ? 0.0f : -INFINITY;
+            w.top32 = 0.0f;
+            __syncthreads();
+        }
         w.top = widen(w.top32);
         w.rate = 92.332482616893657 / par.temperature;  // 64 log2(e)
         w.rate32 = static_cast<float>(1.4426950408889634 / par.temperature);
@@ -215,6 +227,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     // Tokens in order: larger logits first, then smaller indices; those up to (edge, edge_index) are kept.
     float edge = -FLT_MAX;
     uint32_t edge_index = 0xffffffffu;
+    // Of the kept ones above `settled` the thread's sum is `known` already.
+    float settled = INFINITY;
+    uint64_t known = 0;
     auto kept = [&](float v, uint32_t i) { return v > edge || (v == edge && i <= edge_index); };
 
     if constexpr (kFilter) {
@@ -253,107 +268,142 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         };
         auto weight_at = [&](int i) { return weight(w, sh.table, value_of(static_cast<uint32_t>(f.list[i] >> 32))); };
 
-        // The bin of a logit, 0 for the largest; the last takes all that is left.
+        // A logit's place in bins, 0 for the largest; the last bin takes all that is left.
         const float per_bin = kBins / kSpan * w.rate32;
-        auto bin0 = [&](float v) {
-            if (w.infinite) return v == INFINITY ? 0 : kBins - 1;
-            return static_cast<int>(fminf((w.top32 - v) * per_bin, kBins - 1.0f));
+        auto place0 = [&](float v) { return fminf((w.top32 - v) * per_bin, kBins - 1.0f); };
+        // The counts of all blocks' bins in every block (the caller's are in f.mine), and the bin with which the sum
+        // from the first one on reaches `goal`: each bin counts `unit` times its own weight.
+        auto pick = [&](auto weigh, auto goal_of) {
+            __syncthreads();
+            if (split > 1) {
+                for (int i = threadIdx.x; i < kBins; i += kThreads)
+                    if (f.mine[i])
+                        for (uint32_t b = 0; b < split; ++b) atomicAdd(&block_of(&f, b)->bins[i], f.mine[i]);
+                meet();
+            }
+            const uint32_t* bins = split > 1 ? f.bins : f.mine;
+            if (warp == 0) {
+                double here[kBins / 32], sum = 0.0;
+#pragma unroll
+                for (int i = 0; i < kBins / 32; ++i) {
+                    const int b = lane * (kBins / 32) + i;
+                    here[i] = bins[b] ? bins[b] * weigh(b) : 0.0;
+                    sum += here[i];
+                }
+                double upto = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) {
+                    const double y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                const double goal = goal_of(__shfl_sync(0xffffffffu, upto, 31));
+                double before = upto - sum;
+                int mine = -1, any = -1;
+#pragma unroll
+                for (int i = 0; i < kBins / 32; ++i) {
+                    if (here[i] > 0.0) {
+                        any = lane * (kBins / 32) + i;
+                        if (mine < 0 && before + here[i] >= goal) mine = any;
+                    }
+                    before += here[i];
+                }
+                const uint32_t has = __ballot_sync(0xffffffffu, mine >= 0), some = __ballot_sync(0xffffffffu, any >= 0);
+                const int b = has ? __shfl_sync(0xffffffffu, mine, __ffs(has) - 1)
+                                  : some ? __shfl_sync(0xffffffffu, any, 31 - __clz(some)) : 0;
+                if (lane == 0) f.picked = b;
+            }
+            __syncthreads();
+            return static_cast<int>(f.picked);
+        };
+        auto clear_bins = [&] {
+            meet();
+            for (int i = threadIdx.x; i < kBins; i += kThreads) f.bins[i] = f.mine[i] = 0;
+            meet();
         };
         // The last token of the first `want_count`, or of the first whose mass is at least `share_of` of the kept ones'.
-        // Returns false where the kept tokens are all wanted.
         auto threshold = [&](auto by_mass, double share_of, uint32_t want_count) {
             constexpr bool kByMass = decltype(by_mass)::value;
             uint32_t lo = 0, hi = 0, shift = 0;  // keys (lo, hi] after the first time round
-            bool first = true;
-            uint64_t above = 0;      // exact mass, or count, of what lies above the bins
+            uint64_t above = 0;                  // exact mass, or count, of what lies above the bins
             double want = kByMass ? 0.0 : want_count;
-            auto inside = [&](float v, uint32_t i) {
-                if (v == -INFINITY || !kept(v, i)) return false;
-                const uint32_t k = key_of(v);
-                return first || (k > lo && k <= hi);
-            };
-            auto bin = [&](float v) { return first ? bin0(v) : static_cast<int>((hi - key_of(v)) >> shift); };
-            while (true) {
-                // weights in 15 bits of the largest that a bin can hold
+            // one level of bins; true when the threshold is found
+            auto level = [&](auto is_first) {
+                constexpr bool kFirst = decltype(is_first)::value;
+                auto inside = [&](float v, uint32_t i) {
+                    if (v == -INFINITY || !kept(v, i)) return false;
+                    if constexpr (kFirst) return true;
+                    const uint32_t k = key_of(v);
+                    return k > lo && k <= hi;
+                };
+                // (a whole number; the first time with a fraction behind it)
+                auto bin = [&](float v) {
+                    if constexpr (kFirst) return place0(v);
+                    else return static_cast<float>((hi - key_of(v)) >> shift);
+                };
+                const float high = kFirst ? 0.0f : value_of(hi);
 #pragma unroll 4
                 for (uint32_t i = run0; i < run1; ++i) {
-                        const float v = x[i];
-                        if (!inside(v, base + i)) continue;
-                        const int b = bin(v);
-                        uint32_t m = 1;
-                        if constexpr (kByMass) {
-                            if (first && b == kBins - 1) continue;  // (no weight, or next to none)
-                            const float d = w.infinite ? 0.0f : (w.top32 - v) * w.rate32 - (first ? b * (kSpan / kBins) : 0.0f);
-                            float y;
-                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(first ? -d : (w.infinite ? 0.0f : (v - value_of(hi)) * w.rate32)));
-                            m = __float2uint_rn(fminf(y, 1.0f) * 32768.0f);
-                        }
-                        atomicAdd(&f.mine[b], m);
+                    const float v = x[i];
+                    if (!inside(v, base + i)) continue;
+                    const float c = bin(v);
+                    uint32_t m = 1;
+                    if constexpr (kByMass) {
+                        if (kFirst && c >= kBins - 1.0f) continue;  // (no weight, or next to none)
+                        // weights in 15 bits of the largest that the bin can hold
+                        float y;
+                        asm("ex2.approx.ftz.f32 %0, %1;"
+                            : "=f"(y)
+                            : "f"(kFirst ? (truncf(c) - c) * (kSpan / kBins) : (v - high) * w.rate32));
+                        m = __float2uint_rn(fminf(y, 1.0f) * 32768.0f);
                     }
-                __syncthreads();
-                if (split > 1) {
-                    for (int i = threadIdx.x; i < kBins; i += kThreads)
-                        if (f.mine[i])
-                            for (uint32_t b = 0; b < split; ++b) atomicAdd(&block_of(&f, b)->bins[i], f.mine[i]);
-                    meet();
+                    atomicAdd(&f.mine[static_cast<int>(c)], m);
                 }
+                int b = pick([&](int c) { return kByMass && kFirst ? static_cast<double>(exp2f(-c * (kSpan / kBins))) : 1.0; },
+                             [&](double total) {
+                                 if (!kByMass) return want - static_cast<double>(above);
+                                 if (kFirst) return share_of * total;
+                                 return (want - static_cast<double>(above)) * (32768.0 / 8796093022208.0) *
+                                        exp2f((w.top32 - high) * w.rate32);
+                             });
                 const uint32_t* bins = split > 1 ? f.bins : f.mine;
-                // the bin that the sums point at
-                if (warp == 0) {
-                    double here[kBins / 32], sum = 0.0;
-#pragma unroll
-                    for (int i = 0; i < kBins / 32; ++i) {
-                        const int b = lane * (kBins / 32) + i;
-                        here[i] = bins[b];
-                        if (kByMass && first) here[i] *= exp2f(-b * (kSpan / kBins));
-                        sum += here[i];
-                    }
-                    double upto = sum;
-#pragma unroll
-                    for (int o = 1; o < 32; o *= 2) {
-                        const double y = __shfl_up_sync(0xffffffffu, upto, o);
-                        if (lane >= o) upto += y;
-                    }
-                    const double total = __shfl_sync(0xffffffffu, upto, 31);
-                    double goal = want - static_cast<double>(above);
-                    if constexpr (kByMass) goal = first ? share_of * total : goal / (8796093022208.0 / 32768.0) * exp2f((w.top32 - value_of(hi)) * w.rate32);
-                    double before = upto - sum;
-                    int mine = -1, any = -1;
-#pragma unroll
-                    for (int i = 0; i < kBins / 32; ++i) {
-                        if (here[i] > 0.0) {
-                            any = lane * (kBins / 32) + i;
-                            if (mine < 0 && before + here[i] >= goal) mine = any;
-                        }
-                        before += here[i];
-                    }
-                    const uint32_t has = __ballot_sync(0xffffffffu, mine >= 0), some = __ballot_sync(0xffffffffu, any >= 0);
-                    const int b = has ? __shfl_sync(0xffffffffu, mine, __ffs(has) - 1) : __shfl_sync(0xffffffffu, any, 31 - __clz(some));
-                    if (lane == 0) f.picked = b;
-                }
-                __syncthreads();
-                int b = f.picked;
                 // exact sums: all of them the first time, those above the bin, those in it
-                uint64_t over, in;
+                uint64_t over;
                 uint32_t n;
                 if constexpr (kByMass) {
+                    uint64_t sure, in;  // sure: the thread's part of what is above the bin and passes min_p
                     while (true) {
                         uint64_t s_all = 0, s_over = 0, s_in = 0;
                         uint32_t c_in = 0;
-#pragma unroll 4
-                        for (uint32_t i = run0; i < run1; ++i) {
-                                const float v = x[i];
-                                if (!inside(v, base + i)) continue;
-                                const int c = bin(v);
-                                if (!first && c > b) continue;
-                                const uint64_t m = weight(w, sh.table, v);
-                                s_all += m;
-                                if (c < b) s_over += m;
-                                else if (c == b) s_in += m, ++c_in;
+                        sure = 0;
+                        const float b0 = static_cast<float>(b), b1 = static_cast<float>(b + 1);
+                        by_four([&](const float(&v)[4], uint32_t i) {
+                            bool need[4], some = false;
+                            float c[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                need[e] = inside(v[e], i + e);
+                                c[e] = bin(v[e]);
+                                if (!kFirst) need[e] &= c[e] < b1;
+                                some |= need[e];
                             }
+                            if (!some) return;
+                            uint64_t m[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) m[e] = weight(w, sh.table, v[e]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if (!need[e]) m[e] = 0, c[e] = kBins;
+                                if (kFirst) s_all += m[e];
+                                const bool is_over = c[e] < b0, is_in = !is_over && c[e] < b1;
+                                s_over += is_over ? m[e] : 0;
+                                sure += is_over && m[e] >= least ? m[e] : 0;
+                                s_in += is_in ? m[e] : 0;
+                                c_in += is_in;
+                            }
+                        });
                         uint64_t all;
                         uint32_t none;
-                        if (first) {
+                        if constexpr (kFirst) {
                             sum_all(s_all, 0, all, none);
                             want = share_of * static_cast<double>(all);
                         }
@@ -365,22 +415,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                             for (next = b - 1; next > 0 && !bins[next]; --next) {}
                             if (next < 0) next = b;
                         } else if (static_cast<double>(above + over + in) < want) {
-                            for (next = b + 1; next < kBins && !bins[next] && !(first && next == kBins - 1); ++next) {}
+                            for (next = b + 1; next < kBins && !bins[next] && !(kFirst && next == kBins - 1); ++next) {}
                             if (next == kBins) next = b;
                         }
                         if (next == b) break;
                         b = next;
                     }
+                    known += sure;
                 } else {
                     uint64_t c_over = 0;
                     for (int i = lane; i < b; i += 32) c_over += bins[i];
                     over = warp_sum(c_over);
                     n = bins[b];
-                    in = n;
                 }
                 above += over;
                 if (n <= kList) {
-                    const int found = sorted([&](float v, uint32_t i) { return inside(v, i) && bin(v) == b; });
+                    const int found = sorted([&](float v, uint32_t i) { return inside(v, i) && static_cast<int>(bin(v)) == b; });
                     if (rank == 0) {
                         if constexpr (kByMass) {
                             for (int i = threadIdx.x; i < found; i += kThreads) f.mass[i] = weight_at(i);
@@ -397,7 +447,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                                     const bool there = i + lane < found && (static_cast<double>(before + y) >= want || i + lane == found - 1);
                                     const uint32_t who = __ballot_sync(0xffffffffu, there);
                                     if (who) {
-                                        if (lane < split) block_of(&f, lane)->found = f.list[i + __ffs(who) - 1];
+                                        if (lane < split) {
+                                            Filter* to = block_of(&f, lane);
+                                            to->found = f.list[i + __ffs(who) - 1], to->most = f.list[0];
+                                        }
                                         break;
                                     }
                                     before += __shfl_sync(0xffffffffu, y, 31);
@@ -410,19 +463,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                     meet();
                     edge = value_of(static_cast<uint32_t>(f.found >> 32));
                     edge_index = index_at(f.found);
-                    return;
+                    if (kByMass) settled = value_of(static_cast<uint32_t>(f.most >> 32));
+                    return true;
                 }
                 // too many: their keys
                 uint32_t least_key = 0xffffffffu, most_key = 0;
-#pragma unroll 4
                 for (uint32_t i = run0; i < run1; ++i)
-                        if (inside(x[i], base + i) && bin(x[i]) == b) {
-                            const uint32_t k = key_of(x[i]);
-                            least_key = min(least_key, k), most_key = max(most_key, k);
-                        }
-                least_key = __reduce_min_sync(0xffffffffu, least_key);
-                most_key = __reduce_max_sync(0xffffffffu, most_key);
-                share(least_key, most_key);
+                    if (inside(x[i], base + i) && static_cast<int>(bin(x[i])) == b) {
+                        const uint32_t k = key_of(x[i]);
+                        least_key = min(least_key, k), most_key = max(most_key, k);
+                    }
+                share(__reduce_min_sync(0xffffffffu, least_key), __reduce_max_sync(0xffffffffu, most_key));
                 for (uint32_t i = 0; i < split * kWarps; ++i) {
                     least_key = min(least_key, static_cast<uint32_t>(sh.sums[turn][i]));
                     most_key = max(most_key, sh.counts[turn][i]);
@@ -433,8 +484,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                     const float v = value_of(least_key);
                     uint32_t need = want_count - static_cast<uint32_t>(above);
                     if constexpr (kByMass) {
-                        const double each = static_cast<double>(weight(w, sh.table, v));
-                        need = static_cast<uint32_t>(fmin(fmax(ceil((want - static_cast<double>(above)) / fmax(each, 1.0)), 1.0), 4e9));
+                        const double one = static_cast<double>(weight(w, sh.table, v));
+                        need = static_cast<uint32_t>(fmin(fmax(ceil((want - static_cast<double>(above)) / fmax(one, 1.0)), 1.0), 4e9));
                     }
                     need = min(need, n);
                     uint32_t mine = 0;
@@ -458,31 +509,56 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                     meet();
                     edge = v;
                     edge_index = index_at(f.found);
-                    return;
+                    if (kByMass) settled = v;
+                    return true;
                 }
                 lo = least_key - 1, hi = most_key;
                 shift = 0;
                 while ((most_key - least_key) >> shift >= kBins) ++shift;
-                first = false;
-                meet();
-                for (int i = threadIdx.x; i < kBins; i += kThreads) f.bins[i] = f.mine[i] = 0;
-                meet();
-            }
+                clear_bins();
+                return false;
+            };
+            if (!level(std::true_type{}))
+                while (!level(std::false_type{})) {}
         };
 
-        bool count_on = par.top_k && par.top_k < a.vocab;
-        if (count_on) {
-            uint32_t n = 0, n_all;
+        bool count_on = par.top_k && par.top_k < a.vocab, few = false;
+        int n = 0;
+        if (count_on && par.top_k <= min(kList / 2, kThreads * static_cast<int>(split) / 2)) {
+            // As many threads' largest logits are at least the top_k-th of all: with their bins the first top_k tokens
+            // are among few.
+            if (top != -INFINITY) atomicAdd(&f.mine[static_cast<int>(place0(top))], 1u);
+            const uint32_t want = par.top_k;
+            const float last = static_cast<float>(pick([](int) { return 1.0; }, [&](double) { return static_cast<double>(want); }) + 1);
+            const uint32_t* bins = split > 1 ? f.bins : f.mine;
+            uint32_t tops = 0;
+            for (int i = lane; i < kBins; i += 32) tops += bins[i];
+            tops = __reduce_add_sync(0xffffffffu, tops);
+            if (tops >= want && last < kBins) {
+                n = sorted([&](float v, uint32_t) { return v != -INFINITY && place0(v) < last; });
+                few = block_of(&f, 0)->listed <= kList;
+                n = min(n, static_cast<int>(want));
+            }
+            if (!few) clear_bins();
+            else if (split > 1) meet();  // (block 0's count has been read)
+        }
+        if (count_on && !few) {
+            uint32_t c = 0, c_all;
             uint64_t none;
 #pragma unroll 4
-            for (uint32_t i = run0; i < run1; ++i) n += x[i] != -INFINITY;
-            sum_all(0, n, none, n_all);
-            count_on = n_all > par.top_k;
+            for (uint32_t i = run0; i < run1; ++i) c += x[i] != -INFINITY;
+            sum_all(0, c, none, c_all);
+            count_on = c_all > par.top_k;
         }
-        if (count_on) threshold(std::false_type{}, 0.0, par.top_k);
-        if (count_on && par.top_k <= kList) {
+        if (count_on && !few) {
+            threshold(std::false_type{}, 0.0, par.top_k);
+            if (par.top_k <= kList) {
+                n = sorted([&](float v, uint32_t i) { return v != -INFINITY && kept(v, i); });
+                few = true;
+            }
+        }
+        if (few) {
             // all that is kept: a list
-            const int n = sorted([&](float v, uint32_t i) { return v != -INFINITY && kept(v, i); });
             if (rank) return;  // (no other block writes to this one any more)
             for (int i = threadIdx.x; i < n; i += kThreads) f.mass[i] = weight_at(i);
             __syncthreads();
@@ -526,23 +602,24 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
             return;
         }
         if (par.top_p < 1.0) {
-            if (count_on) {
-                meet();
-                for (int i = threadIdx.x; i < kBins; i += kThreads) f.bins[i] = f.mine[i] = 0;
-                meet();
-            }
+            if (count_on) clear_bins();
             threshold(std::true_type{}, fmax(par.top_p, 0.0), 0);
         }
     }
 
     // the draw: sums of the kept tokens, thread by thread
-    uint64_t mine = 0, all = 0;
-#pragma unroll 4
-    for (uint32_t i = run0; i < run1; ++i) {
-        if (!kept(x[i], base + i)) continue;
-        const uint64_t m = weight(w, sh.table, x[i]);
-        if (m >= least) mine += m;
-    }
+    uint64_t mine = known, all = 0;
+    by_four([&](const float(&v)[4], uint32_t i) {
+        bool need[4], some = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) some |= need[e] = kept(v[e], i + e) && v[e] <= settled;
+        if (!some) return;
+        uint64_t m[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] = weight(w, sh.table, v[e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mine += need[e] && m[e] >= least ? m[e] : 0;
+    });
     uint64_t y = mine;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -557,16 +634,24 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     }
     turn ^= 1;
     const uint64_t point = point_of(all);
-    if (sum <= point && point < sum + mine) {
-        for (uint32_t i = run0; i < run1; ++i) {
-            if (!kept(x[i], base + i)) continue;
-            const uint64_t m = weight(w, sh.table, x[i]);
-            if (m < least) continue;
-            if (point < sum + m) {
-                answer(base + i, m, all);
-                break;
+    // the thread whose run it falls into, and with its warp's help the token
+    const uint32_t who = __ballot_sync(0xffffffffu, sum <= point && point < sum + mine);
+    if (who) {
+        const int owner = __ffs(who) - 1;
+        const uint32_t from = __shfl_sync(0xffffffffu, run0, owner), to = __shfl_sync(0xffffffffu, run1, owner);
+        sum = __shfl_sync(0xffffffffu, sum, owner);
+        for (uint32_t i = from; i < to; i += 32) {
+            const float v = i + lane < to ? x[i + lane] : -INFINITY;
+            uint64_t m = kept(v, base + i + lane) ? weight(w, sh.table, v) : 0;
+            if (m < least) m = 0;
+            uint64_t z = m;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const uint64_t q = __shfl_up_sync(0xffffffffu, z, o);
+                if (lane >= o) z += q;
             }
-            sum += m;
+            if (sum + z - m <= point && point < sum + z) answer(base + i + lane, m, all);
+            sum += __shfl_sync(0xffffffffu, z, 31);
         }
     }
     if (split > 1) cg::this_cluster().sync();  // (no block ends while another writes to it)
@@ -601,7 +686,7 @@ template <typename T, bool kFilter> cudaError_t by_vocab(const TokenArgs& a, cud
     while (split * kMaxSlice < a.vocab) split *= 2;
     // few rows: more blocks each, down to 8192 logits
     while (a.rows * split * 2 <= 148 && split < 8 && split * 2 * 8192 <= a.vocab) split *= 2;
-    return launch<T, 512, kFilter>(a, split, s);
+    return a.vocab > 16384 * split ? launch<T, 1024, kFilter>(a, split, s) : launch<T, 512, kFilter>(a, split, s);
 }
 
 template <typename T> cudaError_t by_filter(const TokenArgs& a, cudaStream_t s) {
