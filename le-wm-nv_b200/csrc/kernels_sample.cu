@@ -33,7 +33,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kList = 1024;     // candidates that are sorted
 constexpr int kMaxSplit = 16;   // blocks of a row
-constexpr int kBins = 256;
+constexpr int kBins = 512;
 constexpr uint32_t kMaxSlice = 32768;  // logits of a block
 constexpr float kSpan = 45.0f;  // powers of two that the bins span: weights end there
 
@@ -60,9 +60,9 @@ __device__ __forceinline__ double widen(float x) {
     const uint32_t b = __float_as_uint(x), m = b & 0x7fffffffu;
     return __hiloint2double(static_cast<int>((b & 0x80000000u) | (m == 0 ? 0u : (m >> 3) + 0x38000000u)), static_cast<int>(b << 29));
 }
-// round(2^43 exp((x - top) / temperature)).  2^(n / 64) comes from a table,
-// the rest, below 2^-7, from five terms of the series.
-__device__ __forceinline__ uint64_t weight(const Weights& w, const double* table, float x) {
+// 2^43 exp((x - top) / temperature), rounded to a whole number (a thread's sums of them stay below 2^53, so
+// they are exact).  2^(n / 64) comes from a table, the rest, below 2^-7, from five terms of the series.
+__device__ __forceinline__ double weight(const Weights& w, const double* table, float x) {
     const double y = (widen(x) - w.top) * w.rate;  // 64ths of a power of two
     const double t = y + kMagic, n = t - kMagic;
     const int i = __double2loint(t);
@@ -70,9 +70,9 @@ __device__ __forceinline__ uint64_t weight(const Weights& w, const double* table
     const double r2 = r * r;
     const double p = fma(fma(1.0 / 24.0, r2, 0.5), r2, 1.0) + fma(1.0 / 6.0, r2, 1.0) * r;  // the series to r^4
     const double f = table[i & 63] * p;  // [2^-1/128, 2)
-    const double scaled = __hiloint2double(__double2hiint(f) + (((i >> 6) + 43) << 20), __double2loint(f));
-    const uint64_t m = __double_as_longlong(scaled + kMagic) - __double_as_longlong(kMagic);
-    return static_cast<uint32_t>(__double2hiint(y)) < 0xc0a6a800u ? m : 0;  // (y > -2900: below that it is 2^-45 and less)
+    const int up = static_cast<uint32_t>(__double2hiint(y)) < 0xc0a6a800u ? (((i >> 6) + 43) << 20) : -(1 << 30);  // (y <= -2900: 2^-45 and less)
+    const double scaled = __hiloint2double(max(__double2hiint(f) + up, 0), __double2loint(f));
+    return (scaled + kMagic) - kMagic;
 }
 
 struct Params {
@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         w.rate = 92.332482616893657 / par.temperature;  // 64 log2(e)
         w.rate32 = static_cast<float>(1.4426950408889634 / par.temperature);
     }
-    const uint64_t least = par.min_p > 0.0 ? static_cast<uint64_t>(ceil(par.min_p * 8796093022208.0)) : 1;  // 2^43 min_p
+    const double least = par.min_p > 0.0 ? ceil(par.min_p * 8796093022208.0) : 1.0;  // 2^43 min_p
+    const bool by_min = least > 1.0;
     const float u = a.uniform[row];
     // the point on the sum `all` of kept weights that the random number stands for: the first sum above it is drawn
     auto point_of = [&](uint64_t all) {
@@ -255,8 +256,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
             while (size < n) size *= 2;
             for (int i = n + threadIdx.x; i < size; i += kThreads) f.list[i] = 0;
             __syncthreads();
-            for (int k = 2; k <= size; k *= 2)
-                for (int j = k / 2; j > 0; j /= 2) {
+            // a warp keeps 32 neighbours in registers: steps within them need no barrier
+            for (int k = 2; k <= size; k *= 2) {
+                int j = k / 2;
+                for (; j >= 32; j /= 2) {
                     for (int i = threadIdx.x; i < size / 2; i += kThreads) {
                         const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
                         const uint64_t p = f.list[lo], q = f.list[hi];
@@ -264,9 +267,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                     }
                     __syncthreads();
                 }
+                if (k < 32 && k * 2 <= min(size, 32)) continue;  // (the first ones all at once, below)
+                for (int i = threadIdx.x; i < ((size + 31) & ~31); i += kThreads) {
+                    uint64_t p = i < size ? f.list[i] : 0;
+                    for (int kk = k <= 32 ? 2 : k; kk <= k; kk *= 2)
+                        for (int jj = min(j, kk / 2); jj > 0; jj /= 2) {
+                            const uint64_t q = __shfl_xor_sync(0xffffffffu, p, jj);
+                            const bool larger_first = (i & kk) == 0, is_low = (i & jj) == 0;
+                            if ((p < q) == (larger_first == is_low)) p = q;
+                        }
+                    if (i < size) f.list[i] = p;
+                }
+                __syncthreads();
+            }
             return n;
         };
-        auto weight_at = [&](int i) { return weight(w, sh.table, value_of(static_cast<uint32_t>(f.list[i] >> 32))); };
+        auto weight_at = [&](int i) { return static_cast<uint64_t>(weight(w, sh.table, value_of(static_cast<uint32_t>(f.list[i] >> 32)))); };
 
         // A logit's place in bins, 0 for the largest; the last bin takes all that is left.
         const float per_bin = kBins / kSpan * w.rate32;
@@ -283,13 +299,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
             }
             const uint32_t* bins = split > 1 ? f.bins : f.mine;
             if (warp == 0) {
-                double here[kBins / 32], sum = 0.0;
-#pragma unroll
-                for (int i = 0; i < kBins / 32; ++i) {
+                auto here = [&](int i) {
                     const int b = lane * (kBins / 32) + i;
-                    here[i] = bins[b] ? bins[b] * weigh(b) : 0.0;
-                    sum += here[i];
-                }
+                    return bins[b] ? bins[b] * weigh(b) : 0.0;
+                };
+                double sum = 0.0;
+#pragma unroll 1
+                for (int i = 0; i < kBins / 32; ++i) sum += here(i);
                 double upto = sum;
 #pragma unroll
                 for (int o = 1; o < 32; o *= 2) {
@@ -299,13 +315,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                 const double goal = goal_of(__shfl_sync(0xffffffffu, upto, 31));
                 double before = upto - sum;
                 int mine = -1, any = -1;
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < kBins / 32; ++i) {
-                    if (here[i] > 0.0) {
+                    const double mass = here(i);
+                    if (mass > 0.0) {
                         any = lane * (kBins / 32) + i;
-                        if (mine < 0 && before + here[i] >= goal) mine = any;
+                        if (mine < 0 && before + mass >= goal) mine = any;
                     }
-                    before += here[i];
+                    before += mass;
                 }
                 const uint32_t has = __ballot_sync(0xffffffffu, mine >= 0), some = __ballot_sync(0xffffffffu, any >= 0);
                 const int b = has ? __shfl_sync(0xffffffffu, mine, __ffs(has) - 1)
@@ -372,9 +389,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                 if constexpr (kByMass) {
                     uint64_t sure, in;  // sure: the thread's part of what is above the bin and passes min_p
                     while (true) {
-                        uint64_t s_all = 0, s_over = 0, s_in = 0;
+                        double s_all = 0.0, s_over = 0.0, s_in = 0.0, s_sure = 0.0;
                         uint32_t c_in = 0;
-                        sure = 0;
                         const float b0 = static_cast<float>(b), b1 = static_cast<float>(b + 1);
                         by_four([&](const float(&v)[4], uint32_t i) {
                             bool need[4], some = false;
@@ -383,32 +399,31 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                             for (int e = 0; e < 4; ++e) {
                                 need[e] = inside(v[e], i + e);
                                 c[e] = bin(v[e]);
-                                if (!kFirst) need[e] &= c[e] < b1;
+                                need[e] &= c[e] < (kFirst ? kBins - 1.0f : b1);
                                 some |= need[e];
                             }
                             if (!some) return;
-                            uint64_t m[4];
+                            double m[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) m[e] = weight(w, sh.table, v[e]);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                if (!need[e]) m[e] = 0, c[e] = kBins;
+                                if (!need[e]) continue;
                                 if (kFirst) s_all += m[e];
-                                const bool is_over = c[e] < b0, is_in = !is_over && c[e] < b1;
-                                s_over += is_over ? m[e] : 0;
-                                sure += is_over && m[e] >= least ? m[e] : 0;
-                                s_in += is_in ? m[e] : 0;
-                                c_in += is_in;
+                                if (c[e] < b0) s_over += m[e];
+                                if (by_min && c[e] < b0 && m[e] >= least) s_sure += m[e];
+                                if (c[e] >= b0 && c[e] < b1) s_in += m[e], ++c_in;
                             }
                         });
+                        sure = static_cast<uint64_t>(by_min ? s_sure : s_over);
                         uint64_t all;
                         uint32_t none;
                         if constexpr (kFirst) {
-                            sum_all(s_all, 0, all, none);
+                            sum_all(static_cast<uint64_t>(s_all), 0, all, none);
                             want = share_of * static_cast<double>(all);
                         }
-                        sum_all(s_over, 0, over, none);
-                        sum_all(s_in, c_in, in, n);
+                        sum_all(static_cast<uint64_t>(s_over), 0, over, none);
+                        sum_all(static_cast<uint64_t>(s_in), c_in, in, n);
                         // (a rough sum may have missed by a bin that holds next to nothing)
                         int next = b;
                         if (static_cast<double>(above + over) >= want) {
@@ -484,7 +499,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                     const float v = value_of(least_key);
                     uint32_t need = want_count - static_cast<uint32_t>(above);
                     if constexpr (kByMass) {
-                        const double one = static_cast<double>(weight(w, sh.table, v));
+                        const double one = weight(w, sh.table, v);
                         need = static_cast<uint32_t>(fmin(fmax(ceil((want - static_cast<double>(above)) / fmax(one, 1.0)), 1.0), 4e9));
                     }
                     need = min(need, n);
@@ -578,7 +593,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                         const uint64_t z = __shfl_up_sync(0xffffffffu, y, o);
                         if (lane >= o) y += z;
                     }
-                    const bool keep = i + lane < n && own >= least && (i + lane == 0 || static_cast<double>(before + y - own) < want);
+                    const bool keep = i + lane < n && static_cast<double>(own) >= least && (i + lane == 0 || static_cast<double>(before + y - own) < want);
                     const uint32_t who = __ballot_sync(0xffffffffu, keep);
                     m += __popc(who);
                     if (who != 0xffffffffu) {
@@ -608,18 +623,21 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     }
 
     // the draw: sums of the kept tokens, thread by thread
-    uint64_t mine = known, all = 0;
+    uint64_t all = 0;
+    double rest = 0.0;
     by_four([&](const float(&v)[4], uint32_t i) {
         bool need[4], some = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) some |= need[e] = kept(v[e], i + e) && v[e] <= settled;
         if (!some) return;
-        uint64_t m[4];
+        double m[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) m[e] = weight(w, sh.table, v[e]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mine += need[e] && m[e] >= least ? m[e] : 0;
+        for (int e = 0; e < 4; ++e)
+            if (need[e] && m[e] >= least) rest += m[e];
     });
+    const uint64_t mine = known + static_cast<uint64_t>(rest);
     uint64_t y = mine;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -642,8 +660,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         sum = __shfl_sync(0xffffffffu, sum, owner);
         for (uint32_t i = from; i < to; i += 32) {
             const float v = i + lane < to ? x[i + lane] : -INFINITY;
-            uint64_t m = kept(v, base + i + lane) ? weight(w, sh.table, v) : 0;
-            if (m < least) m = 0;
+            const double own = kept(v, base + i + lane) ? weight(w, sh.table, v) : 0.0;
+            const uint64_t m = own >= least ? static_cast<uint64_t>(own) : 0;
             uint64_t z = m;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
