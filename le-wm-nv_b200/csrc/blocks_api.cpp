@@ -381,7 +381,10 @@ lwm_status lwm_cache_attention_shared_device(lwm_ctx* ctx, const lwm_paged_cache
     LWM_TRY(on_device(ctx, c, "shared attention's prefix",
                       [&](cudaStream_t s) { return lwm::launch_cache_attention_prefix(a, plan.rows, cache->dtype, cache->storage, s); }));
     return on_device(ctx, c, "shared attention's tails",
-                     [&](cudaStream_t s) { return lwm::launch_cache_attention_tail(a, cache->dtype, cache->storage, s); });
+                     [&](cudaStream_t s) {
+                         return lwm::short_tails(a) ? lwm::launch_cache_attention_short_tail(a, cache->dtype, cache->storage, s)
+                                                    : lwm::launch_cache_attention_tail(a, cache->dtype, cache->storage, s);
+                     });
 }
 
 lwm_status lwm_gated_norm_device(lwm_ctx* ctx, const lwm_gated_norm_args* x) {

@@ -182,6 +182,8 @@ double shared_tail_cost(const CacheAttnArgs& a);
 double cache_attention_cost(const CacheAttnArgs& a);
 cudaError_t launch_cache_attention_prefix(const CacheAttnArgs& a, uint32_t block_rows, int dtype, int storage, cudaStream_t s);
 cudaError_t launch_cache_attention_tail(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
+bool short_tails(const CacheAttnArgs& a);  // which of the two kernels for tails
+cudaError_t launch_cache_attention_short_tail(const CacheAttnArgs& a, int dtype, int storage, cudaStream_t s);
 
 struct GatedNormArgs {
     lwm_gated_norm_args a;
