@@ -1139,6 +1139,7 @@ lwm_status lwm_ctx_synchronize(lwm_ctx* ctx) {
             case lwm::kStateErrStarts: return fail(LWM_INVALID_ARGUMENT, state + ": starts are out of order or beyond the packed rows (" + at + ")");
             case lwm::kStateErrNew: return fail(LWM_INVALID_ARGUMENT, state + ": more new tokens (" + at + ") than max_new");
             case lwm::kStateErrSlot: return fail(LWM_INVALID_ARGUMENT, state + ": state slot " + at + " is not in the pool");
+            case lwm::kStateErrWait: return fail(LWM_CUDA_ERROR, state + ": a pipeline wait of the kernel gave up (site " + at + ")");
             default: return fail(LWM_CUDA_ERROR, seq + ": a pipeline wait of the attention kernel gave up (site " + at + ")");
         }
     }

@@ -543,6 +543,7 @@ template <typename T> cudaError_t by_dim(const LinearArgs& a, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_linear_attention(const LinearArgs& a, int dtype, cudaStream_t s) {
+    if (linear_attention_tensor(a, dtype)) return launch_linear_attention_tc(a, s);
     return dtype == LWM_DTYPE_BF16 ? by_dim<bf16>(a, s) : by_dim<__half>(a, s);
 }
 

@@ -37,7 +37,7 @@ struct FastDiv {
 // report at once one is read whole, not one's page with another's sequence.
 constexpr int kCacheErrStarts = 1, kCacheErrNew = 2, kCacheErrLength = 3, kCacheErrPage = 4, kCacheErrWait = 5;
 constexpr int kCacheErrGroup = 6, kCacheErrShared = 7;                      // groups that share a prefix
-constexpr int kStateErrStarts = 8, kStateErrNew = 9, kStateErrSlot = 10;    // linear attention
+constexpr int kStateErrStarts = 8, kStateErrNew = 9, kStateErrSlot = 10, kStateErrWait = 11;  // linear attention
 constexpr uint32_t kCacheErrSequences = 1u << 27;  // as many as a batch may have
 struct CacheReport {
     int code;
@@ -155,6 +155,8 @@ struct LinearArgs {
 };
 constexpr uint32_t kStepTokens = 8;  // up to here the recurrent kernel
 cudaError_t launch_linear_attention(const LinearArgs& a, int dtype, cudaStream_t s);
+bool linear_attention_tensor(const LinearArgs& a, int dtype);  // which of the two kernels for longer sequences
+cudaError_t launch_linear_attention_tc(const LinearArgs& a, cudaStream_t s);
 
 struct TokenArgs {
     const void* logits;
