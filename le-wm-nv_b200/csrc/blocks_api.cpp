@@ -473,7 +473,10 @@ lwm_status lwm_linear_attention_device(lwm_ctx* ctx, const lwm_state_batch* b, c
     a.head_div = lwm::FastDiv(b->heads);
     a.group_div = lwm::FastDiv(b->heads / x->kv_heads);
     a.err = c.cache_err;
-    return on_device(ctx, c, "linear attention", [&](cudaStream_t s) { return lwm::launch_linear_attention(a, x->dtype, s); });
+    uint32_t launches = 1;
+    LWM_TRY(on_device(ctx, c, "linear attention", [&](cudaStream_t s) { return lwm::launch_linear_attention(a, x->dtype, s, &launches); }));
+    lwm::ctx_add_launches(ctx, launches - 1);
+    return LWM_OK;
 }
 
 lwm_status lwm_sample_tokens_device(lwm_ctx* ctx, const lwm_sample_tokens_args* x) {

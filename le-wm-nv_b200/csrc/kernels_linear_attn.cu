@@ -542,8 +542,11 @@ template <typename T> cudaError_t by_dim(const LinearArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t launch_linear_attention(const LinearArgs& a, int dtype, cudaStream_t s) {
-    if (linear_attention_tensor(a, dtype)) return launch_linear_attention_tc(a, s);
+cudaError_t launch_linear_attention(const LinearArgs& a, int dtype, cudaStream_t s, uint32_t* launches) {
+    bool taken = false;
+    *launches = 1;
+    const cudaError_t e = launch_linear_attention_tc(a, dtype, s, &taken, launches);
+    if (taken || e != cudaSuccess) return e;
     return dtype == LWM_DTYPE_BF16 ? by_dim<bf16>(a, s) : by_dim<__half>(a, s);
 }
 

@@ -1,31 +1,39 @@
 // kernels_linear_attn_tc.cu — linear attention with decay over whole histories
 // of bf16 on the tcgen05 tensor cores (lwm_linear_attention_device).
 //
-// A block takes a sequence and head (or, of few long ones, a part along time,
-// the parts of a sequence in a cluster) in chunks of 128 tokens:
+// A block takes a sequence and head, or, of few long ones, a part along time,
+// in chunks of 128 tokens:
 //   P  = Q K^T                     (TMEM), times lambda^(i-j) where j <= i, to bf16 in place
 //   O1 = Q S, O2 = P V             (TMEM), out = scale (lambda^(i+1) O1 + O2)
 //   S  = lambda^m S + K'^T V       (TMEM, 32 bits; a bf16 copy in shared memory for O1)
 // with K' = lambda^(m-1-j) k_j in three parts of 8 bits, so that S keeps them
 // as 32-bit products would.
 //
-// Warpgroups: outputs (a token a thread: P, O1, O2), two for the state (a key
-// channel a thread, half of the value channels: K' 64 tokens at a time, the
-// first part in place of K once P is done, S between its two uses), and one
-// that loads (cp.async: rows behind the sequence's end are zeros).  K and V
-// have two stages, Q is loaded again as soon as both its products are done.
-// All tiles are rows of 64 channels (128 bytes, 128-byte swizzle); K' is an
-// M-major A operand, V and S N-major B operands of that layout.  64 channels
-// have a second half of K' that is zero, as an A operand of 128 rows wants.
+// Warps: four for the outputs (a token a thread: P, O1, O2), eight for the
+// state (a key channel a thread, half of the value channels: K' some tokens at
+// a time, computed while the product before it runs, then S), one that loads
+// by TMA, and an issuer of products for each of the two chains.  K and V have
+// two stages, Q is loaded again as soon as both its products are done.  All
+// tiles are rows of 64 channels (128 bytes, 128-byte swizzle); K' is an M-major
+// A operand, V and S N-major B operands of that layout.  64 channels have a
+// second half of K' that is zero, as an A operand of 128 rows wants.
 //
-// Infinities and NaN among the values are taken out of the tiles and added
-// where they belong, one by one.  Every wait is bounded: one that gives up
-// marks the block, which unwinds.
-#include <cooperative_groups.h>
-
+// Parts: a first launch walks them for the state alone, each from zero, a
+// second one turns what they add into the states before them, and a third one
+// walks them for the outputs.  In between, a part's state (32 bits) lies in the
+// rows of `out` that are the part's own, where nothing is kept yet; so no part is
+// shorter than that many rows, and a call whose out overlaps its inputs is not
+// cut.
+//
+// Rows behind the sequence's end are another's: their keys weigh zero, their
+// values are zeroed.  Infinities and NaN among the values make outputs that
+// are not finite, also of tokens that do not see them; such rows are computed
+// again, term by term.  Every wait is bounded: one that gives up marks the
+// block, which unwinds.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "lwm_linear_attn.cuh"
 #include "lwm_tc.cuh"
@@ -34,29 +42,30 @@ namespace lwm {
 
 namespace {
 
-namespace cg = cooperative_groups;
-
-constexpr int kChunk = 128, kHalf = 64;
-constexpr int kThreads = 512, kOut = 128, kState = 256, kLoad = 128;
-constexpr uint32_t kMostParts = 16;
+constexpr int kChunk = 128;
+constexpr int kThreads = 480, kOut = 128, kState = 256;
+constexpr int kLoadWarp = 12, kStateIssuer = 13, kOutIssuer = 14;
+constexpr uint32_t kMostParts = 64;
+// What a launch does: the whole, the state that a part adds, or the outputs of a part.
+constexpr int kWhole = 0, kAdds = 1, kGoesOn = 2;
 constexpr uint32_t kPCol = 0, kO1Col = 128;
 
 template <int D> struct Shape {
     static constexpr int kPanels = D / 64;
     static constexpr int kTile = kPanels * kChunk * 128;    // bytes of 128 tokens
-    static constexpr int kPart = kPanels * kHalf * 128;     // of 64
+    static constexpr int kRound = D == 64 ? 64 : 32;        // tokens whose K' is there at once
+    static constexpr int kPart = kPanels * kRound * 128;    // of a part of it
     static constexpr int kS = D * D * 2;
-    static constexpr int kQ = 0, kK = kTile, kV = kK + 2 * kTile, kMid = kV + 2 * kTile, kLow = kMid + kPart, kSAt = kLow + kPart;
+    static constexpr int kQ = 0, kK = kTile, kV = kK + 2 * kTile, kParts = kV + 2 * kTile, kSAt = kParts + 3 * kPart;
     static constexpr int kZero = kSAt + kS;                 // 64 channels: the empty half of K'
-    static constexpr int kBytes = kZero + (D == 64 ? kHalf * 128 : 0) + 1024;  // + alignment
+    static constexpr int kBytes = kZero + (D == 64 ? kRound * 128 : 0) + 1024;  // + alignment
     static constexpr uint32_t kO2Col = kO1Col + D, kSCol = kO2Col + D;
 };
 
 struct Control {
-    uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], scores[2], between, pv, s_full, kv, drain;
+    uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], v_raw, scores, weights, between, pv, o_free, parts, kv, s_copy, drain;
     uint32_t tmem;
     int dead;     // a wait gave up
-    int bad[4];   // infinities or NaN were taken out of a V tile (four, as a flag is read after the tile may be free)
     float power[kChunk + 1];  // lambda^i
 };
 
@@ -70,33 +79,86 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Control* c,
     if (atomicExch(&c->dead, 1) == 0) cache_report(err, kStateErrWait, seq, site);
     return false;
 }
-__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-// Whether any thread of a group says so: a group goes on, or gives up, as one, so that none waits for another there.
-__device__ __forceinline__ bool named_any(int id, int threads, bool x) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, %3, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(r)
-        : "r"(static_cast<uint32_t>(x)), "r"(id), "r"(threads)
-        : "memory");
-    return r != 0;
-}
-
 // kind::f16 of bf16 with f32 accumulation, M 128: operands K-major, or transposed (bits 15 and 16).
 __host__ __device__ constexpr uint32_t idesc(uint32_t n, bool a_turned, bool b_turned) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((a_turned ? 1u : 0u) << 15) | ((b_turned ? 1u : 0u) << 16) | ((n >> 3) << 17) |
            ((128u >> 4) << 24);
 }
-// Descriptor of a tile: start, distance of its panels of 64 channels.
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t panel) { return tc::smem_desc(addr, panel, 1024, tc::kSwizzle128); }
+// Descriptors: the low word holds the start and the distance of the panels of 64 channels (in 16 bytes), the high one
+// is a constant (8-row groups 1024 bytes apart, 128-byte swizzle).
+constexpr uint32_t kHigh = (1024u >> 4) | (1u << 14) | (tc::kSwizzle128 << 29);
+__device__ __forceinline__ uint32_t low_desc(uint32_t addr, uint32_t panel) { return (addr >> 4) | ((panel >> 4) << 16); }
+// Two K = 16 steps by a whole warp (one elected lane), the second's operands at fixed distances: issued one by one, a
+// step costs the warp about 100 cycles for its descriptors.
+__device__ __forceinline__ void mma2(uint32_t d, uint32_t al, uint32_t a_step, uint32_t bl, uint32_t b_step, uint32_t id, uint32_t more) {
+    asm volatile(
+        "{\n\t.reg .pred e, m;\n\t.reg .b32 a2, b2;\n\t.reg .b64 x, y;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 m, %7, 0;\n\t"
+        "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%3, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %6, m;\n\t"
+        "add.u32 a2, %1, %2;\n\tadd.u32 b2, %3, %4;\n\tmov.b64 x, {a2, %5};\n\tmov.b64 y, {b2, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %6, 1;\n\t}\n" ::"r"(d),
+        "r"(al), "r"(a_step), "r"(bl), "r"(b_step), "r"(kHigh), "r"(id), "r"(more)
+        : "memory");
+}
+// The same with A in TMEM (8 columns a step).
+__device__ __forceinline__ void mma2_t(uint32_t d, uint32_t at, uint32_t bl, uint32_t b_step, uint32_t id, uint32_t more) {
+    asm volatile(
+        "{\n\t.reg .pred e, m;\n\t.reg .b32 a2, b2;\n\t.reg .b64 y;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 m, %6, 0;\n\t"
+        "mov.b64 y, {%2, %4};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %5, m;\n\t"
+        "add.u32 a2, %1, 8;\n\tadd.u32 b2, %2, %3;\n\tmov.b64 y, {b2, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], y, %5, 1;\n\t}\n" ::"r"(d),
+        "r"(at), "r"(bl), "r"(b_step), "r"(kHigh), "r"(id), "r"(more)
+        : "memory");
+}
+// 64 channels of 128 rows of a head to shared memory (no multicast).
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int channel, int head, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(map), "r"(tc::smem_u32(bar)), "r"(channel), "r"(head), "r"(row)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
 
 // Offset of 16-byte chunk c of row r of a tile whose panels have `rows` rows.
 __device__ __forceinline__ uint32_t chunk_at(uint32_t r, uint32_t c, uint32_t rows) {
     return (c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, 1) linear_tc_kernel(const __grid_constant__ LinearArgs a, uint32_t parts) {
+// The part of a sequence's chunks that one of `parts` blocks has: `per` of them, the last part what is left, and
+// another 2 D - 1 tokens at most, so that each part has rows of `out` for a state.
+struct Part {
+    uint32_t chunks, first, end, count;  // of the sequence; chunks of this part; parts with tokens
+};
+__host__ __device__ __forceinline__ uint32_t chunks_a_part(uint32_t max_new, uint32_t parts) {
+    return ((max_new + kChunk - 1) / kChunk + parts - 1) / parts;
+}
+__device__ __forceinline__ Part part_of(uint32_t n, uint32_t per, uint32_t parts, uint32_t rank, uint32_t d) {
+    Part p;
+    const uint32_t tokens = per * kChunk, full = n / tokens, rest = n - full * tokens;
+    p.chunks = (n + kChunk - 1) / kChunk;
+    p.count = parts == 1 ? 1 : max(1u, rest >= 2 * d ? full + 1 : full);
+    p.first = rank < p.count ? rank * per : p.chunks;
+    p.end = rank + 1 < p.count ? p.first + per : p.chunks;
+    return p;
+}
+// Element i of a part's state in the rows of `out` from `row` on.
+template <int D> __device__ __forceinline__ float* stash(const LinearArgs& a, size_t row, uint32_t h, uint32_t i) {
+    return reinterpret_cast<float*>(static_cast<bf16*>(a.out) + (row + i / (D / 2)) * a.o_ts + h * a.o_hs) + i % (D / 2);
+}
+
+template <int D, int kMode>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_tc_kernel(const __grid_constant__ LinearArgs a, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                     const __grid_constant__ CUtensorMap v_map, uint32_t per, uint32_t parts) {
     using S = Shape<D>;
     constexpr int kSteps = D / 16, kRowChunks = D / 8;
     extern __shared__ uint8_t smem_raw[];
@@ -104,38 +166,39 @@ __global__ void __launch_bounds__(kThreads, 1) linear_tc_kernel(const __grid_con
     Control* const ctl = &ctl_s;
     uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
     const uint32_t base = tc::smem_u32(smem);
-    const int warp = threadIdx.x >> 5;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x % parts, job = blockIdx.x / parts;
     const uint32_t s = a.head_div.div(job), h = job - s * a.heads;
-    const StateView v = state_view(a, s, h == 0 && rank == 0 && threadIdx.x == 0);
-    if (!v.ok) return;  // (the same in a whole cluster)
+    const StateView v = state_view(a, s, kMode != kGoesOn && h == 0 && rank == 0 && threadIdx.x == 0);
+    if (!v.ok) return;
+    const Part part = part_of(v.n, per, parts, rank, D);
+    const uint32_t chunks = part.chunks, first = part.first, end = part.end;
+    if (rank >= part.count || (kMode == kAdds && rank + 1 == part.count)) return;
     const uint32_t hk = a.group_div.div(h);
     float decay = a.log_decay[h];
     if (decay < -200.0f) decay = -200.0f;  // (e^-200 is zero; minus infinity times zero would be NaN)
-    const uint32_t chunks = (v.n + kChunk - 1) / kChunk, per = (chunks + parts - 1) / parts;
-    const uint32_t first = min(rank * per, chunks), end = min(first + per, chunks);
 
     if (threadIdx.x == 0) {
-        tc::mbar_init(&ctl->q_full, kLoad);
-        tc::mbar_init(&ctl->q_empty, 1);
+        tc::mbar_init(&ctl->q_full, 1);
+        tc::mbar_init(&ctl->q_empty, 2);
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(&ctl->k_full[i], kLoad);
-            tc::mbar_init(&ctl->v_full[i], kLoad);
-            tc::mbar_init(&ctl->k_empty[i], 1);
+            tc::mbar_init(&ctl->k_full[i], 1);
+            tc::mbar_init(&ctl->v_full[i], 1);
+            tc::mbar_init(&ctl->k_empty[i], 1 + kState);
             tc::mbar_init(&ctl->v_empty[i], 2);
-            tc::mbar_init(&ctl->scores[i], 1);
         }
-        tc::mbar_init(&ctl->between, 1);
-        tc::mbar_init(&ctl->s_full, kState);
-        tc::mbar_init(&ctl->kv, 1);
-        tc::mbar_init(&ctl->pv, 1);
+        for (uint64_t* b : {&ctl->v_raw, &ctl->scores, &ctl->between, &ctl->pv, &ctl->kv}) tc::mbar_init(b, 1);
+        tc::mbar_init(&ctl->weights, kOut);
+        tc::mbar_init(&ctl->o_free, kOut);
+        tc::mbar_init(&ctl->parts, kState);
+        tc::mbar_init(&ctl->s_copy, kState);
         tc::mbar_init(&ctl->drain, 2);
         ctl->dead = 0;
         tc::mbar_fence_init();
     }
     for (int i = threadIdx.x; i <= kChunk; i += kThreads) ctl->power[i] = expf(decay * i);
     if constexpr (D == 64)
-        for (int i = threadIdx.x; i < kHalf * 8; i += kThreads) *reinterpret_cast<uint4*>(smem + S::kZero + i * 16) = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < S::kRound * 8; i += kThreads) *reinterpret_cast<uint4*>(smem + S::kZero + i * 16) = make_uint4(0, 0, 0, 0);
     tc::fence_async_smem();
     if (warp == 0) tc::tmem_alloc(&ctl->tmem, 512);
     tc::fence_before();
@@ -150,58 +213,46 @@ __global__ void __launch_bounds__(kThreads, 1) linear_tc_kernel(const __grid_con
     auto row_at = [&](uint32_t i) { return static_cast<size_t>(v.start) + i * kChunk; };
 
     // ------------------------------------------------------------ loads
-    // One tile of the chunk's rows into `to`; the caller commits.
-    auto load = [&](const bf16* src, size_t stride, uint32_t i, uint32_t to) {
-        const int t = threadIdx.x - kOut - kState;
-        const uint32_t m = tokens_of(i);
-#pragma unroll 4
-        for (int c = 0; c < kChunk * kRowChunks / kLoad; ++c) {
-            const uint32_t x = c * kLoad + t, r = x / kRowChunks, ch = x % kRowChunks;
-            const bool live = r < m;
-            cp_async16(to + chunk_at(r, ch, kChunk), src + (row_at(i) + (live ? r : 0)) * stride + 8 * ch, live);
-        }
-    };
-    auto loads = [&](bool whole, uint32_t from, uint32_t& use) {
-        // use: chunks that the rings have seen before
+    auto loads = [&] {
+        constexpr bool whole = kMode != kAdds;
+        const uint32_t from = first;
+        uint32_t use = 0;
         bool fine = true;
-        const int t = threadIdx.x - kOut - kState;
-        for (uint32_t i = from; i < end && fine; ++i, ++use) {
-            const uint32_t st = use & 1, round = use >> 1;
-            if (use >= 2) fine = wait(&ctl->k_empty[st], (round - 1) & 1, ctl, 1, err, s);
-            if (fine) load(k_at, a.k_ts, i, base + S::kK + st * S::kTile);
-            cp_commit();
-            if (fine && use >= 2) fine = wait(&ctl->v_empty[st], (round - 1) & 1, ctl, 2, err, s);
-            if (fine) load(v_at, a.v_ts, i, base + S::kV + st * S::kTile);
-            cp_commit();
-            if (fine && whole && i > from) fine = wait(&ctl->q_empty, (i - from - 1) & 1, ctl, 3, err, s);
-            if (fine && whole) load(q_at, a.q_ts, i, base + S::kQ);
-            cp_commit();
-            cp_wait<2>();
-            tc::fence_async_smem();
-            if (fine) tc::mbar_arrive(&ctl->k_full[st]);
-            cp_wait<1>();
-            if (t == 0) ctl->bad[use & 3] = 0;
-            named_sync(3, kLoad);
-            if (fine) {
-#pragma unroll 4
-                for (int c = 0; c < kChunk * kRowChunks / kLoad; ++c) {
-                    const uint32_t x = c * kLoad + t;
-                    uint4* at = reinterpret_cast<uint4*>(smem + S::kV + st * S::kTile + chunk_at(x / kRowChunks, x % kRowChunks, kChunk));
-                    uint4 y = *at;
-                    if (not_finite2<bf16>(y.x) | not_finite2<bf16>(y.y) | not_finite2<bf16>(y.z) | not_finite2<bf16>(y.w)) {
-                        ctl->bad[use & 3] = 1;
-                        *at = make_uint4(finite2<bf16>(y.x), finite2<bf16>(y.y), finite2<bf16>(y.z), finite2<bf16>(y.w));
-                    }
-                }
-                tc::fence_async_smem();
-                tc::mbar_arrive(&ctl->v_full[st]);
+        auto tile = [&](const CUtensorMap* map, uint32_t head, uint32_t i, uint32_t to, uint64_t* bar) {
+            if (lane == 0) {
+                tc::mbar_expect_tx(bar, S::kTile);
+#pragma unroll
+                for (int p = 0; p < S::kPanels; ++p) tma_rows(to + p * kChunk * 128, map, 64 * p, head, static_cast<int>(row_at(i)), bar);
             }
-            cp_wait<0>();
-            tc::fence_async_smem();
-            if (fine && whole) tc::mbar_arrive(&ctl->q_full);
-            fine = !named_any(3, kLoad, !fine);
+            __syncwarp();
+        };
+        for (uint32_t i = from; i < end && fine; ++i, ++use) {
+            const uint32_t st = use & 1, round = use >> 1, m = tokens_of(i);
+            if (use >= 2) fine = wait(&ctl->k_empty[st], (round - 1) & 1, ctl, 1, err, s);
+            if (!fine) break;
+            tile(&k_map, hk, i, base + S::kK + st * S::kTile, &ctl->k_full[st]);
+            if (whole) {
+                if (i > from) fine = wait(&ctl->q_empty, (i - from - 1) & 1, ctl, 3, err, s);
+                if (!fine) break;
+                tile(&q_map, h, i, base + S::kQ, &ctl->q_full);
+            }
+            if (use >= 2) fine = wait(&ctl->v_empty[st], (round - 1) & 1, ctl, 2, err, s);
+            if (!fine) break;
+            const uint32_t v_a = S::kV + st * S::kTile;
+            tile(&v_map, hk, i, base + v_a, m == kChunk ? &ctl->v_full[st] : &ctl->v_raw);
+            if (m < kChunk) {  // (the sequence's last chunk) rows behind it
+                fine = wait(&ctl->v_raw, 0, ctl, 4, err, s);
+                if (!fine) break;
+                for (uint32_t x = m * kRowChunks + lane; x < kChunk * kRowChunks; x += 32)
+                    *reinterpret_cast<uint4*>(smem + v_a + chunk_at(x / kRowChunks, x % kRowChunks, kChunk)) = make_uint4(0, 0, 0, 0);
+                tc::fence_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&ctl->v_full[st]);
+            }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
+        // a block that gave up: its boxes in flight land long before this
+        if (!fine)
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     };
 
     // ------------------------------------------------------------ state
@@ -219,203 +270,247 @@ __global__ void __launch_bounds__(kThreads, 1) linear_tc_kernel(const __grid_con
             *reinterpret_cast<uint4*>(smem + S::kSAt + chunk_at(row, (col0 + c) / 8 + b, D)) = pack<bf16>(f).a;
         }
     };
-    // The state's steps over the chunks from `from` on (TMEM holds it, times the first chunk's decay).  whole: beside
-    // the outputs, else alone.
-    auto states = [&](bool whole, uint32_t from, uint32_t& use, uint32_t& kv_use, float* final_state) {
-        bool fine = true;
-        for (uint32_t i = from; i < end && fine; ++i, ++use) {
-            const uint32_t st = use & 1, round = use >> 1, m = tokens_of(i);
-            uint8_t* const kt = smem + S::kK + st * S::kTile;
-            const uint32_t v_a = base + S::kV + st * S::kTile;
-            fine = wait(&ctl->k_full[st], round & 1, ctl, 10, err, s);
-            if (fine && whole) fine = wait(&ctl->scores[(i - from) & 1], ((i - from) >> 1) & 1, ctl, 11, err, s);  // K is read: its place may change
-            if (fine) fine = wait(&ctl->v_full[st], round & 1, ctl, 12, err, s);
-            const uint32_t halves = m > kHalf ? 2 : 1;
-            for (uint32_t half = 0; half < halves; ++half) {
-                if (fine) {
+    // The state's steps (TMEM holds it, times the first chunk's decay).  The parts of K' are computed while the products
+    // before them run.
+    auto states = [&](float* final_state) {
+        constexpr bool whole = kMode != kAdds;
+        const uint32_t from = first;
+        uint32_t use = 0, kv_use = 0;
+        constexpr int kMine = S::kRound * kRowChunks / kState;  // 16-byte chunks of a round
+        uint4 part[3][kMine];
+        auto split = [&](uint32_t i, uint32_t st, uint32_t round) {
+            const uint32_t m = tokens_of(i);
 #pragma unroll
-                for (int c = 0; c < kHalf * kRowChunks / kState; ++c) {
-                    const uint32_t x = c * kState + t_state, r = x / kRowChunks, ch = x % kRowChunks;
-                    const uint32_t tok = half * kHalf + r;
-                    const float w = tok < m ? ctl->power[m - 1 - tok] : 0.0f;
-                    uint4* const at = reinterpret_cast<uint4*>(kt + chunk_at(tok, ch, kChunk));
-                    float f[8], g[8];
-                    unpack(Vec8<bf16>{*at}, f);
-                    Vec8<bf16> part[3];
+            for (int c = 0; c < kMine; ++c) {
+                const uint32_t x = c * kState + t_state, tok = round * S::kRound + x / kRowChunks;
+                float f[8], g[8];
+                unpack(Vec8<bf16>{*reinterpret_cast<const uint4*>(smem + S::kK + st * S::kTile + chunk_at(tok, x % kRowChunks, kChunk))}, f);
+                const float w = ctl->power[tok < m ? m - 1 - tok : 0];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] *= w;
+                for (int e = 0; e < 8; ++e) f[e] = tok < m ? f[e] * w : 0.0f;
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        part[p] = pack<bf16>(f);
-                        unpack(part[p], g);
+                for (int p = 0; p < 3; ++p) {
+                    const Vec8<bf16> y = pack<bf16>(f);
+                    part[p][c] = y.a;
+                    unpack(y, g);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] -= g[e];
-                    }
-                    *at = part[0].a;
-                    *reinterpret_cast<uint4*>(smem + S::kMid + chunk_at(r, ch, kHalf)) = part[1].a;
-                    *reinterpret_cast<uint4*>(smem + S::kLow + chunk_at(r, ch, kHalf)) = part[2].a;
+                    for (int e = 0; e < 8; ++e) f[e] -= g[e];
                 }
+            }
+            if ((round + 1) * S::kRound >= m) {  // K has been read
+                tc::mbar_arrive(&ctl->k_empty[st]);
+                if (!whole && t_state == 0) tc::mbar_arrive(&ctl->k_empty[st]);  // (as the products with Q say otherwise)
+            }
+        };
+        bool fine = wait(&ctl->k_full[use & 1], (use >> 1) & 1, ctl, 10, err, s);
+        if (fine) split(from, use & 1, 0);
+        for (uint32_t i = from; i < end && fine; ++i, ++use) {
+            const uint32_t st = use & 1, m = tokens_of(i), rounds = (m + S::kRound - 1) / S::kRound;
+            const bool more = i + 1 < end;
+            for (uint32_t round = 0; round < rounds && fine; ++round) {
+#pragma unroll
+                for (int c = 0; c < kMine; ++c) {
+                    const uint32_t x = c * kState + t_state;
+#pragma unroll
+                    for (int p = 0; p < 3; ++p)
+                        *reinterpret_cast<uint4*>(smem + S::kParts + p * S::kPart + chunk_at(x / kRowChunks, x % kRowChunks, S::kRound)) = part[p][c];
                 }
                 tc::fence_async_smem();
                 tc::fence_before();  // (the state's stores, too)
-                fine = !named_any(2, kState, !fine);
-                if (warp == 4 && fine) {
-                    tc::fence_after();
-                    constexpr uint32_t kI = idesc(D, true, true);
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        const uint32_t from_a = p == 0 ? base + S::kK + st * S::kTile + half * kHalf * 128 : base + (p == 1 ? S::kMid : S::kLow);
-                        const uint32_t panel = D == 64 ? base + S::kZero - from_a : (p == 0 ? kChunk : kHalf) * 128;
-#pragma unroll
-                        for (int k = 0; k < kHalf / 16; ++k)
-                            tc::mma_bf16_w(tmem + S::kSCol, tile_desc(from_a + k * 2048, panel),
-                                           tile_desc(v_a + half * kHalf * 128 + k * 2048, kChunk * 128), kI, 1);
-                    }
-                    tc::commit_w(&ctl->kv);
-                    if (half + 1 == halves) {
-                        tc::commit_w(&ctl->k_empty[st]);
-                        tc::commit_w(&ctl->v_empty[st]);
-                        if (!whole) tc::commit_w(&ctl->v_empty[st]);
-                    }
-                    __syncwarp();
+                tc::mbar_arrive(&ctl->parts);
+                if (round + 1 < rounds) {
+                    split(i, st, round + 1);
+                } else if (more) {
+                    fine = wait(&ctl->k_full[st ^ 1], ((use + 1) >> 1) & 1, ctl, 10, err, s);
+                    if (fine) split(i + 1, st ^ 1, 0);
                 }
                 if (fine) fine = wait(&ctl->kv, kv_use & 1, ctl, 13, err, s);
                 ++kv_use;
             }
-            tc::fence_after();
-            // its bf16 copy's last reader is the product of this chunk
+            // the bf16 copy's last reader is the product of this chunk
             if (fine && whole) fine = wait(&ctl->between, (i - from) & 1, ctl, 14, err, s);
-            const bool more = i + 1 < end;
+            if (!fine) break;
+            tc::fence_after();
             const float fade = more ? expm1f(decay * tokens_of(i + 1)) : 0.0f;
-            const bool bad = *static_cast<volatile int*>(&ctl->bad[use & 3]) != 0;
-            if (has_row && fine) {
-#pragma unroll 1
-                for (int c = 0; c < D / 2; c += 16) {
-                    float x[16];
-                    tc::tmem_ld16(t_lane + S::kSCol + col0 + c, x);
+            if (has_row) {
+#pragma unroll
+                for (int c = 0; c < D / 2; c += 32) {
+                    float x[32];
+                    tmem_ld32(t_lane + S::kSCol + col0 + c, x);
                     tc::tmem_ld_wait();
-                    if (bad)
-                        for (uint32_t j = 0; j < m; ++j)
-                            for (int e = 0; e < 16; ++e) {
-                                const float y = static_cast<float>(v_at[(row_at(i) + j) * a.v_ts + col0 + c + e]);
-                                if (!isfinite(y)) x[e] += static_cast<float>(k_at[(row_at(i) + j) * a.k_ts + row]) * ctl->power[m - 1 - j] * y;
-                            }
-                    if (whole && more) copy16(c, x);
-                    if (final_state && !more) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4)
-                            *reinterpret_cast<float4*>(final_state + static_cast<size_t>(row) * D + col0 + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-                    }
-                    if (more || !whole) {
+                    for (int b = 0; b < 32; b += 16) {
+                        float(&y)[16] = *reinterpret_cast<float(*)[16]>(x + b);
+                        if (whole && more) copy16(c + b, y);
+                        if (final_state && !more) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) x[e] = fmaf(x[e], fade, x[e]);
-                        tc::tmem_st16(t_lane + S::kSCol + col0 + c, x);
+                            for (int e = 0; e < 16; e += 4)
+                                *reinterpret_cast<float4*>(final_state + static_cast<size_t>(row) * D + col0 + c + b + e) =
+                                    make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                        }
+                        if (more || !whole) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) y[e] = fmaf(y[e], fade, y[e]);
+                            tc::tmem_st16(t_lane + S::kSCol + col0 + c + b, y);
+                        }
                     }
                 }
                 tc::tmem_st_wait();
             }
             tc::fence_before();
             tc::fence_async_smem();
-            if (whole && more && fine) tc::mbar_arrive(&ctl->s_full);
-            fine = !named_any(2, kState, !fine);
+            if (whole && more) tc::mbar_arrive(&ctl->s_copy);
+        }
+    };
+    // The state's products: O1 = Q S of a chunk, then K'^T V of it in rounds.
+    auto state_products = [&] {
+        constexpr bool whole = kMode != kAdds;
+        const uint32_t from = first;
+        uint32_t use = 0, parts_use = 0;
+        constexpr uint32_t kI = idesc(D, true, true), kB = idesc(D, false, true);
+        bool fine = true;
+        for (uint32_t i = from; i < end && fine; ++i, ++use) {
+            const uint32_t st = use & 1, m = tokens_of(i), rounds = (m + S::kRound - 1) / S::kRound;
+            if (whole) {
+                fine = wait(&ctl->s_copy, (i - from) & 1, ctl, 17, err, s) && wait(&ctl->q_full, (i - from) & 1, ctl, 15, err, s);
+                if (fine && i > from) fine = wait(&ctl->o_free, (i - from - 1) & 1, ctl, 16, err, s);
+                if (!fine) break;
+                tc::fence_after();
+#pragma unroll
+                for (int k = 0; k < kSteps; k += 2)
+                    mma2(tmem + kO1Col, low_desc(base + S::kQ + (k >> 2) * kChunk * 128 + (k & 3) * 32, 16), 2,
+                         low_desc(base + S::kSAt + k * 2048, D * 128), 128, kB, k > 0);
+                tc::commit_w(&ctl->between);
+                tc::commit_w(&ctl->q_empty);
+            }
+            fine = wait(&ctl->v_full[st], (use >> 1) & 1, ctl, 12, err, s);
+            for (uint32_t round = 0; round < rounds && fine; ++round) {
+                fine = wait(&ctl->parts, parts_use++ & 1, ctl, 18, err, s);
+                if (!fine) break;
+                tc::fence_after();
+                const uint32_t v_a = base + S::kV + st * S::kTile + round * S::kRound * 128;
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    const uint32_t k_a = base + S::kParts + p * S::kPart, panel = D == 64 ? base + S::kZero - k_a : S::kRound * 128;
+#pragma unroll
+                    for (int k = 0; k < S::kRound / 16; k += 2)
+                        mma2(tmem + S::kSCol, low_desc(k_a + k * 2048, panel), 128, low_desc(v_a + k * 2048, kChunk * 128), 128, kI, 1);
+                }
+                tc::commit_w(&ctl->kv);
+            }
+            if (!fine) break;
+            tc::commit_w(&ctl->v_empty[st]);
+            if (!whole) tc::commit_w(&ctl->v_empty[st]);
         }
     };
 
     // ---------------------------------------------------------- outputs
-    auto outputs = [&](uint32_t from, uint32_t use) {
+    auto out_products = [&] {
+        const uint32_t from = first;
+        uint32_t use = 0;
+        constexpr uint32_t kP = idesc(kChunk, false, false), kO = idesc(D, false, true);
+        bool fine = true;
+        auto scores = [&](uint32_t i, uint32_t u) {
+            const uint32_t st = u & 1;
+            fine = wait(&ctl->q_full, (i - from) & 1, ctl, 20, err, s) && wait(&ctl->k_full[st], (u >> 1) & 1, ctl, 21, err, s);
+            if (!fine) return;
+            tc::fence_after();
+#pragma unroll
+            for (int k = 0; k < kSteps; k += 2) {
+                const uint32_t off = (k >> 2) * kChunk * 128 + (k & 3) * 32;
+                mma2(tmem + kPCol, low_desc(base + S::kQ + off, 16), 2, low_desc(base + S::kK + st * S::kTile + off, 16), 2, kP, k > 0);
+            }
+            tc::commit_w(&ctl->scores);
+            tc::commit_w(&ctl->q_empty);
+            tc::commit_w(&ctl->k_empty[st]);
+        };
+        scores(from, use);
+        for (uint32_t i = from; i < end && fine; ++i, ++use) {
+            const uint32_t st = use & 1;
+            fine = wait(&ctl->v_full[st], (use >> 1) & 1, ctl, 24, err, s) && wait(&ctl->weights, (i - from) & 1, ctl, 27, err, s);
+            if (fine && i > from) fine = wait(&ctl->o_free, (i - from - 1) & 1, ctl, 28, err, s);
+            if (!fine) break;
+            tc::fence_after();
+#pragma unroll
+            for (int k = 0; k < kChunk / 16; k += 2)
+                mma2_t(tmem + S::kO2Col, tmem + kPCol + 8 * k, low_desc(base + S::kV + st * S::kTile + k * 2048, kChunk * 128), 128, kO, k > 0);
+            tc::commit_w(&ctl->v_empty[st]);
+            tc::commit_w(&ctl->pv);
+            if (i + 1 < end) scores(i + 1, use + 1);  // (over the weights, which the product before it has read)
+        }
+    };
+    auto outputs = [&] {
+        const uint32_t from = first;
         const uint32_t r = threadIdx.x;  // token of the chunk
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
         bool fine = true;
-        const uint32_t q_a = base + S::kQ, s_a = base + S::kSAt;
-        for (uint32_t i = from; i < end && fine; ++i, ++use) {
-            const uint32_t st = use & 1, round = use >> 1, m = tokens_of(i), turn = (i - from) & 1;
-            const uint32_t k_a = base + S::kK + st * S::kTile, v_a = base + S::kV + st * S::kTile;
-            if (warp == 0) {
-                fine = wait(&ctl->q_full, turn, ctl, 20, err, s) && wait(&ctl->k_full[st], round & 1, ctl, 21, err, s);
-                if (fine) {
-                    tc::fence_after();
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        const uint32_t off = (k >> 2) * kChunk * 128 + (k & 3) * 32;
-                        tc::mma_bf16_w(tmem + kPCol, tile_desc(q_a + off, 16), tile_desc(k_a + off, 16), idesc(kChunk, false, false), k > 0);
-                    }
-                    tc::commit_w(&ctl->scores[turn]);
-                    fine = wait(&ctl->s_full, turn, ctl, 22, err, s);
-                }
-                if (fine) {
-                    tc::fence_after();
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        const uint32_t off = (k >> 2) * kChunk * 128 + (k & 3) * 32;
-                        tc::mma_bf16_w(tmem + kO1Col, tile_desc(q_a + off, 16), tile_desc(s_a + k * 2048, D * 128), idesc(D, false, true), k > 0);
-                    }
-                    tc::commit_w(&ctl->between);
-                    tc::commit_w(&ctl->q_empty);
-                }
-            }
-            if (fine) fine = wait(&ctl->scores[turn], ((i - from) >> 1) & 1, ctl, 23, err, s);
+        for (uint32_t i = from; i < end && fine; ++i) {
+            const uint32_t m = tokens_of(i), turn = (i - from) & 1;
+            fine = wait(&ctl->scores, turn, ctl, 23, err, s);
+            if (!fine) break;
             tc::fence_after();
             // weights: what a token does not see is zero
 #pragma unroll 1
-            for (int c = 0; c < kChunk; c += 16) {
-                uint32_t p[8];
-                if (c > warp * 32 + 31) {  // none of the warp's tokens
+            for (int c = 0; c < kChunk; c += 32) {
+                uint32_t p[16];
+                if (c > warp * 32) {  // none of the warp's tokens
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = 0u;
-                    tc::tmem_st8u(lanes + kPCol + c / 2, p);
-                    continue;
+                    for (int e = 0; e < 16; ++e) p[e] = 0u;
+                } else {
+                    float x[32];
+                    tmem_ld32(lanes + kPCol + c, x);
+                    tc::tmem_ld_wait();
+                    const float* const w = ctl->power + (r - c);
+                    if (c < warp * 32) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] *= w[-e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = e <= lane ? x[e] * w[e <= lane ? -e : 0] : 0.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) p[e] = pack2(x[2 * e], x[2 * e + 1], bf16{});
                 }
-                float x[16];
-                tc::tmem_ld16(lanes + kPCol + c, x);
-                tc::tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int apart = static_cast<int>(r) - (c + e);
-                    const float w = ctl->power[max(apart, 0)];
-                    x[e] = apart >= 0 ? x[e] * w : 0.0f;
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = pack2(x[2 * e], x[2 * e + 1], bf16{});
-                tc::tmem_st8u(lanes + kPCol + c / 2, p);
+                tc::tmem_st8u(lanes + kPCol + c / 2, reinterpret_cast<const uint32_t(&)[8]>(p[0]));
+                tc::tmem_st8u(lanes + kPCol + c / 2 + 8, reinterpret_cast<const uint32_t(&)[8]>(p[8]));
             }
             tc::tmem_st_wait();
             tc::fence_before();
-            fine = !named_any(1, kOut, !fine);
-            if (warp == 0 && fine) {
-                fine = wait(&ctl->v_full[st], round & 1, ctl, 24, err, s);
-                if (fine) {
-                    tc::fence_after();
-#pragma unroll
-                    for (int k = 0; k < kChunk / 16; ++k)
-                        tc::mma_bf16_ta_w(tmem + S::kO2Col, tmem + kPCol + 8 * k, tile_desc(v_a + k * 2048, kChunk * 128),
-                                          idesc(D, false, true), k > 0);
-                    tc::commit_w(&ctl->v_empty[st]);
-                    tc::commit_w(&ctl->pv);
-                }
-            }
-            if (fine) fine = wait(&ctl->between, turn, ctl, 25, err, s) && wait(&ctl->pv, turn, ctl, 26, err, s);
+            tc::mbar_arrive(&ctl->weights);
+            fine = wait(&ctl->between, turn, ctl, 25, err, s) && wait(&ctl->pv, turn, ctl, 26, err, s);
+            if (!fine) break;
             tc::fence_after();
-            const bool live = fine && r < m, bad = *static_cast<volatile int*>(&ctl->bad[use & 3]) != 0;
+            const bool live = r < m;
             const float grow = ctl->power[r + 1] * a.scale;
             bf16* const to = static_cast<bf16*>(a.out) + (row_at(i) + r) * a.o_ts + h * a.o_hs;
-            if (bad) {
-                // the values that were left out, for the tokens that see them (before any output, which may be where q is)
+            // a row of O2 that is not finite is computed again, from what it sees (before any output, which may be
+            // where q is)
+            float zero = 0.0f;
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                float y[32];
+                tmem_ld32(lanes + S::kO2Col + c, y);
+                tc::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) zero = fmaf(y[e], 0.0f, zero);
+            }
+            const bool again = live && zero != 0.0f;  // (then it is NaN)
+            if (__any_sync(0xffffffffu, again)) {
 #pragma unroll 1
                 for (int c = 0; c < D; c += 16) {
                     float y[16];
                     tc::tmem_ld16(lanes + S::kO2Col + c, y);
                     tc::tmem_ld_wait();
-                    for (uint32_t j = 0; live && j <= r; ++j) {
-                        float dot = 0.0f;
-                        bool any = false;
-                        for (int e = 0; e < 16; ++e) {
-                            const float z = static_cast<float>(v_at[(row_at(i) + j) * a.v_ts + c + e]);
-                            if (isfinite(z)) continue;
-                            if (!any)
-                                for (int ch = 0; ch < D; ++ch)
-                                    dot = fmaf(static_cast<float>(q_at[(row_at(i) + r) * a.q_ts + ch]), static_cast<float>(k_at[(row_at(i) + j) * a.k_ts + ch]), dot);
-                            any = true;
-                            y[e] += dot * ctl->power[r - j] * z;
+                    if (again) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) y[e] = 0.0f;
+                        for (uint32_t j = 0; j <= r; ++j) {
+                            float dot = 0.0f;
+                            for (int ch = 0; ch < D; ++ch)
+                                dot = fmaf(static_cast<float>(q_at[(row_at(i) + r) * a.q_ts + ch]), static_cast<float>(k_at[(row_at(i) + j) * a.k_ts + ch]), dot);
+                            dot *= ctl->power[r - j];
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) y[e] = fmaf(dot, static_cast<float>(v_at[(row_at(i) + j) * a.v_ts + c + e]), y[e]);
                         }
                     }
                     __syncwarp();
@@ -423,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_tc_kernel(const __grid_con
                     tc::tmem_st_wait();
                 }
             }
-#pragma unroll 1
+#pragma unroll
             for (int c = 0; c < D; c += 16) {
                 float x[16], y[16];
                 tc::tmem_ld16(lanes + kO1Col + c, x);
@@ -440,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_tc_kernel(const __grid_con
                 }
             }
             tc::fence_before();
-            fine = !named_any(1, kOut, !fine);
+            tc::mbar_arrive(&ctl->o_free);
         }
     };
 
@@ -452,74 +547,21 @@ __global__ void __launch_bounds__(kThreads, 1) linear_tc_kernel(const __grid_con
         for (int e = 0; e < 16; ++e) x[e] = fmaf(x[e], fade0, x[e]);
         tc::tmem_st16(t_lane + S::kSCol + col0 + c, x);
     };
+    constexpr bool whole = kMode != kAdds;
     const bool is_state = warp >= 4 && warp < 12;
     const size_t size = static_cast<size_t>(D) * D;
     const float* const before = a.states + (static_cast<size_t>(v.source < 0 ? 0 : v.source) * a.heads + h) * size;
-    // the block with the last tokens has the state after them (where there are none, the first)
-    const bool last = end == chunks && (first < end || (chunks == 0 && rank == 0));
-    float* const after = last && v.target >= 0 ? a.states + (static_cast<size_t>(v.target) * a.heads + h) * size : nullptr;
-    uint32_t use = 0, kv_use = 0;
-    float* const shared = reinterpret_cast<float*>(smem);
-    if (parts > 1) {
-        // What each block's tokens add to a state, then the states before them: element by element, each block a
-        // share of the elements for all of them, over distributed shared memory.
-        const bool walks = rank + 1 < parts && first < end;
-        if (walks) {
-            if (is_state) {
-                float x[16];
-                for (int c = 0; has_row && c < D / 2; c += 16) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = 0.0f;
-                    begin(c, x, false);
-                }
-                tc::tmem_st_wait();
-                states(false, first, use, kv_use, nullptr);
-            } else if (warp >= 12) {
-                loads(false, first, use);
-            }
-            use = end - first;  // (for the warps that did neither)
-        }
-        tc::fence_before();
-        __syncthreads();
-        tc::fence_after();
-        if (is_state && has_row) {
-            for (int c = 0; c < D / 2; c += 16) {
-                float x[16];
-                if (walks) {
-                    tc::tmem_ld16(t_lane + S::kSCol + col0 + c, x);
-                    tc::tmem_ld_wait();
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) shared[(col0 + c + e) * D + row] = walks ? x[e] : 0.0f;
-            }
-        }
-        cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();
-        const uint32_t share = D * D / parts + 1;
-        for (uint32_t x = threadIdx.x; x < share; x += kThreads) {
-            const uint32_t at = rank * share + x;
-            if (at >= D * D) break;
-            float y = v.source < 0 ? 0.0f : before[(at % D) * D + at / D];
-            float added[kMostParts];
-#pragma unroll
-            for (uint32_t b = 0; b < kMostParts; ++b) added[b] = b + 1 < parts ? cluster.map_shared_rank(shared, b)[at] : 0.0f;
-#pragma unroll
-            for (uint32_t b = 0; b < kMostParts; ++b) {
-                if (b >= parts) break;
-                cluster.map_shared_rank(shared, b)[at] = y;
-                const uint32_t done = min(b * per * kChunk, v.n), tokens = min(v.n - done, per * kChunk);
-                y = fmaf(y, expm1f(decay * tokens), y) + added[b];
-            }
-        }
-        cluster.sync();
-    }
+    // the part with the last tokens has the state after them
+    float* const after = whole && end == chunks && v.target >= 0 ? a.states + (static_cast<size_t>(v.target) * a.heads + h) * size : nullptr;
+    const size_t row0 = static_cast<size_t>(v.start) + first * kChunk;
+    const bool stashed = kMode == kGoesOn && part.count > 1;
     if (is_state && has_row) {
         for (int c = 0; c < D / 2; c += 16) {
             float x[16];
-            if (parts > 1) {
+            if (stashed) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = shared[(col0 + c + e) * D + row];
-            } else if (v.source >= 0) {
+                for (int e = 0; e < 16; ++e) x[e] = *stash<D>(a, row0, h, (col0 + c + e) * D + row);
+            } else if (kMode != kAdds && v.source >= 0) {
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
                     const float4 y = *reinterpret_cast<const float4*>(before + static_cast<size_t>(row) * D + col0 + c + e);
@@ -534,24 +576,39 @@ __global__ void __launch_bounds__(kThreads, 1) linear_tc_kernel(const __grid_con
                 for (int e = 0; e < 16; e += 4)
                     *reinterpret_cast<float4*>(after + static_cast<size_t>(row) * D + col0 + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
             }
-            begin(c, x, true);
+            begin(c, x, whole);
         }
         tc::tmem_st_wait();
     }
     tc::fence_before();
     tc::fence_async_smem();
-    __syncthreads();  // (the tiles go where the states were)
+    __syncthreads();  // (before any output: rows of `out` may hold the state)
     tc::fence_after();
-    if (is_state) {
-        if (first < end) tc::mbar_arrive(&ctl->s_full);
-        states(true, first, use, kv_use, after);
-    } else if (warp < 4) {
-        outputs(first, use);
-    } else {
-        loads(true, first, use);
+    if (first < end) {
+        if (is_state) {
+            if (whole) tc::mbar_arrive(&ctl->s_copy);
+            states(after);
+            if (kMode == kAdds && has_row) {
+                for (int c = 0; c < D / 2; c += 16) {
+                    float x[16];
+                    tc::tmem_ld16(t_lane + S::kSCol + col0 + c, x);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) *stash<D>(a, row0, h, (col0 + c + e) * D + row) = x[e];
+                }
+            }
+        } else if (warp < 4) {
+            if (whole) outputs();
+        } else if (warp == kLoadWarp) {
+            loads();
+        } else if (warp == kStateIssuer) {
+            state_products();
+        } else {
+            if (whole) out_products();
+        }
     }
     // every product has read its operands before the block ends
-    if (warp == 0 || warp == 4) {
+    if (warp == kStateIssuer || warp == kOutIssuer) {
         tc::commit_w(&ctl->drain);
         tc::mbar_wait_landing(&ctl->drain, 0);
     }
@@ -561,52 +618,109 @@ __global__ void __launch_bounds__(kThreads, 1) linear_tc_kernel(const __grid_con
     if (warp == 0) tc::tmem_free(tmem, 512);
 }
 
-// Blocks that a sequence and head are cut into along time: as many as run at once (clusters of blocks that fill an SM
-// each: a GPU of 148 has room for fewer than 148 / parts), with two chunks each at least.
+// What the parts of a sequence and head add, into the states before them, element by element.
+template <int D>
+__global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant__ LinearArgs a, uint32_t per, uint32_t parts) {
+    constexpr uint32_t kSlices = D * D / 256;
+    const uint32_t job = blockIdx.x / kSlices, i = (blockIdx.x - job * kSlices) * 256 + threadIdx.x;
+    const uint32_t s = a.head_div.div(job), h = job - s * a.heads;
+    const StateView v = state_view(a, s, false);
+    if (!v.ok) return;
+    const uint32_t count = part_of(v.n, per, parts, 0, D).count;
+    if (count == 1) return;
+    float decay = a.log_decay[h];
+    if (decay < -200.0f) decay = -200.0f;
+    const float fade = expm1f(decay * (per * kChunk));  // (all but the last part are that long)
+    const size_t size = static_cast<size_t>(D) * D;
+    float y = v.source < 0 ? 0.0f : a.states[(static_cast<size_t>(v.source) * a.heads + h) * size + (i % D) * D + i / D];
+#pragma unroll 4
+    for (uint32_t r = 0; r < count; ++r) {
+        float* const at = stash<D>(a, static_cast<size_t>(v.start) + r * per * kChunk, h, i);
+        const float added = r + 1 < count ? *at : 0.0f;
+        *at = y;
+        y = fmaf(y, fade, y) + added;
+    }
+}
+
+// A [tokens, heads, head_dim] tensor in boxes of 128 rows of 64 channels of a head, 128-byte swizzle.
+bool rows_map(const void* p, uint32_t tokens, uint32_t heads, uint32_t d, size_t ts, size_t hs, CUtensorMap* map) {
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found{};
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    if (!encode || ts == 0 || hs == 0 || ts >> 38 || hs >> 38) return false;
+    const cuuint64_t dims[3] = {d, heads, tokens}, strides[2] = {hs * 2, ts * 2};
+    const cuuint32_t box[3] = {64, 1, kChunk}, ones[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, int kMode>
+cudaError_t launch_mode(const LinearArgs& a, const CUtensorMap (&maps)[3], uint32_t per, uint32_t parts, cudaStream_t s) {
+    using S = Shape<D>;
+    static_assert(S::kBytes + sizeof(Control) <= 227 * 1024, "shared memory");
+    auto* kernel = linear_tc_kernel<D, kMode>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (e != cudaSuccess) return e;
+    kernel<<<a.sequences * a.heads * parts, kThreads, S::kBytes, s>>>(a, maps[0], maps[1], maps[2], per, parts);
+    return cudaGetLastError();
+}
+
+// Parts that a sequence and head are cut into: where that is quicker by the blocks that a GPU runs at once and the
+// chunks they have one after another (a chunk costs about as much for the state alone as with its outputs), with four
+// chunks each at least.
 uint32_t parts_of(const LinearArgs& a) {
-    constexpr uint32_t kRoom[] = {0, 148, 74, 44, 33, 25, 22, 16, 15, 8, 8, 8, 8, 8, 8, 7, 7};
-    const uint64_t jobs = static_cast<uint64_t>(a.sequences) * a.heads;
-    const uint32_t chunks = (a.max_new + kChunk - 1) / kChunk;
+    const double jobs = static_cast<double>(a.sequences) * a.heads, chunks = (a.max_new + kChunk - 1) / kChunk;
+    const double chunk_us = a.head_dim == 128 ? 2.6 : 2.0;
     uint32_t best = 1;
-    double least = 1e30;
-    for (uint32_t parts = 1; parts <= kMostParts && parts * 2 <= std::max(chunks, 2u); ++parts) {
-        const double cost = std::ceil(static_cast<double>(jobs) / kRoom[parts]) * ((chunks + parts - 1) / parts * (parts > 1 ? 1.6 : 1.0) + (parts > 1 ? 4.0 : 2.0));
+    double least = std::max(1.0, jobs / 148) * chunks * chunk_us;
+    for (uint32_t parts = 2; parts <= kMostParts && parts * 4 <= chunks; ++parts) {
+        const double cost = std::ceil(jobs * parts / 148) * std::ceil(chunks / parts) * 1.8 * chunk_us + 15.0;
         if (cost < least) least = cost, best = parts;
     }
     return best;
 }
 
-template <int D> cudaError_t launch(const LinearArgs& a, cudaStream_t s) {
-    using S = Shape<D>;
-    static_assert(S::kBytes + sizeof(Control) <= 227 * 1024, "shared memory");
-    auto* kernel = linear_tc_kernel<D>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
+// Whether two tensors' extents meet.
+bool apart(const void* x, size_t x_ts, size_t x_hs, uint32_t x_heads, const void* y, size_t y_ts, size_t y_hs, uint32_t y_heads, const LinearArgs& a) {
+    const auto end = [&](const void* p, size_t ts, size_t hs, uint32_t heads) {
+        return reinterpret_cast<uintptr_t>(p) + ((a.tokens - 1) * ts + (heads - 1) * hs + a.head_dim) * sizeof(bf16);
+    };
+    return end(x, x_ts, x_hs, x_heads) <= reinterpret_cast<uintptr_t>(y) || end(y, y_ts, y_hs, y_heads) <= reinterpret_cast<uintptr_t>(x);
+}
+
+template <int D> cudaError_t launch(const LinearArgs& a, const CUtensorMap (&maps)[3], cudaStream_t s, uint32_t* launches) {
+    const uint32_t kv = a.heads / a.group_div.d;
     uint32_t parts = parts_of(a);
-    if (getenv("LWM_PARTS")) parts = atoi(getenv("LWM_PARTS"));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(a.sequences * a.heads * parts);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = S::kBytes;
-    cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = parts;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, a, parts);
+    if (!apart(a.q, a.q_ts, a.q_hs, a.heads, a.out, a.o_ts, a.o_hs, a.heads, a) || !apart(a.k, a.k_ts, a.k_hs, kv, a.out, a.o_ts, a.o_hs, a.heads, a) ||
+        !apart(a.v, a.v_ts, a.v_hs, kv, a.out, a.o_ts, a.o_hs, a.heads, a))
+        parts = 1;
+    const uint32_t per = chunks_a_part(a.max_new, parts);
+    if (parts == 1) return launch_mode<D, kWhole>(a, maps, per, 1, s);
+    *launches = 3;
+    cudaError_t e = launch_mode<D, kAdds>(a, maps, per, parts, s);
+    if (e != cudaSuccess) return e;
+    linear_parts_kernel<D><<<a.sequences * a.heads * (D * D / 256), 256, 0, s>>>(a, per, parts);
+    e = cudaGetLastError();
+    return e == cudaSuccess ? launch_mode<D, kGoesOn>(a, maps, per, parts, s) : e;
 }
 
 }  // namespace
 
-bool linear_attention_tensor(const LinearArgs& a, int dtype) {
-    return dtype == LWM_DTYPE_BF16 && a.head_dim >= 64 && a.max_new > 64;
-}
-
-cudaError_t launch_linear_attention_tc(const LinearArgs& a, cudaStream_t s) {
-    return a.head_dim == 64 ? launch<64>(a, s) : launch<128>(a, s);
+cudaError_t launch_linear_attention_tc(const LinearArgs& a, int dtype, cudaStream_t s, bool* taken, uint32_t* launches) {
+    *taken = false;
+    if (dtype != LWM_DTYPE_BF16 || a.head_dim < 64 || a.max_new <= 64) return cudaSuccess;
+    CUtensorMap maps[3];
+    const uint32_t kv = a.heads / a.group_div.d;
+    if (!rows_map(a.q, a.tokens, a.heads, a.head_dim, a.q_ts, a.q_hs, &maps[0]) || !rows_map(a.k, a.tokens, kv, a.head_dim, a.k_ts, a.k_hs, &maps[1]) ||
+        !rows_map(a.v, a.tokens, kv, a.head_dim, a.v_ts, a.v_hs, &maps[2]))
+        return cudaSuccess;  // (strides that a tensor map does not take)
+    *taken = true;
+    return a.head_dim == 64 ? launch<64>(a, maps, s, launches) : launch<128>(a, maps, s, launches);
 }
 
 }  // namespace lwm

@@ -154,9 +154,9 @@ struct LinearArgs {
     uint64_t* err;
 };
 constexpr uint32_t kStepTokens = 8;  // up to here the recurrent kernel
-cudaError_t launch_linear_attention(const LinearArgs& a, int dtype, cudaStream_t s);
-bool linear_attention_tensor(const LinearArgs& a, int dtype);  // which of the two kernels for longer sequences
-cudaError_t launch_linear_attention_tc(const LinearArgs& a, cudaStream_t s);
+cudaError_t launch_linear_attention(const LinearArgs& a, int dtype, cudaStream_t s, uint32_t* launches);
+// Longer sequences on tcgen05, where types, widths and strides allow (else `taken` is false and nothing is launched).
+cudaError_t launch_linear_attention_tc(const LinearArgs& a, int dtype, cudaStream_t s, bool* taken, uint32_t* launches);
 
 struct TokenArgs {
     const void* logits;

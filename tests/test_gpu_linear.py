@@ -165,6 +165,14 @@ def test_many_sequences_and_a_long_one(ctx):
     call(ctx, gen(9), F16, 64, 1, 1, [1100, 3], "none", 1100)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("news", [[5000], [700, 0, 4700, 130, 1]], ids=str)
+def test_long_sequences_are_cut_along_time(ctx, d, news):
+    call(ctx, gen(19), BF16, d, 2, 1, news, "mild", max(news))
+    n = len(news)
+    call(ctx, gen(20), BF16, d, 1, 1, news, "none", max(news), slots=n + 2, source=[n + 1] * (n - 1) + [-1], target=list(range(n)))
+
+
 def test_half_precision_keeps_large_and_small_states(ctx):
     """Scores, keys and states far beyond f16's range on either side."""
     g, d, n = gen(10), 64, 130
