@@ -11,9 +11,10 @@
 //
 // Warps: four for the outputs (a token a thread: P, O1, O2), eight for the
 // state (a key channel a thread, half of the value channels: K' some tokens at
-// a time, computed while the product before it runs, then S), one that loads
-// by TMA, and an issuer of products for each of the two chains.  K and V have
-// two stages, Q is loaded again as soon as both its products are done.  All
+// a time, computed while the products before it run, then S), one that loads
+// by TMA, and an issuer of products for each of the two chains.  V has two
+// stages; Q and K are loaded again as soon as their products are done (the state
+// reads its keys from memory, with L2's help).  All
 // tiles are rows of 64 channels (128 bytes, 128-byte swizzle); K' is an M-major
 // A operand, V and S N-major B operands of that layout.  64 channels have a
 // second half of K' that is zero, as an A operand of 128 rows wants.
@@ -43,7 +44,7 @@ namespace lwm {
 namespace {
 
 constexpr int kChunk = 128;
-constexpr int kThreads = 480, kOut = 128, kState = 256;
+constexpr int kThreads = 480, kOut = 128, kState = 256, kOutWarps = 4, kStateWarps = 8;
 constexpr int kLoadWarp = 12, kStateIssuer = 13, kOutIssuer = 14;
 constexpr uint32_t kMostParts = 64;
 // What a launch does: the whole, the state that a part adds, or the outputs of a part.
@@ -53,17 +54,18 @@ constexpr uint32_t kPCol = 0, kO1Col = 128;
 template <int D> struct Shape {
     static constexpr int kPanels = D / 64;
     static constexpr int kTile = kPanels * kChunk * 128;    // bytes of 128 tokens
-    static constexpr int kRound = D == 64 ? 64 : 32;        // tokens whose K' is there at once
+    static constexpr int kRound = 4096 / D;                 // tokens of a round of K', twice 16 bytes a thread
     static constexpr int kPart = kPanels * kRound * 128;    // of a part of it
     static constexpr int kS = D * D * 2;
-    static constexpr int kQ = 0, kK = kTile, kV = kK + 2 * kTile, kParts = kV + 2 * kTile, kSAt = kParts + 3 * kPart;
-    static constexpr int kZero = kSAt + kS;                 // 64 channels: the empty half of K'
+    static constexpr int kQ = 0, kK = kTile, kV = kK + kTile, kParts = kV + 2 * kTile, kSAt = kParts + 6 * kPart;
+    static constexpr int kStage = kSAt + kS;                // outputs on their way, 32 rows of 32 channels a warp
+    static constexpr int kZero = kStage + 4 * 2048;         // 64 channels: the empty half of K'
     static constexpr int kBytes = kZero + (D == 64 ? kRound * 128 : 0) + 1024;  // + alignment
     static constexpr uint32_t kO2Col = kO1Col + D, kSCol = kO2Col + D;
 };
 
 struct Control {
-    uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], v_raw, scores, weights, between, pv, o_free, parts, kv, s_copy, drain;
+    uint64_t q_full, q_empty, k_full, k_empty, v_full[2], v_empty[2], v_raw, scores, weights, between, pv, o_free, parts[2], kv[2], s_copy, drain;
     uint32_t tmem;
     int dead;     // a wait gave up
     float power[kChunk + 1];  // lambda^i
@@ -83,6 +85,11 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Control* c,
 __host__ __device__ constexpr uint32_t idesc(uint32_t n, bool a_turned, bool b_turned) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((a_turned ? 1u : 0u) << 15) | ((b_turned ? 1u : 0u) << 16) | ((n >> 3) << 17) |
            ((128u >> 4) << 24);
+}
+// A warp's arrival, by one lane (32 arrivals at one barrier wait for each other).
+__device__ __forceinline__ void arrive_w(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(bar);
 }
 // Descriptors: the low word holds the start and the distance of the panels of 64 channels (in 16 bytes), the high one
 // is a constant (8-row groups 1024 bytes apart, 128-byte swizzle).
@@ -115,6 +122,10 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, i
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
         "l"(map), "r"(tc::smem_u32(bar)), "r"(channel), "r"(head), "r"(row)
         : "memory");
+}
+// The same rows into L2.
+__device__ __forceinline__ void prefetch_rows(const CUtensorMap* map, int channel, int head, int row) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(channel), "r"(head), "r"(row) : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -182,16 +193,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::mbar_init(&ctl->q_full, 1);
         tc::mbar_init(&ctl->q_empty, 2);
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(&ctl->k_full[i], 1);
             tc::mbar_init(&ctl->v_full[i], 1);
-            tc::mbar_init(&ctl->k_empty[i], 1 + kState);
             tc::mbar_init(&ctl->v_empty[i], 2);
+            tc::mbar_init(&ctl->parts[i], kStateWarps);
+            tc::mbar_init(&ctl->kv[i], 1);
         }
-        for (uint64_t* b : {&ctl->v_raw, &ctl->scores, &ctl->between, &ctl->pv, &ctl->kv}) tc::mbar_init(b, 1);
-        tc::mbar_init(&ctl->weights, kOut);
-        tc::mbar_init(&ctl->o_free, kOut);
-        tc::mbar_init(&ctl->parts, kState);
-        tc::mbar_init(&ctl->s_copy, kState);
+        for (uint64_t* b : {&ctl->k_full, &ctl->k_empty, &ctl->v_raw, &ctl->scores, &ctl->between, &ctl->pv}) tc::mbar_init(b, 1);
+        tc::mbar_init(&ctl->weights, kOutWarps);
+        tc::mbar_init(&ctl->o_free, kOutWarps);
+        tc::mbar_init(&ctl->s_copy, kStateWarps);
         tc::mbar_init(&ctl->drain, 2);
         ctl->dead = 0;
         tc::mbar_fence_init();
@@ -226,12 +236,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
         };
+        // keys (which the state reads from memory) and queries come to L2 two chunks ahead
+        auto ahead = [&](uint32_t i) {
+            if (i >= end || lane >= S::kPanels * (whole ? 2 : 1)) return;
+            if (lane < S::kPanels) prefetch_rows(&k_map, 64 * lane, hk, static_cast<int>(row_at(i)));
+            else prefetch_rows(&q_map, 64 * (lane - S::kPanels), h, static_cast<int>(row_at(i)));
+        };
+        ahead(from + 1);
         for (uint32_t i = from; i < end && fine; ++i, ++use) {
             const uint32_t st = use & 1, round = use >> 1, m = tokens_of(i);
-            if (use >= 2) fine = wait(&ctl->k_empty[st], (round - 1) & 1, ctl, 1, err, s);
-            if (!fine) break;
-            tile(&k_map, hk, i, base + S::kK + st * S::kTile, &ctl->k_full[st]);
+            ahead(i + 2);
             if (whole) {
+                if (i > from) fine = wait(&ctl->k_empty, (i - from - 1) & 1, ctl, 1, err, s);
+                if (!fine) break;
+                tile(&k_map, hk, i, base + S::kK, &ctl->k_full);
                 if (i > from) fine = wait(&ctl->q_empty, (i - from - 1) & 1, ctl, 3, err, s);
                 if (!fine) break;
                 tile(&q_map, h, i, base + S::kQ, &ctl->q_full);
@@ -275,58 +293,61 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto states = [&](float* final_state) {
         constexpr bool whole = kMode != kAdds;
         const uint32_t from = first;
-        uint32_t use = 0, kv_use = 0;
-        constexpr int kMine = S::kRound * kRowChunks / kState;  // 16-byte chunks of a round
-        uint4 part[3][kMine];
-        auto split = [&](uint32_t i, uint32_t st, uint32_t round) {
-            const uint32_t m = tokens_of(i);
+        uint32_t use = 0, turn = 0;  // chunks and rounds so far
+        bool fine = true;
+        // Keys come straight from memory, a round ahead (their tile in shared memory is for P).
+        uint4 raw[2];
+        const int at_tok = t_state / kRowChunks, at_ch = t_state % kRowChunks;  // and kApart tokens later
+        constexpr int kApart = kState / kRowChunks;
+        auto ask = [&](uint32_t i, uint32_t round) {
+            const uint32_t m = tokens_of(i), tok = round * S::kRound + at_tok;
+            const bf16* const k = k_at + (row_at(i) + tok) * a.k_ts + 8 * at_ch;
 #pragma unroll
-            for (int c = 0; c < kMine; ++c) {
-                const uint32_t x = c * kState + t_state, tok = round * S::kRound + x / kRowChunks;
-                float f[8], g[8];
-                unpack(Vec8<bf16>{*reinterpret_cast<const uint4*>(smem + S::kK + st * S::kTile + chunk_at(tok, x % kRowChunks, kChunk))}, f);
-                const float w = ctl->power[tok < m ? m - 1 - tok : 0];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = tok < m ? f[e] * w : 0.0f;
-#pragma unroll
-                for (int p = 0; p < 3; ++p) {
-                    const Vec8<bf16> y = pack<bf16>(f);
-                    part[p][c] = y.a;
-                    unpack(y, g);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] -= g[e];
-                }
-            }
-            if ((round + 1) * S::kRound >= m) {  // K has been read
-                tc::mbar_arrive(&ctl->k_empty[st]);
-                if (!whole && t_state == 0) tc::mbar_arrive(&ctl->k_empty[st]);  // (as the products with Q say otherwise)
-            }
+            for (int c = 0; c < 2; ++c)
+                raw[c] = tok + c * kApart < m ? *reinterpret_cast<const uint4*>(k + c * kApart * a.k_ts) : make_uint4(0, 0, 0, 0);
         };
-        bool fine = wait(&ctl->k_full[use & 1], (use >> 1) & 1, ctl, 10, err, s);
-        if (fine) split(from, use & 1, 0);
+        ask(from, 0);
         for (uint32_t i = from; i < end && fine; ++i, ++use) {
-            const uint32_t st = use & 1, m = tokens_of(i), rounds = (m + S::kRound - 1) / S::kRound;
+            const uint32_t m = tokens_of(i), rounds = (m + S::kRound - 1) / S::kRound;
             const bool more = i + 1 < end;
-            for (uint32_t round = 0; round < rounds && fine; ++round) {
+            for (uint32_t round = 0; round < rounds; ++round, ++turn) {
+                // three parts of 8 bits are all of a 32-bit product: its high half, and twice that of what is left
+                uint4 part[3][2];
 #pragma unroll
-                for (int c = 0; c < kMine; ++c) {
-                    const uint32_t x = c * kState + t_state;
+                for (int c = 0; c < 2; ++c) {
+                    float f[8];
+                    unpack(Vec8<bf16>{raw[c]}, f);
+                    const uint32_t tok = round * S::kRound + at_tok + c * kApart;
+                    const float w = ctl->power[tok < m ? m - 1 - tok : 0];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] *= w;
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) {
+                        uint32_t* const y = &part[p][c].x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t lo = __float_as_uint(f[2 * e]), hi = __float_as_uint(f[2 * e + 1]);
+                            y[e] = __byte_perm(lo, hi, 0x7632);
+                            f[2 * e] -= __uint_as_float(lo & 0xffff0000u);
+                            f[2 * e + 1] -= __uint_as_float(hi & 0xffff0000u);
+                        }
+                    }
+                }
+                if (round + 1 < rounds) ask(i, round + 1);
+                else if (more) ask(i + 1, 0);
+                const uint32_t b = turn & 1;
+                if (turn >= 2) fine = wait(&ctl->kv[b], ((turn >> 1) - 1) & 1, ctl, 13, err, s);  // the round before last is done
+                if (!fine) break;
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int p = 0; p < 3; ++p)
-                        *reinterpret_cast<uint4*>(smem + S::kParts + p * S::kPart + chunk_at(x / kRowChunks, x % kRowChunks, S::kRound)) = part[p][c];
-                }
+                        *reinterpret_cast<uint4*>(smem + S::kParts + (3 * b + p) * S::kPart + chunk_at(at_tok + c * kApart, at_ch, S::kRound)) = part[p][c];
                 tc::fence_async_smem();
-                tc::fence_before();  // (the state's stores, too)
-                tc::mbar_arrive(&ctl->parts);
-                if (round + 1 < rounds) {
-                    split(i, st, round + 1);
-                } else if (more) {
-                    fine = wait(&ctl->k_full[st ^ 1], ((use + 1) >> 1) & 1, ctl, 10, err, s);
-                    if (fine) split(i + 1, st ^ 1, 0);
-                }
-                if (fine) fine = wait(&ctl->kv, kv_use & 1, ctl, 13, err, s);
-                ++kv_use;
+                if (round == 0) tc::fence_before();  // (the state's stores, too)
+                arrive_w(&ctl->parts[b]);
             }
+            if (fine) fine = wait(&ctl->kv[(turn - 1) & 1], ((turn - 1) >> 1) & 1, ctl, 19, err, s);
             // the bf16 copy's last reader is the product of this chunk
             if (fine && whole) fine = wait(&ctl->between, (i - from) & 1, ctl, 14, err, s);
             if (!fine) break;
@@ -359,14 +380,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc::fence_before();
             tc::fence_async_smem();
-            if (whole && more) tc::mbar_arrive(&ctl->s_copy);
+            if (whole && more) arrive_w(&ctl->s_copy);
         }
     };
     // The state's products: O1 = Q S of a chunk, then K'^T V of it in rounds.
     auto state_products = [&] {
         constexpr bool whole = kMode != kAdds;
         const uint32_t from = first;
-        uint32_t use = 0, parts_use = 0;
+        uint32_t use = 0, turn = 0;
         constexpr uint32_t kI = idesc(D, true, true), kB = idesc(D, false, true);
         bool fine = true;
         for (uint32_t i = from; i < end && fine; ++i, ++use) {
@@ -384,19 +405,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::commit_w(&ctl->q_empty);
             }
             fine = wait(&ctl->v_full[st], (use >> 1) & 1, ctl, 12, err, s);
-            for (uint32_t round = 0; round < rounds && fine; ++round) {
-                fine = wait(&ctl->parts, parts_use++ & 1, ctl, 18, err, s);
+            for (uint32_t round = 0; round < rounds && fine; ++round, ++turn) {
+                const uint32_t b = turn & 1;
+                fine = wait(&ctl->parts[b], (turn >> 1) & 1, ctl, 18, err, s);
                 if (!fine) break;
                 tc::fence_after();
-                const uint32_t v_a = base + S::kV + st * S::kTile + round * S::kRound * 128;
+                const uint32_t k_a = base + S::kParts + 3 * b * S::kPart, v_low = low_desc(base + S::kV + st * S::kTile + round * S::kRound * 128, kChunk * 128);
 #pragma unroll
                 for (int p = 0; p < 3; ++p) {
-                    const uint32_t k_a = base + S::kParts + p * S::kPart, panel = D == 64 ? base + S::kZero - k_a : S::kRound * 128;
+                    const uint32_t k_p = k_a + p * S::kPart, panel = D == 64 ? base + S::kZero - k_p : S::kRound * 128;
 #pragma unroll
                     for (int k = 0; k < S::kRound / 16; k += 2)
-                        mma2(tmem + S::kSCol, low_desc(k_a + k * 2048, panel), 128, low_desc(v_a + k * 2048, kChunk * 128), 128, kI, 1);
+                        mma2(tmem + S::kSCol, low_desc(k_p + k * 2048, panel), 128, v_low + k * 128, 128, kI, 1);
                 }
-                tc::commit_w(&ctl->kv);
+                tc::commit_w(&ctl->kv[b]);
             }
             if (!fine) break;
             tc::commit_w(&ctl->v_empty[st]);
@@ -410,21 +432,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t use = 0;
         constexpr uint32_t kP = idesc(kChunk, false, false), kO = idesc(D, false, true);
         bool fine = true;
-        auto scores = [&](uint32_t i, uint32_t u) {
-            const uint32_t st = u & 1;
-            fine = wait(&ctl->q_full, (i - from) & 1, ctl, 20, err, s) && wait(&ctl->k_full[st], (u >> 1) & 1, ctl, 21, err, s);
+        auto scores = [&](uint32_t i) {
+            fine = wait(&ctl->q_full, (i - from) & 1, ctl, 20, err, s) && wait(&ctl->k_full, (i - from) & 1, ctl, 21, err, s);
             if (!fine) return;
             tc::fence_after();
 #pragma unroll
             for (int k = 0; k < kSteps; k += 2) {
                 const uint32_t off = (k >> 2) * kChunk * 128 + (k & 3) * 32;
-                mma2(tmem + kPCol, low_desc(base + S::kQ + off, 16), 2, low_desc(base + S::kK + st * S::kTile + off, 16), 2, kP, k > 0);
+                mma2(tmem + kPCol, low_desc(base + S::kQ + off, 16), 2, low_desc(base + S::kK + off, 16), 2, kP, k > 0);
             }
             tc::commit_w(&ctl->scores);
             tc::commit_w(&ctl->q_empty);
-            tc::commit_w(&ctl->k_empty[st]);
+            tc::commit_w(&ctl->k_empty);
         };
-        scores(from, use);
+        scores(from);
         for (uint32_t i = from; i < end && fine; ++i, ++use) {
             const uint32_t st = use & 1;
             fine = wait(&ctl->v_full[st], (use >> 1) & 1, ctl, 24, err, s) && wait(&ctl->weights, (i - from) & 1, ctl, 27, err, s);
@@ -436,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mma2_t(tmem + S::kO2Col, tmem + kPCol + 8 * k, low_desc(base + S::kV + st * S::kTile + k * 2048, kChunk * 128), 128, kO, k > 0);
             tc::commit_w(&ctl->v_empty[st]);
             tc::commit_w(&ctl->pv);
-            if (i + 1 < end) scores(i + 1, use + 1);  // (over the weights, which the product before it has read)
+            if (i + 1 < end) scores(i + 1);  // (over the weights, which the product before it has read)
         }
     };
     auto outputs = [&] {
@@ -476,24 +497,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc::tmem_st_wait();
             tc::fence_before();
-            tc::mbar_arrive(&ctl->weights);
+            arrive_w(&ctl->weights);
             fine = wait(&ctl->between, turn, ctl, 25, err, s) && wait(&ctl->pv, turn, ctl, 26, err, s);
             if (!fine) break;
             tc::fence_after();
             const bool live = r < m;
             const float grow = ctl->power[r + 1] * a.scale;
-            bf16* const to = static_cast<bf16*>(a.out) + (row_at(i) + r) * a.o_ts + h * a.o_hs;
+            bf16* const out_at = static_cast<bf16*>(a.out) + h * a.o_hs;
             // a row of O2 that is not finite is computed again, from what it sees (before any output, which may be
             // where q is)
-            float zero = 0.0f;
+            float zeros[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
                 float y[32];
                 tmem_ld32(lanes + S::kO2Col + c, y);
                 tc::tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) zero = fmaf(y[e], 0.0f, zero);
+                for (int e = 0; e < 32; ++e) zeros[e & 3] = fmaf(y[e], 0.0f, zeros[e & 3]);
             }
+            const float zero = (zeros[0] + zeros[1]) + (zeros[2] + zeros[3]);
             const bool again = live && zero != 0.0f;  // (then it is NaN)
             if (__any_sync(0xffffffffu, again)) {
 #pragma unroll 1
@@ -518,24 +540,37 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc::tmem_st_wait();
                 }
             }
+            // 32 channels at a time through shared memory, so that a store takes whole runs of 64 bytes
+            uint8_t* const stage = smem + S::kStage + warp * 2048;
+            bf16* to[4];
 #pragma unroll
-            for (int c = 0; c < D; c += 16) {
-                float x[16], y[16];
-                tc::tmem_ld16(lanes + kO1Col + c, x);
-                tc::tmem_ld16(lanes + S::kO2Col + c, y);
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t rr = warp * 32 + 8 * k + (lane >> 2);
+                to[k] = rr < m ? out_at + (row_at(i) + rr) * a.o_ts + 8 * (lane & 3) : nullptr;
+            }
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                float x[32], y[32];
+                tmem_ld32(lanes + kO1Col + c, x);
+                tmem_ld32(lanes + S::kO2Col + c, y);
                 tc::tmem_ld_wait();
-                if (live) {
+                __syncwarp();  // (the rows before these have been read)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        float f[8];
+                for (int b = 0; b < 4; ++b) {
+                    float f[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = fmaf(x[8 * b + e], grow, y[8 * b + e] * a.scale);
-                        store8(to + c + 8 * b, pack<bf16>(f));
-                    }
+                    for (int e = 0; e < 8; ++e) f[e] = fmaf(x[8 * b + e], grow, y[8 * b + e] * a.scale);
+                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((b ^ ((lane >> 1) & 3)) << 4)) = pack<bf16>(f).a;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t rr = 8 * k + (lane >> 2), b = lane & 3;
+                    if (to[k]) *reinterpret_cast<uint4*>(to[k] + c) = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((b ^ ((rr >> 1) & 3)) << 4));
                 }
             }
             tc::fence_before();
-            tc::mbar_arrive(&ctl->o_free);
+            arrive_w(&ctl->o_free);
         }
     };
 
@@ -586,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::fence_after();
     if (first < end) {
         if (is_state) {
-            if (whole) tc::mbar_arrive(&ctl->s_copy);
+            if (whole) arrive_w(&ctl->s_copy);
             states(after);
             if (kMode == kAdds && has_row) {
                 for (int c = 0; c < D / 2; c += 16) {
