@@ -668,12 +668,20 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant
     const float fade = expm1f(decay * (per * kChunk));  // (all but the last part are that long)
     const size_t size = static_cast<size_t>(D) * D;
     float y = v.source < 0 ? 0.0f : a.states[(static_cast<size_t>(v.source) * a.heads + h) * size + (i % D) * D + i / D];
-#pragma unroll 4
-    for (uint32_t r = 0; r < count; ++r) {
-        float* const at = stash<D>(a, static_cast<size_t>(v.start) + r * per * kChunk, h, i);
-        const float added = r + 1 < count ? *at : 0.0f;
-        *at = y;
-        y = fmaf(y, fade, y) + added;
+    // (eight parts are read before the first of them is written)
+    for (uint32_t r0 = 0; r0 < count; r0 += 8) {
+        float* at[8];
+        float added[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            at[e] = stash<D>(a, static_cast<size_t>(v.start) + (r0 + e) * per * kChunk, h, i);
+            added[e] = r0 + e + 1 < count ? *at[e] : 0.0f;
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            if (r0 + e < count) *at[e] = y;
+            y = fmaf(y, fade, y) + added[e];
+        }
     }
 }
 
@@ -710,11 +718,11 @@ cudaError_t launch_mode(const LinearArgs& a, const CUtensorMap (&maps)[3], uint3
 // chunks each at least.
 uint32_t parts_of(const LinearArgs& a) {
     const double jobs = static_cast<double>(a.sequences) * a.heads, chunks = (a.max_new + kChunk - 1) / kChunk;
-    const double chunk_us = a.head_dim == 128 ? 2.6 : 2.0;
+    const double chunk_us = a.head_dim == 128 ? 4.6 : 3.3;
     uint32_t best = 1;
     double least = std::max(1.0, jobs / 148) * chunks * chunk_us;
     for (uint32_t parts = 2; parts <= kMostParts && parts * 4 <= chunks; ++parts) {
-        const double cost = std::ceil(jobs * parts / 148) * std::ceil(chunks / parts) * 1.8 * chunk_us + 15.0;
+        const double cost = std::ceil(jobs * parts / 148) * (std::ceil(chunks / parts) * 1.7 * chunk_us + 8.0) + 12.0;
         if (cost < least) least = cost, best = parts;
     }
     return best;
