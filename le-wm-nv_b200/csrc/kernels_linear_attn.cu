@@ -99,7 +99,7 @@ template <typename T, int D> struct ChunkShape {
     static constexpr int kState = kHalf ? D * kPitch * 4 : D * D * 2;
     static constexpr int kStages = kHalf && D == 128 ? 2 : 3, kStates = kHalf && D == 128 ? 1 : 2;
     static constexpr int kBytes = kStages * 3 * kTile + kStates * kState;
-    static constexpr int kBlocks = D == 128 ? 1 : D == 64 ? 2 : 3;
+    static constexpr int kBlocks = D == 128 ? 1 : 2;
     static_assert(kStages * 3 * kTile >= D * D * 4, "a state goes where the tiles are");
 };
 
@@ -194,47 +194,50 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
                 scale[r] = f.x, back[r] = f.y;
             }
         }
+        // Tensor cores cut off what does not fit a sum, step by step, so a chunk's sums start at zero and are added to
+        // the state with rounding (16384 tokens that hardly fade: off by 6e-6 of the state when summed in place, 6e-7 so).
+        constexpr int kGroup = D == 64 ? 8 : 4;  // tiles at once, for the registers
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n)
+        for (int n0 = 0; n0 < kTiles; n0 += kGroup) {
+            float sum[kGroup][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                st[n][e] = fmaf(st[n][e], fade, st[n][e]);
-                if constexpr (S::kHalf) st[n][e] *= scale[e >> 1];
-            }
+            for (int n = 0; n < kGroup; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            // keys times their decay in parts (bf16 three of 8 bits, f16 two of 11), so that the state keeps them
-            // as a 32-bit product would
-            constexpr int kParts = S::kHalf ? 2 : 3;
-            uint32_t raw[4], x[kParts][4];
-            keys(k, raw);
+            for (int k = 0; k < 4; ++k) {
+                // keys times their decay in parts (bf16 three of 8 bits, f16 two of 11), so that the state keeps them
+                // as a 32-bit product would
+                constexpr int kParts = S::kHalf ? 2 : 3;
+                uint32_t raw[4], x[kParts][4];
+                keys(k, raw);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {  // register e: row g + 8 (e & 1), tokens 2 t (+ 1) + 8 (e >> 1)
-                float2 r = pair_at<T>(raw[e]);
-                r.x *= weight(k, 2 * (e >> 1)) * scale[e & 1], r.y *= weight(k, 2 * (e >> 1) + 1) * scale[e & 1];
+                for (int e = 0; e < 4; ++e) {  // register e: row g + 8 (e & 1), tokens 2 t (+ 1) + 8 (e >> 1)
+                    float2 r = pair_at<T>(raw[e]);
+                    r.x *= weight(k, 2 * (e >> 1)) * scale[e & 1], r.y *= weight(k, 2 * (e >> 1) + 1) * scale[e & 1];
 #pragma unroll
-                for (int q = 0; q < kParts; ++q) {
-                    x[q][e] = pack2(r.x, r.y, T{});
-                    const float2 y = pair_at<T>(x[q][e]);
-                    r.x -= y.x, r.y -= y.y;
+                    for (int q = 0; q < kParts; ++q) {
+                        x[q][e] = pack2(r.x, r.y, T{});
+                        const float2 y = pair_at<T>(x[q][e]);
+                        r.x -= y.x, r.y -= y.y;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < kGroup; n += 2) {
+                    uint32_t b[4];
+                    ldsm4t(b, v_a + tile_at<D>(16 * k + (lane & 15), n0 + n + (lane >> 4)));
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q) {
+                        mma<T>(sum[n], x[q], b[0], b[1]);
+                        mma<T>(sum[n + 1], x[q], b[2], b[3]);
+                    }
                 }
             }
 #pragma unroll
-            for (int n = 0; n < kTiles; n += 2) {
-                uint32_t b[4];
-                ldsm4t(b, v_a + tile_at<D>(16 * k + (lane & 15), n + (lane >> 4)));
+            for (int n = 0; n < kGroup; ++n)
 #pragma unroll
-                for (int q = 0; q < kParts; ++q) {
-                    mma<T>(st[n], x[q], b[0], b[1]);
-                    mma<T>(st[n + 1], x[q], b[2], b[3]);
+                for (int e = 0; e < 4; ++e) {
+                    float& y = st[n0 + n][e];
+                    y = fmaf(sum[n][e], S::kHalf ? back[e >> 1] : 1.0f, fmaf(y, fade, y));
                 }
-            }
-        }
-        if constexpr (S::kHalf) {
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) st[n][e] *= back[e >> 1];
         }
     };
     // the state to shared memory, for the product with Q: bf16, or tf32 for f16 (which has no room for its range)

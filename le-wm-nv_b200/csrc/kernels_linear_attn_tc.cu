@@ -5,7 +5,7 @@
 // in chunks of 128 tokens:
 //   P  = Q K^T                     (TMEM), times lambda^(i-j) where j <= i, to bf16 in place
 //   O1 = Q S, O2 = P V             (TMEM), out = scale (lambda^(i+1) O1 + O2)
-//   S  = lambda^m S + K'^T V       (TMEM, 32 bits; a bf16 copy in shared memory for O1)
+//   S  = lambda^m S + K'^T V       (the product in TMEM, S in registers; a bf16 copy in shared memory for O1)
 // with K' = lambda^(m-1-j) k_j in three parts of 8 bits, so that S keeps them
 // as 32-bit products would.
 //
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool has_row = row < D;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     // the bf16 copy of this thread's part of the state
-    auto copy16 = [&](int c, const float(&x)[16]) {
+    auto copy16 = [&](int c, const float* x) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             float f[8];
@@ -288,9 +288,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<uint4*>(smem + S::kSAt + chunk_at(row, (col0 + c) / 8 + b, D)) = pack<bf16>(f).a;
         }
     };
-    // The state's steps (TMEM holds it, times the first chunk's decay).  The parts of K' are computed while the products
-    // before them run.
-    auto states = [&](float* final_state) {
+    // The state's steps; x is this thread's part of it.  The parts of K' are computed while the products before them run.
+    auto states = [&](float(&x)[D / 2]) {
         constexpr bool whole = kMode != kAdds;
         const uint32_t from = first;
         uint32_t use = 0, turn = 0;  // chunks and rounds so far
@@ -352,31 +351,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (fine && whole) fine = wait(&ctl->between, (i - from) & 1, ctl, 14, err, s);
             if (!fine) break;
             tc::fence_after();
-            const float fade = more ? expm1f(decay * tokens_of(i + 1)) : 0.0f;
+            // Sums in TMEM are cut off, not rounded, at each step: a chunk's are added to the state here.
+            const float fade = expm1f(decay * m);
             if (has_row) {
 #pragma unroll
                 for (int c = 0; c < D / 2; c += 32) {
-                    float x[32];
-                    tmem_ld32(t_lane + S::kSCol + col0 + c, x);
+                    float y[32];
+                    tmem_ld32(t_lane + S::kSCol + col0 + c, y);
                     tc::tmem_ld_wait();
 #pragma unroll
-                    for (int b = 0; b < 32; b += 16) {
-                        float(&y)[16] = *reinterpret_cast<float(*)[16]>(x + b);
-                        if (whole && more) copy16(c + b, y);
-                        if (final_state && !more) {
-#pragma unroll
-                            for (int e = 0; e < 16; e += 4)
-                                *reinterpret_cast<float4*>(final_state + static_cast<size_t>(row) * D + col0 + c + b + e) =
-                                    make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-                        }
-                        if (more || !whole) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) y[e] = fmaf(y[e], fade, y[e]);
-                            tc::tmem_st16(t_lane + S::kSCol + col0 + c + b, y);
-                        }
+                    for (int e = 0; e < 32; ++e) x[c + e] = fmaf(x[c + e], fade, x[c + e]) + y[e];
+                    if (whole && more) {
+                        copy16(c, x + c);
+                        copy16(c + 16, x + c + 16);
                     }
                 }
-                tc::tmem_st_wait();
             }
             tc::fence_before();
             tc::fence_async_smem();
@@ -416,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t k_p = k_a + p * S::kPart, panel = D == 64 ? base + S::kZero - k_p : S::kRound * 128;
 #pragma unroll
                     for (int k = 0; k < S::kRound / 16; k += 2)
-                        mma2(tmem + S::kSCol, low_desc(k_p + k * 2048, panel), 128, v_low + k * 128, 128, kI, 1);
+                        mma2(tmem + S::kSCol, low_desc(k_p + k * 2048, panel), 128, v_low + k * 128, 128, kI, round || p || k);
                 }
                 tc::commit_w(&ctl->kv[b]);
             }
@@ -574,14 +563,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     };
 
-    // A state into TMEM, times the decay of the first chunk, and its bf16 copy.
-    const float fade0 = first < end ? expm1f(decay * tokens_of(first)) : 0.0f;
-    auto begin = [&](int c, float(&x)[16], bool copy) {
-        if (copy) copy16(c, x);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = fmaf(x[e], fade0, x[e]);
-        tc::tmem_st16(t_lane + S::kSCol + col0 + c, x);
-    };
     constexpr bool whole = kMode != kAdds;
     const bool is_state = warp >= 4 && warp < 12;
     const size_t size = static_cast<size_t>(D) * D;
@@ -590,49 +571,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* const after = whole && end == chunks && v.target >= 0 ? a.states + (static_cast<size_t>(v.target) * a.heads + h) * size : nullptr;
     const size_t row0 = static_cast<size_t>(v.start) + first * kChunk;
     const bool stashed = kMode == kGoesOn && part.count > 1;
+    float x[D / 2];
     if (is_state && has_row) {
+#pragma unroll
         for (int c = 0; c < D / 2; c += 16) {
-            float x[16];
             if (stashed) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = *stash<D>(a, row0, h, (col0 + c + e) * D + row);
+                for (int e = 0; e < 16; ++e) x[c + e] = *stash<D>(a, row0, h, (col0 + c + e) * D + row);
             } else if (kMode != kAdds && v.source >= 0) {
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
                     const float4 y = *reinterpret_cast<const float4*>(before + static_cast<size_t>(row) * D + col0 + c + e);
-                    x[e] = y.x, x[e + 1] = y.y, x[e + 2] = y.z, x[e + 3] = y.w;
+                    x[c + e] = y.x, x[c + e + 1] = y.y, x[c + e + 2] = y.z, x[c + e + 3] = y.w;
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+                for (int e = 0; e < 16; ++e) x[c + e] = 0.0f;
             }
-            if (after && first == end) {
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    *reinterpret_cast<float4*>(after + static_cast<size_t>(row) * D + col0 + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-            }
-            begin(c, x, whole);
+            if (whole) copy16(c, x + c);
         }
-        tc::tmem_st_wait();
     }
-    tc::fence_before();
     tc::fence_async_smem();
     __syncthreads();  // (before any output: rows of `out` may hold the state)
-    tc::fence_after();
-    if (first < end) {
-        if (is_state) {
+    if (is_state) {
+        if (first < end) {
             if (whole) arrive_w(&ctl->s_copy);
-            states(after);
-            if (kMode == kAdds && has_row) {
-                for (int c = 0; c < D / 2; c += 16) {
-                    float x[16];
-                    tc::tmem_ld16(t_lane + S::kSCol + col0 + c, x);
-                    tc::tmem_ld_wait();
+            states(x);
+        }
+        if (has_row && (kMode == kAdds || after)) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) *stash<D>(a, row0, h, (col0 + c + e) * D + row) = x[e];
+            for (int c = 0; c < D / 2; c += 4) {
+                if constexpr (kMode == kAdds) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) *stash<D>(a, row0, h, (col0 + c + e) * D + row) = x[c + e];
+                } else {
+                    *reinterpret_cast<float4*>(after + static_cast<size_t>(row) * D + col0 + c) = make_float4(x[c], x[c + 1], x[c + 2], x[c + 3]);
                 }
             }
-        } else if (warp < 4) {
+        }
+    } else if (first < end) {
+        if (warp < 4) {
             if (whole) outputs();
         } else if (warp == kLoadWarp) {
             loads();

@@ -173,6 +173,21 @@ def test_long_sequences_are_cut_along_time(ctx, d, news):
     call(ctx, gen(20), BF16, d, 1, 1, news, "none", max(news), slots=n + 2, source=[n + 1] * (n - 1) + [-1], target=list(range(n)))
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_long_sums_are_rounded_not_cut_off(ctx, d, dtype):
+    """Without decay the state is K^T V.  A rounding at every chunk of 64 tokens or more (two of them) moves its norm
+    by 2^-24 sqrt(2 n / 64) / 2 or so, as their signs differ; sums that are cut off at every step of the tensor cores
+    lean to one side, 4e-6 and more at this length."""
+    g, n = gen(21), 16384
+    q, k, v = (randn(g, n, 1, d, dtype=dtype) for _ in range(3))
+    states, out = torch.zeros(1, 1, d, d, device="cuda"), torch.empty_like(q)
+    L.linear_attention_device(ctx, L.StateBatch(states, ints([0, n]), n), q, k, v, out, torch.zeros(1, device="cuda"))
+    ctx.synchronize()
+    want = k[:, 0].double().T @ v[:, 0].double()
+    assert (states[0, 0].double() - want).norm() <= E32 * (2 * (2 * n / 64) ** 0.5 + 16) * want.norm()
+
+
 def test_half_precision_keeps_large_and_small_states(ctx):
     """Scores, keys and states far beyond f16's range on either side."""
     g, d, n = gen(10), 64, 130
