@@ -110,6 +110,22 @@ def test_ties_go_to_the_lowest_index(ctx):
             run(ctx, logits, u, 1.0, top_k, top_p, min_p)
 
 
+@pytest.mark.parametrize("many", [131072, 262044])
+@pytest.mark.parametrize("step", [3, 40])
+def test_many_tokens_in_one_bin_of_a_large_vocabulary(ctx, many, step):
+    """The most tokens there can be at one logit below a hundred larger ones, at temperatures where it is the first of
+    its bin: a bin's mass is the largest that it can be."""
+    x = torch.full((12, 262144), -float("inf"), device="cuda")
+    x[:, :many] = -float(step)
+    x[:, many:many + 100] = 0.0
+    # (bins are 45 / 512 powers of two: a step of the logits each, or a little less)
+    temperature = torch.tensor([512 / 45 * 1.4426950408889634 * (1 - i * 2.0 ** -21) for i in range(12)], device="cuda")
+    u = torch.rand(12, generator=torch.Generator("cuda").manual_seed(5), device="cuda")
+    for top_p in (0.3, 0.999):
+        run(ctx, x, u, temperature, 0, top_p)
+    run(ctx, x, u, temperature, 60000, 0.9)
+
+
 def test_random_numbers_at_the_edges(ctx):
     for vocab in (5, 3000, 20000):
         logits, _ = logits_of(8, vocab, F32, 3)
