@@ -961,7 +961,9 @@ lwm_status lwm_cache_attention_shared_device(lwm_ctx* ctx, const lwm_paged_cache
  * undefined).  A sequence without tokens hands its state on.  Launches are
  * sized by max_new: with up to 8 new tokens the state is read and written
  * once and the tokens follow each other; longer sequences go by chunks of 64
- * on tensor cores.
+ * or 128 on tensor cores, few long ones cut along time, where `out` lies apart
+ * from q, k and v (a call in place is right too, only slower); its rows may
+ * hold other values until the call's work is done.
  *
  * q, out [tokens, heads, head_dim], k, v [tokens, kv_heads, head_dim] of
  * `dtype` (bf16 or f16; out may be q); query head h and its state use kv head
@@ -969,9 +971,10 @@ lwm_status lwm_cache_attention_shared_device(lwm_ctx* ctx, const lwm_paged_cache
  * (nothing fades) or below; minus infinity: every token starts afresh.
  * In chunks, the weights q.k lambda^n are rounded to dtype for their product
  * with v, the state is rounded to bf16 (f16: to 11 bits of any range) for the
- * product with q, and keys times their decay enter the state with 16 bits
- * (f16: 22).  Infinities and NaN reach later tokens of their sequence and
- * head only.
+ * product with q, and keys times their decay enter the state with 24 bits
+ * (f16: 22 of each key channel's largest), whose sums are in 32 bits and
+ * rounded.  Infinities and NaN reach later tokens of their sequence and head
+ * only; a state that an infinity entered may hold NaN in its place.
  *
  * A sequence whose starts are out of order or above max_new, or whose slots
  * are beyond the pool, is skipped; the next lwm_ctx_synchronize returns

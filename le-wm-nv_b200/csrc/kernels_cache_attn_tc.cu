@@ -34,6 +34,11 @@
 // 32 channels run as 64 whose upper half is zero (by TMA's fill beyond the
 // tensor, or copies of no bytes): the softmax bounds them all the same.
 //
+// A prefix that sequences share (kPrefixKeys) is attended by all rows of its
+// group as if they were one sequence's, in parts of its keys: a part's rows
+// leave in 32 bits, divided by their sum, with that sum's logarithm, and the
+// tails' kernels join them.  Figures stand at shared_plan.
+//
 // TMEM: S (and P) of tile t at column 128 t, O at 256 and 256 + D.  Shared
 // memory: Q, two stages of K and of V, all rows of 64 channels (128 bytes,
 // 128-byte swizzle); K is a K-major operand, V the transposed (N-major) one
@@ -1102,6 +1107,12 @@ cudaError_t launch_cache_attention_tc(const CacheAttnArgs& a, int dtype, int sto
 
 // The prefix's blocks by the same costs: row tiles a block, and parts of the
 // keys, each of which writes 32-bit results that the tails' kernel reads.
+// What bounds the prefix (one B200): with few keys the chain of a block's steps and its start (1024 candidates of 16
+// heads behind 1568 tokens: 26 us, tensor pipe 15 %; the flops alone 8), with many the chain of scores, softmax and
+// product as in a sequence's own attention (64 candidates of 4 tokens and 32 heads behind 65536: 208 us, pipe 53 %, 106
+// at its peak).  8-bit codes: 16 groups of 64 with a window of 4096 75 us, expanding the codes beside that chain.  A part
+// more costs its results in 32 bits, written here and read by the tails; the choice made here was the quickest
+// of all (block, parts) pairs in the cases tried.
 SharedPlan shared_plan(const CacheAttnArgs& a, uint32_t most_splits) {
     const bool wide = a.c.head_dim == 128;
     const uint64_t rows = static_cast<uint64_t>(a.max_tokens) * a.group;

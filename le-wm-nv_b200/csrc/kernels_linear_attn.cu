@@ -4,12 +4,22 @@
 // S one f32 [head_dim, head_dim] state a head.
 //
 // A few tokens a sequence (linear_step_kernel): the state is read once, kept
-// in registers over the tokens, and written once.
+// in registers over the tokens, and written once.  Bound by those bytes: 1024
+// sequences of 16 heads of 64, a token each, 537 MB in 84.6 us, 6.4 TB/s; 256
+// that fork from one state, 16 heads of 128, 268 MB written in 64 us.  Up to 8
+// tokens: 8 of those 1024 take 184 us, in chunks 267, and each token more 16.
 //
 // Whole histories (linear_chunk_kernel): chunks of 64 tokens,
 //   O = lambda^(i+1) Q S + (Q K^T . lambda^(i-j), j <= i) V,
 //   S' = lambda^m S + sum_j lambda^(m-1-j) k_j v_j^T   (m tokens),
-// all four products on mma.sync with the state in the accumulators' registers.
+// all four products on mma.sync with the state in registers: half of the warps
+// keep it, the others compute the outputs of the chunk before.  For f16 (whose
+// states and weights need powers of two a row, and tf32 for Q S), 32 channels,
+// short sequences, and strides that a tensor map does not take; long ones of
+// bf16 with 64 or 128 channels go on tcgen05.  Bound by the products' issue and
+// the fragments' way to them: 16 sequences of 1568 tokens, 16 heads, f16, of 32
+// channels 63 us, of 64 108, of 128 (one block a SM) 353; one of 65536 tokens
+// 371, 595, 2665.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -498,14 +508,15 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
     else run(std::false_type{});
 }
 
-// Blocks that a sequence and head are cut into along time (a cluster): as many as run at once, where they have four
-// chunks each at least.  A cut costs a second walk for the state; 16 heads of 128 channels over 65536 tokens: 5382 us
-// uncut, 1979 in 4 parts (or in 8: a GPU has room for 15 clusters of 8 such blocks), 1502 in 16.
+// Blocks that a sequence and head are cut into along time (a cluster): as many as run at once, where they have two
+// chunks each at least.  A cut costs a second walk for the state, so two parts gain nothing (128 heads of 64 channels
+// over 1024 tokens: 51 us in two, 41 uncut); 16 heads of 64 over 1024 tokens in 8 parts 17 us, 16 heads of 128 channels
+// of bf16 over 65536 tokens 5382 uncut, 1979 in 4 (or in 8: a GPU has room for 15 clusters of 8 such blocks), 1502 in 16.
 uint32_t parts_of(const LinearArgs& a, int resident) {
     const uint64_t jobs = static_cast<uint64_t>(a.sequences) * a.heads, chunks = (a.max_new + kChunk - 1) / kChunk;
     uint32_t parts = 1;
     while (parts < kMostParts && jobs * parts <= 74ull * resident && chunks >= parts * 4) parts *= 2;
-    return parts;
+    return parts < 4 ? 1 : parts;
 }
 
 template <typename T, int D> cudaError_t launch(const LinearArgs& a, cudaStream_t s) {

@@ -19,9 +19,22 @@
 // A operand, V and S N-major B operands of that layout.  64 channels have a
 // second half of K' that is zero, as an A operand of 128 rows wants.
 //
+// What bounds it (one B200): the two chains.  A chunk of 64 channels takes 3.3
+// us, the outputs' four steps one after another (scores, weights, products,
+// stores); one of 128 channels 4.9 us, the state's warps (K' in parts 2.1,
+// waits for the products 1.2, the state 1.0).  16 sequences of 1568 tokens, 16
+// heads of 64: 71 us, 256 blocks on 148 SMs, where the bytes would take 22; one
+// of 65536 tokens, 16 heads of 128: 475 us (the states 197, the joining 10, the
+// outputs 270), where its bytes read twice would take 210.  Measured otherwise:
+// mma.sync with the state in registers 98 and 1502; the state in TMEM alone,
+// summed there, 71 and 456, but off by 2e-5 where nothing fades, as those sums
+// are cut off (now 6e-7); products issued one by one by an elected lane 20 %
+// slower; one part a sequence 2.3 ms for the long one.
+//
 // Parts: a first launch walks them for the state alone, each from zero, a
 // second one turns what they add into the states before them, and a third one
-// walks them for the outputs.  In between, a part's state (32 bits) lies in the
+// walks them for the outputs (blocks of a cluster that hand their states on
+// through distributed shared memory need all of them at once; launches do not).  In between, a part's state (32 bits) lies in the
 // rows of `out` that are the part's own, where nothing is kept yet; so no part is
 // shorter than that many rows, and a call whose out overlaps its inputs is not
 // cut.
@@ -493,8 +506,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool live = r < m;
             const float grow = ctl->power[r + 1] * a.scale;
             bf16* const out_at = static_cast<bf16*>(a.out) + h * a.o_hs;
-            // a row of O2 that is not finite is computed again, from what it sees (before any output, which may be
-            // where q is)
+            // a row of O2 that is not finite is computed again, from what it sees, if values of the chunk are not finite
+            // (before any output, which may be where q is)
             float zeros[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
@@ -506,7 +519,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const float zero = (zeros[0] + zeros[1]) + (zeros[2] + zeros[3]);
             const bool again = live && zero != 0.0f;  // (then it is NaN)
-            if (__any_sync(0xffffffffu, again)) {
+            bool bad = __any_sync(0xffffffffu, again);
+            if (bad) {  // (with finite values it is right as it is)
+                bad = false;
+                for (uint32_t x = lane; x < m * kRowChunks; x += 32) {
+                    float f[8];
+                    unpack(load8(v_at + (row_at(i) + x / kRowChunks) * a.v_ts + 8 * (x % kRowChunks)), f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) bad |= !isfinite(f[e]);
+                }
+                bad = __any_sync(0xffffffffu, bad);
+            }
+            if (bad) {
 #pragma unroll 1
                 for (int c = 0; c < D; c += 16) {
                     float y[16];
@@ -706,7 +730,7 @@ uint32_t parts_of(const LinearArgs& a) {
     return best;
 }
 
-// Whether two tensors' extents meet.
+// Whether two tensors' extents are apart.
 bool apart(const void* x, size_t x_ts, size_t x_hs, uint32_t x_heads, const void* y, size_t y_ts, size_t y_hs, uint32_t y_heads, const LinearArgs& a) {
     const auto end = [&](const void* p, size_t ts, size_t hs, uint32_t heads) {
         return reinterpret_cast<uintptr_t>(p) + ((a.tokens - 1) * ts + (heads - 1) * hs + a.head_dim) * sizeof(bf16);
@@ -732,9 +756,23 @@ template <int D> cudaError_t launch(const LinearArgs& a, const CUtensorMap (&map
 
 }  // namespace
 
+namespace {
+
+// 64 channels: the mma.sync kernel has two blocks a SM, chunks of 64 tokens and cuts that cost less (us, here and there):
+// 64 sequences of 16 heads with 128 tokens 53 and 37, 256 77 and 64, 512 120 and 113, 1024 198 and 211; one of 16 heads
+// with 128 tokens 8.3 and 7.4, 256 10.9 and 12.3, 512, cut along time, 15.6 and 13.6, 1024 26 and 17, 2048 30 and 31.
+// With 128 channels it has one block a SM: 16 heads with 128 tokens 14.9 and 15.0, 1024 sequences and heads 112 and 117.
+bool rather_there(const LinearArgs& a) {
+    const uint64_t jobs = static_cast<uint64_t>(a.sequences) * a.heads;
+    if (a.head_dim != 64) return false;
+    return a.max_new <= 192 || (a.max_new <= 512 && jobs > 148) || (a.max_new >= 384 && a.max_new <= 1024 && jobs * 4 <= 148);
+}
+
+}  // namespace
+
 cudaError_t launch_linear_attention_tc(const LinearArgs& a, int dtype, cudaStream_t s, bool* taken, uint32_t* launches) {
     *taken = false;
-    if (dtype != LWM_DTYPE_BF16 || a.head_dim < 64 || a.max_new <= 64) return cudaSuccess;
+    if (dtype != LWM_DTYPE_BF16 || a.head_dim < 64 || a.max_new <= 64 || rather_there(a)) return cudaSuccess;
     CUtensorMap maps[3];
     const uint32_t kv = a.heads / a.group_div.d;
     if (!rows_map(a.q, a.tokens, a.heads, a.head_dim, a.q_ts, a.q_hs, &maps[0]) || !rows_map(a.k, a.tokens, kv, a.head_dim, a.k_ts, a.k_hs, &maps[1]) ||

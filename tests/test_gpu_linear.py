@@ -7,7 +7,7 @@ Tolerances count roundings.  M is the same recurrence over absolute values, so
 the sum of all magnitudes that enter a value.  In chunks the weights (of the
 operands' type) and the state (bf16 or 11 bits) are rounded once, at most u =
 half a step of the type each and of different parts of M; keys times decay
-keep two parts, u^2.  In 32 bits a value passes through at most one product
+keep two parts at least, u^2.  In 32 bits a value passes through at most one product
 and one sum a token, the sums over channels, and powers of the decay: 2^-24
 each (|log lambda| 64 of them for the power's argument, 4 a chunk to carry
 it)."""
@@ -133,6 +133,12 @@ LENGTHS = [[1], [0, 1, 1], [3, 8, 1, 0], [9], [63, 64], [65, 0, 1, 130], [200, 1
 @pytest.mark.parametrize("heads,kv", [(1, 1), (3, 3), (4, 2)])
 def test_against_the_recurrence(ctx, news, d, dtype, heads, kv):
     call(ctx, gen(1), dtype, d, heads, kv, news, "mild", max(news))
+
+
+@pytest.mark.parametrize("news", [[300, 63, 64, 65, 0, 1, 127], [128, 256, 129, 9], [600], [384, 2, 130] + [1] * 50], ids=str)
+@pytest.mark.parametrize("d", [64, 128])
+def test_lengths_at_the_edges_of_longer_chunks(ctx, news, d):
+    call(ctx, gen(22), BF16, d, 4, 2, news, "mild", max(news))
 
 
 @pytest.mark.parametrize("news", [[1, 2], [5], [70, 129]], ids=str)
@@ -291,6 +297,26 @@ def test_captured_calls_replay(ctx, m):
     ctx.synchronize()
     assert torch.equal(out, first) and torch.equal(states, once)
     del graph
+
+
+@pytest.mark.parametrize("n", [300, 5000])
+def test_infinite_queries_leave_the_other_rows(ctx, n):
+    """Rows that are not finite for their own queries' sake, at finite values: theirs alone."""
+    g, d = gen(23), 64
+    q, k, v = (randn(g, n, 2, d, dtype=BF16) for _ in range(3))
+    a = DECAYS["mild"](2).cuda().float()
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    for o, x in ((clean, q), (out, q.clone())):
+        if o is out:
+            x[7::50, 1] = float("inf")
+            x[n - 1, 0, 3] = float("nan")
+        b = L.StateBatch(torch.zeros(1, 2, d, d, device="cuda"), ints([0, n]), n)
+        L.linear_attention_device(ctx, b, x, k, v, o, a)
+    ctx.synchronize()
+    rows = torch.ones(n, 2, dtype=torch.bool, device="cuda")
+    rows[7::50, 1] = rows[n - 1, 0] = False
+    assert torch.equal(out[rows], clean[rows])
+    assert torch.isnan(out[n - 1, 0]).all() and not torch.isfinite(out[7::50, 1]).any()
 
 
 @pytest.mark.parametrize("news", [1, 70])
