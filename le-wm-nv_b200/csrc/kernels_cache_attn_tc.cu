@@ -1108,7 +1108,7 @@ cudaError_t launch_cache_attention_tc(const CacheAttnArgs& a, int dtype, int sto
 // The prefix's blocks by the same costs: row tiles a block, and parts of the
 // keys, each of which writes 32-bit results that the tails' kernel reads.
 // What bounds the prefix (one B200): with few keys the chain of a block's steps and its start (1024 candidates of 16
-// heads behind 1568 tokens: 26 us, tensor pipe 15 %; the flops alone 8), with many the chain of scores, softmax and
+// heads behind 1568 tokens: 26 us, tensor pipe 15 %; its flops alone 3.4), with many the chain of scores, softmax and
 // product as in a sequence's own attention (64 candidates of 4 tokens and 32 heads behind 65536: 208 us, pipe 53 %, 106
 // at its peak).  8-bit codes: 16 groups of 64 with a window of 4096 75 us, expanding the codes beside that chain.  A part
 // more costs its results in 32 bits, written here and read by the tails; the choice made here was the quickest

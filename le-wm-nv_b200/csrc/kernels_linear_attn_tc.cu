@@ -21,11 +21,12 @@
 //
 // What bounds it (one B200): the two chains.  A chunk of 64 channels takes 3.3
 // us, the outputs' four steps one after another (scores, weights, products,
-// stores); one of 128 channels 4.9 us, the state's warps (K' in parts 2.1,
-// waits for the products 1.2, the state 1.0).  16 sequences of 1568 tokens, 16
-// heads of 64: 71 us, 256 blocks on 148 SMs, where the bytes would take 22; one
+// stores); one of 128 channels 4.6, the state's warps (K' in parts, waits for the
+// products, the state).  16 sequences of 1568 tokens, 16
+// heads of 64: 72 us, 256 blocks on 148 SMs, where the bytes would take 23; one
 // of 65536 tokens, 16 heads of 128: 475 us (the states 197, the joining 10, the
-// outputs 270), where its bytes read twice would take 210.  Measured otherwise:
+// outputs 270), where its bytes (keys and values read twice, 1.70 GB in DRAM)
+// would take 263.  Measured otherwise:
 // mma.sync with the state in registers 98 and 1502; the state in TMEM alone,
 // summed there, 71 and 456, but off by 2e-5 where nothing fades, as those sums
 // are cut off (now 6e-7); products issued one by one by an elected lane 20 %

@@ -4,6 +4,8 @@ reads a vehicle's history once for its candidates, linear attention whose
 states fork from the vehicle's, and the next token drawn from the logits.
 Every step of it is checked against 64 bits on what it read, and a graph of one
 step replays to the same rollout."""
+import os
+
 import numpy as np
 import pytest
 
@@ -185,3 +187,27 @@ def test_tokens_drawn_step_by_step(ctx, dtype, codes, vehicles, candidates, hist
         assert torch.equal(a, b)
     ctx.synchronize()
     del graph
+
+
+def test_the_guides_program_goes_on(ctx):
+    """The integration guide's second program after its first one, each result against 64 bits."""
+    guide = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
+    programs = [b.split("```")[0] for b in guide.split("```python\n")[1:] if "PagedCache" in b.split("```")[0] or "SharedPrefix" in b.split("```")[0]]
+    assert len(programs) == 2
+    names = dict(ctx=ctx, L=L)
+    exec(programs[0], names)
+    before = names["out"].clone()
+    names["out"].fill_(7.0)
+    exec(programs[1], names)
+    h, kv, d, S = names["heads"], names["kv"], names["dim"], names["S"]
+    assert torch.equal(names["out"], before)  # so few run by themselves
+    split = lambda x: (x[:, :h], x[:, h:h + kv], x[:, h + kv:])
+    states = torch.zeros(1, h, d, d, device="cuda")
+    for x, out, news, starts_from, kept in ((names["x"], names["seen"], [40], states, names["states"][:1]),
+                                            (names["y"], names["went"], [1] * S, names["states"][:1].expand(S, -1, -1, -1), names["states"][1:])):
+        want, mag, after, sizes = recurrence(*split(x), names["decay"], news, starts_from, d ** -0.5)
+        tol, state_tol = tolerances(BF16, d, max(news), names["decay"], want, mag, sizes, max(news) <= 8)
+        close(out, want, tol)
+        close(kept, after, state_tol)
+    x, u = names["logits"].double().cpu().numpy(), names["uniform"].double().cpu().numpy()
+    assert [definition(x[s], u[s], 0.9, 200, 0.95, 0.0)[0] for s in range(S)] == names["tokens"].tolist()
