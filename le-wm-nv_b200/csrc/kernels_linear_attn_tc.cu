@@ -14,36 +14,38 @@
 // a time, computed while the products before it run, then S), one that loads
 // by TMA, and an issuer of products for each of the two chains.  V has two
 // stages; Q and K are loaded again as soon as their products are done (the state
-// reads its keys from memory, with L2's help).  All
+// reads its keys from memory, with L2's help).  With 64 channels there is room
+// for two stages of Q and of P, so a chunk's weights are computed beside the
+// product of the one before with V.  All
 // tiles are rows of 64 channels (128 bytes, 128-byte swizzle); K' is an M-major
 // A operand, V and S N-major B operands of that layout.  64 channels have a
 // second half of K' that is zero, as an A operand of 128 rows wants.
 //
-// What bounds it (one B200): the two chains.  A chunk of 64 channels takes 3.3
-// us, the outputs' four steps one after another (scores, weights, products,
-// stores); one of 128 channels 4.6, the state's warps (K' in parts, waits for the
-// products, the state).  16 sequences of 1568 tokens, 16
-// heads of 64: 72 us, 256 blocks on 148 SMs, where the bytes would take 23; one
-// of 65536 tokens, 16 heads of 128: 475 us (the states 197, the joining 10, the
-// outputs 270), where its bytes (keys and values read twice, 1.70 GB in DRAM)
-// would take 263.  Measured otherwise:
-// mma.sync with the state in registers 98 and 1502; the state in TMEM alone,
-// summed there, 71 and 456, but off by 2e-5 where nothing fades, as those sums
-// are cut off (now 6e-7); products issued one by one by an elected lane 20 %
-// slower; one part a sequence 2.3 ms for the long one.
+// What bounds it (one B200): the instructions of the two chains, one after
+// another in few warps.  A chunk of 64 channels takes about 3.3 us, 4000 of its
+// cycles in the output warps and as many in the state's; one of 128 channels
+// 4.6, the state's warps (K' in parts, waits for the products, the state).  16
+// sequences of up to 1568 tokens, 16 heads of 64: 69.5 us, 256 blocks on 148
+// SMs, where the bytes would take 23; one of 65536 tokens, 16 heads of 128: 475
+// us (the states 193, the joining 9, the outputs 273), where its bytes (keys and
+// values read twice, 1.6 GB in DRAM) would take 250.  Measured otherwise:
+// mma.sync with the state in registers 98 and 1502; one stage of Q and P 72;
+// two sums of keys and values in TMEM by turns, so that no wait is left in the
+// state's warps, 73 and 470 (fewer cycles, more of them in each other's way);
+// the state in TMEM alone, summed there, 71 and 456, but off by 2e-5 where
+// nothing fades, as those sums are cut off (now 6e-7).
 //
 // Parts: a first launch walks them for the state alone, each from zero, a
 // second one turns what they add into the states before them, and a third one
-// walks them for the outputs (blocks of a cluster that hand their states on
-// through distributed shared memory need all of them at once; launches do not).  In between, a part's state (32 bits) lies in the
+// walks them for the outputs.  In between, a part's state (32 bits) lies in the
 // rows of `out` that are the part's own, where nothing is kept yet; so no part is
 // shorter than that many rows, and a call whose out overlaps its inputs is not
-// cut.
+// cut (65536 tokens of 16 heads, 64 channels 1.8 ms, 128 channels 3.3 ms).
 //
 // Rows behind the sequence's end are another's: their keys weigh zero, their
 // values are zeroed.  Infinities and NaN among the values make outputs that
-// are not finite, also of tokens that do not see them; such rows are computed
-// again, term by term.  Every wait is bounded: one that gives up marks the
+// are not finite, also of tokens that do not see them; such rows of their chunk
+// are computed again, term by term (about 2.5 ms a chunk).  Every wait is bounded: one that gives up marks the
 // block, which unwinds.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -63,7 +65,6 @@ constexpr int kLoadWarp = 12, kStateIssuer = 13, kOutIssuer = 14;
 constexpr uint32_t kMostParts = 64;
 // What a launch does: the whole, the state that a part adds, or the outputs of a part.
 constexpr int kWhole = 0, kAdds = 1, kGoesOn = 2;
-constexpr uint32_t kPCol = 0, kO1Col = 128;
 
 template <int D> struct Shape {
     static constexpr int kPanels = D / 64;
@@ -71,15 +72,17 @@ template <int D> struct Shape {
     static constexpr int kRound = 4096 / D;                 // tokens of a round of K', twice 16 bytes a thread
     static constexpr int kPart = kPanels * kRound * 128;    // of a part of it
     static constexpr int kS = D * D * 2;
-    static constexpr int kQ = 0, kK = kTile, kV = kK + kTile, kParts = kV + 2 * kTile, kSAt = kParts + 6 * kPart;
+    static constexpr int kAhead = D == 64 ? 2 : 1;          // stages of Q, and of scores and weights: room is there
+    static constexpr int kQ = 0, kK = kAhead * kTile, kV = kK + kTile, kParts = kV + 2 * kTile, kSAt = kParts + 6 * kPart;
     static constexpr int kStage = kSAt + kS;                // outputs on their way, 32 rows of 32 channels a warp
     static constexpr int kZero = kStage + 4 * 2048;         // 64 channels: the empty half of K'
     static constexpr int kBytes = kZero + (D == 64 ? kRound * 128 : 0) + 1024;  // + alignment
-    static constexpr uint32_t kO2Col = kO1Col + D, kSCol = kO2Col + D;
+    static constexpr uint32_t kPCol = 0, kO1Col = kAhead * 128, kO2Col = kO1Col + D, kSCol = kO2Col + D;  // of TMEM
+    static_assert(kSCol + D <= 512, "TMEM");
 };
 
 struct Control {
-    uint64_t q_full, q_empty, k_full, k_empty, v_full[2], v_empty[2], v_raw, scores, weights, between, pv, o_free, parts[2], kv[2], s_copy, drain;
+    uint64_t q_full[2], q_empty[2], k_full, k_empty, v_full[2], v_empty[2], v_raw, scores[2], weights[2], between, pv, o_free, parts[2], kv[2], s_copy, drain;
     uint32_t tmem;
     int dead;     // a wait gave up
     float power[kChunk + 1];  // lambda^i
@@ -204,16 +207,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (decay < -200.0f) decay = -200.0f;  // (e^-200 is zero; minus infinity times zero would be NaN)
 
     if (threadIdx.x == 0) {
-        tc::mbar_init(&ctl->q_full, 1);
-        tc::mbar_init(&ctl->q_empty, 2);
         for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&ctl->q_full[i], 1);
+            tc::mbar_init(&ctl->q_empty[i], 2);
+            tc::mbar_init(&ctl->scores[i], 1);
+            tc::mbar_init(&ctl->weights[i], kOutWarps);
             tc::mbar_init(&ctl->v_full[i], 1);
             tc::mbar_init(&ctl->v_empty[i], 2);
             tc::mbar_init(&ctl->parts[i], kStateWarps);
             tc::mbar_init(&ctl->kv[i], 1);
         }
-        for (uint64_t* b : {&ctl->k_full, &ctl->k_empty, &ctl->v_raw, &ctl->scores, &ctl->between, &ctl->pv}) tc::mbar_init(b, 1);
-        tc::mbar_init(&ctl->weights, kOutWarps);
+        for (uint64_t* b : {&ctl->k_full, &ctl->k_empty, &ctl->v_raw, &ctl->between, &ctl->pv}) tc::mbar_init(b, 1);
         tc::mbar_init(&ctl->o_free, kOutWarps);
         tc::mbar_init(&ctl->s_copy, kStateWarps);
         tc::mbar_init(&ctl->drain, 2);
@@ -234,6 +238,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const auto* const k_at = static_cast<const bf16*>(a.k) + hk * a.k_hs;
     const auto* const v_at = static_cast<const bf16*>(a.v) + hk * a.v_hs;
     auto tokens_of = [&](uint32_t i) { return min(static_cast<uint32_t>(kChunk), v.n - i * kChunk); };
+    // chunk i's stage of Q, scores and weights, and the parity of its turn there
+    constexpr uint32_t kAhead = S::kAhead;
+    auto stage_of = [&](uint32_t i) { return (i - first) % kAhead; };
+    auto turn_of = [&](uint32_t i) { return (i - first) / kAhead & 1; };
     auto row_at = [&](uint32_t i) { return static_cast<size_t>(v.start) + i * kChunk; };
 
     // ------------------------------------------------------------ loads
@@ -264,9 +272,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (i > from) fine = wait(&ctl->k_empty, (i - from - 1) & 1, ctl, 1, err, s);
                 if (!fine) break;
                 tile(&k_map, hk, i, base + S::kK, &ctl->k_full);
-                if (i > from) fine = wait(&ctl->q_empty, (i - from - 1) & 1, ctl, 3, err, s);
+                const uint32_t at = stage_of(i);
+                if (i - from >= kAhead) fine = wait(&ctl->q_empty[at], turn_of(i) ^ 1, ctl, 3, err, s);
                 if (!fine) break;
-                tile(&q_map, h, i, base + S::kQ, &ctl->q_full);
+                tile(&q_map, h, i, base + S::kQ + at * S::kTile, &ctl->q_full[at]);
             }
             if (use >= 2) fine = wait(&ctl->v_empty[st], (round - 1) & 1, ctl, 2, err, s);
             if (!fine) break;
@@ -396,16 +405,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t i = from; i < end && fine; ++i, ++use) {
             const uint32_t st = use & 1, m = tokens_of(i), rounds = (m + S::kRound - 1) / S::kRound;
             if (whole) {
-                fine = wait(&ctl->s_copy, (i - from) & 1, ctl, 17, err, s) && wait(&ctl->q_full, (i - from) & 1, ctl, 15, err, s);
+                fine = wait(&ctl->s_copy, (i - from) & 1, ctl, 17, err, s) && wait(&ctl->q_full[stage_of(i)], turn_of(i), ctl, 15, err, s);
                 if (fine && i > from) fine = wait(&ctl->o_free, (i - from - 1) & 1, ctl, 16, err, s);
                 if (!fine) break;
                 tc::fence_after();
 #pragma unroll
                 for (int k = 0; k < kSteps; k += 2)
-                    mma2(tmem + kO1Col, low_desc(base + S::kQ + (k >> 2) * kChunk * 128 + (k & 3) * 32, 16), 2,
+                    mma2(tmem + S::kO1Col, low_desc(base + S::kQ + stage_of(i) * S::kTile + (k >> 2) * kChunk * 128 + (k & 3) * 32, 16), 2,
                          low_desc(base + S::kSAt + k * 2048, D * 128), 128, kB, k > 0);
                 tc::commit_w(&ctl->between);
-                tc::commit_w(&ctl->q_empty);
+                tc::commit_w(&ctl->q_empty[stage_of(i)]);
             }
             fine = wait(&ctl->v_full[st], (use >> 1) & 1, ctl, 12, err, s);
             for (uint32_t round = 0; round < rounds && fine; ++round, ++turn) {
@@ -436,31 +445,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t kP = idesc(kChunk, false, false), kO = idesc(D, false, true);
         bool fine = true;
         auto scores = [&](uint32_t i) {
-            fine = wait(&ctl->q_full, (i - from) & 1, ctl, 20, err, s) && wait(&ctl->k_full, (i - from) & 1, ctl, 21, err, s);
+            fine = wait(&ctl->q_full[stage_of(i)], turn_of(i), ctl, 20, err, s) && wait(&ctl->k_full, (i - from) & 1, ctl, 21, err, s);
             if (!fine) return;
             tc::fence_after();
 #pragma unroll
             for (int k = 0; k < kSteps; k += 2) {
                 const uint32_t off = (k >> 2) * kChunk * 128 + (k & 3) * 32;
-                mma2(tmem + kPCol, low_desc(base + S::kQ + off, 16), 2, low_desc(base + S::kK + off, 16), 2, kP, k > 0);
+                mma2(tmem + S::kPCol + stage_of(i) * 128, low_desc(base + S::kQ + stage_of(i) * S::kTile + off, 16), 2, low_desc(base + S::kK + off, 16), 2, kP, k > 0);
             }
-            tc::commit_w(&ctl->scores);
-            tc::commit_w(&ctl->q_empty);
+            tc::commit_w(&ctl->scores[stage_of(i)]);
+            tc::commit_w(&ctl->q_empty[stage_of(i)]);
             tc::commit_w(&ctl->k_empty);
         };
         scores(from);
         for (uint32_t i = from; i < end && fine; ++i, ++use) {
             const uint32_t st = use & 1;
-            fine = wait(&ctl->v_full[st], (use >> 1) & 1, ctl, 24, err, s) && wait(&ctl->weights, (i - from) & 1, ctl, 27, err, s);
+            // (over the weights of the chunk before, which their product has read)
+            if (kAhead == 2 && i + 1 < end) scores(i + 1);
+            if (!fine) break;
+            fine = wait(&ctl->v_full[st], (use >> 1) & 1, ctl, 24, err, s) && wait(&ctl->weights[stage_of(i)], turn_of(i), ctl, 27, err, s);
             if (fine && i > from) fine = wait(&ctl->o_free, (i - from - 1) & 1, ctl, 28, err, s);
             if (!fine) break;
             tc::fence_after();
 #pragma unroll
             for (int k = 0; k < kChunk / 16; k += 2)
-                mma2_t(tmem + S::kO2Col, tmem + kPCol + 8 * k, low_desc(base + S::kV + st * S::kTile + k * 2048, kChunk * 128), 128, kO, k > 0);
+                mma2_t(tmem + S::kO2Col, tmem + S::kPCol + stage_of(i) * 128 + 8 * k, low_desc(base + S::kV + st * S::kTile + k * 2048, kChunk * 128), 128, kO, k > 0);
             tc::commit_w(&ctl->v_empty[st]);
             tc::commit_w(&ctl->pv);
-            if (i + 1 < end) scores(i + 1);  // (over the weights, which the product before it has read)
+            if (kAhead == 1 && i + 1 < end) scores(i + 1);  // (over the weights, which the product before it has read)
         }
     };
     auto outputs = [&] {
@@ -468,11 +480,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t r = threadIdx.x;  // token of the chunk
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
         bool fine = true;
-        for (uint32_t i = from; i < end && fine; ++i) {
-            const uint32_t m = tokens_of(i), turn = (i - from) & 1;
-            fine = wait(&ctl->scores, turn, ctl, 23, err, s);
-            if (!fine) break;
+        auto weigh = [&](uint32_t i) {
+            fine = wait(&ctl->scores[stage_of(i)], turn_of(i), ctl, 23, err, s);
+            if (!fine) return;
             tc::fence_after();
+            const uint32_t p_at = lanes + S::kPCol + stage_of(i) * 128;
             // weights: what a token does not see is zero
 #pragma unroll 1
             for (int c = 0; c < kChunk; c += 32) {
@@ -482,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int e = 0; e < 16; ++e) p[e] = 0u;
                 } else {
                     float x[32];
-                    tmem_ld32(lanes + kPCol + c, x);
+                    tmem_ld32(p_at + c, x);
                     tc::tmem_ld_wait();
                     const float* const w = ctl->power + (r - c);
                     if (c < warp * 32) {
@@ -495,14 +507,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) p[e] = pack2(x[2 * e], x[2 * e + 1], bf16{});
                 }
-                tc::tmem_st8u(lanes + kPCol + c / 2, reinterpret_cast<const uint32_t(&)[8]>(p[0]));
-                tc::tmem_st8u(lanes + kPCol + c / 2 + 8, reinterpret_cast<const uint32_t(&)[8]>(p[8]));
+                tc::tmem_st8u(p_at + c / 2, reinterpret_cast<const uint32_t(&)[8]>(p[0]));
+                tc::tmem_st8u(p_at + c / 2 + 8, reinterpret_cast<const uint32_t(&)[8]>(p[8]));
             }
             tc::tmem_st_wait();
             tc::fence_before();
-            arrive_w(&ctl->weights);
+            arrive_w(&ctl->weights[stage_of(i)]);
+        };
+        auto write = [&](uint32_t i) {
+            const uint32_t m = tokens_of(i), turn = (i - from) & 1;
             fine = wait(&ctl->between, turn, ctl, 25, err, s) && wait(&ctl->pv, turn, ctl, 26, err, s);
-            if (!fine) break;
+            if (!fine) return;
             tc::fence_after();
             const bool live = r < m;
             const float grow = ctl->power[r + 1] * a.scale;
@@ -565,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
                 float x[32], y[32];
-                tmem_ld32(lanes + kO1Col + c, x);
+                tmem_ld32(lanes + S::kO1Col + c, x);
                 tmem_ld32(lanes + S::kO2Col + c, y);
                 tc::tmem_ld_wait();
                 __syncwarp();  // (the rows before these have been read)
@@ -585,6 +600,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc::fence_before();
             arrive_w(&ctl->o_free);
+        };
+        if (kAhead == 2) weigh(from);
+        for (uint32_t i = from; i < end && fine; ++i) {
+            // the next chunk's weights beside this one's product with V
+            if (kAhead == 1) weigh(i);
+            else if (i + 1 < end) weigh(i + 1);
+            if (fine) write(i);
         }
     };
 
