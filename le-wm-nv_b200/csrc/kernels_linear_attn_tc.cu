@@ -40,7 +40,7 @@
 // walks them for the outputs.  In between, a part's state (32 bits) lies in the
 // rows of `out` that are the part's own, where nothing is kept yet; so no part is
 // shorter than that many rows, and a call whose out overlaps its inputs is not
-// cut (65536 tokens of 16 heads, 64 channels 1.8 ms, 128 channels 3.3 ms).
+// cut here (most of those go by clusters on mma.sync).
 //
 // Rows behind the sequence's end are another's: their keys weigh zero, their
 // values are zeroed.  Infinities and NaN among the values make outputs that
@@ -761,12 +761,15 @@ bool apart(const void* x, size_t x_ts, size_t x_hs, uint32_t x_heads, const void
     return end(x, x_ts, x_hs, x_heads) <= reinterpret_cast<uintptr_t>(y) || end(y, y_ts, y_hs, y_heads) <= reinterpret_cast<uintptr_t>(x);
 }
 
-template <int D> cudaError_t launch(const LinearArgs& a, const CUtensorMap (&maps)[3], cudaStream_t s, uint32_t* launches) {
+// Whether out's rows may not hold a state, as an input's lie among them.
+bool overlaps(const LinearArgs& a) {
     const uint32_t kv = a.heads / a.group_div.d;
-    uint32_t parts = parts_of(a);
-    if (!apart(a.q, a.q_ts, a.q_hs, a.heads, a.out, a.o_ts, a.o_hs, a.heads, a) || !apart(a.k, a.k_ts, a.k_hs, kv, a.out, a.o_ts, a.o_hs, a.heads, a) ||
-        !apart(a.v, a.v_ts, a.v_hs, kv, a.out, a.o_ts, a.o_hs, a.heads, a))
-        parts = 1;
+    return !apart(a.q, a.q_ts, a.q_hs, a.heads, a.out, a.o_ts, a.o_hs, a.heads, a) || !apart(a.k, a.k_ts, a.k_hs, kv, a.out, a.o_ts, a.o_hs, a.heads, a) ||
+           !apart(a.v, a.v_ts, a.v_hs, kv, a.out, a.o_ts, a.o_hs, a.heads, a);
+}
+
+template <int D> cudaError_t launch(const LinearArgs& a, const CUtensorMap (&maps)[3], cudaStream_t s, uint32_t* launches) {
+    const uint32_t parts = overlaps(a) ? 1 : parts_of(a);
     const uint32_t per = chunks_a_part(a.max_new, parts);
     if (parts == 1) return launch_mode<D, kWhole>(a, maps, per, 1, s);
     *launches = 3;
@@ -785,8 +788,11 @@ namespace {
 // 64 sequences of 16 heads with 128 tokens 53 and 37, 256 77 and 64, 512 120 and 113, 1024 198 and 211; one of 16 heads
 // with 128 tokens 8.3 and 7.4, 256 10.9 and 12.3, 512, cut along time, 15.6 and 13.6, 1024 26 and 17, 2048 30 and 31.
 // With 128 channels it has one block a SM: 16 heads with 128 tokens 14.9 and 15.0, 1024 sequences and heads 112 and 117.
+// Its cuts along time need no room in `out`, so it has the long sequences of a call whose out overlaps its inputs (65536
+// tokens, uncut here and there: 16 heads of 64 channels 1239 and 536, 16 of 128 2065 and 2525, 4 of 128 2057 and 650).
 bool rather_there(const LinearArgs& a) {
     const uint64_t jobs = static_cast<uint64_t>(a.sequences) * a.heads;
+    if (parts_of(a) > 1 && (a.head_dim == 64 || jobs * 16 <= 148) && overlaps(a)) return true;
     if (a.head_dim != 64) return false;
     return a.max_new <= 192 || (a.max_new <= 512 && jobs > 148) || (a.max_new >= 384 && a.max_new <= 1024 && jobs * 4 <= 148);
 }

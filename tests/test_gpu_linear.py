@@ -259,6 +259,29 @@ def test_out_may_be_q_and_results_repeat(ctx):
         assert torch.equal(states[0], states[1]) and torch.equal(states[0], states[2])
 
 
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("where,heads", [("q", 2), ("beside", 2), ("q", 12)])
+def test_long_sequences_in_place(ctx, dtype, d, where, heads):
+    """Out is q, or lies between the rows of a fused projection's output: no row of it may hold a state."""
+    g, n, h = gen(24), 5000, heads
+    fused = randn(g, n, 4 * h, d, dtype=dtype)
+    kept = fused.clone()
+    q, k, v, out = (fused[:, i * h:(i + 1) * h] for i in range(4))
+    if where == "q":
+        out = q
+    a = DECAYS["mild"](h).cuda().float()
+    states = torch.zeros(1, h, d, d, device="cuda")
+    L.linear_attention_device(ctx, L.StateBatch(states, ints([0, n]), n), q, k, v, out, a)
+    ctx.synchronize()
+    first = torch.zeros_like(states)
+    want, mag, after, sizes = recurrence(kept[:, :h], k, v, a, [n], first, d ** -0.5)
+    tol, state_tol = tolerances(dtype, d, n, a, want, mag, sizes, False)
+    close(out, want, tol)
+    close(states, after, state_tol)
+    rest = slice(h, None) if where == "q" else slice(0, 3 * h)
+    assert torch.equal(fused[:, rest], kept[:, rest])
+
+
 def test_a_rollout_in_pieces_is_the_whole(ctx):
     """A history in one call, or in chunks and single tokens with the state handed on."""
     g, n = gen(13), 150
