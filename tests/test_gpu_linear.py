@@ -214,7 +214,18 @@ def test_half_precision_keeps_large_and_small_states(ctx):
 @pytest.mark.parametrize("value", [float("inf"), float("nan")])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_infinities_and_nan_reach_later_tokens_of_their_head_only(ctx, where, value, dtype):
-    g, d, n, at = gen(11), 64, 150, 77
+    infinities(ctx, where, value, dtype, 64, 150, 77)
+
+
+@pytest.mark.parametrize("where", ["v", "k", "q"])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("d,n,at", [(64, 300, 77), (64, 3000, 1600), (128, 300, 200), (128, 3000, 700), (128, 70, 69)])
+def test_infinities_and_nan_in_long_sequences(ctx, where, value, d, n, at):
+    infinities(ctx, where, value, BF16, d, n, at)
+
+
+def infinities(ctx, where, value, dtype, d, n, at):
+    g = gen(11)
     x = {name: randn(g, n, 2, d, dtype=dtype) for name in "qkv"}
     x[where][at, 1, 5] = value
     states = randn(g, 1, 2, d, d)
@@ -300,12 +311,12 @@ def test_a_rollout_in_pieces_is_the_whole(ctx):
     close(states, after, state_tol + 6 * E32 * sizes)
 
 
-@pytest.mark.parametrize("m", [1, 90])
-def test_captured_calls_replay(ctx, m):
+@pytest.mark.parametrize("m,d", [(1, 64), (90, 64), (300, 64), (3000, 64), (300, 128), (3000, 128)])
+def test_captured_calls_replay(ctx, m, d):
     g = gen(14)
-    q, k, v = (randn(g, 2 * m, 2, 64, dtype=BF16) for _ in range(3))
+    q, k, v = (randn(g, 2 * m, 2, d, dtype=BF16) for _ in range(3))
     a = DECAYS["mild"](2).float().cuda()
-    states, out = randn(g, 2, 2, 64, 64), torch.empty_like(q)
+    states, out = randn(g, 2, 2, d, d), torch.empty_like(q)
     held = states.clone()
     b = L.StateBatch(states, ints([0, m, 2 * m]), 2 * m, m)
     L.linear_attention_device(ctx, b, q, k, v, out, a)
@@ -342,17 +353,17 @@ def test_infinite_queries_leave_the_other_rows(ctx, n):
     assert torch.isnan(out[n - 1, 0]).all() and not torch.isfinite(out[7::50, 1]).any()
 
 
-@pytest.mark.parametrize("news", [1, 70])
-def test_what_does_not_fit_is_skipped_and_reported(ctx, news):
+@pytest.mark.parametrize("news,d", [(1, 32), (70, 32), (300, 64), (3000, 64), (300, 128), (3000, 128)])
+def test_what_does_not_fit_is_skipped_and_reported(ctx, news, d):
     g, tokens = gen(15), 3 * news
-    q, k, v = (randn(g, tokens, 1, 32, dtype=BF16) for _ in range(3))
+    q, k, v = (randn(g, tokens, 1, d, dtype=BF16) for _ in range(3))
     a = torch.zeros(1, device="cuda")
     for starts, source, target, message in (
             ([0, news, tokens + 1, tokens], [0, 1, 2], [0, 1, 2], "sequence [12]: starts are out of order or beyond the packed rows"),
             ([0, news, 2 * news, tokens], [0, 9, 2], [0, 1, 2], "sequence 1: state slot 9 is not in the pool"),
             ([0, news, 2 * news, tokens], [0, 1, 2], [0, 3, 2], "sequence 1: state slot 3 is not in the pool"),
             ([0, news, news, tokens], [0, 1, 2], [0, 1, 2], "sequence 2: more new tokens")):
-        states = randn(g, 3, 1, 32, 32)
+        states = randn(g, 3, 1, d, d)
         before, out = states.clone(), torch.full_like(q, 5.0)
         b = L.StateBatch(states, ints(starts), tokens, news, ints(source), ints(target))
         L.linear_attention_device(ctx, b, q, k, v, out, a)
@@ -361,7 +372,7 @@ def test_what_does_not_fit_is_skipped_and_reported(ctx, news):
         ctx.synchronize()
         s = 2 if "sequence 2" in message else 1
         assert torch.equal(states[s], before[s])
-        want, mag, after, sizes = recurrence(q[:news], k[:news], v[:news], a, [news], before[:1], 32 ** -0.5)
-        tol, state_tol = tolerances(BF16, 32, news, a, want, mag, sizes, news <= 8)
+        want, mag, after, sizes = recurrence(q[:news], k[:news], v[:news], a, [news], before[:1], d ** -0.5)
+        tol, state_tol = tolerances(BF16, d, news, a, want, mag, sizes, news <= 8)
         close(out[:news], want, tol)
         close(states[:1], after, state_tol)
