@@ -134,6 +134,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
     float decay = a.log_decay[h];
     if (decay < -200.0f) decay = -200.0f;  // (e^-200 is zero; minus infinity times zero would be NaN)
     for (int i = threadIdx.x; i <= kChunk; i += S::kThreads) power[i] = expf(decay * i);
+    meet();  // (before any warp marks a chunk there)
 
     const uint32_t smem_a = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
     // this block's chunks of the sequence
