@@ -42,10 +42,15 @@ template <int D> struct StepShape {
     static constexpr int kRowGroups = kThreads / kCols, kRows = D / kRowGroups;
 };
 
+template <int D> struct alignas(16) Channels {  // of a token, read four at a time
+    float x[D];
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(StepShape<D>::kThreads) linear_step_kernel(const __grid_constant__ LinearArgs a) {
     using S = StepShape<D>;
-    __shared__ float q_s[D], k_s[D], v_s[D];
+    __shared__ Channels<D> q_s, k_s, v_s;
+    static_assert(alignof(decltype(v_s)) == sizeof(float4), "read as float4");
     __shared__ float4 part[S::kRowGroups][S::kCols];
     const uint32_t s = a.head_div.div(blockIdx.x), h = blockIdx.x - s * a.heads;
     const StateView v = state_view(a, s, h == 0 && threadIdx.x == 0);
@@ -67,14 +72,14 @@ __global__ void __launch_bounds__(StepShape<D>::kThreads) linear_step_kernel(con
             const T* src = w == 0 ? static_cast<const T*>(a.q) + tok * a.q_ts + h * a.q_hs
                            : w == 1 ? static_cast<const T*>(a.k) + tok * a.k_ts + hk * a.k_hs
                                     : static_cast<const T*>(a.v) + tok * a.v_ts + hk * a.v_hs;
-            (w == 0 ? q_s : w == 1 ? k_s : v_s)[ch] = static_cast<float>(src[ch]);
+            (w == 0 ? q_s : w == 1 ? k_s : v_s).x[ch] = static_cast<float>(src[ch]);
         }
         __syncthreads();
-        const float4 x = *reinterpret_cast<const float4*>(v_s + 4 * c);
+        const float4 x = *reinterpret_cast<const float4*>(v_s.x + 4 * c);
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < S::kRows; ++j) {
-            const float k = k_s[r + j * S::kRowGroups], q = q_s[r + j * S::kRowGroups];
+            const float k = k_s.x[r + j * S::kRowGroups], q = q_s.x[r + j * S::kRowGroups];
             st[j].x = fmaf(lambda, st[j].x, k * x.x), o.x = fmaf(q, st[j].x, o.x);
             st[j].y = fmaf(lambda, st[j].y, k * x.y), o.y = fmaf(q, st[j].y, o.y);
             st[j].z = fmaf(lambda, st[j].z, k * x.z), o.z = fmaf(q, st[j].z, o.z);

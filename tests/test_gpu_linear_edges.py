@@ -38,3 +38,20 @@ def test_infinities_in_the_first_chunk_of_many_sequences(ctx, d, dtype):
     assert not torch.isfinite(out[~before][:, :, 3]).any()
     others = [c for c in range(d) if c != 3]
     close(out[:, :, others], want[:, :, others], tol[:, :, others])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_few_tokens_use_every_channel(ctx, d, dtype):
+    """Values whose channels differ by powers of two, over several tokens: each is read from where it was put."""
+    g, n, heads = gen(31), 5, 3
+    q, k = (randn(g, n, heads, d, dtype=dtype) for _ in range(2))
+    v = (randn(g, n, heads, d) * torch.exp2((torch.arange(d, device="cuda") % 9 - 4).float())).to(dtype)
+    a = DECAYS["mild"](heads).cuda()
+    states, out = randn(g, 1, heads, d, d), torch.empty_like(q)
+    want, mag, after, sizes = recurrence(q, k, v, a.float(), [n], states, d ** -0.5)
+    L.linear_attention_device(ctx, L.StateBatch(states, ints([0, n]), n), q, k, v, out, a.float())
+    ctx.synchronize()
+    tol, state_tol = tolerances(dtype, d, n, a, want, mag, sizes, True)
+    close(out, want, tol)
+    close(states, after, state_tol)
