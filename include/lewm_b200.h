@@ -966,7 +966,9 @@ lwm_status lwm_cache_attention_shared_device(lwm_ctx* ctx, const lwm_paged_cache
  * hold other values until the call's work is done.
  *
  * q, out [tokens, heads, head_dim], k, v [tokens, kv_heads, head_dim] of
- * `dtype` (bf16 or f16; out may be q); query head h and its state use kv head
+ * `dtype` (bf16 or f16).  In place: out may be q, and with as many kv_heads as
+ * heads k or v (the same rows and strides; otherwise no element of out is one of
+ * theirs).  Query head h and its state use kv head
  * h / (heads / kv_heads).  log_decay [heads] f32, natural logarithms, zero
  * (nothing fades) or below; minus infinity: every token starts afresh.
  * In chunks, the weights q.k lambda^n are rounded to dtype for their product

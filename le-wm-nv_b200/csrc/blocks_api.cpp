@@ -458,6 +458,16 @@ lwm_status lwm_linear_attention_device(lwm_ctx* ctx, const lwm_state_batch* b, c
     CtxView c;
     if (!lwm::ctx_view(ctx, &c)) return bad("null context");
     if (b->sequences == 0) return LWM_OK;
+    if (b->max_new) {
+        // heads that share keys and values read them at different times: none may write there
+        const auto over = [&](const char* name, const void* p, uint64_t ts, uint64_t hs) {
+            const bool same = x->kv_heads == b->heads && (b->tokens == 1 || ts == x->out_token_stride) &&
+                              (b->heads == 1 || hs == x->out_head_stride);
+            return p != x->out || same ? LWM_OK : bad(std::string("out may be ") + name + " only with as many kv_heads as heads and the same strides");
+        };
+        LWM_TRY(over("k", x->k, x->k_token_stride, x->k_head_stride));
+        LWM_TRY(over("v", x->v, x->v_token_stride, x->v_head_stride));
+    }
     lwm::LinearArgs a{};
     a.q = x->q, a.k = x->k, a.v = x->v, a.out = x->out;
     a.q_ts = x->q_token_stride, a.q_hs = x->q_head_stride;

@@ -51,6 +51,7 @@
 #include <cudaTypedefs.h>
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 
 #include "lwm_linear_attn.cuh"
 #include "lwm_tc.cuh"
@@ -761,6 +762,25 @@ bool apart(const void* x, size_t x_ts, size_t x_hs, uint32_t x_heads, const void
     return end(x, x_ts, x_hs, x_heads) <= reinterpret_cast<uintptr_t>(y) || end(y, y_ts, y_hs, y_heads) <= reinterpret_cast<uintptr_t>(x);
 }
 
+// Whether an element of out may be one of x's (k or v): not where the extents are apart, nor where they interleave in a
+// way that strides show (a fused projection's rows: what a token, or a head, has of each lies apart; heads that have
+// q, k, v and out side by side: so it is for each of them).
+bool may_share(const void* x, size_t x_ts, size_t x_hs, uint32_t x_heads, const LinearArgs& a) {
+    if (apart(x, x_ts, x_hs, x_heads, a.out, a.o_ts, a.o_hs, a.heads, a)) return false;
+    const size_t d = a.head_dim;
+    const auto by = (static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.out)) - static_cast<int64_t>(reinterpret_cast<uintptr_t>(x))) /
+                    static_cast<int64_t>(sizeof(bf16));
+    const auto turn = [&](size_t n) { return static_cast<size_t>((by % static_cast<int64_t>(n) + static_cast<int64_t>(n)) % static_cast<int64_t>(n)); };
+    // repeated every `outer` elements, with this much of either in between
+    const auto beside = [&](size_t outer, size_t x_span, size_t o_span) {
+        return outer && x_span <= turn(outer) && turn(outer) + o_span <= outer;
+    };
+    if (x_ts == a.o_ts && beside(x_ts, (x_heads - 1) * x_hs + d, (a.heads - 1) * a.o_hs + d)) return false;
+    if (x_hs == a.o_hs && beside(x_hs, (a.tokens - 1) * x_ts + d, (a.tokens - 1) * a.o_ts + d)) return false;
+    const size_t all = std::gcd(std::gcd(x_ts, a.o_ts), std::gcd(x_heads > 1 ? x_hs : 0, a.heads > 1 ? a.o_hs : 0));
+    return !beside(all, d, d);
+}
+
 // Whether out's rows may not hold a state, as an input's lie among them.
 bool overlaps(const LinearArgs& a) {
     const uint32_t kv = a.heads / a.group_div.d;
@@ -779,10 +799,6 @@ template <int D> cudaError_t launch(const LinearArgs& a, const CUtensorMap (&map
     e = cudaGetLastError();
     return e == cudaSuccess ? launch_mode<D, kGoesOn>(a, maps, per, parts, s) : e;
 }
-
-}  // namespace
-
-namespace {
 
 // 64 channels: the mma.sync kernel has two blocks a SM, chunks of 64 tokens and cuts that cost less (us, here and there):
 // 64 sequences of 16 heads with 128 tokens 53 and 37, 256 77 and 64, 512 120 and 113, 1024 198 and 211; one of 16 heads
@@ -804,6 +820,9 @@ cudaError_t launch_linear_attention_tc(const LinearArgs& a, int dtype, cudaStrea
     if (dtype != LWM_DTYPE_BF16 || a.head_dim < 64 || a.max_new <= 64 || rather_there(a)) return cudaSuccess;
     CUtensorMap maps[3];
     const uint32_t kv = a.heads / a.group_div.d;
+    // (the state reads its keys from memory beside the outputs of the same chunk, and rows that are computed again
+    // read values; the other kernel has a chunk's in shared memory before it writes)
+    if (may_share(a.k, a.k_ts, a.k_hs, kv, a) || may_share(a.v, a.v_ts, a.v_hs, kv, a)) return cudaSuccess;
     if (!rows_map(a.q, a.tokens, a.heads, a.head_dim, a.q_ts, a.q_hs, &maps[0]) || !rows_map(a.k, a.tokens, kv, a.head_dim, a.k_ts, a.k_hs, &maps[1]) ||
         !rows_map(a.v, a.tokens, kv, a.head_dim, a.v_ts, a.v_hs, &maps[2]))
         return cudaSuccess;  // (strides that a tensor map does not take)

@@ -55,3 +55,76 @@ def test_few_tokens_use_every_channel(ctx, d, dtype):
     tol, state_tol = tolerances(dtype, d, n, a, want, mag, sizes, True)
     close(out, want, tol)
     close(states, after, state_tol)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (BF16, 128), (F16, 64), (BF16, 32)])
+@pytest.mark.parametrize("news", [[1, 8], [300, 70, 1400], [5000]], ids=str)
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_out_may_be_the_keys_or_the_values(ctx, where, news, dtype, d):
+    """In place of k or v, of heads of their own: what a token's state and outputs read is read before it is written."""
+    g, n, heads = gen(32), sum(news), 3
+    x = {name: randn(g, n, heads, d, dtype=dtype) for name in "qkv"}
+    kept = {name: t.clone() for name, t in x.items()}
+    a = DECAYS["mild"](heads).cuda()
+    states = torch.zeros(len(news), heads, d, d, device="cuda")
+    starts = [sum(news[:i]) for i in range(len(news) + 1)]
+    L.linear_attention_device(ctx, L.StateBatch(states, ints(starts), n, max(news)), x["q"], x["k"], x["v"], x[where], a.float())
+    ctx.synchronize()
+    want, mag, after, sizes = recurrence(kept["q"], kept["k"], kept["v"], a.float(), news, torch.zeros_like(states), d ** -0.5)
+    tol, state_tol = tolerances(dtype, d, max(news), a, want, mag, sizes, max(news) <= 8)
+    close(x[where], want, tol)
+    close(states, after, state_tol)
+    for name in "qkv":
+        assert name == where or torch.equal(x[name], kept[name])
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_out_over_values_that_are_not_finite(ctx, value):
+    g, n, heads, d, at = gen(33), 700, 2, 128, 200
+    q, k, v = (randn(g, n, heads, d, dtype=BF16) for _ in range(3))
+    a = DECAYS["mild"](heads).cuda()
+    states = torch.zeros(1, heads, d, d, device="cuda")
+    want, mag, _, sizes = recurrence(q, k, v, a.float(), [n], states, d ** -0.5)
+    tol, _ = tolerances(BF16, d, n, a, want, mag, sizes, False)
+    v[at, 1, 5] = value
+    L.linear_attention_device(ctx, L.StateBatch(states, ints([0, n]), n), q, k, v, v, a.float())
+    ctx.synchronize()
+    close(v[:at], want[:at], tol[:at])
+    assert not torch.isfinite(v[at:, 1, 5]).any()
+    others = [c for c in range(d) if c != 5]
+    close(v[:, :, others], want[:, :, others], tol[:, :, others])
+
+
+@pytest.mark.parametrize("layout", ["rows", "heads", "planes"])
+@pytest.mark.parametrize("n", [300, 1500])
+def test_out_between_keys_and_values(ctx, layout, n):
+    """Fused layouts of which out is a part: no element of it is theirs."""
+    g, heads, d = gen(34), 2, 128
+    shape = {"rows": (n, 4, heads, d), "heads": (n, heads, 4, d), "planes": (heads, 4, n, d)}[layout]
+    fused = randn(g, *shape, dtype=BF16)
+    order = {"rows": (1, 0, 2, 3), "heads": (2, 0, 1, 3), "planes": (1, 2, 0, 3)}[layout]
+    q, k, out, v = fused.permute(order).unbind(0)
+    kept = [t.clone() for t in (q, k, v)]
+    a = DECAYS["mild"](heads).cuda()
+    states = torch.zeros(1, heads, d, d, device="cuda")
+    L.linear_attention_device(ctx, L.StateBatch(states, ints([0, n]), n), q, k, v, out, a.float())
+    ctx.synchronize()
+    want, mag, after, sizes = recurrence(*kept, a.float(), [n], torch.zeros_like(states), d ** -0.5)
+    tol, state_tol = tolerances(BF16, d, n, a, want, mag, sizes, False)
+    close(out, want, tol)
+    close(states, after, state_tol)
+    assert all(torch.equal(x, y) for x, y in zip((q, k, v), kept))
+
+
+def test_out_over_keys_or_values_that_heads_share_is_refused(ctx):
+    n, d = 70, 64
+    fused = torch.zeros(n, 8, d, device="cuda", dtype=BF16)
+    q, other = fused[:, :4], fused[:, 4:]
+    a = torch.zeros(4, device="cuda")
+    b = L.StateBatch(torch.zeros(1, 4, d, d, device="cuda"), ints([0, n]), n)
+    apart = torch.zeros(n, 2, d, device="cuda", dtype=BF16)
+    for name, k, v in (("k", other[:, :2], apart), ("v", apart, other[:, :2])):
+        with pytest.raises(L.LwmError, match=f"out may be {name} only with as many kv_heads as heads and the same strides"):
+            L.linear_attention_device(ctx, b, q, k, v, other, a)
+    with pytest.raises(L.LwmError, match="out may be k only"):  # other strides
+        L.linear_attention_device(ctx, b, q, torch.as_strided(other, (n, 4, d), (4 * d, d, 1), other.storage_offset()), q, other, a)
