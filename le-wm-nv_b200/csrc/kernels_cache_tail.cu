@@ -35,6 +35,14 @@ template <typename T, bool kCodes> __device__ __forceinline__ void values(const 
     else unpack(Vec8<T>{c.w}, f);
 }
 
+// The larger one, NaN where either is (fmaxf leaves NaN out: a row that sees
+// nothing but NaN would look like one that sees nothing).
+__device__ __forceinline__ float max_or_nan(float x, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
+
 template <typename T, int D, bool kCodes, int kRows>
 __global__ void __launch_bounds__(kThreads, kRows == 1 ? 6 : 5) cache_tail_kernel(const __grid_constant__ CacheAttnArgs a, uint32_t heads) {
     using C = Chunk8<T, kCodes>;
@@ -193,10 +201,10 @@ __global__ void __launch_bounds__(kThreads, kRows == 1 ? 6 : 5) cache_tail_kerne
             }
 #pragma unroll
             for (int r = 0; r < kRows; ++r) {
-                float top = fmaxf(fmaxf(sc[r][0], sc[r][1]), fmaxf(sc[r][2], sc[r][3]));
+                float top = max_or_nan(max_or_nan(sc[r][0], sc[r][1]), max_or_nan(sc[r][2], sc[r][3]));
 #pragma unroll
-                for (int o = kLanes; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                top = fmaxf(top, m[r]);
+                for (int o = kLanes; o < 32; o *= 2) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = max_or_nan(top, m[r]);
                 const float down = m[r] == -INFINITY ? 0.0f : exp2_fast(m[r] - top);
                 m[r] = top;
                 if (i == 0) continue;
@@ -248,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, kRows == 1 ? 6 : 5) cache_tail_kerne
         if (!owns) continue;
         // the tail's sum is ll 2^ml; a part's, its logarithm with its values already divided by it
         float top = ll == 0.0f ? -INFINITY : ml;
-        bool nan = false;
+        bool nan = ll != ll;
         auto part_at = [&](uint32_t x) { return x == 0 ? first_log : a.part_log[x * part_rows + row]; };
         if (joined)
             for (uint32_t x = 0; x < a.splits; ++x) {
