@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
     auto update = [&](uint32_t i) {
         const uint32_t k_a = smem_a + (i - first) % S::kStages * 3 * S::kTile + S::kTile, v_a = k_a + S::kTile;
         const uint32_t m = min(static_cast<uint32_t>(kChunk), v.n - i * kChunk);
-        const float fade = expm1f(decay * m);
+        const Fade fade = fade_of(decay * m);
         float scale[2] = {1.0f, 1.0f}, back[2] = {1.0f, 1.0f};
         auto weight = [&](int k, int e) {  // of tokens 16 k + 2 t, + 1, + 8, + 9
             const int left = static_cast<int>(m) - 1 - (16 * k + 2 * t + (e & 1) + 8 * (e >> 1));
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float& y = st[n0 + n][e];
-                    y = fmaf(sum[n][e], S::kHalf ? back[e >> 1] : 1.0f, fmaf(y, fade, y));
+                    y = faded(fade, y, S::kHalf ? sum[n][e] * back[e >> 1] : sum[n][e]);
                 }
         }
     };
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
                     if (b >= parts) break;
                     cluster.map_shared_rank(shared, b)[at_x] = y;
                     const uint32_t done = min(b * per * kChunk, v.n), tokens = min(v.n - done, per * kChunk);
-                    y = fmaf(y, expm1f(decay * tokens), y) + added[b];
+                    y = faded(fade_of(decay * tokens), y, added[b]);
                 }
             }
             meet_cluster();

@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!fine) break;
             tc::fence_after();
             // Sums in TMEM are cut off, not rounded, at each step: a chunk's are added to the state here.
-            const float fade = expm1f(decay * m);
+            const Fade fade = fade_of(decay * m);
             if (has_row) {
 #pragma unroll
                 for (int c = 0; c < D / 2; c += 32) {
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld32(t_lane + S::kSCol + col0 + c, y);
                     tc::tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[c + e] = fmaf(x[c + e], fade, x[c + e]) + y[e];
+                    for (int e = 0; e < 32; ++e) x[c + e] = faded(fade, x[c + e], y[e]);
                     if (whole && more) {
                         copy16(c, x + c);
                         copy16(c + 16, x + c + 16);
@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant
     if (count == 1) return;
     float decay = a.log_decay[h];
     if (decay < -200.0f) decay = -200.0f;
-    const float fade = expm1f(decay * (per * kChunk));  // (all but the last part are that long)
+    const Fade fade = fade_of(decay * (per * kChunk));  // (all but the last part are that long)
     const size_t size = static_cast<size_t>(D) * D;
     float y = v.source < 0 ? 0.0f : a.states[(static_cast<size_t>(v.source) * a.heads + h) * size + (i % D) * D + i / D];
     // (eight parts are read before the first of them is written)
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) {
             if (r0 + e < count) *at[e] = y;
-            y = fmaf(y, fade, y) + added[e];
+            y = faded(fade, y, added[e]);
         }
     }
 }

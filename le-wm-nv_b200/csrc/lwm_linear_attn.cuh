@@ -43,6 +43,25 @@ __device__ __forceinline__ StateView state_view(const LinearArgs& a, uint32_t s,
     return v;
 }
 
+// e^x, x at most zero, as a sum of two floats: the one below the nearest float,
+// and what is left of it.  Near one a single float is off by up to 2^-25, which
+// a state that is multiplied again and again would forget more or less by; far
+// from one, e^x - 1 alone would keep only 2^-24 of one, not of e^x.  (Both are
+// positive, so an infinite state stays infinite.)
+struct Fade {
+    float most, rest;
+};
+__device__ __forceinline__ Fade fade_of(float x) {
+    const float less = expm1f(x);
+    const bool near = x > -0.5f;
+    const float all = near ? 1.0f + less : expf(x);
+    const float lost = near ? less - (all - 1.0f) : 0.0f;  // (exact)
+    const float most = all > 0.0f ? __uint_as_float(__float_as_uint(all) - 1u) : all;
+    return {most, (all - most) + lost};
+}
+// y e^x + added, rounded at y's size once.
+__device__ __forceinline__ float faded(const Fade& f, float y, float added) { return fmaf(y, f.most, fmaf(y, f.rest, added)); }
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
     // a dead row's 16 bytes are filled with zeros, its address is not read
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");

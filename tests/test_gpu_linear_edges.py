@@ -3,7 +3,7 @@ finite in the first chunk of many blocks at once."""
 import pytest
 
 import lewm_b200 as L
-from test_gpu_linear import BF16, DECAYS, F16, close, gen, ints, randn, recurrence, tolerances
+from test_gpu_linear import BF16, DECAYS, E32, F16, close, gen, ints, randn, recurrence, tolerances
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -128,3 +128,57 @@ def test_out_over_keys_or_values_that_heads_share_is_refused(ctx):
             L.linear_attention_device(ctx, b, q, k, v, other, a)
     with pytest.raises(L.LwmError, match="out may be k only"):  # other strides
         L.linear_attention_device(ctx, b, q, torch.as_strided(other, (n, 4, d), (4 * d, d, 1), other.storage_offset()), q, other, a)
+
+
+# ---- what a state keeps while nothing is added to it, or little
+
+FADES = [(9, -0.5), (64, -0.27), (64, -1.0), (128, -0.135), (130, -0.5), (300, -0.2), (700, -0.1), (5000, -0.012), (3000, -2.0 ** -12),
+         (2000, 0.0)]
+
+
+def kept_tolerance(dtype, n, rate, out, mag, sizes):
+    """A chunk of 64 tokens or more (or a part of them) multiplies the state once: the exponent is off by 2^-24 of it,
+    its exponential by two steps of 2^-24 and what follows by two more, the sums of a chunk by three; a cut along time
+    joins parts once more.  Keys of a chunk: in two parts or more of the type (f16 down to 2^-38 of the largest of a
+    channel).  Outputs: the state's rounding for its product with q, and their own."""
+    u = torch.finfo(dtype).eps / 2
+    state = E32 * (2 * abs(rate) * n + 8 * (n / 64 + 2)) + 1.01 * u * u + 64 * 2.0 ** -38
+    return mag * (state + 1.01 * u + 200 * E32) + u * (out.abs() * 1.001 + torch.finfo(dtype).tiny), sizes * state + 1e-44
+
+
+@pytest.mark.parametrize("n,rate", FADES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("keys", [0, 40])
+def test_states_that_nothing_is_added_to_keep_what_is_left(ctx, d, dtype, n, rate, keys):
+    """Tokens whose keys are zero (behind some whose keys are not): the state is what the decay leaves of it, to the
+    precision of what is left, however little that is."""
+    g, heads, n = gen(35), 2, n + keys
+    q, k, v = (randn(g, n, heads, d, dtype=dtype) for _ in range(3))
+    k[keys:] = 0
+    a = torch.tensor([rate, rate / 2], device="cuda", dtype=torch.float64)
+    states, out = randn(g, 1, heads, d, d), torch.empty_like(q)
+    want, mag, after, sizes = recurrence(q, k, v, a.float(), [n], states, d ** -0.5)
+    L.linear_attention_device(ctx, L.StateBatch(states, ints([0, n]), n), q, k, v, out, a.float())
+    ctx.synchronize()
+    tol, state_tol = kept_tolerance(dtype, n, rate, want, mag, sizes)
+    close(states, after, state_tol)
+    close(out, want, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_many_short_sequences_keep_what_is_left(ctx, d, dtype):
+    """The same for more sequences than are cut along time, of one chunk and of two."""
+    g, heads, news = gen(36), 4, [64, 128, 130, 0, 100] * 12
+    n, s = sum(news), len(news)
+    q, v = (randn(g, n, heads, d, dtype=dtype) for _ in range(2))
+    k = torch.zeros_like(q)
+    a = torch.tensor([-0.1, -0.2, -0.35, -0.5], device="cuda", dtype=torch.float64)
+    states, out = randn(g, s, heads, d, d), torch.empty_like(q)
+    want, mag, after, sizes = recurrence(q, k, v, a.float(), news, states, d ** -0.5)
+    L.linear_attention_device(ctx, L.StateBatch(states, ints([sum(news[:i]) for i in range(s + 1)]), n, 130), q, k, v, out, a.float())
+    ctx.synchronize()
+    tol, state_tol = kept_tolerance(dtype, 130, -0.5, want, mag, sizes)
+    close(states, after, state_tol)
+    close(out, want, tol)
