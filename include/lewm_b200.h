@@ -968,9 +968,12 @@ lwm_status lwm_cache_attention_shared_device(lwm_ctx* ctx, const lwm_paged_cache
  * q, out [tokens, heads, head_dim], k, v [tokens, kv_heads, head_dim] of
  * `dtype` (bf16 or f16).  In place: out may be q, and with as many kv_heads as
  * heads k or v (the same rows and strides; otherwise no element of out is one of
- * theirs).  Query head h and its state use kv head
- * h / (heads / kv_heads).  log_decay [heads] f32, natural logarithms, zero
- * (nothing fades) or below; minus infinity: every token starts afresh.
+ * theirs).  Query head h and its state use kv head h / (heads / kv_heads).
+ * log_decay [heads] f32, natural logarithms, zero (nothing fades) or below;
+ * minus infinity: every token starts afresh.  The factor of a token or a chunk
+ * is held to 2^-23 of its distance from one, so tokens that come one by one
+ * forget as a history does, but for the state's rounding to 32 bits at each:
+ * what a token fades by less than 2^-25 of a value is lost there.
  * In chunks, the weights q.k lambda^n are rounded to dtype for their product
  * with v, the state is rounded to bf16 (f16: to 11 bits of any range) for the
  * product with q, and keys times their decay enter the state with 24 bits

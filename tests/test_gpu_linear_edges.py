@@ -182,3 +182,38 @@ def test_many_short_sequences_keep_what_is_left(ctx, d, dtype):
     tol, state_tol = kept_tolerance(dtype, 130, -0.5, want, mag, sizes)
     close(states, after, state_tol)
     close(out, want, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("keys", [0.0, 1.0 / 64])
+def test_single_tokens_forget_as_a_history_does(ctx, d, dtype, keys):
+    """4096 calls of a token each, at log decays whose factor lies between two floats.  A state rounds twice a token,
+    half a step at most each, their signs at random: its norm moves by 2^-24 sqrt(2 n) or less (twice that allowed,
+    and 16 steps for what is common to all).  Without keys the signs are not at random: a token takes |a| 2^23 steps
+    and more off an element, whose part of a step stays alike until the element has moved, so c = a^2 n 2^23 times
+    in the run (once at least) a new sign begins, and the norm moves by n / c sqrt(c) times the root mean square of a
+    rounding, 0.29 steps of 2^-23 at most.  A factor that is rounded once is off by up to 2^-25 a token, all to one
+    side: 2^-13 after so many."""
+    g, n, a = gen(37), 4096, torch.tensor([-2.0 ** -12, -3e-5, -1e-6, -0.01], device="cuda", dtype=torch.float64)
+    heads = a.numel()
+    q, k, v = (randn(g, n, heads, d, dtype=dtype) for _ in range(3))
+    k *= keys
+    first = randn(g, 1, heads, d, d)
+    a = a.float().double()
+    left = torch.exp(a[None] * torch.arange(n - 1, -1, -1, device="cuda", dtype=torch.float64)[:, None])[..., None]
+    want = torch.exp(a * n)[:, None, None] * first[0].double() + torch.einsum("nhk,nhv->hkv", k.double() * left, v.double())
+    limit = E32 * (2 * (2 * n) ** 0.5 + 16 + (0.58 * n / (a * a * n * 2.0 ** 23).clamp(min=1.0).sqrt() if keys == 0 else 0.0))
+    steps, out = first.clone(), torch.empty_like(q)
+    b = L.StateBatch(steps, ints([0, 1]), 1)
+    for i in range(n):
+        L.linear_attention_device(ctx, b, q[i:i + 1], k[i:i + 1], v[i:i + 1], out[i:i + 1], a.float())
+    history = first.clone()
+    L.linear_attention_device(ctx, L.StateBatch(history, ints([0, n]), n), q, k, v, torch.empty_like(q), a.float())
+    eights = first.clone()
+    for i in range(0, n, 8):
+        L.linear_attention_device(ctx, L.StateBatch(eights, ints([0, 8]), 8), q[i:i + 8], k[i:i + 8], v[i:i + 8], out[i:i + 8], a.float())
+    ctx.synchronize()
+    for got in (steps, history, eights):
+        off = (got[0].double() - want).norm(dim=(1, 2)) / want.norm(dim=(1, 2))
+        assert (off <= limit + (1.01 * (torch.finfo(dtype).eps / 2) ** 2 if got is history else 0.0)).all(), off
