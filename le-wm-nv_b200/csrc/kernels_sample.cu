@@ -42,9 +42,10 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kList = 1024;     // candidates that are sorted
-constexpr int kMaxSplit = 16;   // blocks of a row
+constexpr uint32_t kMaxSplit = 8;      // blocks of a row
 constexpr int kBins = 512;
 constexpr uint32_t kMaxSlice = 32768;  // logits of a block
+static_assert(kMaxSplit * kMaxSlice >= kSampleVocab, "a row fits its blocks");
 constexpr float kSpan = 45.0f;  // powers of two that the bins span: weights end there
 constexpr float kUnits = 8192.0f;
 static_assert(kUnits * kSampleVocab < 4294967296.0f, "a bin's mass");
@@ -693,8 +694,7 @@ template <typename T, int kThreads, bool kFilter> cudaError_t launch(const Token
     const int vectors = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.stride * sizeof(T) % 16 == 0;
     const uint32_t slice = ((a.vocab + split - 1) / split + 7) / 8 * 8;
     cudaError_t e = cudaSuccess;
-    if (split > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess && slice * 4 > 16384) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice * 4);
+    if (slice * 4 > 16384) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice * 4);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.rows * split);
@@ -716,7 +716,7 @@ template <typename T, bool kFilter> cudaError_t by_vocab(const TokenArgs& a, cud
     uint32_t split = 1;
     while (split * kMaxSlice < a.vocab) split *= 2;
     // few rows: more blocks each, down to 8192 logits
-    while (a.rows * split * 2 <= 148 && split < 8 && split * 2 * 8192 <= a.vocab) split *= 2;
+    while (a.rows * split * 2 <= 148 && split < kMaxSplit && split * 2 * 8192 <= a.vocab) split *= 2;
     return a.vocab > 16384 * split ? launch<T, 1024, kFilter>(a, split, s) : launch<T, 512, kFilter>(a, split, s);
 }
 
