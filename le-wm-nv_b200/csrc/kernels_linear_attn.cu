@@ -42,20 +42,6 @@ template <int D> struct StepShape {
     static constexpr int kRowGroups = kThreads / kCols, kRows = D / kRowGroups;
 };
 
-// Two products and sums at once.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(r)
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)), "l"(reinterpret_cast<const uint64_t&>(c)));
-    return reinterpret_cast<const float2&>(r);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-    return reinterpret_cast<const float2&>(r);
-}
-
 template <int D> struct alignas(16) Channels {  // of a token, read four at a time
     float x[D];
 };
@@ -80,7 +66,6 @@ __global__ void __launch_bounds__(StepShape<D>::kThreads) linear_step_kernel(con
     // As the chunks do it: with lambda rounded to 32 bits a head that forgets 1 / 4096 a token would be off by 1e-4 of
     // that.  (What a token fades by less than 2^-25 of the state is lost in the state's own rounding.)
     const Fade fade = fade_of(a.log_decay[h]);
-    const float2 most = make_float2(fade.most, fade.most), rest = make_float2(fade.rest, fade.rest);
     const uint32_t hk = a.group_div.div(h);
     for (uint32_t i = 0; i < v.n; ++i) {
         const size_t tok = v.start + i;
@@ -98,8 +83,7 @@ __global__ void __launch_bounds__(StepShape<D>::kThreads) linear_step_kernel(con
         for (int j = 0; j < S::kRows; ++j) {
             const float k = k_s.x[r + j * S::kRowGroups], q = q_s.x[r + j * S::kRowGroups];
             auto next = [&](float& s0, float& s1, float x0, float x1, float& o0, float& o1) {
-                // (faded, with k v in the place of what is added)
-                const float2 y = fma2(most, make_float2(s0, s1), fma2(make_float2(k, k), make_float2(x0, x1), mul2(rest, make_float2(s0, s1))));
+                const float2 y = faded(fade, make_float2(s0, s1), make_float2(x0, x1), make_float2(k, k));
                 const float2 z = fma2(make_float2(q, q), y, make_float2(o0, o1));
                 s0 = y.x, s1 = y.y, o0 = z.x, o1 = z.y;
             };
@@ -146,6 +130,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
     constexpr int kSteps = D / 16, kTiles = D / 8, kCols = kTiles / S::kSplit;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float power[kChunk + 1];  // lambda^i
+    __shared__ Fade fades[2 + kMostParts];      // of a whole chunk, of the last one, of each block's tokens
     __shared__ uint32_t bad_chunk[S::kStages];  // the last chunk there whose values are not all finite
     if (threadIdx.x < S::kStages) bad_chunk[threadIdx.x] = 0xffffffffu;
     // (called from either kind of warp)
@@ -160,12 +145,16 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
     float decay = a.log_decay[h];
     if (decay < -200.0f) decay = -200.0f;  // (e^-200 is zero; minus infinity times zero would be NaN)
     for (int i = threadIdx.x; i <= kChunk; i += S::kThreads) power[i] = expf(decay * i);
-    meet();  // (before any warp marks a chunk there)
-
     const uint32_t smem_a = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
     // this block's chunks of the sequence
     const uint32_t chunks = (v.n + kChunk - 1) / kChunk, per = (chunks + parts - 1) / parts;
     const uint32_t first = min(rank * per, chunks), end = min(first + per, chunks);
+    if (threadIdx.x < 2 + parts) {
+        const uint32_t b = threadIdx.x - 2, before = min(b * per * kChunk, v.n);
+        const uint32_t tokens = threadIdx.x == 0 ? kChunk : threadIdx.x == 1 ? (v.n + kChunk - 1) % kChunk + 1 : min(v.n - before, per * kChunk);
+        fades[threadIdx.x] = fade_of(decay * tokens);
+    }
+    meet();  // (what is set up so far, before any warp uses it, or marks a chunk)
     constexpr int kRowChunks = D / 8, kEach = kChunk * kRowChunks / S::kThreads;
     auto load = [&](uint32_t i, bool with_q) {
         if (i < end) {
@@ -199,7 +188,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
     auto update = [&](uint32_t i) {
         const uint32_t k_a = smem_a + (i - first) % S::kStages * 3 * S::kTile + S::kTile, v_a = k_a + S::kTile;
         const uint32_t m = min(static_cast<uint32_t>(kChunk), v.n - i * kChunk);
-        const Fade fade = fade_of(decay * m);
+        const Fade fade = fades[m < kChunk];
         float scale[2] = {1.0f, 1.0f}, back[2] = {1.0f, 1.0f};
         auto weight = [&](int k, int e) {  // of tokens 16 k + 2 t, + 1, + 8, + 9
             const int left = static_cast<int>(m) - 1 - (16 * k + 2 * t + (e & 1) + 8 * (e >> 1));
@@ -271,9 +260,16 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
 #pragma unroll
             for (int n = 0; n < kGroup; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float& y = st[n0 + n][e];
-                    y = faded(fade, y, S::kHalf ? sum[n][e] * back[e >> 1] : sum[n][e]);
+                for (int e = 0; e < 4; e += 2) {
+                    float* const y = &st[n0 + n][e];
+                    if constexpr (S::kHalf && D == 128) {  // (pairs: 4 % for the registers that hold them)
+                        y[0] = faded(fade, y[0], sum[n][e] * back[e >> 1]);
+                        y[1] = faded(fade, y[1], sum[n][e + 1] * back[e >> 1]);
+                    } else {
+                        const float2 x = make_float2(y[0], y[1]), added = make_float2(sum[n][e], sum[n][e + 1]);
+                        const float2 z = S::kHalf ? faded(fade, x, added, make_float2(back[e >> 1], back[e >> 1])) : faded(fade, x, added);
+                        y[0] = z.x, y[1] = z.y;
+                    }
                 }
         }
     };
@@ -499,8 +495,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
                 for (uint32_t b = 0; b < kMostParts; ++b) {
                     if (b >= parts) break;
                     cluster.map_shared_rank(shared, b)[at_x] = y;
-                    const uint32_t done = min(b * per * kChunk, v.n), tokens = min(v.n - done, per * kChunk);
-                    y = faded(fade_of(decay * tokens), y, added[b]);
+                    y = faded(fades[2 + b], y, added[b]);
                 }
             }
             meet_cluster();

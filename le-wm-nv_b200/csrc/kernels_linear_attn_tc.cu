@@ -87,6 +87,7 @@ struct Control {
     uint32_t tmem;
     int dead;     // a wait gave up
     float power[kChunk + 1];  // lambda^i
+    Fade fades[2];            // of a whole chunk, and of the sequence's last one
 };
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Control* c, int site, uint64_t* err, uint32_t seq) {
@@ -226,6 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::mbar_fence_init();
     }
     for (int i = threadIdx.x; i <= kChunk; i += kThreads) ctl->power[i] = expf(decay * i);
+    if (threadIdx.x < 2) ctl->fades[threadIdx.x] = fade_of(decay * (threadIdx.x ? (v.n + kChunk - 1) % kChunk + 1 : kChunk));
     if constexpr (D == 64)
         for (int i = threadIdx.x; i < S::kRound * 8; i += kThreads) *reinterpret_cast<uint4*>(smem + S::kZero + i * 16) = make_uint4(0, 0, 0, 0);
     tc::fence_async_smem();
@@ -376,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!fine) break;
             tc::fence_after();
             // Sums in TMEM are cut off, not rounded, at each step: a chunk's are added to the state here.
-            const Fade fade = fade_of(decay * m);
+            const Fade fade = ctl->fades[m < kChunk];
             if (has_row) {
 #pragma unroll
                 for (int c = 0; c < D / 2; c += 32) {
@@ -384,7 +386,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld32(t_lane + S::kSCol + col0 + c, y);
                     tc::tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[c + e] = faded(fade, x[c + e], y[e]);
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 z = faded(fade, make_float2(x[c + e], x[c + e + 1]), make_float2(y[e], y[e + 1]));
+                        x[c + e] = z.x, x[c + e + 1] = z.y;
+                    }
                     if (whole && more) {
                         copy16(c, x + c);
                         copy16(c + 16, x + c + 16);

@@ -61,6 +61,25 @@ __device__ __forceinline__ Fade fade_of(float x) {
 }
 // y e^x + added, rounded at y's size once.
 __device__ __forceinline__ float faded(const Fade& f, float y, float added) { return fmaf(y, f.most, fmaf(y, f.rest, added)); }
+// Two products and sums at once.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(r)
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)), "l"(reinterpret_cast<const uint64_t&>(c)));
+    return reinterpret_cast<const float2&>(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return reinterpret_cast<const float2&>(r);
+}
+__device__ __forceinline__ float2 faded(const Fade& f, float2 y, float2 added) {
+    return fma2(y, make_float2(f.most, f.most), fma2(y, make_float2(f.rest, f.rest), added));
+}
+__device__ __forceinline__ float2 faded(const Fade& f, float2 y, float2 added, float2 times) {  // added times times
+    return fma2(y, make_float2(f.most, f.most), fma2(added, times, mul2(y, make_float2(f.rest, f.rest))));
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
     // a dead row's 16 bytes are filled with zeros, its address is not read
