@@ -914,16 +914,18 @@ lwm_status lwm_cache_attention_device(lwm_ctx* ctx, const lwm_paged_cache* cache
  * group's sequences name pages that hold the same tokens there (the same pages
  * as a rule, and for a page that the prefix ends in a copy of each sequence's
  * own); a call may read them from the first sequence's.  New tokens lie behind
- * the prefix.  max_tokens is at least the packed rows of any group,
- * max_length (0: the table's reach) and max_tail (0: the batch's max_length
- * less this one, if both are given) say how long prefixes and what follows
- * them get, for the shape of the launch only.
+ * the prefix.  max_tokens is at least the packed rows of any group (launches and
+ * the choice below are sized by count groups of so many: say it where there are
+ * several groups, the batch's tokens make each as large as all), max_length (0:
+ * the table's reach) and max_tail (0: the batch's max_length less this one, if
+ * both are given) say how long prefixes and what follows them get, for the shape
+ * of the launch only.
  *
  * workspace: 16-byte aligned, at least as many bytes as
  * lwm_cache_attention_shared_workspace says for the same arguments (tensors
- * may be null there; none are needed, 0, where the sequences are so few or the prefix
- * so short that lwm_cache_attention_device costs less; it runs then).  It holds
- * nothing between calls; calls in flight at once need one each.
+ * may be null there; none are needed, 0, where the sequences are so few or the
+ * prefix so short that lwm_cache_attention_device costs less; it runs then).  It
+ * holds nothing between calls; calls in flight at once need one each.
  *
  * A group whose sequences or rows are out of order or above max_tokens, or
  * whose prefix is beyond the table, is skipped with the sequences that it
@@ -971,9 +973,9 @@ lwm_status lwm_cache_attention_shared_device(lwm_ctx* ctx, const lwm_paged_cache
  * theirs).  Query head h and its state use kv head h / (heads / kv_heads).
  * log_decay [heads] f32, natural logarithms, zero (nothing fades) or below;
  * minus infinity: every token starts afresh.  The factor of a token or a chunk
- * is held to 2^-23 of its distance from one, so tokens that come one by one
- * forget as a history does, but for the state's rounding to 32 bits at each:
- * what a token fades by less than 2^-25 of a value is lost there.
+ * is held to 2^-22 of its distance from one, and to 2^-22 of itself, so tokens
+ * that come one by one forget as a history does, but for the state's rounding to
+ * 32 bits at each: what a token fades by less than 2^-25 of a value is lost there.
  * In chunks, the weights q.k lambda^n are rounded to dtype for their product
  * with v, the state is rounded to bf16 (f16: to 11 bits of any range) for the
  * product with q, and keys times their decay enter the state with 24 bits
@@ -1022,7 +1024,9 @@ lwm_status lwm_linear_attention_device(lwm_ctx* ctx, const lwm_state_batch* batc
  *
  * logits: rows `stride` elements apart (any alignment of the type; whole
  * 16-byte rows load faster), vocab up to 2^18; uniform [rows] f32 in [0, 1)
- * (others count as the nearest); tokens [rows] int32.  Parameters of each row, f32
+ * (others count as the nearest); tokens [rows] int32.  Temperatures above 0 count
+ * as at least 1e-30 and at most 1e30, logits below the smallest normal f32 as
+ * about zero.  Parameters of each row, f32
  * (top_ks int32) [rows] device arrays or NULL for the one value: there,
  * temperatures not above 0 take the largest logit, top_ks below 1 and top_ps
  * from 1 on (or NaN) keep all, min_ps not above 0 too.  Weights have a relative error

@@ -28,9 +28,10 @@
 //
 // Tails (kTailKeys): what lies behind a prefix that a group shares, joined with
 // the prefix's parts, which another kernel leaves in the workspace; it may
-// start beside that one and waits for it only before the join (64 candidates of
-// 4 tokens with tails up to 64 tokens, 32 heads over 8 of 128: 50 us, most of
-// them beside a prefix of 208).
+// start beside that one and waits for it only before the join, of the first head
+// where a warp has several (64 candidates of 4 tokens with tails up to 64 tokens,
+// 32 heads over 8 of 128, a head a block: 50 us, most of them beside a prefix of
+// 208).
 //
 // 8-bit codes become halves in registers: e4m3 is exact in fp16.  The
 // contraction's order is free, so a thread's 16 bytes of a key are the four

@@ -8,13 +8,15 @@
 // channels; everything is in 32 bits on CUDA cores: the products of one row
 // with a dozen keys are too few for the tensor cores' 16 x 8 tiles, of which
 // they would fill one row.  The prefix's parts are asked for together with the
-// keys, and joined at the end.
+// keys, and joined at the end.  The grid may start beside the prefix's, but a
+// warp waits for that before the join of its first head, so one head a warp runs
+// ahead at most: with four heads a warp nearly nothing overlaps.
 //
 // What bounds it (one B200): instructions, and each head's chain of keys, scores
 // and join.  1024 candidates of 16 heads of 64 with up to 16 tokens of their own
-// (bf16): 18 us, where their 35 MB of keys, values and rows and the parts' 8
-// would take 7 (the tensor-core kernel for few rows: 42; the whole call 57.8 us
-// with that, 43.0 with this).  The next head's keys asked for ahead: 48.9 and
+// (bf16): 18 us behind the prefix's 26, where their 35 MB of keys, values and
+// rows and the parts' 8 would take 7 (the tensor-core kernel for few rows: 42;
+// the whole call 57.8 us with that, 43.0 with this).  The next head's keys asked for ahead: 48.9 and
 // 59.8, the registers cost a block or two of the SM's six.  4 rows a warp:
 // slower than tensor cores (16 vehicles' 64 candidates, 4 rows, 8-bit codes:
 // 118 instead of 91), so up to 2, and tails up to 128 tokens.

@@ -4,10 +4,14 @@
 // S one f32 [head_dim, head_dim] state a head.
 //
 // A few tokens a sequence (linear_step_kernel): the state is read once, kept
-// in registers over the tokens, and written once.  Bound by those bytes: 1024
-// sequences of 16 heads of 64, a token each, 537 MB in 84.6 us, 6.4 TB/s; 256
-// that fork from one state, 16 heads of 128, 268 MB written in 64 us.  Up to 8
-// tokens: 8 of those 1024 take 184 us, in chunks 267, and each token more 16.
+// in registers over the tokens, and written once.  Where every sequence has a
+// state of its own that is bound by those bytes: 1024 sequences of 16 heads of
+// 64, a token each, 537 MB in 84.2 us, 6.4 TB/s.  256 that fork from one state,
+// 16 heads of 128, write 268 MB in 61 us, which a plain fill would do in 38:
+// there each block's way from its state (in the L2) over the sums to its stores
+// is the bound, one after the other, with two blocks of 8 warps an SM for their
+// 107 registers (DRAM 41 %, L2 45 %).  Up to 8 tokens: 8 of those 1024 take 186
+// us, in chunks 283, and each token more 17, the latency of its loads.
 //
 // Whole histories (linear_chunk_kernel): chunks of 64 tokens,
 //   O = lambda^(i+1) Q S + (Q K^T . lambda^(i-j), j <= i) V,
@@ -15,11 +19,16 @@
 // all four products on mma.sync with the state in registers: half of the warps
 // keep it, the others compute the outputs of the chunk before.  For f16 (whose
 // states and weights need powers of two a row, and tf32 for Q S), 32 channels,
-// short sequences, and strides that a tensor map does not take; long ones of
-// bf16 with 64 or 128 channels go on tcgen05.  Bound by the products' issue and
-// the fragments' way to them: 16 sequences of 1568 tokens, 16 heads, f16, of 32
-// channels 63 us, of 64 108, of 128 (one block a SM) 353; one of 65536 tokens
-// 371, 595, 2665.
+// short sequences, strides that a tensor map does not take, and an out that may
+// lie on keys or values; long ones of bf16 with 64 or 128 channels go on
+// tcgen05.  Bound by the products' issue and the fragments' way to them: 16
+// sequences of 1568 tokens, 16 heads, f16, of 32 channels 62 us, of 64 109, of
+// 128 (one block a SM) 359; one of 65536 tokens 367, 609, 2669.
+//
+// What is rounded to 16 bits: a row's weights, as operands of their product
+// with v (a rounding costs them half a step each, of either sign, as that of
+// the output does), and the state's copy for the product with q (f16: 11 bits
+// by tf32).  The state itself and what enters it keep 22 bits and more.
 #include <cooperative_groups.h>
 
 #include <algorithm>

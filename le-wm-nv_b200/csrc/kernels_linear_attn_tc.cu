@@ -7,7 +7,9 @@
 //   O1 = Q S, O2 = P V             (TMEM), out = scale (lambda^(i+1) O1 + O2)
 //   S  = lambda^m S + K'^T V       (the product in TMEM, S in registers; a bf16 copy in shared memory for O1)
 // with K' = lambda^(m-1-j) k_j in three parts of 8 bits, so that S keeps them
-// as 32-bit products would.
+// as 32-bit products would.  P and the copy of S are rounded to bf16 as operands
+// have to be: half a step each, of either sign, which in a sum costs about what
+// rounding the output does (errors of 0.0023 against 0.0017 for the latter alone).
 //
 // Warps: four for the outputs (a token a thread: P, O1, O2), eight for the
 // state (a key channel a thread, half of the value channels: K' some tokens at
@@ -25,22 +27,27 @@
 // another in few warps.  A chunk of 64 channels takes about 3.3 us, 4000 of its
 // cycles in the output warps and as many in the state's; one of 128 channels
 // 4.6, the state's warps (K' in parts, waits for the products, the state).  16
-// sequences of up to 1568 tokens, 16 heads of 64: 69.5 us, 256 blocks on 148
-// SMs, where the bytes would take 23; one of 65536 tokens, 16 heads of 128: 475
-// us (the states 193, the joining 9, the outputs 273), where its bytes (keys and
-// values read twice, 1.6 GB in DRAM) would take 250.  Measured otherwise:
+// sequences of up to 1568 tokens, 16 heads of 64: 68.5 us, 256 blocks on 148
+// SMs, where the bytes would take 23; one of 65536 tokens, 16 heads of 128: 458
+// to 474 us (the states 192, the joining 9, the outputs 270), where its bytes
+// (keys and values read twice, 1.6 GB in DRAM) would take 250.  Measured
+// otherwise, when these took 69.5 and 475:
 // mma.sync with the state in registers 98 and 1502; one stage of Q and P 72;
 // two sums of keys and values in TMEM by turns, so that no wait is left in the
 // state's warps, 73 and 470 (fewer cycles, more of them in each other's way);
 // the state in TMEM alone, summed there, 71 and 456, but off by 2e-5 where
 // nothing fades, as those sums are cut off (now 6e-7).
 //
+// A head's factor for a chunk is the sum of two floats (Fade), the same for a
+// chunk, a part and a single token, whatever is left of a state.
+//
 // Parts: a first launch walks them for the state alone, each from zero, a
 // second one turns what they add into the states before them, and a third one
 // walks them for the outputs.  In between, a part's state (32 bits) lies in the
 // rows of `out` that are the part's own, where nothing is kept yet; so no part is
 // shorter than that many rows, and a call whose out overlaps its inputs is not
-// cut here (most of those go by clusters on mma.sync).
+// cut here (most of those go by clusters on mma.sync, and all whose out may lie
+// on keys or values).
 //
 // Rows behind the sequence's end are another's: their keys weigh zero, their
 // values are zeroed.  Infinities and NaN among the values make outputs that
@@ -806,11 +813,12 @@ template <int D> cudaError_t launch(const LinearArgs& a, const CUtensorMap (&map
 }
 
 // 64 channels: the mma.sync kernel has two blocks a SM, chunks of 64 tokens and cuts that cost less (us, here and there):
-// 64 sequences of 16 heads with 128 tokens 53 and 37, 256 77 and 64, 512 120 and 113, 1024 198 and 211; one of 16 heads
-// with 128 tokens 8.3 and 7.4, 256 10.9 and 12.3, 512, cut along time, 15.6 and 13.6, 1024 26 and 17, 2048 30 and 31.
-// With 128 channels it has one block a SM: 16 heads with 128 tokens 14.9 and 15.0, 1024 sequences and heads 112 and 117.
+// 64 sequences of 16 heads with 128 tokens 53 and 36, 256 77 and 62, 512 120 and 111, 1024 187 and 208; one of 16 heads
+// with 128 tokens 8.3 and 7.4, 256 10.7 and 12.1, 512, cut along time, 15.6 and 12.8, 1024 26 and 15.4, 2048 29 and 28.
+// With 128 channels it has one block a SM: 16 heads with 128 tokens 14.7 and 17.8, 1024 sequences and heads 112 and 143.
 // Its cuts along time need no room in `out`, so it has the long sequences of a call whose out overlaps its inputs (65536
-// tokens, uncut here and there: 16 heads of 64 channels 1239 and 536, 16 of 128 2065 and 2525, 4 of 128 2057 and 650).
+// tokens, uncut here and there: 16 heads of 64 channels 1239 and 537, 16 of 128 2015 and 2529, 4 of 128 2057 and 657).
+// All with heads of their own keys and sequences of one length; ragged batches and shared heads go by the same rule.
 bool rather_there(const LinearArgs& a) {
     const uint64_t jobs = static_cast<uint64_t>(a.sequences) * a.heads;
     if (parts_of(a) > 1 && (a.head_dim == 64 || jobs * 16 <= 148) && overlaps(a)) return true;

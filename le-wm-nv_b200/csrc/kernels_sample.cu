@@ -19,7 +19,7 @@
 // rest of the call works on that alone.
 //
 // What bounds it (one B200): instructions.  256 rows of 32000 f32 logits with
-// top_p 0.95 take 105 us, of which their 33 MB from memory would be 5: two
+// top_p 0.95 take 104 us, of which their 33 MB from memory would be 5: two
 // passes that compute weights of 64 bits (28000 cycles of a block, the double
 // precision units of its SM the limit), a histogram of 32000 shared atomics, a
 // sort (11000 cycles) and about twenty barriers, for two blocks a SM one after

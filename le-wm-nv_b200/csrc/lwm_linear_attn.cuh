@@ -61,6 +61,7 @@ __device__ __forceinline__ Fade fade_of(float x) {
 }
 // y e^x + added, rounded at y's size once.
 __device__ __forceinline__ float faded(const Fade& f, float y, float added) { return fmaf(y, f.most, fmaf(y, f.rest, added)); }
+
 // Two products and sums at once.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     uint64_t r;

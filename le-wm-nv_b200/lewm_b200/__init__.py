@@ -1470,8 +1470,10 @@ def cache_attention_device(ctx: Context, cache: PagedCache, batch: CacheBatch, q
 class SharedPrefix:
     """lwm_shared_prefix: groups [count + 1] (sequences [groups[g], groups[g +
     1]) share their first tokens) and lengths [count] of those prefixes, int32
-    device tensors; bounds of a group's packed rows (None: the batch's), of a
-    prefix and of what follows it (0: not known)."""
+    device tensors; bounds of a group's packed rows (None: the batch's, which
+    makes each of several groups as large as all of them for the choice and the
+    shape of the launch: say it there), of a prefix and of what follows it (0:
+    not known)."""
 
     def __init__(self, groups, lengths, max_tokens: Optional[int] = None, max_length: int = 0, max_tail: int = 0):
         if groups.dim() != 1 or groups.shape[0] < 1:
@@ -1578,8 +1580,9 @@ class StateBatch:
 def linear_attention_device(ctx: Context, batch: StateBatch, q, k, v, out, log_decay, scale: Optional[float] = None) -> None:
     """out = linear attention of q [tokens, heads, head_dim] over k, v [tokens,
     kv_heads, head_dim] and the batch's states, which go on to their targets;
-    log_decay [heads] float32 (scale None: head_dim ** -0.5).  `out` and the
-    states are ready on the context's stream."""
+    log_decay [heads] float32 (scale None: head_dim ** -0.5).  `out` may be q, and
+    with as many kv_heads as heads k or v.  `out` and the states are ready on the
+    context's stream."""
     if batch.device_index != ctx.device:
         raise LwmError(1, f"states must be on cuda:{ctx.device}, got {batch.device}")
     if k.dim() != 3:
@@ -1605,7 +1608,8 @@ def sample_tokens_device(ctx: Context, logits, uniform, tokens, log_probs=None, 
     """tokens [rows] int32 = a token of each row of logits [rows, vocab], drawn
     with the random numbers uniform [rows] float32 in [0, 1) from what top_k,
     top_p and min_p keep; log_probs [rows] float32 its log-probability there.
-    Each parameter is a number or a [rows] tensor (float32, top_k int32).
+    Each parameter is a number or a [rows] tensor (float32, top_k int32);
+    temperatures count as 1e-30 to 1e30, those not above 0 take the largest logit.
     Outputs are ready on the context's stream."""
     if logits.dim() != 2:
         raise LwmError(1, f"logits must be [rows, vocab], got {list(logits.shape)}")
