@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, kCodes, kRows, kShared>::kB
                 // (the prefix's rows are the group's)
                 joined = group.ok && v.start >= group.start && v.start + v.n <= group.start + group.n;
                 shared = group.shared;
-                const bool reaches = joined && v.n && static_cast<uint64_t>(v.n) + shared > v.length;
+                const bool reaches = joined && shared && v.n && static_cast<uint64_t>(v.n) + shared > v.length;
                 if (reaches && h0 == 0 && tile == 0 && rank == 0 && lane == 0) cache_report(a.c.err, kCacheErrShared, s, shared);
                 if (!joined || reaches) v.n = 0;
             }

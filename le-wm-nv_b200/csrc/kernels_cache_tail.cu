@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kThreads, kRows == 1 ? 6 : 5) cache_tail_kerne
                 const GroupView group = group_view(a, g, false);
                 joined = group.ok && v.start >= group.start && v.start + v.n <= group.start + group.n;  // (the prefix's rows)
                 shared = group.shared;
-                const bool reaches = joined && v.n && static_cast<uint64_t>(v.n) + shared > v.length;
+                const bool reaches = joined && shared && v.n && static_cast<uint64_t>(v.n) + shared > v.length;
                 if (reaches && h0 == 0 && lane == 0) cache_report(a.c.err, kCacheErrShared, s, shared);
                 if (!joined || reaches) v.n = 0;
             }
