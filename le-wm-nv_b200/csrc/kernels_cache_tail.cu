@@ -16,10 +16,10 @@
 // and join.  1024 candidates of 16 heads of 64 with up to 16 tokens of their own
 // (bf16): 18 us behind the prefix's 26, where their 35 MB of keys, values and
 // rows and the parts' 8 would take 7 (the tensor-core kernel for few rows: 42;
-// the whole call 57.8 us with that, 43.0 with this).  The next head's keys asked for ahead: 48.9 and
-// 59.8, the registers cost a block or two of the SM's six.  4 rows a warp:
-// slower than tensor cores (16 vehicles' 64 candidates, 4 rows, 8-bit codes:
-// 118 instead of 91), so up to 2, and tails up to 128 tokens.
+// the whole call 57.8 us with that, 43.0 with this).  The next head's keys asked
+// for ahead: 48.9 and 59.8, the registers cost a block or two of the SM's six.  4
+// rows a warp: slower than tensor cores (16 vehicles' 64 candidates, 4 rows,
+// 8-bit codes: 118 instead of 91), so up to 2, and tails up to 128 tokens.
 #include "lwm_blocks.cuh"
 #include "lwm_cache_attn.cuh"
 

@@ -541,8 +541,9 @@ __global__ void __launch_bounds__(ChunkShape<T, D>::kThreads, ChunkShape<T, D>::
 
 // Blocks that a sequence and head are cut into along time (a cluster): as many as run at once, where they have two
 // chunks each at least.  A cut costs a second walk for the state, so two parts gain nothing (128 heads of 64 channels
-// over 1024 tokens: 51 us in two, 41 uncut); 16 heads of 64 over 1024 tokens in 8 parts 17 us, 16 heads of 128 channels
-// of bf16 over 65536 tokens 5382 uncut, 1979 in 4 (or in 8: a GPU has room for 15 clusters of 8 such blocks), 1502 in 16.
+// over 1024 tokens: 51 us in two, 41 uncut); 16 heads of 64 over 1024 tokens in 8 parts 15.4 us, 16 heads of 128 channels
+// of bf16 over 65536 tokens 2529 in 16 (before a chunk's sums were rounded into the state: 5382 uncut, 1979 in 4, or in
+// 8, as a GPU has room for 15 clusters of 8 such blocks, 1502 in 16).
 uint32_t parts_of(const LinearArgs& a, int resident) {
     const uint64_t jobs = static_cast<uint64_t>(a.sequences) * a.heads, chunks = (a.max_new + kChunk - 1) / kChunk;
     uint32_t parts = 1;
